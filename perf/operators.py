@@ -10,7 +10,7 @@ scale (E8M0), held in 4 bits (E2M1, two per byte, the even column in the low hal
 The scale of a block is 2^(floor(log2(largest magnitude)) - E), E the exponent of the element type's largest
 value (2 for E2M1, 8 for E4M3), its exponent kept within -127..127; elements are rounded to the nearest value
 of their type, ties to the even code, beyond its largest value to that.  Rows are padded with zeros to a
-multiple of 128 columns; a block of zeros has the smallest scale.  Layer sizes are those of the denoiser's
+multiple of 128 columns, a row's scales to a multiple of 16; a block of zeros has the smallest scale.  Layer sizes are those of the denoiser's
 linears (hidden 6144, key / value width 1536, MLP 16384), row counts from one token to a 1024-pixel
 image's 4096 latent tokens with 256 text tokens.
 """
@@ -127,14 +127,15 @@ def _pad(x):
 
 
 def _encode(x, fmt):
-    """f32 [M, K] -> codes (uint8 [M, Kp / 2] or float8_e4m3fn [M, Kp]) and scales (float8_e8m0fnu [M, Kp / 32])."""
+    """f32 [M, K] -> codes (uint8 [M, Kp / 2] or float8_e4m3fn [M, Kp]) and scales (float8_e8m0fnu, a
+    row's padded to whole 16 bytes)."""
     x = _pad(x)
     b = x.view(x.shape[0], -1, 32)
     amax = b.abs().amax(-1)
     e = torch.frexp(amax).exponent - 1 - EMAX[fmt]
     e = torch.where(amax > 0, e, -127).clamp(-127, 127)
     v = torch.ldexp(b, -e[..., None]).view(x.shape)
-    scales = (e + 127).to(torch.uint8).view(torch.float8_e8m0fnu)
+    scales = torch.nn.functional.pad((e + 127).to(torch.uint8), (0, -e.shape[1] % 16)).view(torch.float8_e8m0fnu)
     if fmt == E4M3:
         return v.clamp(-448, 448).to(torch.float8_e4m3fn), scales
     a = v.abs()
@@ -151,7 +152,8 @@ def _decode(codes, scales):
         v = torch.where(c >= 8, -1.0, 1.0) * table[(c & 7).int()]
     else:
         v = codes.float()
-    s = torch.ldexp(torch.ones((), device=codes.device), scales.view(torch.uint8).int() - 127)
+    s = scales.view(torch.uint8)[:, :v.shape[1] // 32].int() - 127
+    s = torch.ldexp(torch.ones((), device=codes.device), s)
     return (v.view(v.shape[0], -1, 32) * s[..., None]).view(v.shape)
 
 
@@ -227,11 +229,12 @@ def _held64(x, fmt):
     # the spacing of the element type's values around each magnitude
     step = torch.exp2(torch.floor(torch.log2(mag.clamp_min(2.0 ** low))) - bits)
     q = torch.round(mag / step) * step
+    scale = torch.cat([scale, scale.new_full((len(scale), -scale.shape[1] % 16), 2.0 ** -127)], 1)
     return (torch.sign(v) * q.clamp_max(most)).reshape(x.shape), scale
 
 
 def _times64(q, scale):
-    return (q.reshape(q.shape[0], -1, 32) * scale[..., None]).reshape(q.shape)
+    return (q.reshape(q.shape[0], -1, 32) * scale[:, :q.shape[1] // 32, None]).reshape(q.shape)
 
 
 def exact(case, seed):
