@@ -373,6 +373,52 @@ int svdq_attention_fwd_qnorm(const void* q, int64_t ldq, const void* k, const vo
                              int Hkv, float scale, const void* cos, const void* sin, int64_t ldcs, float eps, void* o,
                              int64_t ldo, void* workspace, hipStream_t stream);
 
+/* ---- Microscaled (MX) blocks -------------------------------------------------------------------
+ * 32 consecutive values of a row share an E8M0 scale byte s, 2^(s - 127) (255: the block is not a
+ * number); elements are E2M1 (4 bits, two per byte, the even column in the low half) or E4M3 (8 bits), as
+ * the OCP Microscaling specification v1.0 defines them.  No counterpart in the reference, whose
+ * activations and weights are INT4 groups.
+ *
+ * A matrix of R rows and K columns is held as codes, R rows of kp elements (kp = K rounded up to 128,
+ * zero codes beyond K; kp / 2 or kp bytes), and scales, R rows of sp bytes (sp = 16 * ceil(K / 512), 0
+ * beyond kp / 32), both contiguous and 16-byte aligned.
+ *
+ * Quantising a block: s = max(floor(log2(max |v|)) - E, -127) + 127 with E = 2 (E2M1) or 8 (E4M3);
+ * codes are the nearest values to v / 2^(s - 127), ties to even, beyond the largest value (6, 448) to that.
+ * A block with an infinity or a NaN gets s = 255 and zero codes; what reads it gets NaN. */
+#define SVDQ_MX_E2M1 0
+#define SVDQ_MX_E4M3 1
+
+/* bf16 x [M, K] (row stride ldx >= K, any alignment; 16-byte aligned rows and K % 8 == 0 run
+ * fastest) into MX blocks; every byte of codes and scales is written.  M = 0 does nothing. */
+int svdq_mx_quantize(const void* x, int64_t ldx, int M, int K, int fmt, void* codes, void* scales, hipStream_t stream);
+
+/* MX blocks back to contiguous bf16 y [M, K]: exact but for values below bf16's range. */
+int svdq_mx_dequantize(const void* codes, const void* scales, int M, int K, int fmt, void* y, hipStream_t stream);
+
+/* y [M, ldy] (bf16, or float32 with out_f32 = 1) = a w^T + bias: a [M, K] MX codes of format fmt with
+ * their scales, w [N, K] E2M1 codes with theirs, bias [N] bf16 or null.  Sums in float32, one rounding at
+ * the store.  E4M3 with bf16 output: within 8 consecutive k the matrix instruction drops what lies below
+ * 2^-13 of the largest product (about 1e-5 of a result); with float32 output, and E2M1, nothing is
+ * dropped.  M = 0 does nothing. */
+int svdq_mx_gemm(const void* a, const void* a_scales, int fmt, const void* w, const void* w_scales, const void* bias,
+                 int M, int N, int K, void* y, int64_t ldy, int out_f32, hipStream_t stream);
+
+/* The SwiGLU product silu(g) * u of bf16 g, u [M, K] (row strides ldg, ldu) in float32, into MX blocks
+ * (not rounded to bf16 first). */
+int svdq_silu_mul_mx(const void* g, int64_t ldg, const void* u, int64_t ldu, int M, int K, int fmt, void* codes,
+                     void* scales, hipStream_t stream);
+
+/* svdq_rms_norm_modulate and svdq_residual_rms_norm_modulate with the normed row in MX blocks:
+ *   y = x * rsqrt(mean(x^2) + eps) * w + shift   in float32, quantised (not rounded to bf16 first)
+ * of x, or of xo = bf16(x + g * v), which is stored.  H % 8 == 0, 16-byte aligned pointers and row
+ * strides (multiples of 8); xo may equal x. */
+int svdq_rms_norm_modulate_mx(const void* x, int64_t ldx, const void* w, const void* shift, int T, int H, float eps,
+                              int fmt, void* codes, void* scales, hipStream_t stream);
+int svdq_residual_rms_norm_modulate_mx(const void* x, int64_t ldx, const void* v, int64_t ldv, const void* g,
+                                       const void* w, const void* shift, int T, int H, float eps, int fmt, void* xo,
+                                       int64_t ldxo, void* codes, void* scales, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

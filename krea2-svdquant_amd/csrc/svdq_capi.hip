@@ -717,3 +717,133 @@ int svdq_w4a16_gemm_siblings(const svdq_w4a16_sibling* layers, int count, int M,
 }
 
 }  // extern "C"
+
+namespace {
+
+int mx_checks(const char* fn, int M, int K, int fmt, const void* codes, const void* scales) {
+  if (fmt != SVDQ_MX_E2M1 && fmt != SVDQ_MX_E4M3) return fail(SVDQ_ERR_ARG, "%s: element format %d", fn, fmt);
+  if (M < 0 || K <= 0 || K > 1 << 30) return fail(SVDQ_ERR_SHAPE, "%s: M=%d, K=%d (0 < K <= 2^30)", fn, M, K);
+  if (M && (!codes || !scales)) return fail(SVDQ_ERR_ARG, "%s: null pointer", fn);
+  if (!aligned16(codes) || !aligned16(scales))
+    return fail(SVDQ_ERR_ALIGN, "%s: codes and scales must be 16-byte aligned", fn);
+  return SVDQ_OK;
+}
+
+bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
+
+// one thread per 8 columns, 256 to a workgroup
+bool mx_too_many(int64_t M, int64_t K) { return M * ((K + 511) / 512 * 64) / 256 >= INT32_MAX; }
+
+}  // namespace
+
+extern "C" {
+
+int svdq_mx_quantize(const void* x, int64_t ldx, int M, int K, int fmt, void* codes, void* scales, hipStream_t stream) {
+  if (int e = mx_checks("mx_quantize", M, K, fmt, codes, scales)) return e;
+  if (M == 0) return ok();
+  if (!x) return fail(SVDQ_ERR_ARG, "mx_quantize: null pointer");
+  if (ldx < K || mx_too_many(M, K)) return fail(SVDQ_ERR_SHAPE, "mx_quantize: M=%d, K=%d, ldx=%lld", M, K, (long long)ldx);
+  if (!aligned2(x)) return fail(SVDQ_ERR_ALIGN, "mx_quantize: x must be 2-byte aligned");
+  return launched(svdq::launch_mx_quantize(static_cast<const uint16_t*>(x), ldx, M, K, fmt, static_cast<uint8_t*>(codes),
+                                           static_cast<uint8_t*>(scales), stream),
+                  "mx_quantize");
+}
+
+int svdq_mx_dequantize(const void* codes, const void* scales, int M, int K, int fmt, void* y, hipStream_t stream) {
+  if (int e = mx_checks("mx_dequantize", M, K, fmt, codes, scales)) return e;
+  if (M == 0) return ok();
+  if (!y) return fail(SVDQ_ERR_ARG, "mx_dequantize: null pointer");
+  if (mx_too_many(M, K)) return fail(SVDQ_ERR_SHAPE, "mx_dequantize: M=%d, K=%d", M, K);
+  if (!aligned2(y)) return fail(SVDQ_ERR_ALIGN, "mx_dequantize: y must be 2-byte aligned");
+  return launched(svdq::launch_mx_dequantize(static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), M,
+                                             K, fmt, static_cast<uint16_t*>(y), stream),
+                  "mx_dequantize");
+}
+
+int svdq_mx_gemm(const void* a, const void* a_scales, int fmt, const void* w, const void* w_scales, const void* bias,
+                 int M, int N, int K, void* y, int64_t ldy, int out_f32, hipStream_t stream) {
+  if (int e = mx_checks("mx_gemm", M, K, fmt, a, a_scales)) return e;
+  if (N <= 0 || ldy < N) return fail(SVDQ_ERR_SHAPE, "mx_gemm: N=%d, ldy=%lld", N, (long long)ldy);
+  if (out_f32 != 0 && out_f32 != 1) return fail(SVDQ_ERR_ARG, "mx_gemm: out_f32=%d", out_f32);
+  if (M == 0) return ok();
+  if (!w || !w_scales || !y) return fail(SVDQ_ERR_ARG, "mx_gemm: null pointer");
+  if (!aligned16(w) || !aligned16(w_scales))
+    return fail(SVDQ_ERR_ALIGN, "mx_gemm: codes and scales must be 16-byte aligned");
+  if (!aligned2(bias) || reinterpret_cast<uintptr_t>(y) % (out_f32 ? 4 : 2))
+    return fail(SVDQ_ERR_ALIGN, "mx_gemm: bias and y must be aligned to their elements");
+  svdq::MxGemmParams p{};
+  p.a = static_cast<const uint8_t*>(a);
+  p.as = static_cast<const uint8_t*>(a_scales);
+  p.w = static_cast<const uint8_t*>(w);
+  p.ws = static_cast<const uint8_t*>(w_scales);
+  p.bias = static_cast<const uint16_t*>(bias);
+  p.y = y;
+  p.ldy = ldy;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  return launched(svdq::launch_mx_gemm(p, fmt, out_f32 == 1, stream), "mx_gemm");
+}
+
+int svdq_silu_mul_mx(const void* g, int64_t ldg, const void* u, int64_t ldu, int M, int K, int fmt, void* codes,
+                     void* scales, hipStream_t stream) {
+  if (int e = mx_checks("silu_mul_mx", M, K, fmt, codes, scales)) return e;
+  if (M == 0) return ok();
+  if (!g || !u) return fail(SVDQ_ERR_ARG, "silu_mul_mx: null pointer");
+  if (ldg < K || ldu < K || mx_too_many(M, K))
+    return fail(SVDQ_ERR_SHAPE, "silu_mul_mx: M=%d, K=%d, ldg=%lld, ldu=%lld", M, K, (long long)ldg, (long long)ldu);
+  if (!aligned2(g) || !aligned2(u)) return fail(SVDQ_ERR_ALIGN, "silu_mul_mx: inputs must be 2-byte aligned");
+  return launched(svdq::launch_silu_mul_mx(static_cast<const uint16_t*>(g), ldg, static_cast<const uint16_t*>(u), ldu, M,
+                                           K, fmt, static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), stream),
+                  "silu_mul_mx");
+}
+
+}  // extern "C"
+
+namespace {
+
+int norm_mx_checks(const char* fn, const void* x, int64_t ldx, const void* w, const void* shift, int T, int H,
+                   float eps, int fmt, const void* codes, const void* scales) {
+  if (int e = mx_checks(fn, T, H, fmt, codes, scales)) return e;
+  if (H % 8) return fail(SVDQ_ERR_SHAPE, "%s: H=%d (H %% 8 == 0)", fn, H);
+  if (!(eps >= 0.0f)) return fail(SVDQ_ERR_ARG, "%s: eps must be >= 0", fn);
+  if (T && (!x || !w || !shift)) return fail(SVDQ_ERR_ARG, "%s: null pointer", fn);
+  if (ldx < H || ldx % 8 || !aligned16(x) || !aligned16(w) || !aligned16(shift))
+    return fail(SVDQ_ERR_ALIGN, "%s: 16-byte aligned pointers, row strides >= H and multiples of 8", fn);
+  return SVDQ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int svdq_rms_norm_modulate_mx(const void* x, int64_t ldx, const void* w, const void* shift, int T, int H, float eps,
+                              int fmt, void* codes, void* scales, hipStream_t stream) {
+  const char* fn = "rms_norm_modulate_mx";
+  if (int e = norm_mx_checks(fn, x, ldx, w, shift, T, H, eps, fmt, codes, scales)) return e;
+  if (T == 0) return ok();
+  return launched(svdq::launch_rms_norm_mx(static_cast<const uint16_t*>(x), ldx, nullptr, 0, nullptr,
+                                           static_cast<const uint16_t*>(w), static_cast<const uint16_t*>(shift), T, H,
+                                           eps, fmt, nullptr, 0, static_cast<uint8_t*>(codes),
+                                           static_cast<uint8_t*>(scales), stream),
+                  fn);
+}
+
+int svdq_residual_rms_norm_modulate_mx(const void* x, int64_t ldx, const void* v, int64_t ldv, const void* g,
+                                       const void* w, const void* shift, int T, int H, float eps, int fmt, void* xo,
+                                       int64_t ldxo, void* codes, void* scales, hipStream_t stream) {
+  const char* fn = "residual_rms_norm_modulate_mx";
+  if (int e = norm_mx_checks(fn, x, ldx, w, shift, T, H, eps, fmt, codes, scales)) return e;
+  if (T && (!v || !g || !xo)) return fail(SVDQ_ERR_ARG, "%s: null pointer", fn);
+  if (ldv < H || ldxo < H || ldv % 8 || ldxo % 8 || !aligned16(v) || !aligned16(g) || !aligned16(xo))
+    return fail(SVDQ_ERR_ALIGN, "%s: 16-byte aligned pointers, row strides >= H and multiples of 8", fn);
+  if (T == 0) return ok();
+  return launched(svdq::launch_rms_norm_mx(static_cast<const uint16_t*>(x), ldx, static_cast<const uint16_t*>(v), ldv,
+                                           static_cast<const uint16_t*>(g), static_cast<const uint16_t*>(w),
+                                           static_cast<const uint16_t*>(shift), T, H, eps, fmt,
+                                           static_cast<uint16_t*>(xo), ldxo, static_cast<uint8_t*>(codes),
+                                           static_cast<uint8_t*>(scales), stream),
+                  fn);
+}
+
+}  // extern "C"

@@ -172,4 +172,29 @@ hipError_t launch_attention_fwd(const uint16_t* q, const uint16_t* k, const uint
                                 float qeps = 0.0f);
 long attention_workspace_bytes(int T, int H);
 
+// Microscaled blocks (svdq_mx.hip, svdq_mx_gemm.hip); fmt 0 = E2M1, 1 = E4M3, storage as in svdq_mx.h.
+// Strides in elements; inputs of any alignment and width but the norm's (16-byte rows, H % 8 == 0).
+hipError_t launch_mx_quantize(const uint16_t* x, long ldx, long M, int K, int fmt, uint8_t* codes, uint8_t* scales,
+                              hipStream_t st);
+hipError_t launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, long M, int K, int fmt, uint16_t* y,
+                                hipStream_t st);
+// silu(g) * u into MX blocks
+hipError_t launch_silu_mul_mx(const uint16_t* g, long ldg, const uint16_t* u, long ldu, long M, int K, int fmt,
+                              uint8_t* codes, uint8_t* scales, hipStream_t st);
+// the adaptive RMS norm of x, or (v not null) of xo = bf16(x + g v), into MX blocks
+hipError_t launch_rms_norm_mx(const uint16_t* x, long ldx, const uint16_t* v, long ldv, const uint16_t* g,
+                              const uint16_t* w, const uint16_t* shift, int T, int H, float eps, int fmt, uint16_t* xo,
+                              long ldxo, uint8_t* codes, uint8_t* scales, hipStream_t st);
+struct MxGemmParams {
+  const uint8_t* a;         // [M] rows of E2M1 or E4M3 codes
+  const uint8_t* as;        // their scales
+  const uint8_t* w;         // [N] rows of E2M1 codes
+  const uint8_t* ws;
+  const uint16_t* bias;     // [N] bf16 or null
+  void* y;                  // [M, ldy] bf16 or f32
+  long ldy;
+  int M, N, K;
+};
+hipError_t launch_mx_gemm(const MxGemmParams& p, int fmt, bool out_f32, hipStream_t st);
+
 }  // namespace svdq

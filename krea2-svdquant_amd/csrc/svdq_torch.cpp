@@ -265,6 +265,197 @@ std::vector<Tensor> linear_siblings(const Tensor& x, const std::vector<Tensor>& 
   return ys;
 }
 
+// ---- Microscaled blocks --------------------------------------------------------------------------
+// Codes are uint8 [..., kp / 2] (E2M1) or float8_e4m3fn [..., kp] (E4M3), scales float8_e8m0fnu [..., sp], with
+// kp and sp as in svdq_gfx950.h.  Native operators like the linears: a prompt-sized call is shorter on the
+// GPU than a Python operator's checks and allocations.
+
+int64_t mx_kp(int64_t k) { return (k + 127) / 128 * 128; }
+int64_t mx_sp(int64_t k) { return (k + 511) / 512 * 16; }
+int64_t mx_row_bytes(int64_t k, int64_t fmt) { return fmt == SVDQ_MX_E4M3 ? mx_kp(k) : mx_kp(k) / 2; }
+
+void check_fmt(int64_t fmt) {
+  TORCH_CHECK_VALUE(fmt == SVDQ_MX_E2M1 || fmt == SVDQ_MX_E4M3, "fmt=", fmt);
+}
+
+// [..., K] as rows: the last dimension dense, the leading ones flattened (a copy where they have no common stride)
+struct Rows {
+  Tensor t;
+  int64_t m, k, ld;
+  std::vector<int64_t> lead;
+
+  // aligned: 16-byte rows, copied where they are not
+  Rows(const char* name, const Tensor& x, bool aligned = false) {
+    TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16, name, " must be bfloat16, got ", x.scalar_type());
+    TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, name, " must be [..., K] with K > 0, got ", x.sizes());
+    lead = x.sizes().vec();
+    k = lead.back();
+    lead.pop_back();
+    m = 1;
+    for (int64_t d : lead) m *= d;
+    TORCH_CHECK_VALUE(m <= INT32_MAX && k <= 1 << 30, name, ": ", m, " rows of ", k, " columns are too many");
+    t = x.reshape({m, k});
+    if (t.stride(1) != 1 && k > 1) t = t.contiguous();
+    ld = m > 1 ? t.stride(0) : k;
+    if (ld < k || (aligned && (ld % 8 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16))) {
+      t = at::empty({m, k}, t.options()).copy_(t);
+      ld = k;
+    }
+  }
+};
+
+// new codes and scales of the rows of x
+std::tuple<Tensor, Tensor> mx_empty(const Rows& r, int64_t fmt) {
+  std::vector<int64_t> cs = r.lead, ss = r.lead;
+  cs.push_back(mx_row_bytes(r.k, fmt));
+  ss.push_back(mx_sp(r.k));
+  return {at::empty(cs, r.t.options().dtype(fmt == SVDQ_MX_E4M3 ? at::kFloat8_e4m3fn : at::kByte)),
+          at::empty(ss, r.t.options().dtype(at::kFloat8_e8m0fnu))};
+}
+
+// codes and their scales, checked: format, rows and padded columns
+struct Mx {
+  int64_t fmt, m, kp;
+  std::vector<int64_t> lead;
+
+  Mx(const char* name, const Tensor& codes, const Tensor& scales, c10::Device dev) {
+    const auto dt = codes.scalar_type();
+    TORCH_CHECK_TYPE(dt == at::kByte || dt == at::kFloat8_e4m3fn, name, " must be uint8 (E2M1) or float8_e4m3fn codes, got ", dt);
+    check_tensor(name, codes, dev, dt);
+    check_tensor("their scales", scales, dev, at::kFloat8_e8m0fnu);
+    fmt = dt == at::kByte ? SVDQ_MX_E2M1 : SVDQ_MX_E4M3;
+    TORCH_CHECK_VALUE(codes.dim() >= 1, name, " must be [..., K], got ", codes.sizes());
+    lead = codes.sizes().vec();
+    kp = lead.back() * (fmt == SVDQ_MX_E2M1 ? 2 : 1);
+    lead.pop_back();
+    m = 1;
+    for (int64_t d : lead) m *= d;
+    TORCH_CHECK_VALUE(kp > 0 && kp % 128 == 0 && kp <= 1 << 30 && m <= INT32_MAX, name,
+                      " must hold rows of a multiple of 128 values, got ", codes.sizes());
+    std::vector<int64_t> want = lead;
+    want.push_back(mx_sp(kp));
+    TORCH_CHECK_VALUE(scales.sizes() == at::IntArrayRef(want), name, "' scales must be ", at::IntArrayRef(want), ", got ",
+                      scales.sizes());
+  }
+};
+
+hipStream_t stream_of(c10::Device dev) { return c10::hip::getCurrentHIPStream(dev.index()); }
+
+std::tuple<Tensor, Tensor> mx_quantize(const Tensor& x, int64_t fmt) {
+  check_fmt(fmt);
+  const c10::DeviceGuard guard(x.device());
+  const Rows r("x", x);
+  auto [codes, scales] = mx_empty(r, fmt);
+  check_status("svdq_mx_quantize", svdq_mx_quantize(ptr(r.t), r.ld, (int)r.m, (int)r.k, (int)fmt, ptr(codes), ptr(scales),
+                                                    stream_of(x.device())));
+  return {codes, scales};
+}
+
+Tensor mx_dequantize(const Tensor& codes, const Tensor& scales, int64_t k) {
+  const c10::DeviceGuard guard(codes.device());
+  const Mx a("codes", codes, scales, codes.device());
+  TORCH_CHECK_VALUE(k > 0 && mx_kp(k) == a.kp, "k=", k, " does not pad to the codes' ", a.kp, " columns");
+  std::vector<int64_t> shape = a.lead;
+  shape.push_back(k);
+  Tensor y = at::empty(shape, codes.options().dtype(at::kBFloat16));
+  check_status("svdq_mx_dequantize", svdq_mx_dequantize(ptr(codes), ptr(scales), (int)a.m, (int)k, (int)a.fmt, ptr(y),
+                                                        stream_of(codes.device())));
+  return y;
+}
+
+// y [lead..., N] = a w^T + bias of checked activation blocks (codes at a, scales at as)
+Tensor mx_product(const void* a, const void* as, int64_t fmt, int64_t m, int64_t kp, std::vector<int64_t> lead,
+                  const Tensor& w, const Tensor& w_scales, const OptTensor& bias, bool out_f32) {
+  const c10::Device dev = w.device();
+  const Mx b("w", w, w_scales, dev);
+  TORCH_CHECK_TYPE(b.fmt == SVDQ_MX_E2M1, "w must be uint8 (E2M1) codes");
+  TORCH_CHECK_VALUE(w.dim() == 2 && b.m > 0, "w must be [N, K / 2] codes, got ", w.sizes());
+  TORCH_CHECK_VALUE(b.kp == kp, "rows of ", kp, " values (padded) against a weight of ", b.kp);
+  if (bias.has_value()) {
+    check_tensor("bias", *bias, dev, at::kBFloat16);
+    TORCH_CHECK_VALUE(bias->numel() == b.m, "bias must have ", b.m, " entries, got ", bias->numel());
+  }
+  lead.push_back(b.m);
+  Tensor y = at::empty(lead, w.options().dtype(out_f32 ? at::kFloat : at::kBFloat16));
+  check_status("svdq_mx_gemm", svdq_mx_gemm(a, as, (int)fmt, ptr(w), ptr(w_scales), ptr(bias), (int)m, (int)b.m, (int)kp,
+                                            ptr(y), b.m, out_f32, stream_of(dev)));
+  return y;
+}
+
+Tensor mx_gemm(const Tensor& a, const Tensor& a_scales, const Tensor& w, const Tensor& w_scales, const OptTensor& bias,
+               bool out_f32) {
+  const c10::DeviceGuard guard(w.device());
+  const Mx r("a", a, a_scales, w.device());
+  return mx_product(ptr(a), ptr(a_scales), r.fmt, r.m, r.kp, r.lead, w, w_scales, bias, out_f32);
+}
+
+Tensor mx_linear(const Tensor& x, const Tensor& w, const Tensor& w_scales, const OptTensor& bias, int64_t fmt,
+                 bool out_f32) {
+  check_fmt(fmt);
+  const c10::DeviceGuard guard(w.device());
+  TORCH_CHECK_VALUE(x.device() == w.device(), "x is on ", x.device(), ", expected ", w.device());
+  const Rows r("x", x);
+  const int64_t codes = r.m * mx_row_bytes(r.k, fmt);   // rows of 64 bytes and more: 16-byte aligned scales behind
+  const Tensor work = at::empty({codes + r.m * mx_sp(r.k)}, r.t.options().dtype(at::kByte));
+  uint8_t* base = ptr<uint8_t>(work);
+  check_status("svdq_mx_quantize", svdq_mx_quantize(ptr(r.t), r.ld, (int)r.m, (int)r.k, (int)fmt, base, base + codes,
+                                                    stream_of(w.device())));
+  return mx_product(base, base + codes, fmt, r.m, mx_kp(r.k), r.lead, w, w_scales, bias, out_f32);
+}
+
+std::tuple<Tensor, Tensor> silu_mul_mx(const Tensor& gate, const Tensor& up, int64_t fmt) {
+  check_fmt(fmt);
+  const c10::DeviceGuard guard(gate.device());
+  TORCH_CHECK_VALUE(up.device() == gate.device(), "up is on ", up.device(), ", expected ", gate.device());
+  TORCH_CHECK_VALUE(up.sizes() == gate.sizes(), "gate ", gate.sizes(), " and up ", up.sizes(), " differ");
+  const Rows g("gate", gate), u("up", up);
+  auto [codes, scales] = mx_empty(g, fmt);
+  check_status("svdq_silu_mul_mx", svdq_silu_mul_mx(ptr(g.t), g.ld, ptr(u.t), u.ld, (int)g.m, (int)g.k, (int)fmt,
+                                                    ptr(codes), ptr(scales), stream_of(gate.device())));
+  return {codes, scales};
+}
+
+// a vector [H] of the norms, 16-byte aligned
+Tensor norm_vector(const char* name, const Tensor& t, int64_t h, c10::Device dev) {
+  check_tensor(name, t, dev, at::kBFloat16);
+  TORCH_CHECK_VALUE(t.numel() == h, name, " must have ", h, " elements, got ", t.numel());
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 ? t.clone() : t;
+}
+
+std::tuple<Tensor, Tensor> rms_norm_modulate_mx(const Tensor& x, const Tensor& weight, const Tensor& shift, double eps,
+                                                int64_t fmt) {
+  check_fmt(fmt);
+  const c10::DeviceGuard guard(x.device());
+  const Rows r("x", x, true);
+  TORCH_CHECK_VALUE(r.k % 8 == 0, "rows must be multiples of 8 values, got ", r.k);
+  const Tensor w = norm_vector("weight", weight, r.k, x.device()), s = norm_vector("shift", shift, r.k, x.device());
+  auto [codes, scales] = mx_empty(r, fmt);
+  check_status("svdq_rms_norm_modulate_mx",
+               svdq_rms_norm_modulate_mx(ptr(r.t), r.ld, ptr(w), ptr(s), (int)r.m, (int)r.k, (float)eps, (int)fmt,
+                                         ptr(codes), ptr(scales), stream_of(x.device())));
+  return {codes, scales};
+}
+
+std::tuple<Tensor, Tensor, Tensor> residual_rms_norm_modulate_mx(const Tensor& x, const Tensor& v, const Tensor& gate,
+                                                                 const Tensor& weight, const Tensor& shift, double eps,
+                                                                 int64_t fmt) {
+  check_fmt(fmt);
+  const c10::DeviceGuard guard(x.device());
+  TORCH_CHECK_VALUE(v.device() == x.device(), "v is on ", v.device(), ", expected ", x.device());
+  TORCH_CHECK_VALUE(v.sizes() == x.sizes(), "v ", v.sizes(), " must match x ", x.sizes());
+  const Rows r("x", x, true), rv("v", v, true);
+  TORCH_CHECK_VALUE(r.k % 8 == 0, "rows must be multiples of 8 values, got ", r.k);
+  const Tensor g = norm_vector("gate", gate, r.k, x.device()), w = norm_vector("weight", weight, r.k, x.device()),
+               s = norm_vector("shift", shift, r.k, x.device());
+  Tensor xo = at::empty(x.sizes(), r.t.options());
+  auto [codes, scales] = mx_empty(r, fmt);
+  check_status("svdq_residual_rms_norm_modulate_mx",
+               svdq_residual_rms_norm_modulate_mx(ptr(r.t), r.ld, ptr(rv.t), rv.ld, ptr(g), ptr(w), ptr(s), (int)r.m,
+                                                  (int)r.k, (float)eps, (int)fmt, ptr(xo), r.k, ptr(codes), ptr(scales),
+                                                  stream_of(x.device())));
+  return {xo, codes, scales};
+}
+
 }  // namespace
 
 // The torch that this file was compiled against, found in the file by kernels/hip/lib.py ahead of
@@ -280,12 +471,35 @@ TORCH_LIBRARY_FRAGMENT(svdq, m) {
       "linear_siblings(Tensor x, Tensor[] srs, Tensor[] l2, Tensor?[] lora_down, Tensor?[] lora_mult, "
       "int group_size, int[] rtp, Tensor[] weight, Tensor[] weight_scales, Tensor[] l1cat, Tensor?[] bias, "
       "int operand, bool out_f32, bool exact) -> Tensor[]");
+  m.def("mx_quantize(Tensor x, int fmt) -> (Tensor, Tensor)");
+  m.def("mx_dequantize(Tensor codes, Tensor scales, int k) -> Tensor");
+  m.def("mx_gemm(Tensor a, Tensor a_scales, Tensor w, Tensor w_scales, Tensor? bias, bool out_f32) -> Tensor");
+  m.def("mx_linear(Tensor x, Tensor w, Tensor w_scales, Tensor? bias, int fmt, bool out_f32) -> Tensor");
+  m.def("silu_mul_mx(Tensor gate, Tensor up, int fmt) -> (Tensor, Tensor)");
+  m.def("rms_norm_modulate_mx(Tensor x, Tensor weight, Tensor shift, float eps, int fmt) -> (Tensor, Tensor)");
+  m.def(
+      "residual_rms_norm_modulate_mx(Tensor x, Tensor v, Tensor gate, Tensor weight, Tensor shift, float eps, int fmt) "
+      "-> (Tensor, Tensor, Tensor)");
 }
 TORCH_LIBRARY_IMPL(svdq, CUDA, m) {
   m.impl("linear", TORCH_FN(linear));
   m.impl("linear_siblings", TORCH_FN(linear_siblings));
+  m.impl("mx_quantize", TORCH_FN(mx_quantize));
+  m.impl("mx_dequantize", TORCH_FN(mx_dequantize));
+  m.impl("mx_gemm", TORCH_FN(mx_gemm));
+  m.impl("mx_linear", TORCH_FN(mx_linear));
+  m.impl("silu_mul_mx", TORCH_FN(silu_mul_mx));
+  m.impl("rms_norm_modulate_mx", TORCH_FN(rms_norm_modulate_mx));
+  m.impl("residual_rms_norm_modulate_mx", TORCH_FN(residual_rms_norm_modulate_mx));
 }
 TORCH_LIBRARY_IMPL(svdq, Autograd, m) {
   m.impl("linear", torch::autograd::autogradNotImplementedFallback());
   m.impl("linear_siblings", torch::autograd::autogradNotImplementedFallback());
+  m.impl("mx_quantize", torch::autograd::autogradNotImplementedFallback());
+  m.impl("mx_dequantize", torch::autograd::autogradNotImplementedFallback());
+  m.impl("mx_gemm", torch::autograd::autogradNotImplementedFallback());
+  m.impl("mx_linear", torch::autograd::autogradNotImplementedFallback());
+  m.impl("silu_mul_mx", torch::autograd::autogradNotImplementedFallback());
+  m.impl("rms_norm_modulate_mx", torch::autograd::autogradNotImplementedFallback());
+  m.impl("residual_rms_norm_modulate_mx", torch::autograd::autogradNotImplementedFallback());
 }

@@ -36,6 +36,10 @@ SVDQ_EPI_MUL_SIGMOID = 1
 SVDQ_EPI_SILU_MUL = 2
 SVDQ_EPI_RESIDUAL_GATE = 3
 
+# element formats of microscaled blocks
+SVDQ_MX_E2M1 = 0
+SVDQ_MX_E4M3 = 1
+
 # sibling layers of one svdq_w4a4_gemm_siblings / svdq_w4a16_gemm_siblings call (SVDQ_MAX_SIBLINGS)
 SVDQ_MAX_SIBLINGS = 4
 
@@ -100,6 +104,13 @@ SIGNATURES = {
     "svdq_attention_fwd": (_I, [_P, _L, _P, _P, _L, _I, _I, _I, ctypes.c_float, _P, _L, _P, _P]),
     "svdq_attention_fwd_qnorm": (_I, [_P, _L, _P, _P, _L, _I, _I, _I, ctypes.c_float, _P, _P, _L, ctypes.c_float,
                                       _P, _L, _P, _P]),
+    "svdq_mx_quantize": (_I, [_P, _L, _I, _I, _I, _P, _P, _P]),
+    "svdq_mx_dequantize": (_I, [_P, _P, _I, _I, _I, _P, _P]),
+    "svdq_mx_gemm": (_I, [_P, _P, _I, _P, _P, _P, _I, _I, _I, _P, _L, _I, _P]),
+    "svdq_silu_mul_mx": (_I, [_P, _L, _P, _L, _I, _I, _I, _P, _P, _P]),
+    "svdq_rms_norm_modulate_mx": (_I, [_P, _L, _P, _P, _I, _I, ctypes.c_float, _I, _P, _P, _P]),
+    "svdq_residual_rms_norm_modulate_mx": (_I, [_P, _L, _P, _L, _P, _P, _P, _I, _I, ctypes.c_float, _I, _P, _L, _P,
+                                                _P, _P]),
 }
 
 lock = threading.RLock()

@@ -480,8 +480,10 @@ def load_native() -> dict:
             lib.load_torch_ops()
             torch.library.register_fake("svdq::linear", _linear_fake)
             torch.library.register_fake("svdq::linear_siblings", _linear_siblings_fake)
-            _native_ops.update(linear=torch.ops.svdq.linear.default,
-                               linear_siblings=torch.ops.svdq.linear_siblings.default)
+            for name, fake in _MX_FAKES.items():
+                torch.library.register_fake(f"svdq::{name}", fake)
+            _native_ops.update({name: getattr(torch.ops.svdq, name).default
+                                for name in ("linear", "linear_siblings", *_MX_FAKES)})
     return _native_ops
 
 
@@ -510,6 +512,104 @@ def linear_siblings(*args) -> list[Tensor]:
     """``svdq::linear_siblings``: ``linear`` of sibling layers over one x, their activation passes and
     GEMMs grouped as by ``act_quant_siblings``, ``w4a4_gemm_siblings`` and ``w4a16_gemm_siblings``."""
     return _native("linear_siblings", *args)
+
+
+# ---- microscaled (MX) blocks -------------------------------------------------------------------
+# Blocks of 32 consecutive values of a row share an E8M0 scale; elements are E2M1 or E4M3.  Codes are
+# uint8 [..., kp / 2] (E2M1: two per byte, the even column in the low half) or float8_e4m3fn [..., kp], scales
+# float8_e8m0fnu [..., sp]; kp = K rounded up to 128 (zero codes), sp = 16 * ceil(K / 512).
+MX_FORMATS = {"e2m1": lib.SVDQ_MX_E2M1, "fp4": lib.SVDQ_MX_E2M1, "e4m3": lib.SVDQ_MX_E4M3, "fp8": lib.SVDQ_MX_E4M3}
+
+
+def mx_shapes(k: int, fmt: str) -> tuple[int, int]:
+    """Columns of the codes and of the scales of rows of ``k`` values."""
+    _need(fmt in MX_FORMATS, ValueError, f"fmt must be one of {sorted(MX_FORMATS)}, got {fmt!r}")
+    kp = (k + 127) // 128 * 128
+    return (kp if MX_FORMATS[fmt] == lib.SVDQ_MX_E4M3 else kp // 2), (k + 511) // 512 * 16
+
+
+def _mx_quantize_fake(x, fmt):
+    cols, sp = mx_shapes(x.shape[-1], "e4m3" if fmt == lib.SVDQ_MX_E4M3 else "e2m1")
+    return (x.new_empty((*x.shape[:-1], cols), dtype=torch.float8_e4m3fn if fmt == lib.SVDQ_MX_E4M3 else torch.uint8),
+            x.new_empty((*x.shape[:-1], sp), dtype=torch.float8_e8m0fnu))
+
+
+def _mx_out_fake(x, w, out_f32):
+    return x.new_empty((*x.shape[:-1], w.shape[0]), dtype=torch.float32 if out_f32 else torch.bfloat16)
+
+
+_MX_FAKES = {
+    "mx_quantize": _mx_quantize_fake,
+    "mx_dequantize": lambda codes, scales, k: codes.new_empty((*codes.shape[:-1], k), dtype=torch.bfloat16),
+    "mx_gemm": lambda a, a_scales, w, w_scales, bias, out_f32: _mx_out_fake(a, w, out_f32),
+    "mx_linear": lambda x, w, w_scales, bias, fmt, out_f32: _mx_out_fake(x, w, out_f32),
+    "silu_mul_mx": lambda gate, up, fmt: _mx_quantize_fake(gate, fmt),
+    "rms_norm_modulate_mx": lambda x, weight, shift, eps, fmt: _mx_quantize_fake(x, fmt),
+    "residual_rms_norm_modulate_mx": lambda x, v, gate, weight, shift, eps, fmt: (
+        x.new_empty(x.shape), *_mx_quantize_fake(x, fmt)),
+}
+
+
+def _mx(op: str, t: Tensor, *args):
+    if not t.is_cuda:
+        raise RuntimeError(f"svdq::{op} needs GPU tensors")
+    return _native(op, *args)
+
+
+def _mx_fmt(fmt: str) -> int:
+    code = MX_FORMATS.get(fmt)
+    if code is None:
+        raise ValueError(f"fmt must be one of {sorted(MX_FORMATS)}, got {fmt!r}")
+    return code
+
+
+def mx_quantize(x: Tensor, fmt: str = "e2m1") -> tuple[Tensor, Tensor]:
+    """``svdq::mx_quantize``: bf16 ``x`` [..., K] into MX blocks, ``(codes, scales)``.
+
+    A block's scale is ``2^max(floor(log2(amax)) - E, -127)`` (E = 2 for ``"e2m1"``, 8 for ``"e4m3"``), its codes
+    the nearest values to ``x / scale``, ties to even, beyond the largest value (6, 448) to that.  A block with an
+    infinity or a NaN reads back as NaN."""
+    return _mx("mx_quantize", x, x, _mx_fmt(fmt))
+
+
+def mx_dequantize(codes: Tensor, scales: Tensor, k: int) -> Tensor:
+    """``svdq::mx_dequantize``: the bf16 values [..., k] that MX blocks hold (exact but below bf16's range)."""
+    return _mx("mx_dequantize", codes, codes, scales, k)
+
+
+def mx_gemm(a: Tensor, a_scales: Tensor, w: Tensor, w_scales: Tensor, bias: Optional[Tensor] = None,
+            out_f32: bool = False) -> Tensor:
+    """``svdq::mx_gemm``: ``a w^T + bias`` of MX activations ``a`` [..., K] (either format) and an E2M1 weight ``w``
+    [N, K], both as ``mx_quantize`` gives them; bf16 (or float32) [..., N], sums in float32.  With E4M3
+    activations and bf16 output the matrix instruction drops, within 8 consecutive k, what lies below 2^-13 of the
+    largest product (about 1e-5 of a result); otherwise every product counts in full."""
+    return _mx("mx_gemm", a, a, a_scales, w, w_scales, bias, out_f32)
+
+
+def mx_linear(x: Tensor, w: Tensor, w_scales: Tensor, bias: Optional[Tensor] = None, fmt: str = "e2m1",
+              out_f32: bool = False) -> Tensor:
+    """``svdq::mx_linear``: ``mx_gemm(*mx_quantize(x, fmt), w, w_scales, bias, out_f32)`` in one call."""
+    return _mx("mx_linear", x, x, w, w_scales, bias, _mx_fmt(fmt), out_f32)
+
+
+def silu_mul_mx(gate: Tensor, up: Tensor, fmt: str = "e4m3") -> tuple[Tensor, Tensor]:
+    """``svdq::silu_mul_mx``: the SwiGLU product ``silu(gate) * up`` of bf16 tensors of one shape, in float32, into
+    MX blocks ``(codes, scales)``."""
+    return _mx("silu_mul_mx", gate, gate, up, _mx_fmt(fmt))
+
+
+def rms_norm_modulate_mx(x: Tensor, weight: Tensor, shift: Tensor, eps: float,
+                         fmt: str = "e4m3") -> tuple[Tensor, Tensor]:
+    """``svdq::rms_norm_modulate_mx``: ``x * rsqrt(mean(x^2) + eps) * weight + shift`` over the last dimension of a
+    bf16 ``x`` [..., H] (H % 8 == 0), in float32, into MX blocks ``(codes, scales)``."""
+    return _mx("rms_norm_modulate_mx", x, x, weight, shift, eps, _mx_fmt(fmt))
+
+
+def residual_rms_norm_modulate_mx(x: Tensor, v: Tensor, gate: Tensor, weight: Tensor, shift: Tensor, eps: float,
+                                  fmt: str = "e4m3") -> tuple[Tensor, Tensor, Tensor]:
+    """``svdq::residual_rms_norm_modulate_mx``: ``xo = torch.addcmul(x, gate, v)`` (bf16, one rounding) and
+    ``rms_norm_modulate_mx(xo, weight, shift, eps, fmt)`` in one pass; ``(xo, codes, scales)``."""
+    return _mx("residual_rms_norm_modulate_mx", x, x, v, gate, weight, shift, eps, _mx_fmt(fmt))
 
 
 # ---- stand-in block normalizations -------------------------------------------------------------

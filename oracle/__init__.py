@@ -19,6 +19,8 @@ Modules
               (``src/krea2_svdquant/quant/svd.py:119-163``) in CPU torch bf16,
               and float64 evaluators of the W4A4 / W4A16 quantized math,
               including the LoRA side branch (``runtime/linear.py:11-45``).
+``mx``        microscaled blocks (quantise, encode, decode) in 64 bits from the
+              format definitions; the reference has none.
 ``synth``     seeded synthetic layer states following
               ``quant/svd.py:26-116`` and ``scripts/convert_simulated.py:184-208``.
 
