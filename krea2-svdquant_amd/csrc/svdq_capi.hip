@@ -764,6 +764,7 @@ int svdq_mx_gemm(const void* a, const void* a_scales, int fmt, const void* w, co
                  int M, int N, int K, void* y, int64_t ldy, int out_f32, hipStream_t stream) {
   if (int e = mx_checks("mx_gemm", M, K, fmt, a, a_scales)) return e;
   if (N <= 0 || ldy < N) return fail(SVDQ_ERR_SHAPE, "mx_gemm: N=%d, ldy=%lld", N, (long long)ldy);
+  if (K > 1 << 22) return fail(SVDQ_ERR_SHAPE, "mx_gemm: K=%d exceeds 2^22 (a tile's offsets are 32 bits)", K);
   if (out_f32 != 0 && out_f32 != 1) return fail(SVDQ_ERR_ARG, "mx_gemm: out_f32=%d", out_f32);
   if (M == 0) return ok();
   if (!w || !w_scales || !y) return fail(SVDQ_ERR_ARG, "mx_gemm: null pointer");
