@@ -400,9 +400,13 @@ int svdq_mx_dequantize(const void* codes, const void* scales, int M, int K, int 
  * their scales, w [N, K] E2M1 codes with theirs, bias [N] bf16 or null.  Sums in float32, one rounding at
  * the store.  E4M3 with bf16 output: within 8 consecutive k the matrix instruction drops what lies below
  * 2^-13 of the largest product (about 1e-5 of a result); with float32 output, and E2M1, nothing is
- * dropped.  M = 0 does nothing. */
+ * dropped.  K at most 2^22.  M = 0 does nothing. */
 int svdq_mx_gemm(const void* a, const void* a_scales, int fmt, const void* w, const void* w_scales, const void* bias,
                  int M, int N, int K, void* y, int64_t ldy, int out_f32, hipStream_t stream);
+
+/* Block tile (*rows of a by *cols of w; either may be null) of the kernel that svdq_mx_gemm runs for these sizes;
+ * returns 1, 2 for the kernel for few rows, 0 for other arguments.  For callers that report which kernel ran (tests). */
+int svdq_mx_gemm_tile(int M, int N, int K, int fmt, int* rows, int* cols);
 
 /* The SwiGLU product silu(g) * u of bf16 g, u [M, K] (row strides ldg, ldu) in float32, into MX blocks
  * (not rounded to bf16 first). */

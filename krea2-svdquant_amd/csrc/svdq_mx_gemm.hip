@@ -23,8 +23,6 @@
 
 namespace svdq {
 
-int mx_gemm_tile_choice(int M, int N, int K, int fmt);
-
 namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -41,22 +39,27 @@ __device__ __forceinline__ i32x8 operand(const MxFrag<MX_E4M3>& f) {
   return __builtin_bit_cast(i32x8, __builtin_shufflevector(f.q[0], f.q[1], 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// a = hi + lo by the top bit of the E4M3 exponents
+__device__ __forceinline__ void split(const MxFrag<MX_E4M3>& a, MxFrag<MX_E4M3>& hi, MxFrag<MX_E4M3>& lo) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      // 0xFF where the exponent is 8 or more: v_perm's selectors 8 and 9 (10 and 11) repeat the top bits of bytes 1 and 3
+      // of its second (first) operand
+      const uint32_t x = a.q[i][d], mask = __builtin_amdgcn_perm(x << 9, x << 1, 0x090B080Au);
+      hi.q[i][d] = x & mask;
+      lo.q[i][d] = x & ~mask;
+    }
+}
+
 // acc += w a on one step of 64: scale byte SEL of ws and of as.  EXACT: in two halves by the E4M3 exponent.
 template <int AF, bool EXACT, int SEL>
 __device__ __forceinline__ f32x16 mx_mfma(const MxFrag<MX_E2M1>& w, const MxFrag<AF>& a, f32x16 acc, uint32_t ws,
                                           uint32_t as) {
   if constexpr (EXACT && AF == MX_E4M3) {
     MxFrag<AF> hi, lo;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        // 0xFF where the exponent is 8 or more: v_perm's selectors 8 and 9 (10 and 11) repeat the top bits of bytes 1 and 3 of
-        // its second (first) operand
-        const uint32_t x = a.q[i][d], mask = __builtin_amdgcn_perm(x << 9, x << 1, 0x090B080Au);
-        hi.q[i][d] = x & mask;
-        lo.q[i][d] = x & ~mask;
-      }
+    split(a, hi, lo);
     acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(w), operand(lo), acc, 4, 0, SEL, (int)ws, SEL, (int)as);
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(w), operand(hi), acc, 4, 0, SEL, (int)ws, SEL, (int)as);
   } else {
@@ -72,30 +75,43 @@ __device__ __forceinline__ void for_each_index(F&& f, std::integer_sequence<int,
 
 // Block tile BM x BN (BM = 32 TM WM rows of a, BN = 32 TN WN rows of w), WM x WN waves of TM x TN accumulators.
 //
-// A stage is 128 columns of K in a ring of NBUF LDS buffers filled by DMA: rows of a (64 bytes E2M1, 128 bytes
-// E4M3) and of w (64 bytes) in chunks of 16 bytes, a row's chunk c at slot c ^ f(row), which spreads sixteen
-// consecutive rows' chunk over the 64 banks (f = row / 4 mod 4 in rows of 64 bytes, row / 2 mod 8 in rows of 128) while
-// the DMA's lanes still read whole rows.  Scales come four stages at a time, 16 bytes a row, and are taken into
-// registers at once, so they need no second buffer.
+// A stage is SPS matrix steps of 64 columns of K, 2 or 4, in a ring of NB LDS buffers filled by DMA.  Rows lie in chunks
+// of 16 bytes, chunk c at slot c ^ f(row), which spreads sixteen consecutive rows' chunk over the 64 banks (rows of 64
+// bytes: f = row / 4 mod 4, of 128: row / 2 mod 8, of 256: row mod 16) while the DMA's lanes still read whole rows.
+// Scales come CH 16-byte groups a row at a time (a group: 512 columns), and are taken into registers a group at a time,
+// so they need no second buffer.
 //
-// A stage is two matrix steps of 64.  Its first step's operands are read during the stage before, its second's
-// during its first step's products; between the two ("mid-stage") the wave waits for the next stage's bytes and for
-// the other waves, after which everything of this stage has been read: its buffer takes stage s + NBUF.  So the one
-// barrier per stage has matrix instructions queued on both sides.
-template <int AF, bool F32, int TM, int TN, int WM, int WN, int NB>
+// A load fills a cache line of 128 bytes.  Two steps of E2M1 codes are half a line, so stages of two steps read every
+// line twice, and what bounds the large tiles is what the L2 delivers (M = 4352, N = 16384, K = 6144, 256 x 256: 248 us,
+// on lines read once 224).  Stages of four steps read whole lines; the 256 x 256 tiles, whose LDS holds only two of
+// those, take four of two steps and fetch the rows of every second stage in reverse order, so that its first half finds
+// the lines of the stage before in the 32 KB of L1: 236 us.  For the same reason scales come in CH = 2 groups (one
+// group at a time, a line of 128 bytes for 16: 248, none at all 232).
+//
+// A step's operands are read during the step before it.  Ahead of a stage's last step the wave waits for the next
+// stage's bytes and for the other waves: by then everything of this stage has been read, its buffer takes stage s + NB,
+// and the last step reads the next stage's first operands.  So the one barrier per stage has matrix instructions
+// queued on both sides.
+template <int AF, bool F32, int TM, int TN, int WM, int WN, int SPS, int NB>
 struct MxTile {
-  static constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, NBUF = NB;
-  static constexpr int RA = AF == MX_E4M3 ? 128 : 64;                       // bytes of a row of a per stage
-  static constexpr int TA = BM * RA / 1024, TB = BN * 64 / 1024;            // DMA instructions of 1024 bytes
+  static constexpr int NW = WM * WN, BM = 32 * TM * WM, BN = 32 * TN * WN, CH = 2;
+  static constexpr int RW = 32 * SPS, RA = AF == MX_E4M3 ? 2 * RW : RW;     // bytes of a row of w and of a per stage
+  static constexpr int TA = BM * RA / 1024, TB = BN * RW / 1024;            // DMA instructions of 1024 bytes
   static constexpr int DA = TA / NW, D = DA + TB / NW;                      // per wave and stage
-  static constexpr int TS = (BM + BN + 63) / 64, E = (TS + NW - 1) / NW;    // of scales, per four stages
-  static constexpr int OB = TA * 1024, BUF = (TA + TB) * 1024, OS = NBUF * BUF;
-  static constexpr int LDS = OS + TS * 1024;
+  static constexpr int TS = (BM + BN) * CH / 64, E = (TS + NW - 1) / NW;    // of scales, per CH groups
+  static constexpr int OB = TA * 1024, BUF = (TA + TB) * 1024, OS = NB * BUF, LDS = OS + TS * 1024;
   static constexpr int GROUPS = 160 * 1024 / LDS;                           // workgroups that a CU's LDS holds
+  static constexpr bool TURN = RW < 128;                                    // every second stage in reverse order
   static_assert(LDS <= 160 * 1024, "LDS");
-  static_assert(NBUF >= 3 && TA % NW == 0 && TB % NW == 0, "whole instructions per wave");
-  static_assert(NBUF * D + E <= 63, "vmcnt counts to 63");
+  static_assert(NB >= 2 && TA % NW == 0 && TB % NW == 0 && (BM + BN) * CH % 64 == 0 && NW % 4 == 0, "whole instructions");
+  static_assert(NB * D + E <= 63, "vmcnt counts to 63");
 };
+
+// f(row) of rows of `bytes`
+template <int BYTES>
+__device__ __forceinline__ int mx_turn(int row) {
+  return BYTES == 64 ? row >> 2 & 3 : BYTES == 128 ? row >> 1 & 7 : row & 15;
+}
 
 template <int N>
 __device__ __forceinline__ void landed_and_met() {
@@ -107,57 +123,63 @@ __device__ __forceinline__ void dma16_at(const void* at, uint32_t lds) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(at), "{m0}"(lds) : "memory");
 }
 
-template <int AF, bool F32, int TM, int TN, int WM, int WN, int NB>
-__global__ void __launch_bounds__(64 * WM * WN, (MxTile<AF, F32, TM, TN, WM, WN, NB>::GROUPS > 1 ? 2 : 1))
+template <int AF, bool F32, int TM, int TN, int WM, int WN, int SPS, int NB>
+__global__ void __launch_bounds__(64 * WM * WN, (MxTile<AF, F32, TM, TN, WM, WN, SPS, NB>::GROUPS > 1 ? 2 : 1))
     mx_gemm_tile_kernel(MxGemmParams p, int nbm, int nbn, int group_m) {
-  using T = MxTile<AF, F32, TM, TN, WM, WN, NB>;
+  using T = MxTile<AF, F32, TM, TN, WM, WN, SPS, NB>;
   __shared__ __attribute__((aligned(1024))) uint8_t sm[T::LDS];
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
   int bm, bn;
   tile_coords(blockIdx.x, nbm, nbn, group_m, bm, bn);
   const int m0 = bm * T::BM, n0 = bn * T::BN;
-  const int nst = (int)(mx_kp(p.K) / 128), sp = (int)mx_sp(p.K);
+  const int steps = (int)(mx_kp(p.K) / 64), nst = (steps + SPS - 1) / SPS, sp = (int)mx_sp(p.K);   // steps is even
   const long pa = mx_row_bytes(p.K, AF), pw = mx_kp(p.K) / 2;
   const uint32_t lds0 = lds_offset(sm);
 
-  // Instruction i of a stage moves 1024 bytes: 16 (8) rows of 4 (8) chunks, a's rows first.  A wave's d-th is
-  // wave + NW d: DA of a's, then w's.
+  // Instruction i of a stage moves 1024 bytes, 1024 / RA rows of a or 1024 / RW of w, a's first.  A wave's d-th is
+  // wave + NW d: DA of a's, then w's.  The chunk of a lane is the same in all of a's, and in all of w's.
+  constexpr int CA = T::RA / 16, CW = T::RW / 16;
   const uint8_t *src_a = p.a + (long)m0 * pa, *src_w = p.w + (long)n0 * pw;
   const uint32_t ldsw = lds0 + 1024 * wave;
+  const int chunk_a = lane % CA ^ mx_turn<T::RA>(64 / CA * wave + lane / CA);
+  const int chunk_w = lane % CW ^ mx_turn<T::RW>(64 / CW * wave + lane / CW);
   uint32_t off[T::D];
 #pragma unroll
   for (int d = 0; d < T::D; ++d) {
     const bool a = d < T::DA;
-    const int rows = a ? 1024 / T::RA : 16, cpr = a ? T::RA / 16 : 4;
-    const int row = (wave + T::NW * (a ? d : d - T::DA)) * rows + lane / cpr, slot = lane % cpr;
-    const int chunk = slot ^ (cpr == 8 ? row >> 1 & 7 : row >> 2 & 3);
-    off[d] = (uint32_t)(min(row, (a ? p.M - m0 : p.N - n0) - 1) * (a ? pa : pw) + 16 * chunk);
+    const int cpr = a ? CA : CW, row = (wave + T::NW * (a ? d : d - T::DA)) * (64 / cpr) + lane / cpr;
+    off[d] = (uint32_t)(min(row, (a ? p.M - m0 : p.N - n0) - 1) * (a ? pa : pw) + 16 * (a ? chunk_a : chunk_w));
   }
+  // a last stage of two steps out of four has no second half to read: its first half again
+  const uint32_t back_a = chunk_a >= CA / 2 ? T::RA / 2 : 0, back_w = chunk_w >= CW / 2 ? T::RW / 2 : 0;
   const uint8_t* ssrc[T::E];
+  int spart = lane % T::CH;   // this lane's 16 bytes of a row's 16 CH
 #pragma unroll
   for (int e = 0; e < T::E; ++e) {
-    const int r = 64 * min(wave + T::NW * e, T::TS - 1) + lane;
+    const int r = (64 * min(wave + T::NW * e, T::TS - 1) + lane) / T::CH;
     ssrc[e] = r < T::BM ? p.as + (long)min(m0 + r, p.M - 1) * sp : p.ws + (long)min(n0 + r - T::BM, p.N - 1) * sp;
   }
-  // Every stage fetches the one NBUF further on; past the last stage the last one again, into a buffer that nothing
+  // Every stage fetches the one NB further on; past the last stage the last one again, into a buffer that nothing
   // reads any more, so that the number of loads under way, which the waits count, is the same throughout.
-  int ahead = 1;
-  auto fetch = [&](uint32_t buf, int d) {   // this wave's instruction d, into the buffer at byte buf
-    dma16(d < T::DA ? src_a : src_w, off[d], ldsw + 1024 * T::NW * d + buf);
-    if (d == T::D - 1) {
-      src_a += ahead < nst ? T::RA : 0;
-      src_w += ahead < nst ? 64 : 0;
+  int ahead = 0;
+  const bool odd = SPS == 4 && steps % 4;
+  uint32_t half = odd && nst == 1 ? ~0u : 0u;
+  auto fetch = [&](uint32_t buf, int i, bool turned) {   // this wave's i-th instruction, into the buffer at byte buf
+    const int d = T::TURN && turned ? T::D - 1 - i : i;
+    const uint32_t o = SPS == 4 ? off[d] - (half & (d < T::DA ? back_a : back_w)) : off[d];
+    dma16(d < T::DA ? src_a : src_w, o, ldsw + 1024 * T::NW * d + buf);
+    if (i == T::D - 1) {
       ++ahead;
+      src_a += ahead < nst ? T::RA : 0;
+      src_w += ahead < nst ? T::RW : 0;
+      if (SPS == 4) half = odd && ahead >= nst - 1 ? ~0u : 0u;
     }
   };
-  auto fetch_scales = [&](int super) {
-    const int more = 4 * (super + 1) < nst ? 16 : 0;
+  auto fetch_scales = [&](int chunk) {   // the chunk-th CH groups; beyond a row's scales its last again
+    const int at = 16 * min(T::CH * chunk + spart, sp / 16 - 1);
 #pragma unroll
-    for (int e = 0; e < T::E; ++e) {
-      dma16_at(ssrc[e], lds0 + T::OS + 1024 * min(wave + T::NW * e, T::TS - 1));
-      ssrc[e] += more;
-    }
+    for (int e = 0; e < T::E; ++e) dma16_at(ssrc[e] + at, lds0 + T::OS + 1024 * min(wave + T::NW * e, T::TS - 1));
   };
 
   const int ra = 32 * TM * wm + lr, rw = 32 * TN * wn + lr;   // this lane's row of its first tiles
@@ -169,103 +191,124 @@ __global__ void __launch_bounds__(64 * WM * WN, (MxTile<AF, F32, TM, TN, WM, WN,
   auto read = [&](uint32_t buf, int j, int r) {
     const uint8_t* b = sm + buf;
     if (r < TN) {
-      fw[j][r].q[0] = *reinterpret_cast<const u32x4*>(b + T::OB + (rw + 32 * r) * 64 + 16 * ((2 * j + h) ^ (lr >> 2 & 3)));
+      fw[j & 1][r].q[0] = *reinterpret_cast<const u32x4*>(b + T::OB + (rw + 32 * r) * T::RW + 16 * ((2 * j + h) ^ mx_turn<T::RW>(lr)));
     } else {
       const int t = (r - TN) / AR, u = (r - TN) % AR;
       const uint8_t* row = b + (ra + 32 * t) * T::RA;
-      if (AF == MX_E4M3) fa[j][t].q[u] = *reinterpret_cast<const u32x4*>(row + 16 * ((4 * j + 2 * u + h) ^ (lr >> 1 & 7)));
-      else fa[j][t].q[0] = *reinterpret_cast<const u32x4*>(row + 16 * ((2 * j + h) ^ (lr >> 2 & 3)));
+      if (AF == MX_E4M3) fa[j & 1][t].q[u] = *reinterpret_cast<const u32x4*>(row + 16 * ((4 * j + 2 * u + h) ^ mx_turn<T::RA>(lr)));
+      else fa[j & 1][t].q[0] = *reinterpret_cast<const u32x4*>(row + 16 * ((2 * j + h) ^ mx_turn<T::RA>(lr)));
     }
   };
-  auto read_scales = [&] {   // of the next four stages
-    const uint8_t* b = sm + T::OS;
+  auto read_scales = [&](int part) {   // the part-th group of the chunk
+    const uint8_t* b = sm + T::OS + 16 * part;
 #pragma unroll
-    for (int t = 0; t < TM; ++t) sa[t] = *reinterpret_cast<const u32x4*>(b + (ra + 32 * t) * 16);
+    for (int t = 0; t < TM; ++t) sa[t] = *reinterpret_cast<const u32x4*>(b + (ra + 32 * t) * 16 * T::CH);
 #pragma unroll
-    for (int t = 0; t < TN; ++t) sw[t] = *reinterpret_cast<const u32x4*>(b + (T::BM + rw + 32 * t) * 16);
+    for (int t = 0; t < TN; ++t) sw[t] = *reinterpret_cast<const u32x4*>(b + (T::BM + rw + 32 * t) * 16 * T::CH);
   };
 
   f32x16 acc[TN][TM] = {};
+  constexpr int D1 = (T::D + 1) / 2, D0 = T::D - D1;   // issued in a last step, in the first that follows
   fetch_scales(0);
 #pragma unroll
-  for (int s = 0; s < T::NBUF - 1; ++s)
+  for (int s = 0; s < NB; ++s)
 #pragma unroll
-    for (int d = 0; d < T::D; ++d) fetch(s * T::BUF, d);
-#pragma unroll
-  for (int d = 0; d < (T::D + 1) / 2; ++d) fetch((T::NBUF - 1) * T::BUF, d);
-  landed_and_met<(T::NBUF - 2) * T::D + (T::D + 1) / 2>();
-  read_scales();
+    for (int d = 0; d < (s == NB - 1 ? D1 : T::D); ++d) fetch(s * T::BUF, d, s & 1);
+  landed_and_met<(NB - 2) * T::D + D1>();
+  read_scales(0);
 #pragma unroll
   for (int r = 0; r < READS; ++r) read(0, 0, r);
 
-  // One stage, from the buffer at cur, with the scales in element S of sa and sw.  Memory instructions are spread over
-  // the products: a wave issues in order, and a block of them ahead of the products leaves the matrix unit idle while
-  // their queues drain.  The LDS reads go first, one behind each product, so that they are over when they are needed;
-  // the DMA instructions of stage s + NBUF - 1 are issued half in the second step of stage s - 1, after its mid-stage
-  // freed their buffer, half in the first step of stage s.  No branch in between: the compiler would move the first
-  // step's products below it, past the barrier.
-  constexpr int D1 = (T::D + 1) / 2, D0 = T::D - D1;   // in a second step, in the first step that follows
-  uint32_t cur = 0, nxt = T::BUF, free_ = (T::NBUF - 1) * T::BUF;
-  auto stage = [&](auto sub, auto wait, auto next_scales) {
-    constexpr int S = decltype(sub)::value;
-    // this lane's blocks are h and 2 + h of the stage's four: bytes 0 and 2 after the shift
-    uint32_t ca[TM], cw[TN];
+  // Step J: its products, with a memory instruction or more behind each: a wave issues in order, and a block of them
+  // ahead of the products leaves the matrix unit idle while their queues drain.  The READS reads of the next step go
+  // first, so that they are over when they are needed, then ND DMA instructions.  The scales are in dword Q of sa and sw.
+  uint32_t cur = 0, nxt = NB == 1 ? 0 : T::BUF, free_ = (NB - 1) * T::BUF;
+  uint32_t ca[TM], cw[TN];
+  auto pick = [&](int q) {   // this lane's blocks of a pair of steps are h and 2 + h of dword q: bytes 0 and 2 after the shift
 #pragma unroll
-    for (int t = 0; t < TM; ++t) ca[t] = sa[t][S] >> (8 * h);
+    for (int t = 0; t < TM; ++t) ca[t] = sa[t][q] >> (8 * h);
 #pragma unroll
-    for (int t = 0; t < TN; ++t) cw[t] = sw[t][S] >> (8 * h);
-    auto products = [&](auto step, auto nd, auto&& rd, auto&& dma) {
-      constexpr int J = decltype(step)::value, ND = decltype(nd)::value, OPS = READS + ND;
-      constexpr int PER = (OPS + PRODUCTS - 1) / PRODUCTS;   // behind each product
-      // DMA instructions as far apart as the products behind the reads allow
-      constexpr int LEFT = PRODUCTS - (READS + PER - 1) / PER, GAP = PER == 1 && ND && LEFT / ND > 1 ? LEFT / ND : 1;
+    for (int t = 0; t < TN; ++t) cw[t] = sw[t][q] >> (8 * h);
+  };
+  auto step = [&](auto jj, auto nd, auto&& rd, auto&& dma) {
+    constexpr int J = decltype(jj)::value, ND = decltype(nd)::value, OPS = READS + ND;
+    constexpr int PER = (OPS + PRODUCTS - 1) / PRODUCTS;   // behind each product
+    // DMA instructions as far apart as the products behind the reads allow
+    constexpr int LEFT = PRODUCTS - READS, GAP = PER == 1 && ND && LEFT / (ND ? ND : 1) > 1 ? LEFT / (ND ? ND : 1) : 1;
 #pragma unroll
-      for (int i = 0; i < PRODUCTS; ++i) {
-        const int x = i / TM, t = i % TM;
-        acc[x][t] = mx_mfma<AF, F32, 2 * J>(fw[J][x], fa[J][t], acc[x][t], cw[x], ca[t]);
-        if (GAP > 1) {
-          if (i < READS) rd(i);
-          else if ((i - READS) % GAP == 0 && (i - READS) / GAP < ND) dma((i - READS) / GAP);
-        } else {
+    for (int i = 0; i < PRODUCTS; ++i) {
+      const int x = i / TM, t = i % TM;
+      acc[x][t] = mx_mfma<AF, F32, 2 * (J & 1)>(fw[J & 1][x], fa[J & 1][t], acc[x][t], cw[x], ca[t]);
+      if (GAP > 1) {
+        if (i < READS) rd(i);
+        else if ((i - READS) % GAP == 0 && (i - READS) / GAP < ND) dma((i - READS) / GAP);
+      } else {
 #pragma unroll
-          for (int o = i * PER; o < (i + 1) * PER && o < OPS; ++o) {
-            if (o < READS) rd(o);
-            else dma(o - READS);
-          }
+        for (int o = i * PER; o < (i + 1) * PER && o < OPS; ++o) {
+          if (o < READS) rd(o);
+          else dma(o - READS);
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  using None = std::integral_constant<int, 0>;
+  // One stage of parity PAR, its scales in dwords q .. of sa and sw.  No branch in it: the compiler would move products
+  // below it, past the barrier.  At the barrier everything up to stage s + NB - 1 has been issued, and scales ahead of
+  // the last of it, so stage s + 1 has landed when at most the stages after that are under way.
+  auto stage = [&](auto par, int q, auto&& scales) {
+    constexpr int PAR = decltype(par)::value;
+    auto late = [&](int d) { fetch(free_, D1 + d, (PAR + NB - 1) & 1); };   // what the step before left of its stage
+    auto inner = [&](auto jj) {
+      constexpr int J = decltype(jj)::value;
+      if (J % 2 == 0) pick(q + J / 2);
+      step(jj, std::integral_constant<int, J == 0 ? D0 : 0>{}, [&](int r) { read(cur, J + 1, r); }, late);
     };
-    products(std::integral_constant<int, 0>{}, std::integral_constant<int, D0>{}, [&](int r) { read(cur, 1, r); },
-             [&](int d) { fetch(free_, D1 + d); });
-    landed_and_met<decltype(wait)::value>();
-    next_scales();
-    products(std::integral_constant<int, 1>{}, std::integral_constant<int, D1>{}, [&](int r) { read(nxt, 0, r); },
-             [&](int d) { fetch(cur, d); });
+    for_each_index(inner, std::make_integer_sequence<int, SPS - 1>{});
+    landed_and_met<(NB - 2) * T::D>();
+    scales();   // the last step's are picked
+    step(std::integral_constant<int, SPS - 1>{}, std::integral_constant<int, D1>{}, [&](int r) { read(nxt, 0, r); },
+         [&](int d) { fetch(cur, d, (PAR + NB) & 1); });
     free_ = cur;
     cur = nxt;
     nxt = nxt + T::BUF == T::OS ? 0 : nxt + T::BUF;
   };
-  // Mid-stage of s, everything up to stage s + NBUF - 1 has been issued, and stage s + 1 has landed when only what was
-  // issued after it is under way: NBUF - 2 stages, and the scales, which are issued at the mid-stage of S = 0.
-  constexpr int WAIT = (T::NBUF - 2) * T::D;
-  int s0 = 0;
-  for (; s0 + 4 <= nst; s0 += 4)
-    for_each_index([&](auto sub) {
-      constexpr int S = decltype(sub)::value;
-      stage(sub, std::integral_constant<int, WAIT + (S >= 1 && S <= T::NBUF - 2 ? T::E : 0)>{}, [&] {
-        if (S == 0) fetch_scales(s0 / 4 + 1);
-        if (S == 3) read_scales();
+  // A group of scales lasts PG stages.  A chunk's last group is read at the end of the group before; a stage later
+  // (every wave has read it) the next chunk is fetched, and lands by the end of the chunk.
+  constexpr int PG = 8 / SPS, PC = T::CH * PG, QS = SPS / 2;   // stages per group and per chunk, dwords per stage
+  const int full = steps / SPS;
+  int s = 0;
+  for (; s + PC <= full; s += PC)
+    for_each_index([&](auto ii) {
+      constexpr int I = decltype(ii)::value;
+      stage(std::integral_constant<int, I % 2>{}, I % PG * QS, [&] {
+        if (I % PG == PG - 1) read_scales((I / PG + 1) % T::CH);
+        if (I == PC - PG) fetch_scales(s / PC + 1);
       });
-    }, std::make_integer_sequence<int, 4>{});
-  // up to three more; no further scales to fetch
+    }, std::make_integer_sequence<int, PC>{});
+  // what is left of the last chunk, a stage's scales at a time from LDS
+  int left = 1;
+  auto next_scales = [&] {
+    const uint8_t* b = sm + T::OS + 4 * QS * left++;
+#pragma unroll
+    for (int t = 0; t < TM; ++t)
+#pragma unroll
+      for (int k = 0; k < QS; ++k) sa[t][k] = *reinterpret_cast<const uint32_t*>(b + (ra + 32 * t) * 16 * T::CH + 4 * k);
+#pragma unroll
+    for (int t = 0; t < TN; ++t)
+#pragma unroll
+      for (int k = 0; k < QS; ++k) sw[t][k] = *reinterpret_cast<const uint32_t*>(b + (T::BM + rw + 32 * t) * 16 * T::CH + 4 * k);
+  };
 #pragma unroll 1
-  for (int s = s0; s < nst; ++s) {
-    stage(std::integral_constant<int, 0>{}, std::integral_constant<int, WAIT>{}, [] {});
-#pragma unroll
-    for (int t = 0; t < TM; ++t) sa[t] = __builtin_shufflevector(sa[t], sa[t], 1, 2, 3, 0);
-#pragma unroll
-    for (int t = 0; t < TN; ++t) sw[t] = __builtin_shufflevector(sw[t], sw[t], 1, 2, 3, 0);
+  for (; s + 2 <= full; s += 2) {
+    stage(std::integral_constant<int, 0>{}, 0, next_scales);
+    stage(std::integral_constant<int, 1>{}, 0, next_scales);
+  }
+  if (s < full) stage(std::integral_constant<int, 0>{}, 0, next_scales);
+  if (odd) {
+    pick(0);
+    step(std::integral_constant<int, 0>{}, None{}, [&](int r) { read(cur, 1, r); }, [](int) {});
+    step(std::integral_constant<int, 1>{}, None{}, [](int) {}, [](int) {});
   }
   // nothing of the DMA may be under way when the next workgroup takes this one's LDS
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -326,33 +369,206 @@ __global__ void __launch_bounds__(64 * WM * WN, (MxTile<AF, F32, TM, TN, WM, WN,
   }
 }
 
-template <int AF, bool F32, int TM, int TN, int WM, int WN, int NB>
+// acc += w a of 16 x 16 on a step of 128: lane l supplies row l % 16 of each, E2M1 the 32 codes k = 32 (l / 16) ..,
+// E4M3 k = 16 (l / 16) .. + 15 and 64 + 16 (l / 16) .. + 15; the scale (byte 0) of its row's block l / 16.
+template <int AF, bool EXACT>
+__device__ __forceinline__ f32x4 mx_mfma16(const MxFrag<MX_E2M1>& w, const MxFrag<AF>& a, f32x4 acc, uint32_t ws,
+                                           uint32_t as) {
+  if constexpr (EXACT && AF == MX_E4M3) {
+    MxFrag<AF> hi, lo;
+    split(a, hi, lo);
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w), operand(lo), acc, 4, 0, 0, (int)ws, 0, (int)as);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w), operand(hi), acc, 4, 0, 0, (int)ws, 0, (int)as);
+  } else {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w), operand(a), acc, 4, AF == MX_E4M3 ? 0 : 4, 0,
+                                                            (int)ws, 0, (int)as);
+  }
+}
+
+// Few rows of a (16 at most): what counts is reading w once, from as many places at once as possible.  A workgroup of
+// 8 waves takes 16 columns of the output and all of K; the waves take units of 256 columns of K in turn (whole cache
+// lines of w) and add their sums through LDS in wave order.  Each wave has a ring of U units in LDS to itself, filled
+// by DMA whose lanes read whole lines (operands loaded straight to registers, 16 bytes from each of 64 lines an
+// instruction, took twice as long), so the waves need no barrier before the sums.  MR = 8 or 16 rows of a are held;
+// rows beyond M repeat the last.
+template <int AF, int MR, int U>
+struct MxRows {
+  static constexpr int NW = 8;
+  static constexpr int RA = AF == MX_E4M3 ? 256 : 128, OA = 2048, OSC = OA + MR * RA, UNIT = OSC + 256;
+  static constexpr int DA = MR * RA / 1024, D = 2 + DA + 1;   // DMA instructions of a unit: w, a, scales
+  static constexpr int LDS = NW * U * UNIT;
+  static_assert(LDS <= 160 * 1024 && NW * 1024 <= LDS, "LDS");
+};
+
+template <int AF, bool F32, int MR, int U>
+__global__ void __launch_bounds__(512) mx_gemm_rows_kernel(MxGemmParams p) {
+  using T = MxRows<AF, MR, U>;
+  __shared__ __attribute__((aligned(1024))) uint8_t sm[T::LDS];
+  const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, b = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = blockIdx.x * 16;
+  const int kp = (int)mx_kp(p.K), sp = (int)mx_sp(p.K), nst = kp / 128, units = (nst + 1) / 2;
+  const long pa = mx_row_bytes(p.K, AF), pw = kp / 2;
+  const uint32_t lds0 = lds_offset(sm) + wave * U * T::UNIT;
+  const uint8_t* mine = sm + wave * U * T::UNIT;
+
+  // A DMA lane's row and chunk of 16 bytes; chunk c of a row lies at slot c ^ f(row), f = row / 2 mod 8 (rows of 128
+  // bytes) or row (rows of 256): sixteen rows' chunk over all banks.
+  constexpr int CA = T::RA / 16;
+  uint32_t off_w[2], off_a[T::DA];
+  int chunk_w[2], chunk_a[T::DA];
+#pragma unroll
+  for (int d = 0; d < 2; ++d) {
+    const int row = 8 * d + lane / 8;
+    chunk_w[d] = lane % 8 ^ (row >> 1 & 7);
+    off_w[d] = (uint32_t)(min(row, p.N - n0 - 1) * pw);
+  }
+#pragma unroll
+  for (int d = 0; d < T::DA; ++d) {
+    const int row = (64 / CA) * d + lane / CA;
+    chunk_a[d] = lane % CA ^ (AF == MX_E4M3 ? row & 15 : row >> 1 & 7);
+    off_a[d] = (uint32_t)(min(row, p.M - 1) * pa);
+  }
+  const uint8_t* src_w = p.w + (long)n0 * pw;
+  // scale dwords of a unit: lanes 0..31 w's rows, then a's, each row's first step and then its second
+  const uint8_t* ssrc = (lane < 32 ? p.ws + (long)min(n0 + lr, p.N - 1) * sp : p.as + (long)min(lr, p.M - 1) * sp) +
+                        4 * (lane >> 4 & 1);
+  auto fetch = [&](int unit, int buf) {
+    const uint32_t to = lds0 + buf * T::UNIT;
+    const bool half = 2 * unit + 1 >= nst;   // an odd last step: the unit's second half is its first again
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+      dma16(src_w, off_w[d] + 128 * unit + 16 * (half ? chunk_w[d] & 3 : chunk_w[d]), to + 1024 * d);
+#pragma unroll
+    for (int d = 0; d < T::DA; ++d)
+      dma16(p.a, off_a[d] + T::RA * unit + 16 * (half ? chunk_a[d] & (CA / 2 - 1) : chunk_a[d]), to + T::OA + 1024 * d);
+    const uint8_t* at = ssrc + 8 * unit;
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(at), "{m0}"(to + T::OSC) : "memory");
+  };
+
+  const int mine_units = wave < units ? (units - wave + T::NW - 1) / T::NW : 0;
+  f32x4 acc = {};
+  const int ma = min(lr, MR - 1);
+  if (mine_units) {
+    // units past the last are the last again, into a buffer that is not read: the waits count the same loads throughout
+    auto unit_of = [&](int i) { return wave + T::NW * min(i, mine_units - 1); };
+#pragma unroll
+    for (int i = 0; i < U; ++i) fetch(unit_of(i), i);
+    int buf = 0;
+#pragma unroll 1
+    for (int i = 0; i < mine_units; ++i) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((U - 1) * T::D) : "memory");
+      const uint8_t* u = mine + buf * T::UNIT;
+      MxFrag<MX_E2M1> fw[2];
+      MxFrag<AF> fa[2];
+      uint32_t sw[2], sa[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        fw[j].q[0] = *reinterpret_cast<const u32x4*>(u + 128 * lr + 16 * ((4 * j + b) ^ (lr >> 1 & 7)));
+        const uint8_t* row = u + T::OA + T::RA * ma;
+        if (AF == MX_E4M3) {
+          fa[j].q[0] = *reinterpret_cast<const u32x4*>(row + 16 * ((8 * j + b) ^ ma));
+          fa[j].q[AF == MX_E4M3] = *reinterpret_cast<const u32x4*>(row + 16 * ((8 * j + 4 + b) ^ ma));
+        } else {
+          fa[j].q[0] = *reinterpret_cast<const u32x4*>(row + 16 * ((4 * j + b) ^ (ma >> 1 & 7)));
+        }
+        sw[j] = *reinterpret_cast<const uint32_t*>(u + T::OSC + 4 * (16 * j + lr)) >> (8 * b);
+        sa[j] = *reinterpret_cast<const uint32_t*>(u + T::OSC + 128 + 4 * (16 * j + lr)) >> (8 * b);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // all of the unit is in registers
+      fetch(unit_of(i + U), buf);
+      buf = buf + 1 == U ? 0 : buf + 1;
+      acc = mx_mfma16<AF, F32>(fw[0], fa[0], acc, sw[0], sa[0]);
+      if (2 * unit_of(i) + 1 < nst) acc = mx_mfma16<AF, F32>(fw[1], fa[1], acc, sw[1], sa[1]);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+  __syncthreads();   // every ring is done with; their memory takes the sums
+  f32x4* red = reinterpret_cast<f32x4*>(sm);
+  red[64 * wave + lane] = acc;
+  __syncthreads();
+  // register r of lane (lr, b): row lr of a, column 4 b + r of w
+  const int m = tid >> 4, n = tid & 15;
+  if (m >= p.M || m >= 16 || n0 + n >= p.N) return;
+  float v = 0.0f;
+#pragma unroll
+  for (int k = 0; k < T::NW; ++k) v += reinterpret_cast<const float*>(sm)[4 * (64 * k + 16 * (n / 4) + m) + n % 4];
+  if (p.bias) v += bf16f(p.bias[n0 + n]);
+  const long at = (long)m * p.ldy + n0 + n;
+  if (F32) static_cast<float*>(p.y)[at] = v;
+  else static_cast<uint16_t*>(p.y)[at] = (uint16_t)pack_bf16x2(v, 0.0f);
+}
+
+template <int AF, bool F32, int TM, int TN, int WM, int WN, int SPS, int NB>
 hipError_t launch_tile(const MxGemmParams& p, hipStream_t st) {
-  using T = MxTile<AF, F32, TM, TN, WM, WN, NB>;
+  using T = MxTile<AF, F32, TM, TN, WM, WN, SPS, NB>;
   const long nbm = (p.M + T::BM - 1) / T::BM, nbn = (p.N + T::BN - 1) / T::BN;
   if (nbm * nbn > INT32_MAX) return hipErrorInvalidValue;
-  mx_gemm_tile_kernel<AF, F32, TM, TN, WM, WN, NB>
+  mx_gemm_tile_kernel<AF, F32, TM, TN, WM, WN, SPS, NB>
       <<<(unsigned)(nbm * nbn), 64 * WM * WN, 0, st>>>(p, (int)nbm, (int)nbn, 4);
   return hipGetLastError();
 }
 
-// Block tiles: 64 x 64, 128 x 128, 256 x 256 rows of a by rows of w.
+template <int AF, bool F32, int MR, int U>
+hipError_t launch_rows(const MxGemmParams& p, hipStream_t st) {
+  mx_gemm_rows_kernel<AF, F32, MR, U><<<(unsigned)((p.N + 15) / 16), 512, 0, st>>>(p);
+  return hipGetLastError();
+}
+
 template <int AF, bool F32>
 hipError_t launch_any(const MxGemmParams& p, hipStream_t st) {
   constexpr bool E8 = AF == MX_E4M3;
-  switch (mx_gemm_tile_choice(p.M, p.N, p.K, AF)) {
-    case 0: return launch_tile<AF, F32, 1, 1, 2, 2, 4>(p, st);
-    case 1: return launch_tile<AF, F32, 2, 2, 2, 2, E8 ? 3 : 4>(p, st);
+  int rows, cols;
+  switch (mx_gemm_tile(p.M, p.N, p.K, AF, rows, cols)) {
+    case MX_ROWS:
+      if constexpr (!E8)
+        if (p.M > 8) return launch_rows<AF, F32, 16, 2>(p, st);
+      return launch_rows<AF, F32, 8, E8 ? 2 : 3>(p, st);
+    case 0: return launch_tile<AF, F32, 1, 1, 2, 2, E8 ? 2 : 4, E8 ? 4 : 3>(p, st);
+    case 1: return launch_tile<AF, F32, E8 ? 1 : 2, E8 ? 2 : 1, 2, 2, E8 ? 2 : 4, E8 ? 4 : 3>(p, st);
+    case 2: return launch_tile<AF, F32, 2, 2, 2, 2, E8 ? 2 : 4, 3>(p, st);
     // E4M3 with float32 output needs registers for the halves of its operands
-    default: return launch_tile<AF, F32, E8 && F32 ? 2 : 4, 4, 2, 2, E8 && !F32 ? 3 : 4>(p, st);
+    default: return launch_tile<AF, F32, E8 && F32 ? 2 : 4, 4, 2, 2, 2, E8 && !F32 ? 3 : 4>(p, st);
   }
 }
 
 }  // namespace
 
-int mx_gemm_tile_choice(int M, int N, int K, int fmt) {
-  const long big = (long)((M + 255) / 256) * ((N + 255) / 256), mid = (long)((M + 127) / 128) * ((N + 127) / 128);
-  return big >= 200 ? 2 : mid >= 200 ? 1 : 0;
+// Which kernel runs a product.  Up to 8 rows of a (16 of E2M1), unless 64 x 64 tiles fill the CUs: the rows kernel
+// (M = 1, K = 6144: N = 6144 6.7 us E2M1, 6.4 E4M3, the tiles 9.1, 9.9; N = 16384 11.9 and 11.3, the tiles 10.6, 11.2).
+// Else the block tile that takes least by its rounds: us[n - 1] microseconds per 1024 columns of K with n workgroups on
+// a CU, and 2 us a round, as measured at K = 6144 (M x N and us of the tiles in order; E2M1: 77 x 6144 9.1 10.5 14.0 34,
+// 256 x 6144 13.3 11.5 14.7 34, 256 x 16384 26.1 21.9 19.1 38, 4352 x 16384 - - 312 236; E4M3: 77 x 6144 9.9 12.6 18.9 30,
+// 256 x 6144 17.4 15.0 20.5 30, 256 x 16384 34.5 28.6 25.0 35, 4352 x 16384 - - 375 336).
+int mx_gemm_tile(int M, int N, int K, int fmt, int& rows, int& cols) {
+  struct Tile {
+    int rows, cols, slots;
+    float us[3];
+  };
+  static const Tile tiles[2][MX_TILES] = {
+      {{64, 64, 3, {1.2f, 1.9f, 2.9f}}, {128, 64, 2, {1.6f, 3.2f}}, {128, 128, 1, {2.75f}}, {256, 256, 1, {7.0f}}},
+      {{64, 64, 3, {1.35f, 2.6f, 3.9f}}, {64, 128, 2, {2.1f, 4.4f}}, {128, 128, 2, {3.8f, 6.6f}}, {256, 256, 1, {10.0f}}}};
+  const int e8 = fmt == MX_E4M3;
+  if (M <= (e8 ? 8 : 16) && N < 64 * 256) {
+    rows = M <= 8 ? 8 : 16;
+    cols = 16;
+    return MX_ROWS;
+  }
+  int best = 0;
+  float least = 0.0f;
+  for (int i = 0; i < MX_TILES; ++i) {
+    const Tile& t = tiles[e8][i];
+    const long n = (((long)M + t.rows - 1) / t.rows) * (((long)N + t.cols - 1) / t.cols), whole = n / (256 * t.slots),
+               rest = (n % (256 * t.slots) + 255) / 256;
+    const float us = whole * (2.0f + t.us[t.slots - 1] * (K / 1024.0f)) + (rest ? 2.0f + t.us[rest - 1] * (K / 1024.0f) : 0.0f);
+    if (i == 0 || us < least) {
+      best = i;
+      least = us;
+    }
+  }
+  rows = tiles[e8][best].rows;
+  cols = tiles[e8][best].cols;
+  return best;
 }
 
 hipError_t launch_mx_gemm(const MxGemmParams& p, int fmt, bool out_f32, hipStream_t st) {

@@ -107,6 +107,7 @@ SIGNATURES = {
     "svdq_mx_quantize": (_I, [_P, _L, _I, _I, _I, _P, _P, _P]),
     "svdq_mx_dequantize": (_I, [_P, _P, _I, _I, _I, _P, _P]),
     "svdq_mx_gemm": (_I, [_P, _P, _I, _P, _P, _P, _I, _I, _I, _P, _L, _I, _P]),
+    "svdq_mx_gemm_tile": (_I, [_I, _I, _I, _I, ctypes.POINTER(_I), ctypes.POINTER(_I)]),
     "svdq_silu_mul_mx": (_I, [_P, _L, _P, _L, _I, _I, _I, _P, _P, _P]),
     "svdq_rms_norm_modulate_mx": (_I, [_P, _L, _P, _P, _I, _I, ctypes.c_float, _I, _P, _P, _P]),
     "svdq_residual_rms_norm_modulate_mx": (_I, [_P, _L, _P, _L, _P, _P, _P, _I, _I, ctypes.c_float, _I, _P, _L, _P,
@@ -185,6 +186,13 @@ def w4a4_tile(m: int, ns, k: int, group: int, rtp: int = 32) -> tuple[int, int, 
 def w4a16_tile(m: int, ns, k: int, group: int, rtp: int = 32) -> tuple[int, int, int]:
     """The same for the W4A16 GEMM (``svdq_w4a16_gemm_tile``)."""
     return _tile("svdq_w4a16_gemm_tile", m, ns, k, group, rtp)
+
+
+def mx_tile(m: int, n: int, k: int, fmt: int) -> tuple[int, int, int]:
+    """(1, or 2 for the kernel for few rows; tile rows; tile columns) of an MX product (``svdq_mx_gemm_tile``)."""
+    rows, cols = _I(), _I()
+    kind = load().svdq_mx_gemm_tile(m, n, k, fmt, ctypes.byref(rows), ctypes.byref(cols))
+    return int(kind), rows.value, cols.value
 
 
 def w4a4_tile_cols(m: int, n: int, k: int, group: int, operand: int) -> int:

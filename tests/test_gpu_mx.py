@@ -121,6 +121,34 @@ def test_product(dev, fmt, m, n, k):
         check_product(ops.mx_gemm(*t, bias), a, w, f64(bias))
 
 
+# sizes that each kernel is chosen for, with ragged edges on both sides: (kind, rows, columns) as lib.mx_tile gives them
+TILES = {"e2m1": {(2, 8, 16): (7, 1000), (2, 16, 16): (13, 1000), (1, 64, 64): (70, 3000), (1, 128, 64): (250, 6100),
+                  (1, 128, 128): (500, 8100), (1, 256, 256): (1990, 8100)},
+         "e4m3": {(2, 8, 16): (7, 1000), (1, 64, 64): (70, 3000), (1, 64, 128): (250, 6100), (1, 128, 128): (500, 8100),
+                  (1, 256, 256): (1990, 8100)}}
+
+
+@pytest.mark.parametrize("k", [128, 384, 640, 1000, 2304, 2432])   # one stage, halves of one, ends within a chunk of scales
+@pytest.mark.parametrize("fmt,tile", [(f, t) for f in FMTS for t in TILES[f]])
+def test_every_tile(dev, fmt, tile, k):
+    m, n = TILES[fmt][tile]
+    assert lib.mx_tile(m, n, k, ops.MX_FORMATS[fmt]) == tile
+    x, w = _act(dev, m, k, seed=1), _act(dev, n, k, seed=2)
+    a, b = ops.mx_quantize(x, fmt), ops.mx_quantize(w)
+    bias = _act(dev, n, seed=3)
+    av, bv = (torch.from_numpy(values(*t)).to(dev) for t in (a, b))   # float64 on the card: torch's product there
+    y, mag = av @ bv.T + bias.double(), av.abs() @ bv.abs().T + bias.double().abs()
+    bound = 1.01 * (av.shape[1] + 1) * 2.0 ** -24 * mag   # as mx_util.product_bound
+    got = ops.mx_gemm(*a, *b, bias, True).double()
+    assert ((got - y).abs() <= bound).all()
+    if fmt == "e4m3":
+        ma, mb = (t.abs().reshape(len(t), -1, mx.BLOCK).amax(-1) for t in (av, bv))
+        bound = bound + 4 * 7 * 2.0 ** -13 * 2 * (ma @ mb.T)   # as mx_util.dropped
+    bound = bound + 2.0 ** -8 * (y.abs() + bound)
+    got = ops.mx_gemm(*a, *b, bias).double()
+    assert ((got - y).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("m,n", [(5, 40), (40, 72), (300, 300)])
 def test_product_is_blockwise(dev, fmt, m, n):
