@@ -789,10 +789,11 @@ int svdq_mx_gemm(const void* a, const void* a_scales, int fmt, const void* w, co
 int svdq_mx_gemm_tile(int M, int N, int K, int fmt, int* rows, int* cols) {
   if (M <= 0 || N <= 0 || K <= 0 || K > 1 << 22 || (fmt != SVDQ_MX_E2M1 && fmt != SVDQ_MX_E4M3)) return 0;
   int r = 0, c = 0;
-  const int tile = svdq::mx_gemm_tile(M, N, K, fmt, r, c);
+  bool split = false;
+  const int tile = svdq::mx_gemm_tile(M, N, K, fmt, r, c, split);
   if (rows) *rows = r;
   if (cols) *cols = c;
-  return tile == svdq::MX_ROWS ? 2 : 1;
+  return tile == svdq::MX_ROWS ? 2 : split ? 3 : 1;
 }
 
 int svdq_silu_mul_mx(const void* g, int64_t ldg, const void* u, int64_t ldu, int M, int K, int fmt, void* codes,

@@ -196,8 +196,9 @@ struct MxGemmParams {
   int M, N, K;
 };
 hipError_t launch_mx_gemm(const MxGemmParams& p, int fmt, bool out_f32, hipStream_t st);
-// the kernel that runs it: a block tile (0 .. MX_TILES - 1) or the kernel for few rows, and its rows of a by rows of w
+// the kernel that runs it: a block tile (0 .. MX_TILES - 1) or the kernel for few rows, its rows of a by rows of w, and
+// whether a second launch of smaller tiles takes the last rows
 constexpr int MX_TILES = 4, MX_ROWS = -1;
-int mx_gemm_tile(int M, int N, int K, int fmt, int& rows, int& cols);
+int mx_gemm_tile(int M, int N, int K, int fmt, int& rows, int& cols, bool& split);
 
 }  // namespace svdq

@@ -233,15 +233,14 @@ __global__ void __launch_bounds__(64 * WM * WN, (MxTile<AF, F32, TM, TN, WM, WN,
   auto step = [&](auto jj, auto nd, auto&& rd, auto&& dma) {
     constexpr int J = decltype(jj)::value, ND = decltype(nd)::value, OPS = READS + ND;
     constexpr int PER = (OPS + PRODUCTS - 1) / PRODUCTS;   // behind each product
-    // DMA instructions as far apart as the products behind the reads allow
-    constexpr int LEFT = PRODUCTS - READS, GAP = PER == 1 && ND && LEFT / (ND ? ND : 1) > 1 ? LEFT / (ND ? ND : 1) : 1;
+    constexpr int EVERY = ND == 0 ? PRODUCTS + 1 : ND > PRODUCTS ? 1 : PRODUCTS / (ND ? ND : 1);   // PER = 1: a DMA instruction behind every so manyth
 #pragma unroll
     for (int i = 0; i < PRODUCTS; ++i) {
       const int x = i / TM, t = i % TM;
       acc[x][t] = mx_mfma<AF, F32, 2 * (J & 1)>(fw[J & 1][x], fa[J & 1][t], acc[x][t], cw[x], ca[t]);
-      if (GAP > 1) {
-        if (i < READS) rd(i);
-        else if ((i - READS) % GAP == 0 && (i - READS) / GAP < ND) dma((i - READS) / GAP);
+      if (PER == 1) {
+        if (i % EVERY == EVERY - 1 && i / EVERY < ND) dma(i / EVERY);
+        else if (i - (i / EVERY < ND ? i / EVERY : ND) < READS) rd(i - (i / EVERY < ND ? i / EVERY : ND));
       } else {
 #pragma unroll
         for (int o = i * PER; o < (i + 1) * PER && o < OPS; ++o) {
@@ -310,62 +309,63 @@ __global__ void __launch_bounds__(64 * WM * WN, (MxTile<AF, F32, TM, TN, WM, WN,
     step(std::integral_constant<int, 0>{}, None{}, [&](int r) { read(cur, 1, r); }, [](int) {});
     step(std::integral_constant<int, 1>{}, None{}, [](int) {}, [](int) {});
   }
-  // nothing of the DMA may be under way when the next workgroup takes this one's LDS
+  // Register 4 q + r of lane (lr, h): row lr of a, column 8 q + 4 h + r of w.  32 rows at a time go through LDS, each wave
+  // in a part of its own, and out as whole rows of its tile (stored from the registers, 32 bytes to each of 32 rows an
+  // instruction: M = 4352, N = 16384, K = 6144 235 us, so 231), past the L2, whose lines the operands need and which
+  // would be written back in one go at the kernel's end (231 -> 221).  Nothing of the DMA may be under way when LDS is
+  // used again, here or by the next workgroup.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-
-  // Register 4 q + r of lane (lr, h): row lr of a, column 8 q + 4 h + r of w.  bf16: the halves of a row exchange
-  // runs of four, so that a lane stores eight consecutive columns.
-  const int mrow = m0 + 32 * TM * wm + lr, ncol = n0 + 32 * TN * wn;
-  const bool wide = p.ldy % 8 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
+  __syncthreads();
+  constexpr int ES = F32 ? 4 : 2, COLS = 32 * TN, PITCH = COLS * ES + 16, PER = 16 / ES;   // bytes; elements in 16
+  static_assert(T::NW * 32 * PITCH <= T::LDS, "LDS");
+  uint8_t* stage_out = sm + wave * 32 * PITCH;
+  const int mw = m0 + 32 * TM * wm, nw = n0 + COLS * wn;
+  const bool wide = p.ldy % PER == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
+  f32x4 bias[TN][4];
 #pragma unroll
-  for (int i = 0; i < TN; ++i) {
-    const int c0 = ncol + 32 * i;
-    if (c0 >= p.N) continue;
-    float b[16];
+  for (int i = 0; i < TN; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int c = c0 + 8 * (r / 4) + 4 * h + r % 4;
-      b[r] = p.bias && c < p.N ? bf16f(p.bias[c]) : 0.0f;
+      const int c = nw + 32 * i + 8 * (r / 4) + 4 * h + r % 4;
+      bias[i][r / 4][r % 4] = p.bias && c < p.N ? bf16f(p.bias[c]) : 0.0f;
     }
 #pragma unroll
-    for (int t = 0; t < TM; ++t) {
-      const int m = mrow + 32 * t;
-      float v[16];
+  for (int t = 0; t < TM; ++t) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = acc[i][t][r] + b[r];
-      if (F32) {
-        float* row = static_cast<float*>(p.y) + (long)m * p.ldy;
+    for (int i = 0; i < TN; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int c = c0 + 8 * q + 4 * h;
-          if (m < p.M) {
-            if (wide && c + 4 <= p.N) *reinterpret_cast<f32x4*>(row + c) = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
-            else
-              for (int r = 0; r < 4; ++r)
-                if (c + r < p.N) row[c + r] = v[4 * q + r];
-          }
-        }
-      } else {
-        uint16_t* row = static_cast<uint16_t*>(p.y) + (long)m * p.ldy;
+      for (int q = 0; q < 4; ++q) {
+        f32x4 v;
 #pragma unroll
-        for (int q = 0; q < 4; q += 2) {
-          u32x4 o = {pack_bf16x2(v[4 * q], v[4 * q + 1]), pack_bf16x2(v[4 * q + 2], v[4 * q + 3]),
-                     pack_bf16x2(v[4 * q + 4], v[4 * q + 5]), pack_bf16x2(v[4 * q + 6], v[4 * q + 7])};
-          // lanes h = 0: columns 8 q .. + 3 and (from the other half) + 4 .. 7; h = 1: 8 (q + 1) ..
-          uint32_t x0 = o[0], x1 = o[1], y0 = o[2], y1 = o[3];
-          permlane32_swap(x0, y0);
-          permlane32_swap(x1, y1);
-          const u32x4 w = {x0, x1, y0, y1};
-          const int c = c0 + 8 * (q + h);
-          if (m < p.M) {
-            if (wide && c + 8 <= p.N) *reinterpret_cast<u32x4*>(row + c) = w;
-            else
-              for (int r = 0; r < 8; ++r)
-                if (c + r < p.N) row[c + r] = (uint16_t)(w[r / 2] >> (16 * (r % 2)));
-          }
+        for (int r = 0; r < 4; ++r) v[r] = acc[i][t][4 * q + r] + bias[i][q][r];
+        uint8_t* to = stage_out + lr * PITCH + (32 * i + 8 * q + 4 * h) * ES;
+        if (F32) *reinterpret_cast<f32x4*>(to) = v;
+        else *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own writes, read by its other lanes
+    const int rows = min(32, p.M - (mw + 32 * t)), cols = min(COLS, p.N - nw);
+    uint8_t* out = static_cast<uint8_t*>(p.y) + ((long)(mw + 32 * t) * p.ldy + nw) * ES;
+    if (wide && cols % PER == 0) {
+      constexpr int LPR = COLS / PER;   // lanes per row
+#pragma unroll
+      for (int k = 0; k < 32 * LPR / 64; ++k) {
+        const int row = (64 * k + lane) / LPR, c = (64 * k + lane) % LPR;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(stage_out + row * PITCH + 16 * c);
+        if (row < rows && PER * c < cols) __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(out + (long)row * p.ldy * ES + 16 * c));
+      }
+    } else {
+#pragma unroll 4
+      for (int k = 0; k < 32 * COLS / 64; ++k) {
+        const int row = (64 * k + lane) / COLS, c = (64 * k + lane) % COLS;
+        const uint8_t* from = stage_out + row * PITCH + c * ES;
+        if (row < rows && c < cols) {
+          uint8_t* to = out + (long)row * p.ldy * ES + c * ES;
+          if (F32) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+          else *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
         }
       }
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 }
 
@@ -516,10 +516,9 @@ hipError_t launch_rows(const MxGemmParams& p, hipStream_t st) {
 }
 
 template <int AF, bool F32>
-hipError_t launch_any(const MxGemmParams& p, hipStream_t st) {
+hipError_t launch_kernel(int tile, const MxGemmParams& p, hipStream_t st) {
   constexpr bool E8 = AF == MX_E4M3;
-  int rows, cols;
-  switch (mx_gemm_tile(p.M, p.N, p.K, AF, rows, cols)) {
+  switch (tile) {
     case MX_ROWS:
       if constexpr (!E8)
         if (p.M > 8) return launch_rows<AF, F32, 16, 2>(p, st);
@@ -532,43 +531,76 @@ hipError_t launch_any(const MxGemmParams& p, hipStream_t st) {
   }
 }
 
+// Block tiles: rows of a, of w, workgroups that share a CU, and microseconds per 1024 columns of K with n of them on a
+// CU (us[n - 1]); a round takes 2 us besides.  As measured at K = 6144 (M x N and us of the tiles in order; E2M1: 77 x
+// 6144 9.2 10.5 14.0 34, 256 x 6144 13.3 11.5 14.7 34, 256 x 16384 26.1 21.9 18.4 38, 4352 x 16384 - - 306 231; E4M3:
+// 77 x 6144 9.9 12.6 18.9 30, 256 x 6144 17.4 15.0 20.5 30, 256 x 16384 34.5 28.6 24.9 35, 4352 x 16384 - - 375 330).
+struct MxTileCost {
+  int rows, cols, slots;
+  float us[3];
+};
+const MxTileCost kTiles[2][MX_TILES] = {
+    {{64, 64, 3, {1.2f, 1.9f, 2.9f}}, {128, 64, 2, {1.6f, 3.2f}}, {128, 128, 1, {2.75f}}, {256, 256, 1, {7.2f}}},
+    {{64, 64, 3, {1.35f, 2.6f, 3.9f}}, {64, 128, 2, {2.1f, 4.4f}}, {128, 128, 2, {3.8f, 6.6f}}, {256, 256, 1, {10.3f}}}};
+
+float tile_us(const MxTileCost& t, long tiles, int K) {
+  const long whole = tiles / (256 * t.slots), rest = (tiles % (256 * t.slots) + 255) / 256;
+  return whole * (2.0f + t.us[t.slots - 1] * (K / 1024.0f)) + (rest ? 2.0f + t.us[rest - 1] * (K / 1024.0f) : 0.0f);
+}
+
+long tiles_of(const MxTileCost& t, long M, long N) { return ((M + t.rows - 1) / t.rows) * ((N + t.cols - 1) / t.cols); }
+
+struct MxChoice {
+  int tile;
+  float us;
+  int large;   // rows that go to the large tiles ahead of a launch of smaller ones for the others, 0: one launch
+};
+
+// Up to 8 rows of a (16 of E2M1), unless 64 x 64 tiles fill the CUs, run the rows kernel (M = 1, K = 6144: N = 6144 6.7 us
+// E2M1, 6.4 E4M3, the tiles 9.1, 9.9; N = 16384 11.9 and 11.3, the tiles 10.6, 11.2); else the tile that takes least
+// by its rounds.  A last round of large tiles that leaves most CUs idle costs nearly as much as a full one, so the
+// rows behind the whole rounds go to smaller tiles where that is less: M = 4352, N = 16384, K = 6144 is 4 rounds and 64
+// tiles more, 241 us in one launch, 228 with the last 256 rows on 128 x 128 tiles (E4M3 333, 314); M = 3000, N = K =
+// 6144 85, 67.
+MxChoice choose(long M, long N, int K, int fmt) {
+  const int e8 = fmt == MX_E4M3;
+  if (M <= (e8 ? 8 : 16) && N < 64 * 256) return {MX_ROWS, 10.0f, 0};
+  MxChoice best{0, tile_us(kTiles[e8][0], tiles_of(kTiles[e8][0], M, N), K), 0};
+  for (int i = 1; i < MX_TILES; ++i) {
+    const float us = tile_us(kTiles[e8][i], tiles_of(kTiles[e8][i], M, N), K);
+    if (us < best.us) best = {i, us, 0};
+  }
+  const MxTileCost& t = kTiles[e8][MX_TILES - 1];
+  const long nbn = (N + t.cols - 1) / t.cols, blocks = tiles_of(t, M, N) / 256 * 256 / nbn, rows = blocks * t.rows;
+  if (blocks > 0 && rows < M) {
+    const float us = tile_us(t, blocks * nbn, K) + choose(M - rows, N, K, fmt).us + 2.0f;
+    if (us < 0.97f * best.us) best = {MX_TILES - 1, us, (int)rows};
+  }
+  return best;
+}
+
+template <int AF, bool F32>
+hipError_t launch_any(const MxGemmParams& p, hipStream_t st) {
+  const MxChoice c = choose(p.M, p.N, p.K, AF);
+  if (c.large == 0) return launch_kernel<AF, F32>(c.tile, p, st);
+  MxGemmParams q = p;
+  q.M = c.large;
+  if (hipError_t e = launch_kernel<AF, F32>(c.tile, q, st)) return e;
+  q.M = p.M - c.large;
+  q.a += c.large * mx_row_bytes(p.K, AF);
+  q.as += c.large * mx_sp(p.K);
+  q.y = static_cast<uint8_t*>(p.y) + c.large * p.ldy * (F32 ? 4 : 2);
+  return launch_any<AF, F32>(q, st);
+}
+
 }  // namespace
 
-// Which kernel runs a product.  Up to 8 rows of a (16 of E2M1), unless 64 x 64 tiles fill the CUs: the rows kernel
-// (M = 1, K = 6144: N = 6144 6.7 us E2M1, 6.4 E4M3, the tiles 9.1, 9.9; N = 16384 11.9 and 11.3, the tiles 10.6, 11.2).
-// Else the block tile that takes least by its rounds: us[n - 1] microseconds per 1024 columns of K with n workgroups on
-// a CU, and 2 us a round, as measured at K = 6144 (M x N and us of the tiles in order; E2M1: 77 x 6144 9.1 10.5 14.0 34,
-// 256 x 6144 13.3 11.5 14.7 34, 256 x 16384 26.1 21.9 19.1 38, 4352 x 16384 - - 312 236; E4M3: 77 x 6144 9.9 12.6 18.9 30,
-// 256 x 6144 17.4 15.0 20.5 30, 256 x 16384 34.5 28.6 25.0 35, 4352 x 16384 - - 375 336).
-int mx_gemm_tile(int M, int N, int K, int fmt, int& rows, int& cols) {
-  struct Tile {
-    int rows, cols, slots;
-    float us[3];
-  };
-  static const Tile tiles[2][MX_TILES] = {
-      {{64, 64, 3, {1.2f, 1.9f, 2.9f}}, {128, 64, 2, {1.6f, 3.2f}}, {128, 128, 1, {2.75f}}, {256, 256, 1, {7.0f}}},
-      {{64, 64, 3, {1.35f, 2.6f, 3.9f}}, {64, 128, 2, {2.1f, 4.4f}}, {128, 128, 2, {3.8f, 6.6f}}, {256, 256, 1, {10.0f}}}};
-  const int e8 = fmt == MX_E4M3;
-  if (M <= (e8 ? 8 : 16) && N < 64 * 256) {
-    rows = M <= 8 ? 8 : 16;
-    cols = 16;
-    return MX_ROWS;
-  }
-  int best = 0;
-  float least = 0.0f;
-  for (int i = 0; i < MX_TILES; ++i) {
-    const Tile& t = tiles[e8][i];
-    const long n = (((long)M + t.rows - 1) / t.rows) * (((long)N + t.cols - 1) / t.cols), whole = n / (256 * t.slots),
-               rest = (n % (256 * t.slots) + 255) / 256;
-    const float us = whole * (2.0f + t.us[t.slots - 1] * (K / 1024.0f)) + (rest ? 2.0f + t.us[rest - 1] * (K / 1024.0f) : 0.0f);
-    if (i == 0 || us < least) {
-      best = i;
-      least = us;
-    }
-  }
-  rows = tiles[e8][best].rows;
-  cols = tiles[e8][best].cols;
-  return best;
+int mx_gemm_tile(int M, int N, int K, int fmt, int& rows, int& cols, bool& split) {
+  const MxChoice c = choose(M, N, K, fmt);
+  split = c.large > 0;
+  rows = c.tile == MX_ROWS ? (M <= 8 ? 8 : 16) : kTiles[fmt == MX_E4M3][c.tile].rows;
+  cols = c.tile == MX_ROWS ? 16 : kTiles[fmt == MX_E4M3][c.tile].cols;
+  return c.tile;
 }
 
 hipError_t launch_mx_gemm(const MxGemmParams& p, int fmt, bool out_f32, hipStream_t st) {

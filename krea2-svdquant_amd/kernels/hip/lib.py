@@ -189,7 +189,7 @@ def w4a16_tile(m: int, ns, k: int, group: int, rtp: int = 32) -> tuple[int, int,
 
 
 def mx_tile(m: int, n: int, k: int, fmt: int) -> tuple[int, int, int]:
-    """(1, or 2 for the kernel for few rows; tile rows; tile columns) of an MX product (``svdq_mx_gemm_tile``)."""
+    """(1, 2: the kernel for few rows, 3: a second launch for the last rows; tile rows; columns) of an MX product (``svdq_mx_gemm_tile``)."""
     rows, cols = _I(), _I()
     kind = load().svdq_mx_gemm_tile(m, n, k, fmt, ctypes.byref(rows), ctypes.byref(cols))
     return int(kind), rows.value, cols.value

@@ -131,7 +131,15 @@ TILES = {"e2m1": {(2, 8, 16): (7, 1000), (2, 16, 16): (13, 1000), (1, 64, 64): (
 @pytest.mark.parametrize("k", [128, 384, 640, 1000, 2304, 2432])   # one stage, halves of one, ends within a chunk of scales
 @pytest.mark.parametrize("fmt,tile", [(f, t) for f in FMTS for t in TILES[f]])
 def test_every_tile(dev, fmt, tile, k):
-    m, n = TILES[fmt][tile]
+    _check_tile(dev, fmt, tile, *TILES[fmt][tile], k)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_last_rows_on_smaller_tiles(dev, fmt):
+    _check_tile(dev, fmt, (3, 256, 256), 2200, 8100, 3000)
+
+
+def _check_tile(dev, fmt, tile, m, n, k):
     assert lib.mx_tile(m, n, k, ops.MX_FORMATS[fmt]) == tile
     x, w = _act(dev, m, k, seed=1), _act(dev, n, k, seed=2)
     a, b = ops.mx_quantize(x, fmt), ops.mx_quantize(w)
