@@ -70,14 +70,15 @@ __device__ __forceinline__ uint32_t mx_block_top(const float (&v)[8]) {
 }
 
 // Chunk c (eight columns from 8 c) of a row into MX blocks: the four lanes of a block call it together.
-// Chunks beyond kp write only their share of the scales' padding (v is zero there).
-template <int FMT>
+// Chunks beyond kp write only their share of the scales' padding (v is zero there).  PAST: E4M3 codes past the L2.
+template <int FMT, bool PAST = false>
 __device__ __forceinline__ void mx_store8(const float (&v)[8], int c, int kp, uint8_t* __restrict__ codes,
                                           uint8_t* __restrict__ scales) {
   const uint32_t s = mx_scale_byte<FMT>(mx_block_top(v));
   const u32x2 o = mx_encode8<FMT>(v, s);
   if (8 * c < kp) {
     if (FMT == MX_E2M1) *reinterpret_cast<uint32_t*>(codes + 4 * c) = o[0];
+    else if (PAST) __builtin_nontemporal_store(o, reinterpret_cast<u32x2*>(codes + 8 * c));
     else *reinterpret_cast<u32x2*>(codes + 8 * c) = o;
   }
   if ((c & 3) == 0) scales[c >> 2] = (uint8_t)s;

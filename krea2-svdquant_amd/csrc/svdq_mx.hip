@@ -36,93 +36,126 @@ __device__ __forceinline__ void load8(const uint16_t* __restrict__ row, int c, i
   }
 }
 
-// silu(g) u = g u / (1 + exp(-g)) in float32.  exp(-g) overflows to infinity for g < -88.7, where the quotient is -0
-// as it should be to float32's smallest normal; g = -infinity gives NaN (as in torch's float32 formula).
-__device__ __forceinline__ float silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) u = g u / (1 + exp(-g)) in float32.  exp(-g) = 2^t, t = -g log2(e) as the rounded product t0 and what it and the
+// rounded constant leave, 2^t = 2^t0 (1 + ln(2) (t - t0)), within 1.5 units of 2^-23; the reciprocal of 1 + exp(-g) by
+// v_rcp_f32 and one Newton step; g u is exact, so the result rounds once more.  Few instructions, because the pass is close to being bound by them: with expf and the correctly rounded
+// quotient M = 4352, K = 16384, E4M3 took 74.9 us, so SILU_AFTER.  Beyond |g| = 87 the exponent is held there: 1 + exp(-g)
+// is 1 above, and below the product's magnitude is under 2^-118 |u|, taken as 0 (so is g = -infinity's).
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  const float c = __builtin_amdgcn_fmed3f(g, -87.0f, 87.0f);
+  const float t0 = c * -1.44269502f;
+  const float rest = __builtin_fmaf(c, -1.92596303e-8f, __builtin_fmaf(c, -1.44269502f, -t0));
+  const float e0 = __builtin_amdgcn_exp2f(t0), e = __builtin_fmaf(e0, 0.693147181f * rest, e0);
+  const float d = 1.0f + e, r = __builtin_amdgcn_rcpf(d), r1 = __builtin_fmaf(r, __builtin_fmaf(-d, r, 1.0f), r);
+  return (g < -87.0f ? 0.0f : g) * u * r1;
+}
 
-// One thread per chunk of 8 columns, sp * 4 chunks a row (the scales' padding included).  A workgroup takes 256
-// consecutive chunks of the row-major list, its first one's row by one uniform 64-bit division.
+// A wave takes units of 64 chunks (512 columns: 16 bytes of scales) of one row, UNITS of them at a time, whose loads are
+// all under way before the first is used; rows and columns are wave-uniform (scalar) arithmetic.
 // GATE: the SwiGLU product silu(x) * u, else x itself.
-template <int FMT, bool VEC, bool GATE>
+template <int FMT, bool VEC, bool GATE, int UNITS>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(const uint16_t* __restrict__ x, long ldx,
-                                                          const uint16_t* __restrict__ u, long ldu, long M, int K,
+                                                          const uint16_t* __restrict__ u, long ldu, long units, int K,
                                                           uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  const int kp = (int)mx_kp(K), sp = (int)mx_sp(K), per_row = 4 * sp;
-  const long first = (long)blockIdx.x * 256;
-  const long row0 = first / per_row;
-  const uint32_t in = (uint32_t)(first - row0 * per_row) + threadIdx.x;
-  const long row = row0 + in / (uint32_t)per_row;
-  const int c = (int)(in % (uint32_t)per_row);
-  if (row >= M) return;   // per_row % 64 == 0: the four lanes of a block leave together
-  float v[8];
-  load8<VEC>(x + row * ldx, c, K, v);
-  if (GATE) {
-    float w[8];
-    load8<VEC>(u + row * ldu, c, K, w);
+  const int kp = (int)mx_kp(K), sp = (int)mx_sp(K), per_row = sp / 16, lane = threadIdx.x & 63;
+  const long first = ((long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * UNITS;
+  float v[UNITS][8], w[UNITS][8];
+  long row = first / per_row;
+  int part = (int)(first - row * per_row);
+  const long row0 = row;
+  const int part0 = part;
+  auto next = [&] {
+    if (++part == per_row) {
+      part = 0;
+      ++row;
+    }
+  };
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 8 * c + i < K ? silu_mul(v[i], w[i]) : 0.0f;
-  }
-  mx_store8<FMT>(v, c, kp, codes + row * mx_row_bytes(K, FMT), scales + row * sp);
+  for (int i = 0; i < UNITS; ++i, next())
+    if (first + i < units) {
+      load8<VEC>(x + row * ldx, 64 * part + lane, K, v[i]);
+      if (GATE) load8<VEC>(u + row * ldu, 64 * part + lane, K, w[i]);
+    }
+  row = row0;
+  part = part0;
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i, next())
+    if (first + i < units) {
+      const int c = 64 * part + lane;
+      if (GATE) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[i][k] = VEC ? 8 * c < K ? silu_mul(v[i][k], w[i][k]) : 0.0f
+                                                  : 8 * c + k < K ? silu_mul(v[i][k], w[i][k]) : 0.0f;
+      }
+      mx_store8<FMT>(v[i], c, kp, codes + row * mx_row_bytes(K, FMT), scales + row * sp);
+    }
 }
 
-// Eight E2M1 or E4M3 codes as float32, without their scale.
-template <int FMT>
-__device__ __forceinline__ void decode8(u32x2 q, float (&v)[8]) {
-  if (FMT == MX_E2M1) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t m = (q[0] >> (4 * i)) & 7u;
-      // 0, 0.5, 1, 1.5, 2, 3, 4, 6: exponent m / 2, mantissa bit m % 2; the first two are 0 and 0.5
-      const float a = m < 2 ? 0.5f * m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
-      v[i] = __uint_as_float(__float_as_uint(a) | ((q[0] >> (4 * i + 3)) & 1u) << 31);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[i], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[i], true);
-      v[4 * i] = a[0];
-      v[4 * i + 1] = a[1];
-      v[4 * i + 2] = b[0];
-      v[4 * i + 3] = b[1];
-    }
-  }
-}
-
-// Codes and scales back to bf16 [M, K]: code times 2^(s - 127), exact in bf16 but for values below its normal range.
-template <int FMT, bool VEC>
+// Codes and scales back to bf16 [M, K]: code times 2^(s - 127), exact in bf16 but for values below its normal range.  A wave
+// takes units of 64 chunks as above; a lane's eight codes are converted under their scale by four instructions.
+template <int FMT, bool VEC, int UNITS>
 __global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t* __restrict__ codes,
-                                                            const uint8_t* __restrict__ scales, long M, int K,
+                                                            const uint8_t* __restrict__ scales, long units, int K,
                                                             uint16_t* __restrict__ y) {
-  const int per_row = (K + 7) / 8;
-  const long first = (long)blockIdx.x * 256;
-  const long row0 = first / per_row;
-  const uint32_t in = (uint32_t)(first - row0 * per_row) + threadIdx.x;
-  const long row = row0 + in / (uint32_t)per_row;
-  const int c = (int)(in % (uint32_t)per_row);
-  if (row >= M) return;
-  const uint8_t* src = codes + row * mx_row_bytes(K, FMT);
-  u32x2 q = {0, 0};
-  if (FMT == MX_E2M1) q[0] = *reinterpret_cast<const uint32_t*>(src + 4 * c);
-  else q = *reinterpret_cast<const u32x2*>(src + 8 * c);
-  const uint32_t s = scales[row * mx_sp(K) + (c >> 2)];
-  float v[8];
-  decode8<FMT>(q, v);
+  const int sp = (int)mx_sp(K), per_row = sp / 16, lane = threadIdx.x & 63;
+  const long first = ((long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * UNITS;
+  u32x2 q[UNITS];
+  uint32_t s[UNITS];
+  long row = first / per_row;
+  int part = (int)(first - row * per_row);
+  const long row0 = row;
+  const int part0 = part;
+  auto next = [&] {
+    if (++part == per_row) {
+      part = 0;
+      ++row;
+    }
+  };
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = s == 255u ? __builtin_nanf("") : ldexpf(v[i], (int)s - 127);
-  uint16_t* dst = y + row * K + 8 * c;
-  u32x4 o;
+  for (int i = 0; i < UNITS; ++i, next()) {
+    const int c = 64 * part + lane;
+    q[i] = u32x2{0, 0};
+    s[i] = 0;
+    if (first + i < units && 8 * c < K) {
+      const uint8_t* src = codes + row * mx_row_bytes(K, FMT);
+      if (FMT == MX_E2M1) q[i][0] = *reinterpret_cast<const uint32_t*>(src + 4 * c);
+      else q[i] = *reinterpret_cast<const u32x2*>(src + 8 * c);
+      s[i] = scales[row * sp + (c >> 2)];
+    }
+  }
+  row = row0;
+  part = part0;
 #pragma unroll
-  for (int d = 0; d < 4; ++d) o[d] = pack_bf16x2(v[2 * d], v[2 * d + 1]);
-  if (VEC) {
-    *reinterpret_cast<u32x4*>(dst) = o;
-  } else {
+  for (int i = 0; i < UNITS; ++i, next()) {
+    const int c = 64 * part + lane;
+    if (first + i >= units || 8 * c >= K) continue;
+    const float scale = __uint_as_float(s[i] << 23);
+    u32x4 o;
+    if (FMT == MX_E2M1) {
+      o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[i][0], scale, 0));
+      o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[i][0], scale, 1));
+      o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[i][0], scale, 2));
+      o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q[i][0], scale, 3));
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (8 * c + i < K) dst[i] = (uint16_t)(o[i / 2] >> (16 * (i % 2)));
+      for (int d = 0; d < 2; ++d) {
+        o[2 * d] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[i][d], scale, false));
+        o[2 * d + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[i][d], scale, true));
+      }
+    }
+    if (s[i] == 255u) o = u32x4{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
+    uint16_t* dst = y + row * K + 8 * c;
+    if (VEC) {
+      *reinterpret_cast<u32x4*>(dst) = o;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (8 * c + k < K) dst[k] = (uint16_t)(o[k / 2] >> (16 * (k % 2)));
+    }
   }
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
+__device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
   return v;
@@ -130,9 +163,15 @@ __device__ __forceinline__ float wave_sum(float v) {
 
 // Adaptive RMS norm into MX blocks, one 256-thread workgroup per row of H (H % 8 == 0):
 //   RES: xo = bf16(x + g v) (one rounding; written, and the row that is normalized), else xo = x
-//   y = xo rsqrt(mean(xo^2) + eps) w + shift in float32, quantised
+//   y = xo rsqrt(mean(xo^2) + eps) w + shift, rounded to float32 about once, quantised
+// A value near the middle of two codes takes the other one for an error in its last bits, and the whole row shares its
+// mean: the mean is summed in 64 bits, its root's reciprocal kept as r0 + r1, xo w (with a power of two) is exact, and
+// y = (xo w) r0 + shift + (xo w) r1 by two fused products.
 // Thread t takes chunks t, t + 256, ...: the first NR stay in registers between the passes, those beyond are read
-// again (RES: from xo, written by the same thread).
+// again (RES: from xo, written by the same thread).  HBM-bound: 4.03 (E4M3) or 3.53 bytes a value beside x and v.  NR is
+// the row's own count, so that short rows keep few registers, and stores of what is not read again here go past the L2:
+// M = 4352, H = 6144, E4M3, through the operator 39.7 -> 30.8 us (6.1 TB/s; a copy of 107 MB 11.8 us, from the cache in
+// front of HBM).
 template <int FMT, int NR, bool RES>
 __global__ void __launch_bounds__(256) rms_norm_mx_kernel(const uint16_t* __restrict__ x, long ldx,
                                                           const uint16_t* __restrict__ v, long ldv,
@@ -140,11 +179,11 @@ __global__ void __launch_bounds__(256) rms_norm_mx_kernel(const uint16_t* __rest
                                                           const uint16_t* __restrict__ shift, int H, float eps,
                                                           uint16_t* __restrict__ xo, long ldxo,
                                                           uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  __shared__ float part[4];
+  __shared__ double part[4];
   const int tid = threadIdx.x, nc = H / 8, kp = (int)mx_kp(H), sp = (int)mx_sp(H);
   const uint16_t* xr = x + (long)blockIdx.x * ldx;
   uint16_t* xor_ = RES ? xo + (long)blockIdx.x * ldxo : nullptr;
-  auto row_chunk = [&](int c) {
+  auto row_chunk = [&](int c, bool again) {   // again: the chunk will be read again
     u32x4 r = ld16(xr + 8 * c);
     if (RES) {
       const u32x4 gv = ld16(g + 8 * c), vv = ld16(v + (long)blockIdx.x * ldv + 8 * c);
@@ -152,30 +191,37 @@ __global__ void __launch_bounds__(256) rms_norm_mx_kernel(const uint16_t* __rest
       for (int d = 0; d < 4; ++d)
         r[d] = pack_bf16x2(__builtin_fmaf(bf16lo(gv[d]), bf16lo(vv[d]), bf16lo(r[d])),
                            __builtin_fmaf(bf16hi(gv[d]), bf16hi(vv[d]), bf16hi(r[d])));
-      *reinterpret_cast<u32x4*>(xor_ + 8 * c) = r;
+      if (again) *reinterpret_cast<u32x4*>(xor_ + 8 * c) = r;
+      else __builtin_nontemporal_store(r, reinterpret_cast<u32x4*>(xor_ + 8 * c));
     }
     return r;
   };
-  float ss = 0.0f;
+  double ss = 0.0;
   auto add = [&](u32x4 r) {
 #pragma unroll
     for (int d = 0; d < 4; ++d) {
-      ss = __builtin_fmaf(bf16lo(r[d]), bf16lo(r[d]), ss);
-      ss = __builtin_fmaf(bf16hi(r[d]), bf16hi(r[d]), ss);
+      const double a = bf16lo(r[d]), b = bf16hi(r[d]);
+      ss = __builtin_fma(a, a, ss);
+      ss = __builtin_fma(b, b, ss);
     }
   };
   u32x4 keep[NR];
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
     const int c = tid + 256 * i;
-    keep[i] = c < nc ? row_chunk(c) : u32x4{};
+    keep[i] = c < nc ? row_chunk(c, false) : u32x4{};
     add(keep[i]);
   }
-  for (int c = tid + 256 * NR; c < nc; c += 256) add(row_chunk(c));
+  for (int c = tid + 256 * NR; c < nc; c += 256) add(row_chunk(c, true));
   ss = wave_sum(ss);
   if ((tid & 63) == 0) part[tid >> 6] = ss;
   __syncthreads();
-  const float r = 1.0f / sqrtf((part[0] + part[1] + part[2] + part[3]) / (float)H + eps);
+  const double mean = (part[0] + part[1] + part[2] + part[3]) / (double)H + (double)eps;
+  // the root's reciprocal as 2^k (r0 + r1): x 2^k w is exact and of ordinary size whatever the row's
+  const double root = rsqrt(mean);
+  const float pow2 = fmaxf(__uint_as_float(__float_as_uint((float)root) & 0x7F800000u), 1.17549435e-38f);
+  const double scaled = root / (double)pow2;
+  const float r0 = (float)scaled, r1 = (float)(scaled - (double)r0);
   uint8_t* crow = codes + (long)blockIdx.x * mx_row_bytes(H, FMT);
   uint8_t* srow = scales + (long)blockIdx.x * sp;
   auto put = [&](int c, u32x4 raw) {
@@ -186,9 +232,12 @@ __global__ void __launch_bounds__(256) rms_norm_mx_kernel(const uint16_t* __rest
       unpack8(ld16(w + 8 * c), wv);
       unpack8(ld16(shift + 8 * c), sv);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = __builtin_fmaf(f[i] * r, wv[i], sv[i]);
+      for (int i = 0; i < 8; ++i) {
+        const float t = f[i] * pow2 * wv[i];
+        f[i] = __builtin_fmaf(t, r1, __builtin_fmaf(t, r0, sv[i]));
+      }
     }
-    mx_store8<FMT>(f, c, kp, crow, srow);
+    mx_store8<FMT, true>(f, c, kp, crow, srow);
   };
   // 4 sp chunks a row, the scales' padding included; 4 sp % 64 == 0, so a wave's lanes are in or out together
 #pragma unroll
@@ -200,18 +249,27 @@ __global__ void __launch_bounds__(256) rms_norm_mx_kernel(const uint16_t* __rest
     put(c, c < nc ? ld16((RES ? xor_ : xr) + 8 * c) : u32x4{});
 }
 
+template <int FMT, bool GATE, int UNITS>
+hipError_t quantize_by(bool vec, const uint16_t* x, long ldx, const uint16_t* u, long ldu, long units, int K,
+                       uint8_t* codes, uint8_t* scales, hipStream_t st) {
+  const long blocks = (units + 4 * UNITS - 1) / (4 * UNITS);
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  if (vec)
+    mx_quantize_kernel<FMT, true, GATE, UNITS><<<(unsigned)blocks, 256, 0, st>>>(x, ldx, u, ldu, units, K, codes, scales);
+  else
+    mx_quantize_kernel<FMT, false, GATE, UNITS><<<(unsigned)blocks, 256, 0, st>>>(x, ldx, u, ldu, units, K, codes, scales);
+  return hipGetLastError();
+}
+
 template <int FMT, bool GATE>
 hipError_t quantize(const uint16_t* x, long ldx, const uint16_t* u, long ldu, long M, int K, uint8_t* codes,
                     uint8_t* scales, hipStream_t st) {
-  const long blocks = (M * 4 * mx_sp(K) + 255) / 256;
-  if (blocks > INT32_MAX) return hipErrorInvalidValue;
   const uintptr_t at = reinterpret_cast<uintptr_t>(x) | (GATE ? reinterpret_cast<uintptr_t>(u) : 0);
   const bool vec = at % 16 == 0 && ldx % 8 == 0 && (!GATE || ldu % 8 == 0) && K % 8 == 0;
-  if (vec)
-    mx_quantize_kernel<FMT, true, GATE><<<(unsigned)blocks, 256, 0, st>>>(x, ldx, u, ldu, M, K, codes, scales);
-  else
-    mx_quantize_kernel<FMT, false, GATE><<<(unsigned)blocks, 256, 0, st>>>(x, ldx, u, ldu, M, K, codes, scales);
-  return hipGetLastError();
+  const long units = M * (mx_sp(K) / 16);
+  // units: M = 4352, K = 6144 and 16384, E4M3, UNITS = 1 / 2 / 4: quantising 14.8 13.9 14.8 and 40.6 35.3 38.8 us, the
+  // SwiGLU product 21.4 23.9 - and 62.0 66.1 -
+  return quantize_by<FMT, GATE, GATE ? 1 : 2>(vec, x, ldx, u, ldu, units, K, codes, scales, st);
 }
 
 template <int FMT, bool RES, class... A>
@@ -220,7 +278,10 @@ hipError_t norm(int T, int H, hipStream_t st, A... a) {
     case 1: rms_norm_mx_kernel<FMT, 1, RES><<<T, 256, 0, st>>>(a...); break;
     case 2: rms_norm_mx_kernel<FMT, 2, RES><<<T, 256, 0, st>>>(a...); break;
     case 3: rms_norm_mx_kernel<FMT, 3, RES><<<T, 256, 0, st>>>(a...); break;
-    default: rms_norm_mx_kernel<FMT, 4, RES><<<T, 256, 0, st>>>(a...);
+    case 4: rms_norm_mx_kernel<FMT, 4, RES><<<T, 256, 0, st>>>(a...); break;
+    case 5: rms_norm_mx_kernel<FMT, 5, RES><<<T, 256, 0, st>>>(a...); break;
+    case 6: rms_norm_mx_kernel<FMT, 6, RES><<<T, 256, 0, st>>>(a...); break;
+    default: rms_norm_mx_kernel<FMT, 8, RES><<<T, 256, 0, st>>>(a...);
   }
   return hipGetLastError();
 }
@@ -239,20 +300,21 @@ hipError_t launch_silu_mul_mx(const uint16_t* g, long ldg, const uint16_t* u, lo
                         : quantize<MX_E2M1, true>(g, ldg, u, ldu, M, K, codes, scales, st);
 }
 
+template <int FMT>
+static hipError_t dequantize(const uint8_t* codes, const uint8_t* scales, long M, int K, uint16_t* y, hipStream_t st) {
+  constexpr int UNITS = 2;
+  const long units = M * (mx_sp(K) / 16), blocks = (units + 4 * UNITS - 1) / (4 * UNITS);
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  if (K % 8 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0)
+    mx_dequantize_kernel<FMT, true, UNITS><<<(unsigned)blocks, 256, 0, st>>>(codes, scales, units, K, y);
+  else
+    mx_dequantize_kernel<FMT, false, UNITS><<<(unsigned)blocks, 256, 0, st>>>(codes, scales, units, K, y);
+  return hipGetLastError();
+}
+
 hipError_t launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, long M, int K, int fmt, uint16_t* y,
                                 hipStream_t st) {
-  const long blocks = (M * ((K + 7) / 8) + 255) / 256;
-  if (blocks > INT32_MAX) return hipErrorInvalidValue;
-  const bool vec = K % 8 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
-  const unsigned n = (unsigned)blocks;
-  if (fmt == MX_E4M3) {
-    if (vec) mx_dequantize_kernel<MX_E4M3, true><<<n, 256, 0, st>>>(codes, scales, M, K, y);
-    else mx_dequantize_kernel<MX_E4M3, false><<<n, 256, 0, st>>>(codes, scales, M, K, y);
-  } else {
-    if (vec) mx_dequantize_kernel<MX_E2M1, true><<<n, 256, 0, st>>>(codes, scales, M, K, y);
-    else mx_dequantize_kernel<MX_E2M1, false><<<n, 256, 0, st>>>(codes, scales, M, K, y);
-  }
-  return hipGetLastError();
+  return fmt == MX_E4M3 ? dequantize<MX_E4M3>(codes, scales, M, K, y, st) : dequantize<MX_E2M1>(codes, scales, M, K, y, st);
 }
 
 hipError_t launch_rms_norm_mx(const uint16_t* x, long ldx, const uint16_t* v, long ldv, const uint16_t* g,

@@ -292,6 +292,16 @@ def test_norm_layouts_and_rows_that_are_not_finite(dev, fmt):
     assert torch.equal(y[2, 32:], ops.mx_dequantize(*t, 1024).float()[2, 32:])
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+def test_norm_of_rows_of_any_size(dev, fmt):
+    # magnitudes whose squares, sums and products with the weight leave float32's range
+    scale = torch.tensor([1e-38, 1e-30, 1e-20, 1.0, 1e15, 1e25, 1e37], device=dev)
+    x = (_act(dev, 7, 640, seed=1, dtype=torch.float32).clamp(-20, 20) * scale[:, None]).to(torch.bfloat16)
+    w, shift = _act(dev, 640, seed=4), _act(dev, 640, seed=5)
+    for eps in (0.0, 1e-6):
+        check_blocks(*ops.rms_norm_modulate_mx(x, w, shift, eps, fmt), *_norm64(f64(x), f64(w), f64(shift), eps))
+
+
 # ---- SwiGLU product ----
 def _silu64(g, u):
     """y, and how far float32's evaluation may be from it: exp to 2 units of 2^-23, the sum, the quotient and the
