@@ -266,8 +266,8 @@ std::vector<Tensor> linear_siblings(const Tensor& x, const std::vector<Tensor>& 
 }
 
 // ---- Microscaled blocks --------------------------------------------------------------------------
-// Codes are uint8 [..., kp / 2] (E2M1) or float8_e4m3fn [..., kp] (E4M3), scales float8_e8m0fnu [..., sp], with
-// kp and sp as in svdq_gfx950.h.  Native operators like the linears: a prompt-sized call is shorter on the
+// Codes are uint8 [..., kp / 2] (E2M1) or float8_e4m3fn [..., kp] (E4M3), scales float8_e8m0fnu [..., sp] (taken as uint8
+// bytes too), with kp and sp as in svdq_gfx950.h.  Native operators like the linears: a prompt-sized call is shorter on the
 // GPU than a Python operator's checks and allocations.
 
 int64_t mx_kp(int64_t k) { return (k + 127) / 128 * 128; }
@@ -322,7 +322,7 @@ struct Mx {
     const auto dt = codes.scalar_type();
     TORCH_CHECK_TYPE(dt == at::kByte || dt == at::kFloat8_e4m3fn, name, " must be uint8 (E2M1) or float8_e4m3fn codes, got ", dt);
     check_tensor(name, codes, dev, dt);
-    check_tensor("their scales", scales, dev, at::kFloat8_e8m0fnu);
+    check_tensor("their scales", scales, dev, scales.scalar_type() == at::kByte ? at::kByte : at::kFloat8_e8m0fnu);
     fmt = dt == at::kByte ? SVDQ_MX_E2M1 : SVDQ_MX_E4M3;
     TORCH_CHECK_VALUE(codes.dim() >= 1, name, " must be [..., K], got ", codes.sizes());
     lead = codes.sizes().vec();

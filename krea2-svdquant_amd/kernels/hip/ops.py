@@ -517,7 +517,7 @@ def linear_siblings(*args) -> list[Tensor]:
 # ---- microscaled (MX) blocks -------------------------------------------------------------------
 # Blocks of 32 consecutive values of a row share an E8M0 scale; elements are E2M1 or E4M3.  Codes are
 # uint8 [..., kp / 2] (E2M1: two per byte, the even column in the low half) or float8_e4m3fn [..., kp], scales
-# float8_e8m0fnu [..., sp]; kp = K rounded up to 128 (zero codes), sp = 16 * ceil(K / 512).
+# float8_e8m0fnu [..., sp] (taken as uint8 bytes too); kp = K rounded up to 128 (zero codes), sp = 16 * ceil(K / 512).
 MX_FORMATS = {"e2m1": lib.SVDQ_MX_E2M1, "fp4": lib.SVDQ_MX_E2M1, "e4m3": lib.SVDQ_MX_E4M3, "fp8": lib.SVDQ_MX_E4M3}
 
 

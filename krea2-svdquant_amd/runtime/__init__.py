@@ -1,3 +1,4 @@
 from .linear import SVDQuantLinear, SVDQuantLoRAAdapter
+from .mx_linear import MXLinear
 
-__all__ = ["SVDQuantLinear", "SVDQuantLoRAAdapter"]
+__all__ = ["MXLinear", "SVDQuantLinear", "SVDQuantLoRAAdapter"]

@@ -32,6 +32,10 @@ the torch ops); the gated residual adds run as ``torch.addcmul`` (on the CPU eve
 the stores of to_gate, ff.up, to_out.0 and ff.down instead.  The linears that read the same input
 (to_q, to_k, to_v, to_gate; ff.gate, ff.up) run their GEMMs as one launch by default
 (``run_grouped``; bit-identical to calling them one after another).
+
+``random(..., linears="mx")`` builds the blocks on ``MXLinear`` layers instead.  Their norms and SwiGLU products then
+come as E4M3 MX blocks (``svdq::rms_norm_modulate_mx``, ``svdq::residual_rms_norm_modulate_mx``,
+``svdq::silu_mul_mx``), one quantised activation for all layers that read it and no bf16 copy of it.
 """
 from __future__ import annotations
 
@@ -47,6 +51,7 @@ from torch import Tensor, nn
 from ..kernels.hip import ops as hip_ops
 from ..quant.state import SVDQuantLinearState
 from .linear import SVDQuantLinear
+from .mx_linear import MXLinear
 from .siblings import run_concurrent, run_grouped
 
 LINEAR_NAMES = ("attn.to_q", "attn.to_k", "attn.to_v", "attn.to_gate", "attn.to_out.0",
@@ -95,6 +100,13 @@ def random_quantized_state(n: int, k: int, *, rank: int = 32, group_size: int = 
         smooth_scale=smooth.to(torch.bfloat16), qweight=qweight, weight_scales=scales.to(torch.float16),
         l1=(randn(n, rank) * 0.05).to(torch.bfloat16), l2=(randn(rank, k) / math.sqrt(k)).to(torch.bfloat16),
         bias=None, group_size=group_size, original_shape=(n, k), qweight_packed=True, padded_in_features=kp)
+
+
+def random_mx_linear(n: int, k: int, *, device: torch.device | str = "cuda", generator: torch.Generator | None = None,
+                     activation: str = "e4m3") -> MXLinear:
+    """A random-init ``MXLinear`` of a N(0, 1 / k) weight."""
+    w = torch.randn(n, k, device=torch.device(device), generator=generator) / math.sqrt(k)
+    return MXLinear.from_dense(w, activation=activation)
 
 
 def rms_norm(x: Tensor, eps: float = 1e-6, weight: Optional[Tensor] = None) -> Tensor:
@@ -235,9 +247,32 @@ class Krea2StandInBlock(nn.Module):
         one after another; all three give bit-identical outputs."""
         mod = self.modulation if modulation is None else modulation
         if fused:
+            if self._on_mx():
+                raise NotImplementedError("MXLinear layers have no fused store ops")
             return self._forward_fused(x, cos, sin, self.linears(), tuple(m.to(x.dtype) for m in mod), siblings)
         x, (g_f, y_f) = self._forward_deferred(x, cos, sin, linear, mod, siblings, None)
         return torch.addcmul(x, g_f, y_f)
+
+    def _on_mx(self) -> bool:
+        return all(isinstance(m, MXLinear) for m in self.linears().values())
+
+    def _forward_mx(self, x: Tensor, cos: Tensor, sin: Tensor, mods: tuple, weights: tuple,
+                    pending: Optional[tuple[Tensor, Tensor]]) -> tuple[Tensor, tuple[Tensor, Tensor]]:
+        """``_forward_deferred`` on ``MXLinear`` layers: the norms and the SwiGLU product leave MX blocks, which all
+        layers behind them read."""
+        shift_a, _, gate_a, shift_f, _, gate_f = mods
+        a, f, eps, fmt = self.attn, self.ff, 1e-6, "e4m3"
+        t = x.shape[0]
+        if pending is None:
+            h = hip_ops.rms_norm_modulate_mx(x, weights[0], shift_a, eps, fmt)
+        else:
+            x, *h = hip_ops.residual_rms_norm_modulate_mx(x, pending[1], pending[0], weights[0], shift_a, eps, fmt)
+        q, k, v = (m.forward_mx(*h).view(t, -1, self.dims.head_dim) for m in (a.to_q, a.to_k, a.to_v))
+        o = attention(head_norm_rope(q, cos, sin), head_norm_rope(k, cos, sin), v)
+        o = a.to_out[0](gate_mul_sigmoid(o, a.to_gate.forward_mx(*h)))
+        x, *h = hip_ops.residual_rms_norm_modulate_mx(x, o, gate_a, weights[1], shift_f, eps, fmt)
+        h = hip_ops.silu_mul_mx(f.gate.forward_mx(*h), f.up.forward_mx(*h), fmt)
+        return x, (gate_f, f.down.forward_mx(*h))
 
     def _norm_weights(self, mod: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tensor]:
         """``1 + scale`` of the two norms, computed once per modulation tensor (storage, version,
@@ -258,6 +293,8 @@ class Krea2StandInBlock(nn.Module):
         d = self.dims
         shift_a, scale_a, gate_a, shift_f, scale_f, gate_f = (m.to(x.dtype) for m in mod)
         w_a, w_f = self._norm_weights(mod, x.dtype)
+        if x.is_cuda and linear is _module_linear and self._on_mx():
+            return self._forward_mx(x, cos, sin, (shift_a, scale_a, gate_a, shift_f, scale_f, gate_f), (w_a, w_f), pending)
         lin = self.linears()
         t = x.shape[0]
 
@@ -347,15 +384,19 @@ class Krea2StandInTransformer(nn.Module):
 
     @classmethod
     def random(cls, dims: Krea2Dims = Krea2Dims(), *, rank: int = 32, group_size: int = 64,
-               backend: str = "hip_gfx950", device: torch.device | str = "cuda", seed: int = 0
-               ) -> "Krea2StandInTransformer":
-        """Random-init model with every quantized linear resident on ``device``."""
+               backend: str = "hip_gfx950", device: torch.device | str = "cuda", seed: int = 0,
+               linears: str = "svdquant") -> "Krea2StandInTransformer":
+        """Random-init model with every quantized linear resident on ``device``: ``linears`` "svdquant"
+        (``SVDQuantLinear`` of ``rank``, ``group_size`` and ``backend``) or "mx" (``MXLinear``)."""
+        if linears not in ("svdquant", "mx"):
+            raise ValueError(f"linears must be 'svdquant' or 'mx', got {linears!r}")
         dev = torch.device(device)
         gen = torch.Generator(device=dev).manual_seed(seed)
         blocks = []
         for _ in range(dims.layers):
-            layers = {name: SVDQuantLinear(random_quantized_state(n, k, rank=rank, group_size=group_size,
-                                                                  device=dev, generator=gen), backend=backend)
+            layers = {name: random_mx_linear(n, k, device=dev, generator=gen) if linears == "mx" else
+                      SVDQuantLinear(random_quantized_state(n, k, rank=rank, group_size=group_size,
+                                                            device=dev, generator=gen), backend=backend)
                       for name, (n, k) in dims.linear_shapes().items()}
             mod = torch.randn(6, dims.hidden, device=dev, generator=gen) * 0.1
             mod[2] = mod[2].abs() + 0.2   # attention gate

@@ -398,6 +398,56 @@ def test_streams_and_graphs(dev):
             assert torch.equal(out, eager)
 
 
+@pytest.mark.parametrize("activation", FMTS)
+def test_module(dev, activation):
+    from krea2_svdquant_amd import MXLinear
+    dense = _act(dev, 200, 300, seed=1, dtype=torch.float32) * 0.05
+    bias = _act(dev, 200, seed=2)
+    layer = MXLinear.from_dense(dense, bias, activation=activation)
+    x = _act(dev, 5, 7, 300, seed=3)
+    y = layer(x)
+    assert torch.equal(y, ops.mx_linear(x, *quantize_mx(dense), bias, activation))
+    assert torch.equal(y, layer.forward_mx(*layer.quantize(x)))
+    assert torch.equal(layer.dense_weight(), torch.from_numpy(values(*quantize_mx(dense))[:, :300]).float().to(dev))
+    moved = MXLinear.from_dense(torch.zeros_like(dense), torch.zeros_like(bias), activation=activation)
+    moved.load_state_dict(layer.cpu().state_dict())
+    assert torch.equal(moved.to(dev, torch.bfloat16)(x), y)   # byte buffers do not change type
+    with pytest.raises(ValueError, match="300"):
+        moved(x[..., :299])
+
+
+def test_block_on_mx_layers(dev):
+    from krea2_svdquant_amd.runtime import krea2_standin as ks
+    dims = ks.Krea2Dims(layers=2, hidden=256, heads=2, kv_heads=1, head_dim=128, mlp=520)
+    model = ks.Krea2StandInTransformer.random(dims, linears="mx", device=dev, seed=5)
+    x = _act(dev, 70, 256, seed=1)
+    cos, sin = ks.rope_tables(70, 128, dev, torch.bfloat16)
+    t, pending = x, None
+    for blk in model.transformer_blocks:   # the block's operators one by one
+        shift_a, scale_a, gate_a, shift_f, scale_f, gate_f = blk.modulation
+        lin = blk.linears()
+        if pending is None:
+            a = ops.rms_norm_modulate_mx(t, 1 + scale_a, shift_a, EPS, "e4m3")
+        else:
+            t, *a = ops.residual_rms_norm_modulate_mx(t, pending[1], pending[0], 1 + scale_a, shift_a, EPS, "e4m3")
+        q, k, v, g = (lin[f"attn.to_{n}"].forward_mx(*a) for n in ("q", "k", "v", "gate"))
+        q, k, v = (z.view(70, -1, 128) for z in (q, k, v))
+        o = ks.attention(ks.head_norm_rope(q, cos, sin), ks.head_norm_rope(k, cos, sin), v)
+        o = lin["attn.to_out.0"](ks.gate_mul_sigmoid(o, g))
+        t, *a = ops.residual_rms_norm_modulate_mx(t, o, gate_a, 1 + scale_f, shift_f, EPS, "e4m3")
+        f = ops.silu_mul_mx(lin["ff.gate"].forward_mx(*a), lin["ff.up"].forward_mx(*a), "e4m3")
+        pending = gate_f, lin["ff.down"].forward_mx(*f)
+    want = torch.addcmul(t, *pending)
+    assert want.isfinite().all()
+    assert torch.equal(model(x), want)
+    # the linears alone replaced: the norms and products are rounded to bf16 ahead of their quantising
+    calls = []
+    model(x, linear=lambda name, mod, z: calls.append(name) or mod(z))
+    assert len(calls) == 16
+    with pytest.raises(NotImplementedError):
+        model(x, fused=True)
+
+
 def test_refusals(dev):
     x = _act(dev, 4, 256)
     codes, scales = ops.mx_quantize(x)
@@ -415,7 +465,7 @@ def test_refusals(dev):
     with pytest.raises(TypeError):
         ops.mx_dequantize(codes.int(), scales, 256)
     with pytest.raises(TypeError):
-        ops.mx_dequantize(codes, scales.view(torch.uint8), 256)
+        ops.mx_dequantize(codes, scales.float(), 256)
     with pytest.raises(ValueError, match="contiguous"):
         ops.mx_dequantize(codes[:, ::2], scales, 128)
     with pytest.raises(TypeError):   # an 8-bit weight

@@ -156,3 +156,26 @@ def test_c_entries_take_no_rows():
     lib.call("svdq_rms_norm_modulate_mx", None, 64, None, None, 0, 64, zero, 0, None, None, None)
     lib.call("svdq_residual_rms_norm_modulate_mx", None, 64, None, 64, None, None, None, 0, 64, zero, 0, None, 64, None,
              None, None)
+
+
+def test_module_on_the_cpu():
+    from krea2_svdquant_amd import MXLinear
+    w = torch.randn(6, 40)
+    layer = MXLinear.from_dense(w, torch.zeros(6))
+    assert layer.weight_codes.shape == (6, 64) and layer.weight_scales.dtype == torch.uint8 and layer.bias.dtype == torch.bfloat16
+    assert torch.equal(layer.dense_weight(), dequantize_mx(*quantize_mx(w), 40))
+    assert set(layer.state_dict()) == {"weight_codes", "weight_scales", "bias"}
+    with pytest.raises(RuntimeError, match="GPU"):
+        layer(torch.zeros(2, 40, dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        layer(torch.zeros(2, 41, dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        MXLinear.from_dense(w, activation="int8")
+    with pytest.raises(ValueError):
+        MXLinear(layer.weight_codes, layer.weight_scales, in_features=200)
+    with pytest.raises(ValueError):
+        MXLinear(layer.weight_codes, layer.weight_scales[:, :8], in_features=40)
+    with pytest.raises(ValueError):
+        MXLinear(layer.weight_codes, layer.weight_scales, torch.zeros(5), in_features=40)
+    with pytest.raises(ValueError):
+        MXLinear.from_dense(w[0])
