@@ -39,7 +39,7 @@ __device__ __forceinline__ void load8(const uint16_t* __restrict__ row, int c, i
 // silu(g) u = g u / (1 + exp(-g)) in float32.  exp(-g) = 2^t, t = -g log2(e) as the rounded product t0 and what it and the
 // rounded constant leave, 2^t = 2^t0 (1 + ln(2) (t - t0)), within 1.5 units of 2^-23; the reciprocal of 1 + exp(-g) by
 // v_rcp_f32 and one Newton step; g u is exact, so the result rounds once more.  Few instructions, because the pass is close to being bound by them: with expf and the correctly rounded
-// quotient M = 4352, K = 16384, E4M3 took 74.9 us, so SILU_AFTER.  Beyond |g| = 87 the exponent is held there: 1 + exp(-g)
+// quotient M = 4352, K = 16384, E4M3 took 74.9 us, so 63.3.  Beyond |g| = 87 the exponent is held there: 1 + exp(-g)
 // is 1 above, and below the product's magnitude is under 2^-118 |u|, taken as 0 (so is g = -infinity's).
 __device__ __forceinline__ float silu_mul(float g, float u) {
   const float c = __builtin_amdgcn_fmed3f(g, -87.0f, 87.0f);
@@ -267,9 +267,10 @@ hipError_t quantize(const uint16_t* x, long ldx, const uint16_t* u, long ldu, lo
   const uintptr_t at = reinterpret_cast<uintptr_t>(x) | (GATE ? reinterpret_cast<uintptr_t>(u) : 0);
   const bool vec = at % 16 == 0 && ldx % 8 == 0 && (!GATE || ldu % 8 == 0) && K % 8 == 0;
   const long units = M * (mx_sp(K) / 16);
-  // units: M = 4352, K = 6144 and 16384, E4M3, UNITS = 1 / 2 / 4: quantising 14.8 13.9 14.8 and 40.6 35.3 38.8 us, the
-  // SwiGLU product 21.4 23.9 - and 62.0 66.1 -
-  return quantize_by<FMT, GATE, GATE ? 1 : 2>(vec, x, ldx, u, ldu, units, K, codes, scales, st);
+  // Two units a wave where there are waves enough: M = 4352, K = 6144 and 16384, E4M3, 1 / 2 / 4 units: quantising 14.8 13.9
+  // 14.8 and 40.6 35.3 38.8 us, the SwiGLU product 21.4 23.9 - and 62.0 66.1 -.
+  if (!GATE && units >= 16384) return quantize_by<FMT, GATE, 2>(vec, x, ldx, u, ldu, units, K, codes, scales, st);
+  return quantize_by<FMT, GATE, 1>(vec, x, ldx, u, ldu, units, K, codes, scales, st);
 }
 
 template <int FMT, bool RES, class... A>
@@ -300,16 +301,23 @@ hipError_t launch_silu_mul_mx(const uint16_t* g, long ldg, const uint16_t* u, lo
                         : quantize<MX_E2M1, true>(g, ldg, u, ldu, M, K, codes, scales, st);
 }
 
-template <int FMT>
-static hipError_t dequantize(const uint8_t* codes, const uint8_t* scales, long M, int K, uint16_t* y, hipStream_t st) {
-  constexpr int UNITS = 2;
-  const long units = M * (mx_sp(K) / 16), blocks = (units + 4 * UNITS - 1) / (4 * UNITS);
+template <int FMT, int UNITS>
+static hipError_t dequantize_by(const uint8_t* codes, const uint8_t* scales, long units, int K, uint16_t* y,
+                                hipStream_t st) {
+  const long blocks = (units + 4 * UNITS - 1) / (4 * UNITS);
   if (blocks > INT32_MAX) return hipErrorInvalidValue;
   if (K % 8 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0)
     mx_dequantize_kernel<FMT, true, UNITS><<<(unsigned)blocks, 256, 0, st>>>(codes, scales, units, K, y);
   else
     mx_dequantize_kernel<FMT, false, UNITS><<<(unsigned)blocks, 256, 0, st>>>(codes, scales, units, K, y);
   return hipGetLastError();
+}
+
+template <int FMT>
+static hipError_t dequantize(const uint8_t* codes, const uint8_t* scales, long M, int K, uint16_t* y, hipStream_t st) {
+  const long units = M * (mx_sp(K) / 16);
+  return units >= 16384 ? dequantize_by<FMT, 2>(codes, scales, units, K, y, st)
+                        : dequantize_by<FMT, 1>(codes, scales, units, K, y, st);
 }
 
 hipError_t launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, long M, int K, int fmt, uint16_t* y,

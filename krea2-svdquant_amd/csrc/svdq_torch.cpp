@@ -294,7 +294,7 @@ struct Rows {
     m = 1;
     for (int64_t d : lead) m *= d;
     TORCH_CHECK_VALUE(m <= INT32_MAX && k <= 1 << 30, name, ": ", m, " rows of ", k, " columns are too many");
-    t = x.reshape({m, k});
+    t = x.dim() == 2 ? x : x.reshape({m, k});
     if (t.stride(1) != 1 && k > 1) t = t.contiguous();
     ld = m > 1 ? t.stride(0) : k;
     if (ld < k || (aligned && (ld % 8 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16))) {

@@ -36,7 +36,7 @@ def _check_quantized(x, fmt):
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("m,k", [(1, 1), (1, 8), (3, 31), (2, 32), (5, 33), (7, 127), (4, 128), (3, 136), (2, 511),
-                                 (2, 512), (3, 520), (33, 1000), (1, 6144), (65, 1187), (3, 16384)])
+                                 (2, 512), (3, 520), (33, 1000), (1, 6144), (65, 1187), (3, 16384), (17000, 40), (16999, 41)])
 def test_quantize(dev, fmt, m, k):
     _check_quantized(_act(dev, m, k, seed=k), fmt)
 
@@ -313,7 +313,7 @@ def _silu64(g, u):
 
 
 @pytest.mark.parametrize("fmt", FMTS)
-@pytest.mark.parametrize("m,k", [(1, 1), (3, 31), (2, 32), (3, 130), (7, 1000), (2, 1187), (5, 6144), (2, 16384)])
+@pytest.mark.parametrize("m,k", [(1, 1), (3, 31), (2, 32), (3, 130), (7, 1000), (2, 1187), (5, 6144), (2, 16384), (16999, 41)])
 def test_silu(dev, fmt, m, k):
     g, u = _act(dev, m, k, seed=1) * 3, _act(dev, m, k, seed=2)
     codes, scales = ops.silu_mul_mx(g, u, fmt)

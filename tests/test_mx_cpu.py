@@ -179,3 +179,16 @@ def test_module_on_the_cpu():
         MXLinear(layer.weight_codes, layer.weight_scales, torch.zeros(5), in_features=40)
     with pytest.raises(ValueError):
         MXLinear.from_dense(w[0])
+
+
+@pytest.mark.skipif(not lib.LIB_PATH.exists(), reason="library not built")
+def test_kernels_stay_in_registers():
+    from tests.test_kernel_resources import _kernel_metadata
+    meta = {k: v["private_segment_fixed_size"] for k, v in _kernel_metadata().items() if "mx_" in k or "_mx_" in k}
+    names = ("mx_quantize_kernel", "mx_dequantize_kernel", "rms_norm_mx_kernel", "mx_gemm_rows_kernel")
+    for name in names:
+        assert any(name in k for k in meta), name
+        assert all(v == 0 for k, v in meta.items() if name in k), name
+    # the largest block tiles use all 512 registers and keep a few addresses of their epilogue in scratch
+    tiles = [v for k, v in meta.items() if "mx_gemm_tile_kernel" in k]
+    assert len(tiles) >= 16 and max(tiles) <= 32
