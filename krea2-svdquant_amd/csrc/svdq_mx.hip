@@ -36,18 +36,48 @@ __device__ __forceinline__ void load8(const uint16_t* __restrict__ row, int c, i
   }
 }
 
-// silu(g) u = g u / (1 + exp(-g)) in float32.  exp(-g) = 2^t, t = -g log2(e) as the rounded product t0 and what it and the
-// rounded constant leave, 2^t = 2^t0 (1 + ln(2) (t - t0)), within 1.5 units of 2^-23; the reciprocal of 1 + exp(-g) by
-// v_rcp_f32 and one Newton step; g u is exact, so the result rounds once more.  Few instructions, because the pass is close to being bound by them: with expf and the correctly rounded
-// quotient M = 4352, K = 16384, E4M3 took 74.9 us, so 63.3.  Beyond |g| = 87 the exponent is held there: 1 + exp(-g)
-// is 1 above, and below the product's magnitude is under 2^-118 |u|, taken as 0 (so is g = -infinity's).
-__device__ __forceinline__ float silu_mul(float g, float u) {
+// silu(g) u = g u / (1 + exp(-g)) in float32 for g >= -87.  exp(-g) = 2^t, t = -g log2(e) as the rounded product t0 and
+// what it and the rounded constant leave, 2^t = 2^t0 (1 + ln(2) (t - t0)), within 1.5 units of 2^-23; the reciprocal of
+// 1 + exp(-g) by v_rcp_f32 and one Newton step; g u is exact unless it overflows, so the result rounds once more.  Few
+// instructions, because the pass is close to being bound by them: with expf and the correctly rounded quotient M = 4352,
+// K = 16384, E4M3 took 74.9 us, so 63.3.  Above g = 87 the exponent is held there: 1 + exp(-g) is 1.
+__device__ __forceinline__ float silu_factor(float g) {   // 1 / (1 + exp(-g))
   const float c = __builtin_amdgcn_fmed3f(g, -87.0f, 87.0f);
   const float t0 = c * -1.44269502f;
   const float rest = __builtin_fmaf(c, -1.92596303e-8f, __builtin_fmaf(c, -1.44269502f, -t0));
   const float e0 = __builtin_amdgcn_exp2f(t0), e = __builtin_fmaf(e0, 0.693147181f * rest, e0);
-  const float d = 1.0f + e, r = __builtin_amdgcn_rcpf(d), r1 = __builtin_fmaf(r, __builtin_fmaf(-d, r, 1.0f), r);
-  return (g < -87.0f ? 0.0f : g) * u * r1;
+  const float d = 1.0f + e, r = __builtin_amdgcn_rcpf(d);
+  return __builtin_fmaf(r, __builtin_fmaf(-d, r, 1.0f), r);
+}
+
+// The same product for every g and u, by way of u's exponent: u = m 2^x, g m is of ordinary size.  Below g = -87,
+// 1 / (1 + exp(-g)) is exp(g) to 2^-125 = 2^t0 as above, t0 = n + f with the whole n into the exponent; below -10000 the result is
+// 0 as there.
+__device__ __forceinline__ float silu_mul_any(float g, float u) {
+  const float m = __builtin_amdgcn_frexp_mantf(u);
+  const int x = __builtin_amdgcn_frexp_expf(u);
+  const float c = fmaxf(g, -10000.0f), t0 = c * 1.44269502f, n = rintf(t0);
+  const float rest = __builtin_fmaf(c, 1.92596303e-8f, __builtin_fmaf(c, 1.44269502f, -t0));
+  const float e0 = __builtin_amdgcn_exp2f(t0 - n), e = __builtin_fmaf(e0, 0.693147181f * rest, e0);
+  const bool far = g < -87.0f;
+  return ldexpf(g * m * (far ? e : silu_factor(g)), (far ? (int)n : 0) + x);
+}
+
+// v[i] = silu(v[i]) u[i].  The longer way round only where a gate is below -87 or a product left float32's range.
+__device__ __forceinline__ void silu_mul8(float (&v)[8], const float (&u)[8]) {
+  float least = 0.0f, most = 0.0f, y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    y[i] = v[i] * u[i] * silu_factor(v[i]);
+    least = fminf(least, v[i]);
+    most = fmaxf(most, fabsf(y[i]));
+  }
+  if (least < -87.0f || most > 3.40282347e38f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = silu_mul_any(v[i], u[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = y[i];
 }
 
 // A wave takes units of 64 chunks (512 columns: 16 bytes of scales) of one row, UNITS of them at a time, whose loads are
@@ -82,11 +112,7 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const uint16_t* __rest
   for (int i = 0; i < UNITS; ++i, next())
     if (first + i < units) {
       const int c = 64 * part + lane;
-      if (GATE) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[i][k] = VEC ? 8 * c < K ? silu_mul(v[i][k], w[i][k]) : 0.0f
-                                                  : 8 * c + k < K ? silu_mul(v[i][k], w[i][k]) : 0.0f;
-      }
+      if (GATE) silu_mul8(v[i], w[i]);   // columns beyond K: 0 times 0
       mx_store8<FMT>(v[i], c, kp, codes + row * mx_row_bytes(K, FMT), scales + row * sp);
     }
 }

@@ -338,6 +338,31 @@ def test_silu_layouts_and_extremes(dev, fmt):
     assert torch.equal(y.isnan(), bad)
 
 
+@pytest.mark.parametrize("fmt", FMTS)
+def test_silu_whole_range(dev, fmt):
+    # Gates from -700 to 80 with up of 2^-120 .. 2^127: gate * up passes float32's range where the product does not, and a
+    # far negative gate leaves an ordinary product of a large up.  Relative as in _silu64 (under 8 x 2^-24), and below
+    # float32's normal range half its smallest step, 2^-150, twice (the product's rounding and the last scaling's).
+    g = torch.cat([torch.linspace(-700, -60, 1600), torch.linspace(-100, 80, 1600), torch.linspace(-4, 4, 800)])
+    g = g.to(torch.bfloat16).repeat(8, 1)
+    e = torch.tensor([127, 126, 124, 120, 100, 60, -60, -120], dtype=torch.float64)[:, None]
+    u = (2.0 ** e * (1 + torch.arange(4000, dtype=torch.float64) % 128 / 128)).to(torch.bfloat16)
+    u[:, 1::2] *= -1
+    with np.errstate(over="ignore"):
+        y = f64(g) / (1 + np.exp(-f64(g))) * f64(u)
+    inside = np.abs(y) < 2.0 ** 128 * (1 - 2.0 ** -20)   # what float32 holds; elsewhere a gate of zero stands instead
+    g, y = g.masked_fill(~torch.from_numpy(inside), 0.0), np.where(inside, y, 0.0)
+    codes, scales = ops.silu_mul_mx(g.to(dev), u.to(dev), fmt)
+    check_blocks(codes, scales, y, 8 * 2.0 ** -24 * np.abs(y) + 2.0 ** -149)
+    # an infinite gate gives no number, like the formula
+    x = torch.ones(1, 64, device=dev, dtype=torch.bfloat16)
+    for at in (-float("inf"), float("inf")):
+        bad = x.clone()
+        bad[0, 3] = at
+        out = ops.mx_dequantize(*ops.silu_mul_mx(bad, x, fmt), 64)
+        assert out[:, :32].isnan().all() and out[:, 32:].isfinite().all()
+
+
 # ---- together ----
 def _ff_weights(dev, h, f):
     return {name: quantize_mx(_act(dev, n, k, seed=i, dtype=torch.float32) * 0.05)
