@@ -58,11 +58,16 @@ __device__ __forceinline__ u32x2 mx_encode8(const float (&v)[8], uint32_t s) {
   return s == 255u ? u32x2{0, 0} : o;
 }
 
-// The largest magnitude (float32 bits) of eight values, then of the four lanes 4 i .. 4 i + 3 that hold a block.
-__device__ __forceinline__ uint32_t mx_block_top(const float (&v)[8]) {
+// The largest magnitude (float32 bits; a NaN's pass infinity's) of eight values.
+__device__ __forceinline__ uint32_t mx_chunk_top(const float (&v)[8]) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  return top;
+}
+
+// The largest of the four lanes 4 i .. 4 i + 3 that hold a block.
+__device__ __forceinline__ uint32_t mx_block_top(uint32_t top) {
   // quad_perm [1, 0, 3, 2], then [2, 3, 0, 1]
   top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0xB1, 0xF, 0xF, true));
   top = max(top, (uint32_t)__builtin_amdgcn_mov_dpp((int)top, 0x4E, 0xF, 0xF, true));
@@ -70,11 +75,11 @@ __device__ __forceinline__ uint32_t mx_block_top(const float (&v)[8]) {
 }
 
 // Chunk c (eight columns from 8 c) of a row into MX blocks: the four lanes of a block call it together.
-// Chunks beyond kp write only their share of the scales' padding (v is zero there).  PAST: E4M3 codes past the L2.
+// top: mx_chunk_top(v).  Chunks beyond kp write only their share of the scales' padding (v is zero there).  PAST: E4M3 codes past the L2.
 template <int FMT, bool PAST = false>
-__device__ __forceinline__ void mx_store8(const float (&v)[8], int c, int kp, uint8_t* __restrict__ codes,
+__device__ __forceinline__ void mx_store8(const float (&v)[8], uint32_t top, int c, int kp, uint8_t* __restrict__ codes,
                                           uint8_t* __restrict__ scales) {
-  const uint32_t s = mx_scale_byte<FMT>(mx_block_top(v));
+  const uint32_t s = mx_scale_byte<FMT>(mx_block_top(top));
   const u32x2 o = mx_encode8<FMT>(v, s);
   if (8 * c < kp) {
     if (FMT == MX_E2M1) *reinterpret_cast<uint32_t*>(codes + 4 * c) = o[0];

@@ -40,7 +40,7 @@ __device__ __forceinline__ void load8(const uint16_t* __restrict__ row, int c, i
 // what it and the rounded constant leave, 2^t = 2^t0 (1 + ln(2) (t - t0)), within 1.5 units of 2^-23; the reciprocal of
 // 1 + exp(-g) by v_rcp_f32 and one Newton step; g u is exact unless it overflows, so the result rounds once more.  Few
 // instructions, because the pass is close to being bound by them: with expf and the correctly rounded quotient M = 4352,
-// K = 16384, E4M3 took 74.9 us, so 63.3.  Above g = 87 the exponent is held there: 1 + exp(-g) is 1.
+// K = 16384, E4M3 took 74.9 us, so 65.4 with the check for the range's ends below (62.9 without).  Above g = 87 the exponent is held there: 1 + exp(-g) is 1.
 __device__ __forceinline__ float silu_factor(float g) {   // 1 / (1 + exp(-g))
   const float c = __builtin_amdgcn_fmed3f(g, -87.0f, 87.0f);
   const float t0 = c * -1.44269502f;
@@ -63,21 +63,24 @@ __device__ __forceinline__ float silu_mul_any(float g, float u) {
   return ldexpf(g * m * (far ? e : silu_factor(g)), (far ? (int)n : 0) + x);
 }
 
-// v[i] = silu(v[i]) u[i].  The longer way round only where a gate is below -87 or a product left float32's range.
-__device__ __forceinline__ void silu_mul8(float (&v)[8], const float (&u)[8]) {
-  float least = 0.0f, most = 0.0f, y[8];
+// v[i] = silu(v[i]) u[i]; returns mx_chunk_top(v).  The longer way round only where a gate is below -87 or a product left
+// float32's range.
+__device__ __forceinline__ uint32_t silu_mul8(float (&v)[8], const float (&u)[8]) {
+  float least = 0.0f, y[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     y[i] = v[i] * u[i] * silu_factor(v[i]);
     least = fminf(least, v[i]);
-    most = fmaxf(most, fabsf(y[i]));
   }
-  if (least < -87.0f || most > 3.40282347e38f) {
+  uint32_t top = mx_chunk_top(y);
+  if (__builtin_expect(least < -87.0f || top >= 0x7F800000u, 0)) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = silu_mul_any(v[i], u[i]);
+    top = mx_chunk_top(y);
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = y[i];
+  return top;
 }
 
 // A wave takes units of 64 chunks (512 columns: 16 bytes of scales) of one row, UNITS of them at a time, whose loads are
@@ -112,8 +115,8 @@ __global__ void __launch_bounds__(256) mx_quantize_kernel(const uint16_t* __rest
   for (int i = 0; i < UNITS; ++i, next())
     if (first + i < units) {
       const int c = 64 * part + lane;
-      if (GATE) silu_mul8(v[i], w[i]);   // columns beyond K: 0 times 0
-      mx_store8<FMT>(v[i], c, kp, codes + row * mx_row_bytes(K, FMT), scales + row * sp);
+      const uint32_t top = GATE ? silu_mul8(v[i], w[i]) : mx_chunk_top(v[i]);   // columns beyond K: 0 times 0
+      mx_store8<FMT>(v[i], top, c, kp, codes + row * mx_row_bytes(K, FMT), scales + row * sp);
     }
 }
 
@@ -263,7 +266,7 @@ __global__ void __launch_bounds__(256) rms_norm_mx_kernel(const uint16_t* __rest
         f[i] = __builtin_fmaf(t, r1, __builtin_fmaf(t, r0, sv[i]));
       }
     }
-    mx_store8<FMT, true>(f, c, kp, crow, srow);
+    mx_store8<FMT, true>(f, mx_chunk_top(f), c, kp, crow, srow);
   };
   // 4 sp chunks a row, the scales' padding included; 4 sp % 64 == 0, so a wave's lanes are in or out together
 #pragma unroll
@@ -294,7 +297,7 @@ hipError_t quantize(const uint16_t* x, long ldx, const uint16_t* u, long ldu, lo
   const bool vec = at % 16 == 0 && ldx % 8 == 0 && (!GATE || ldu % 8 == 0) && K % 8 == 0;
   const long units = M * (mx_sp(K) / 16);
   // Two units a wave where there are waves enough: M = 4352, K = 6144 and 16384, E4M3, 1 / 2 / 4 units: quantising 14.8 13.9
-  // 14.8 and 40.6 35.3 38.8 us, the SwiGLU product 21.4 23.9 - and 62.0 66.1 -.
+  // 14.8 and 40.6 35.3 38.8 us, the SwiGLU product (before it looked for the range's ends) 21.4 23.9 - and 62.0 66.1 -.
   if (!GATE && units >= 16384) return quantize_by<FMT, GATE, 2>(vec, x, ldx, u, ldu, units, K, codes, scales, st);
   return quantize_by<FMT, GATE, 1>(vec, x, ldx, u, ldu, units, K, codes, scales, st);
 }
