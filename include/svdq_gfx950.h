@@ -385,7 +385,10 @@ int svdq_attention_fwd_qnorm(const void* q, int64_t ldq, const void* k, const vo
  *
  * Quantising a block: s = max(floor(log2(max |v|)) - E, -127) + 127 with E = 2 (E2M1) or 8 (E4M3);
  * codes are the nearest values to v / 2^(s - 127), ties to even, beyond the largest value (6, 448) to that.
- * A block with an infinity or a NaN gets s = 255 and zero codes; what reads it gets NaN. */
+ * A block with an infinity or a NaN gets s = 255 and zero codes; what reads it gets NaN.
+ *
+ * Rows times units of 512 columns (rounded up) are limited to 2^26 - 1, rows of the norms to 2^24 - 1: more
+ * threads than a launch holds. */
 #define SVDQ_MX_E2M1 0
 #define SVDQ_MX_E4M3 1
 
@@ -400,7 +403,7 @@ int svdq_mx_dequantize(const void* codes, const void* scales, int M, int K, int 
  * their scales, w [N, K] E2M1 codes with theirs, bias [N] bf16 or null.  Sums in float32, one rounding at
  * the store.  E4M3 with bf16 output: within 8 consecutive k the matrix instruction drops what lies below
  * 2^-13 of the largest product (about 1e-5 of a result); with float32 output, and E2M1, nothing is
- * dropped.  K at most 2^22.  M = 0 does nothing. */
+ * dropped.  K at most 2^22, M N / 4096 (each rounded up to 64) under 2^24.  M = 0 does nothing. */
 int svdq_mx_gemm(const void* a, const void* a_scales, int fmt, const void* w, const void* w_scales, const void* bias,
                  int M, int N, int K, void* y, int64_t ldy, int out_f32, hipStream_t stream);
 

@@ -731,8 +731,12 @@ int mx_checks(const char* fn, int M, int K, int fmt, const void* codes, const vo
 
 bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
 
-// one thread per 8 columns, 256 to a workgroup
-bool mx_too_many(int64_t M, int64_t K) { return M * ((K + 511) / 512 * 64) / 256 >= INT32_MAX; }
+// A launch holds less than 2^32 threads; these take a wave per row and 512 columns at most.
+int mx_launch_checks(const char* fn, int64_t M, int64_t K) {
+  if (M * ((K + 511) / 512) * 64 > UINT32_MAX)
+    return fail(SVDQ_ERR_SHAPE, "%s: M=%lld, K=%lld are too many for a launch", fn, (long long)M, (long long)K);
+  return SVDQ_OK;
+}
 
 }  // namespace
 
@@ -742,7 +746,8 @@ int svdq_mx_quantize(const void* x, int64_t ldx, int M, int K, int fmt, void* co
   if (int e = mx_checks("mx_quantize", M, K, fmt, codes, scales)) return e;
   if (M == 0) return ok();
   if (!x) return fail(SVDQ_ERR_ARG, "mx_quantize: null pointer");
-  if (ldx < K || mx_too_many(M, K)) return fail(SVDQ_ERR_SHAPE, "mx_quantize: M=%d, K=%d, ldx=%lld", M, K, (long long)ldx);
+  if (ldx < K) return fail(SVDQ_ERR_SHAPE, "mx_quantize: M=%d, K=%d, ldx=%lld", M, K, (long long)ldx);
+  if (int e = mx_launch_checks("mx_quantize", M, K)) return e;
   if (!aligned2(x)) return fail(SVDQ_ERR_ALIGN, "mx_quantize: x must be 2-byte aligned");
   return launched(svdq::launch_mx_quantize(static_cast<const uint16_t*>(x), ldx, M, K, fmt, static_cast<uint8_t*>(codes),
                                            static_cast<uint8_t*>(scales), stream),
@@ -753,7 +758,7 @@ int svdq_mx_dequantize(const void* codes, const void* scales, int M, int K, int 
   if (int e = mx_checks("mx_dequantize", M, K, fmt, codes, scales)) return e;
   if (M == 0) return ok();
   if (!y) return fail(SVDQ_ERR_ARG, "mx_dequantize: null pointer");
-  if (mx_too_many(M, K)) return fail(SVDQ_ERR_SHAPE, "mx_dequantize: M=%d, K=%d", M, K);
+  if (int e = mx_launch_checks("mx_dequantize", M, K)) return e;
   if (!aligned2(y)) return fail(SVDQ_ERR_ALIGN, "mx_dequantize: y must be 2-byte aligned");
   return launched(svdq::launch_mx_dequantize(static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), M,
                                              K, fmt, static_cast<uint16_t*>(y), stream),
@@ -766,6 +771,8 @@ int svdq_mx_gemm(const void* a, const void* a_scales, int fmt, const void* w, co
   if (N <= 0 || ldy < N) return fail(SVDQ_ERR_SHAPE, "mx_gemm: N=%d, ldy=%lld", N, (long long)ldy);
   if (K > 1 << 22) return fail(SVDQ_ERR_SHAPE, "mx_gemm: K=%d exceeds 2^22 (a tile's offsets are 32 bits)", K);
   if (out_f32 != 0 && out_f32 != 1) return fail(SVDQ_ERR_ARG, "mx_gemm: out_f32=%d", out_f32);
+  if (((int64_t)M + 63) / 64 * (((int64_t)N + 63) / 64) > UINT32_MAX / 256)   // in the smallest tiles
+    return fail(SVDQ_ERR_SHAPE, "mx_gemm: M=%d, N=%d are too many for a launch", M, N);
   if (M == 0) return ok();
   if (!w || !w_scales || !y) return fail(SVDQ_ERR_ARG, "mx_gemm: null pointer");
   if (!aligned16(w) || !aligned16(w_scales))
@@ -801,7 +808,8 @@ int svdq_silu_mul_mx(const void* g, int64_t ldg, const void* u, int64_t ldu, int
   if (int e = mx_checks("silu_mul_mx", M, K, fmt, codes, scales)) return e;
   if (M == 0) return ok();
   if (!g || !u) return fail(SVDQ_ERR_ARG, "silu_mul_mx: null pointer");
-  if (ldg < K || ldu < K || mx_too_many(M, K))
+  if (int e = mx_launch_checks("silu_mul_mx", M, K)) return e;
+  if (ldg < K || ldu < K)
     return fail(SVDQ_ERR_SHAPE, "silu_mul_mx: M=%d, K=%d, ldg=%lld, ldu=%lld", M, K, (long long)ldg, (long long)ldu);
   if (!aligned2(g) || !aligned2(u)) return fail(SVDQ_ERR_ALIGN, "silu_mul_mx: inputs must be 2-byte aligned");
   return launched(svdq::launch_silu_mul_mx(static_cast<const uint16_t*>(g), ldg, static_cast<const uint16_t*>(u), ldu, M,
@@ -817,6 +825,7 @@ int norm_mx_checks(const char* fn, const void* x, int64_t ldx, const void* w, co
                    float eps, int fmt, const void* codes, const void* scales) {
   if (int e = mx_checks(fn, T, H, fmt, codes, scales)) return e;
   if (H % 8) return fail(SVDQ_ERR_SHAPE, "%s: H=%d (H %% 8 == 0)", fn, H);
+  if (T > (int)(UINT32_MAX / 256)) return fail(SVDQ_ERR_SHAPE, "%s: T=%d rows are too many for a launch", fn, T);
   if (!(eps >= 0.0f)) return fail(SVDQ_ERR_ARG, "%s: eps must be >= 0", fn);
   if (T && (!x || !w || !shift)) return fail(SVDQ_ERR_ARG, "%s: null pointer", fn);
   if (ldx < H || ldx % 8 || !aligned16(x) || !aligned16(w) || !aligned16(shift))

@@ -147,6 +147,24 @@ def test_c_entries_refuse_before_any_launch(fn, args, status, needle):
     assert e.value.status == status
 
 
+MANY = 2 ** 24    # a workgroup of 256 threads per row: 2^32 threads
+
+
+@pytest.mark.parametrize("fn,args", [
+    ("svdq_mx_quantize", (P, 8, 2 ** 26, 8, 0, P, P)),                     # a wave of 64 threads per row
+    ("svdq_mx_quantize", (P, 1024, 2 ** 25, 1024, 1, P, P)),
+    ("svdq_mx_dequantize", (P, P, 2 ** 26, 8, 0, P)),
+    ("svdq_silu_mul_mx", (P, 8, P, 8, 2 ** 26, 8, 0, P, P)),
+    ("svdq_rms_norm_modulate_mx", (P, 8, P, P, MANY, 8, ctypes.c_float(0), 0, P, P)),
+    ("svdq_residual_rms_norm_modulate_mx", (P, 8, P, 8, P, P, P, MANY, 8, ctypes.c_float(0), 0, P, 8, P, P)),
+    ("svdq_mx_gemm", (P, P, 0, P, P, None, 2 ** 30, 2 ** 14, 64, P, 2 ** 14, 0)),
+])
+def test_c_entries_refuse_launches_of_too_many_threads(fn, args):
+    with pytest.raises(lib.SVDQError, match="too many") as e:
+        lib.call(fn, *args, None)
+    assert e.value.status == -2
+
+
 def test_c_entries_take_no_rows():
     zero = ctypes.c_float(0)
     lib.call("svdq_mx_quantize", None, 64, 0, 64, 0, None, None, None)
