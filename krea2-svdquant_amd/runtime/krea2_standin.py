@@ -34,7 +34,7 @@ the stores of to_gate, ff.up, to_out.0 and ff.down instead.  The linears that re
 (``run_grouped``; bit-identical to calling them one after another).
 
 ``random(..., linears="mx")`` builds the blocks on ``MXLinear`` layers instead.  Their norms and SwiGLU products then
-come as E4M3 MX blocks (``svdq::rms_norm_modulate_mx``, ``svdq::residual_rms_norm_modulate_mx``,
+come as MX blocks in the layers' format (E4M3) (``svdq::rms_norm_modulate_mx``, ``svdq::residual_rms_norm_modulate_mx``,
 ``svdq::silu_mul_mx``), one quantised activation for all layers that read it and no bf16 copy of it.
 """
 from __future__ import annotations
@@ -247,31 +247,36 @@ class Krea2StandInBlock(nn.Module):
         one after another; all three give bit-identical outputs."""
         mod = self.modulation if modulation is None else modulation
         if fused:
-            if self._on_mx():
+            if any(isinstance(m, MXLinear) for m in self.linears().values()):
                 raise NotImplementedError("MXLinear layers have no fused store ops")
             return self._forward_fused(x, cos, sin, self.linears(), tuple(m.to(x.dtype) for m in mod), siblings)
         x, (g_f, y_f) = self._forward_deferred(x, cos, sin, linear, mod, siblings, None)
         return torch.addcmul(x, g_f, y_f)
 
     def _on_mx(self) -> bool:
-        return all(isinstance(m, MXLinear) for m in self.linears().values())
+        """All layers are ``MXLinear``, those that read one activation in one format."""
+        a, f = self.attn, self.ff
+        return (all(isinstance(m, MXLinear) for m in self.linears().values())
+                and len({m.activation for m in (a.to_q, a.to_k, a.to_v, a.to_gate)}) == 1
+                and f.gate.activation == f.up.activation)
 
     def _forward_mx(self, x: Tensor, cos: Tensor, sin: Tensor, mods: tuple, weights: tuple,
                     pending: Optional[tuple[Tensor, Tensor]]) -> tuple[Tensor, tuple[Tensor, Tensor]]:
         """``_forward_deferred`` on ``MXLinear`` layers: the norms and the SwiGLU product leave MX blocks, which all
         layers behind them read."""
         shift_a, _, gate_a, shift_f, _, gate_f = mods
-        a, f, eps, fmt = self.attn, self.ff, 1e-6, "e4m3"
+        a, f, eps = self.attn, self.ff, 1e-6
         t = x.shape[0]
         if pending is None:
-            h = hip_ops.rms_norm_modulate_mx(x, weights[0], shift_a, eps, fmt)
+            h = hip_ops.rms_norm_modulate_mx(x, weights[0], shift_a, eps, a.to_q.activation)
         else:
-            x, *h = hip_ops.residual_rms_norm_modulate_mx(x, pending[1], pending[0], weights[0], shift_a, eps, fmt)
+            x, *h = hip_ops.residual_rms_norm_modulate_mx(x, pending[1], pending[0], weights[0], shift_a, eps,
+                                                          a.to_q.activation)
         q, k, v = (m.forward_mx(*h).view(t, -1, self.dims.head_dim) for m in (a.to_q, a.to_k, a.to_v))
         o = attention(head_norm_rope(q, cos, sin), head_norm_rope(k, cos, sin), v)
         o = a.to_out[0](gate_mul_sigmoid(o, a.to_gate.forward_mx(*h)))
-        x, *h = hip_ops.residual_rms_norm_modulate_mx(x, o, gate_a, weights[1], shift_f, eps, fmt)
-        h = hip_ops.silu_mul_mx(f.gate.forward_mx(*h), f.up.forward_mx(*h), fmt)
+        x, *h = hip_ops.residual_rms_norm_modulate_mx(x, o, gate_a, weights[1], shift_f, eps, f.gate.activation)
+        h = hip_ops.silu_mul_mx(f.gate.forward_mx(*h), f.up.forward_mx(*h), f.down.activation)
         return x, (gate_f, f.down.forward_mx(*h))
 
     def _norm_weights(self, mod: Tensor, dtype: torch.dtype) -> tuple[Tensor, Tensor]:

@@ -473,6 +473,36 @@ def test_block_on_mx_layers(dev):
         model(x, fused=True)
 
 
+@pytest.mark.parametrize("kinds", [("e2m1", "e2m1"), ("e2m1", "e4m3")])
+def test_block_keeps_its_layers_formats(dev, kinds):
+    # Zero modulation shifts and scales of one: norms and products of the block in the formats that its layers name, whole
+    # blocks of one format on the operators with MX outputs, siblings of two formats each on its own quantised input.
+    from krea2_svdquant_amd.runtime import krea2_standin as ks
+    dims = ks.Krea2Dims(layers=1, hidden=256, heads=2, kv_heads=1, head_dim=128, mlp=520)
+    model = ks.Krea2StandInTransformer.random(dims, linears="mx", device=dev, seed=5)
+    blk = model.transformer_blocks[0]
+    lin = blk.linears()
+    for i, m in enumerate(lin.values()):
+        m.activation = kinds[i % 2]
+    seen = []
+    hooks = {n: getattr(ops, n) for n in ("mx_linear", "rms_norm_modulate_mx", "residual_rms_norm_modulate_mx", "silu_mul_mx")}
+    try:
+        for n, f in hooks.items():
+            setattr(ops, n, lambda *args, n=n, f=f: seen.append((n, args[-1])) or f(*args))
+        y = model(_act(dev, 70, 256, seed=1))
+    finally:
+        for n, f in hooks.items():
+            setattr(ops, n, f)
+    assert y.isfinite().all()
+    if kinds[0] == kinds[1]:
+        assert {n for n, _ in seen} == set(hooks) and {fmt for _, fmt in seen} == {"e2m1"}
+    else:
+        assert sorted(fmt for n, fmt in seen if n == "mx_linear") == ["e2m1"] * 4 + ["e4m3"] * 4 and len(seen) == 8
+    blk.ff.down = torch.nn.Linear(520, 256, device=dev, dtype=torch.bfloat16)   # some MX layers
+    with pytest.raises(NotImplementedError):
+        model(_act(dev, 70, 256, seed=1), fused=True)
+
+
 def test_refusals(dev):
     x = _act(dev, 4, 256)
     codes, scales = ops.mx_quantize(x)
