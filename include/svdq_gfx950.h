@@ -387,8 +387,8 @@ int svdq_attention_fwd_qnorm(const void* q, int64_t ldq, const void* k, const vo
  * codes are the nearest values to v / 2^(s - 127), ties to even, beyond the largest value (6, 448) to that.
  * A block with an infinity or a NaN gets s = 255 and zero codes; what reads it gets NaN.
  *
- * Rows times units of 512 columns (rounded up) are limited to 2^26 - 1, rows of the norms to 2^24 - 1: more
- * threads than a launch holds. */
+ * Rows times units of 512 columns (rounded up) are limited to 2^26 - 1 (the SwiGLU product 2^26 - 4), rows of the
+ * norms to 2^24 - 1: beyond them are more threads than a launch holds. */
 #define SVDQ_MX_E2M1 0
 #define SVDQ_MX_E4M3 1
 

@@ -731,9 +731,11 @@ int mx_checks(const char* fn, int M, int K, int fmt, const void* codes, const vo
 
 bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
 
-// A launch holds less than 2^32 threads; these take a wave per row and 512 columns at most.
-int mx_launch_checks(const char* fn, int64_t M, int64_t K) {
-  if (M * ((K + 511) / 512) * 64 > UINT32_MAX)
+// A launch holds less than 2^32 threads, in whole workgroups of four waves.  per_wave: the units of 512 columns of a row
+// that a wave takes at these sizes (quantising and reading back 2, the SwiGLU product 1).
+int mx_launch_checks(const char* fn, int64_t M, int64_t K, int per_wave) {
+  const int64_t units = M * ((K + 511) / 512), groups = (units + 4 * per_wave - 1) / (4 * per_wave);
+  if (units * 64 > UINT32_MAX || groups * 256 > UINT32_MAX)
     return fail(SVDQ_ERR_SHAPE, "%s: M=%lld, K=%lld are too many for a launch", fn, (long long)M, (long long)K);
   return SVDQ_OK;
 }
@@ -747,7 +749,7 @@ int svdq_mx_quantize(const void* x, int64_t ldx, int M, int K, int fmt, void* co
   if (M == 0) return ok();
   if (!x) return fail(SVDQ_ERR_ARG, "mx_quantize: null pointer");
   if (ldx < K) return fail(SVDQ_ERR_SHAPE, "mx_quantize: M=%d, K=%d, ldx=%lld", M, K, (long long)ldx);
-  if (int e = mx_launch_checks("mx_quantize", M, K)) return e;
+  if (int e = mx_launch_checks("mx_quantize", M, K, 2)) return e;
   if (!aligned2(x)) return fail(SVDQ_ERR_ALIGN, "mx_quantize: x must be 2-byte aligned");
   return launched(svdq::launch_mx_quantize(static_cast<const uint16_t*>(x), ldx, M, K, fmt, static_cast<uint8_t*>(codes),
                                            static_cast<uint8_t*>(scales), stream),
@@ -758,7 +760,7 @@ int svdq_mx_dequantize(const void* codes, const void* scales, int M, int K, int 
   if (int e = mx_checks("mx_dequantize", M, K, fmt, codes, scales)) return e;
   if (M == 0) return ok();
   if (!y) return fail(SVDQ_ERR_ARG, "mx_dequantize: null pointer");
-  if (int e = mx_launch_checks("mx_dequantize", M, K)) return e;
+  if (int e = mx_launch_checks("mx_dequantize", M, K, 2)) return e;
   if (!aligned2(y)) return fail(SVDQ_ERR_ALIGN, "mx_dequantize: y must be 2-byte aligned");
   return launched(svdq::launch_mx_dequantize(static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), M,
                                              K, fmt, static_cast<uint16_t*>(y), stream),
@@ -808,7 +810,7 @@ int svdq_silu_mul_mx(const void* g, int64_t ldg, const void* u, int64_t ldu, int
   if (int e = mx_checks("silu_mul_mx", M, K, fmt, codes, scales)) return e;
   if (M == 0) return ok();
   if (!g || !u) return fail(SVDQ_ERR_ARG, "silu_mul_mx: null pointer");
-  if (int e = mx_launch_checks("silu_mul_mx", M, K)) return e;
+  if (int e = mx_launch_checks("silu_mul_mx", M, K, 1)) return e;
   if (ldg < K || ldu < K)
     return fail(SVDQ_ERR_SHAPE, "silu_mul_mx: M=%d, K=%d, ldg=%lld, ldu=%lld", M, K, (long long)ldg, (long long)ldu);
   if (!aligned2(g) || !aligned2(u)) return fail(SVDQ_ERR_ALIGN, "silu_mul_mx: inputs must be 2-byte aligned");

@@ -1,0 +1,22 @@
+"""Microscaled operators on the CPU: launches at the end of what a grid holds, calls in place, the layer's bias under
+moves to another type, and when a block takes its operators with microscaled outputs."""
+import ctypes
+
+import pytest
+import torch
+
+from krea2_svdquant_amd import MXLinear
+from krea2_svdquant_amd.kernels.hip import lib
+
+P = ctypes.c_void_p(0x1000)    # never read: the calls below fail on the host
+Q = ctypes.c_void_p(0x2000)
+ZERO = ctypes.c_float(0)
+
+
+@pytest.mark.skipif(not lib.LIB_PATH.exists(), reason="library not built")
+@pytest.mark.parametrize("m,k", [(2 ** 26 - 1, 8), (2 ** 26 - 3, 512), (2 ** 25 - 1, 1024)])
+def test_swiglu_refuses_the_last_partial_workgroup_beyond_a_launch(m, k):
+    # workgroups of 256 threads take four units of 512 columns: 2^24 of them hold 2^32 threads
+    with pytest.raises(lib.SVDQError, match="too many") as e:
+        lib.call("svdq_silu_mul_mx", P, k, P, k, m, k, 0, P, P, None)
+    assert e.value.status == -2
