@@ -194,8 +194,8 @@ __device__ __forceinline__ double wave_sum(double v) {
 //   RES: xo = bf16(x + g v) (one rounding; written, and the row that is normalized), else xo = x
 //   y = xo rsqrt(mean(xo^2) + eps) w + shift, rounded to float32 about once, quantised
 // A value near the middle of two codes takes the other one for an error in its last bits, and the whole row shares its
-// mean: the mean is summed in 64 bits, its root's reciprocal kept as r0 + r1, xo w (with a power of two) is exact, and
-// y = (xo w) r0 + shift + (xo w) r1 by two fused products.
+// mean: the mean is summed in 64 bits, its root's reciprocal kept as r0 + r1, xo w (with a power of two) is exact (but for
+// values under 2^-126 of the row's root mean square), and y = (xo w) r0 + shift + (xo w) r1 by two fused products.
 // Thread t takes chunks t, t + 256, ...: the first NR stay in registers between the passes, those beyond are read
 // again (RES: from xo, written by the same thread).  HBM-bound: 4.03 (E4M3) or 3.53 bytes a value beside x and v.  NR is
 // the row's own count, so that short rows keep few registers, and stores of what is not read again here go past the L2:
@@ -246,9 +246,10 @@ __global__ void __launch_bounds__(256) rms_norm_mx_kernel(const uint16_t* __rest
   if ((tid & 63) == 0) part[tid >> 6] = ss;
   __syncthreads();
   const double mean = (part[0] + part[1] + part[2] + part[3]) / (double)H + (double)eps;
-  // the root's reciprocal as 2^k (r0 + r1): x 2^k w is exact and of ordinary size whatever the row's
+  // The root's reciprocal as 2^k (r0 + r1), so that x 2^k w is of ordinary size whatever the row's.  k within -126 .. 127: rows
+  // of bf16 subnormals without eps have reciprocals up to 2^148, whose rest r0 and r1 take (r0 in [1, 2) otherwise).
   const double root = rsqrt(mean);
-  const float pow2 = fmaxf(__uint_as_float(__float_as_uint((float)root) & 0x7F800000u), 1.17549435e-38f);
+  const float pow2 = fminf(fmaxf(__uint_as_float(__float_as_uint((float)root) & 0x7F800000u), 0x1p-126f), 0x1p127f);
   const double scaled = root / (double)pow2;
   const float r0 = (float)scaled, r1 = (float)(scaled - (double)r0);
   uint8_t* crow = codes + (long)blockIdx.x * mx_row_bytes(H, FMT);

@@ -1,0 +1,43 @@
+"""Microscaled operators at the ends of their ranges: rows of the smallest values, rows longer than a workgroup keeps,
+calls in place, products that drop nothing on every tile, equal bits from every tile, layers that were moved to another
+type, blocks whose layers carry hooks."""
+import numpy as np
+import pytest
+import torch
+
+from krea2_svdquant_amd.kernels.hip import lib, ops
+from oracle import mx
+from tests.mx_util import check_blocks, f64, values
+
+pytestmark = pytest.mark.gpu
+FMTS = list(mx.FORMATS)
+
+
+def _randn(dev, *shape, seed, dtype=torch.bfloat16):
+    return torch.randn(shape, device=dev, generator=torch.Generator(device=dev).manual_seed(seed)).to(dtype)
+
+
+def _norm64(x, w, shift, eps):
+    """y = t + shift, t = x w / root, and how far the kernel may be from it: t is (x w 2^k) (r0 + r1), x w 2^k exact
+    (16 bits) and r0 + r1 the root's reciprocal to 2^-47; two fused products round to float32, 2^-24 of their result
+    each (of y up to 2^-24 of t), or half of 2^-149 below its normal range.  The reference here is off by a few 2^-53
+    of t and shift: taken with the 2^-46 of t."""
+    t = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * w
+    y = t + shift
+    return y, 2.1 * 2.0 ** -24 * np.abs(y) + 2.0 ** -46 * (np.abs(t) + np.abs(shift)) + 2.0 ** -149
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_norm_of_the_smallest_rows(dev, fmt):
+    # without eps the reciprocal root of a row of bf16 subnormals passes float32's range; the normed row does not
+    scale = torch.tensor([2.0 ** -133, 3e-40, 1e-39, 3e-39, 1e-38], device=dev)
+    x = (_randn(dev, 5, 640, seed=1, dtype=torch.float32).clamp(-20, 20) * scale[:, None]).to(torch.bfloat16)
+    x[0] = 0
+    x[0, 77] = 2.0 ** -133   # the smallest bf16 alone
+    assert (x != 0).any(1).all()
+    w, shift = _randn(dev, 640, seed=2), _randn(dev, 640, seed=3)
+    for eps in (0.0, 1e-6):
+        check_blocks(*ops.rms_norm_modulate_mx(x, w, shift, eps, fmt), *_norm64(f64(x), f64(w), f64(shift), eps))
+    # a row of zeros without eps has no direction: NaN, as the formula's 0 / 0
+    codes, scales = ops.rms_norm_modulate_mx(torch.zeros_like(x), w, shift, 0.0, fmt)
+    assert ops.mx_dequantize(codes, scales, 640).isnan().all()
