@@ -859,6 +859,8 @@ int svdq_residual_rms_norm_modulate_mx(const void* x, int64_t ldx, const void* v
   if (T && (!v || !g || !xo)) return fail(SVDQ_ERR_ARG, "%s: null pointer", fn);
   if (ldv < H || ldxo < H || ldv % 8 || ldxo % 8 || !aligned16(v) || !aligned16(g) || !aligned16(xo))
     return fail(SVDQ_ERR_ALIGN, "%s: 16-byte aligned pointers, row strides >= H and multiples of 8", fn);
+  if (xo == x && ldxo != ldx && T > 1)   // a row would be written over another that is not read yet
+    return fail(SVDQ_ERR_SHAPE, "%s: ldx=%lld, ldxo=%lld in place", fn, (long long)ldx, (long long)ldxo);
   if (T == 0) return ok();
   return launched(svdq::launch_rms_norm_mx(static_cast<const uint16_t*>(x), ldx, static_cast<const uint16_t*>(v), ldv,
                                            static_cast<const uint16_t*>(g), static_cast<const uint16_t*>(w),

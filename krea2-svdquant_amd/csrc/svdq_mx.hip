@@ -201,13 +201,14 @@ __device__ __forceinline__ double wave_sum(double v) {
 // the row's own count, so that short rows keep few registers, and stores of what is not read again here go past the L2:
 // M = 4352, H = 6144, E4M3, through the operator 39.7 -> 30.8 us (6.1 TB/s; a copy of 107 MB 11.8 us, from the cache in
 // front of HBM).
+// xo may be x, so neither is restrict: each thread reads a chunk of x before it writes that chunk of xo.
 template <int FMT, int NR, bool RES>
-__global__ void __launch_bounds__(256) rms_norm_mx_kernel(const uint16_t* __restrict__ x, long ldx,
-                                                          const uint16_t* __restrict__ v, long ldv,
-                                                          const uint16_t* __restrict__ g, const uint16_t* __restrict__ w,
+__global__ void __launch_bounds__(256) rms_norm_mx_kernel(const uint16_t* x, long ldx, const uint16_t* __restrict__ v,
+                                                          long ldv, const uint16_t* __restrict__ g,
+                                                          const uint16_t* __restrict__ w,
                                                           const uint16_t* __restrict__ shift, int H, float eps,
-                                                          uint16_t* __restrict__ xo, long ldxo,
-                                                          uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+                                                          uint16_t* xo, long ldxo, uint8_t* __restrict__ codes,
+                                                          uint8_t* __restrict__ scales) {
   __shared__ double part[4];
   const int tid = threadIdx.x, nc = H / 8, kp = (int)mx_kp(H), sp = (int)mx_sp(H);
   const uint16_t* xr = x + (long)blockIdx.x * ldx;

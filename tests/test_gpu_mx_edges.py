@@ -41,3 +41,31 @@ def test_norm_of_the_smallest_rows(dev, fmt):
     # a row of zeros without eps has no direction: NaN, as the formula's 0 / 0
     codes, scales = ops.rms_norm_modulate_mx(torch.zeros_like(x), w, shift, 0.0, fmt)
     assert ops.mx_dequantize(codes, scales, 640).isnan().all()
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m,h", [(3, 6144), (2, 16384), (3, 16392), (2, 20000), (5, 33000)])
+def test_norm_of_long_rows(dev, fmt, m, h):
+    # beyond 16384 values a row's chunks are read again after the mean
+    x, v = _randn(dev, m, h, seed=1), _randn(dev, m, h, seed=2)
+    gate, w, shift = (_randn(dev, h, seed=s) for s in (3, 4, 5))
+    check_blocks(*ops.rms_norm_modulate_mx(x, w, shift, 1e-6, fmt), *_norm64(f64(x), f64(w), f64(shift), 1e-6))
+    xo, codes, scales = ops.residual_rms_norm_modulate_mx(x, v, gate, w, shift, 1e-6, fmt)
+    assert torch.equal(xo, torch.addcmul(x, gate, v))
+    check_blocks(codes, scales, *_norm64(f64(xo), f64(w), f64(shift), 1e-6))
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("m,h,ld", [(1, 8, 8), (70, 512, 520), (300, 6144, 6144), (9, 20000, 20008)])
+def test_norm_in_place(dev, fmt, m, h, ld):
+    buf, v = _randn(dev, m, ld, seed=1), _randn(dev, m, h, seed=2)
+    gate, w, shift = (_randn(dev, h, seed=s) for s in (3, 4, 5))
+    want = ops.residual_rms_norm_modulate_mx(buf[:, :h], v, gate, w, shift, 1e-6, fmt)
+    behind = buf[:, h:].clone()
+    codes, scales = torch.empty_like(want[1]), torch.empty_like(want[2])
+    lib.call("svdq_residual_rms_norm_modulate_mx", buf.data_ptr(), ld, v.data_ptr(), h, gate.data_ptr(), w.data_ptr(),
+             shift.data_ptr(), m, h, 1e-6, ops.MX_FORMATS[fmt], buf.data_ptr(), ld, codes.data_ptr(), scales.data_ptr(),
+             torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(buf[:, :h], want[0]) and torch.equal(buf[:, h:], behind)
+    assert torch.equal(codes.view(torch.uint8), want[1].view(torch.uint8))
+    assert torch.equal(scales.view(torch.uint8), want[2].view(torch.uint8))

@@ -20,3 +20,12 @@ def test_swiglu_refuses_the_last_partial_workgroup_beyond_a_launch(m, k):
     with pytest.raises(lib.SVDQError, match="too many") as e:
         lib.call("svdq_silu_mul_mx", P, k, P, k, m, k, 0, P, P, None)
     assert e.value.status == -2
+
+
+@pytest.mark.skipif(not lib.LIB_PATH.exists(), reason="library not built")
+def test_norm_refuses_rows_of_another_stride_in_place():
+    # a row would be written over another workgroup's
+    args = lambda xo, ldxo: (P, 64, Q, 64, Q, Q, Q, 2, 64, ZERO, 0, xo, ldxo, Q, Q, None)
+    with pytest.raises(lib.SVDQError, match="ldxo") as e:
+        lib.call("svdq_residual_rms_norm_modulate_mx", *args(P, 72))
+    assert e.value.status == -2
