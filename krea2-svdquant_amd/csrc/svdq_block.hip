@@ -46,14 +46,15 @@ __device__ __forceinline__ u32x4 addcmul8(u32x4 x, u32x4 g, u32x4 v) {
 // 44.2 us (4.84 TB/s; a copy of the same streams 43.4) -> 41.7 with NR = 3 -> 39.7 (5.40 TB/s); through the
 // torch operator 44.4 -> 42.0; T = 16384: 149.6 -> 139.2; T = 128: 3.93 -> 3.70.  No gain:
 // non-temporal loads as well (1101 rows 10.5 -> 12.1), 512 workgroups of several rows each (T = 16384: 144).
+// xo may be x, so neither is restrict: each thread reads a chunk of x before it writes that chunk of xo.
 template <int NR, bool RES = false>
-__global__ void __launch_bounds__(256) rms_norm_modulate_kernel(const uint16_t* __restrict__ x, long ldx,
+__global__ void __launch_bounds__(256) rms_norm_modulate_kernel(const uint16_t* x, long ldx,
                                                                 const uint16_t* __restrict__ w,
                                                                 const uint16_t* __restrict__ shift, int H,
                                                                 float eps, uint16_t* __restrict__ y, long ldy,
                                                                 const uint16_t* __restrict__ v = nullptr,
                                                                 long ldv = 0, const uint16_t* __restrict__ g = nullptr,
-                                                                uint16_t* __restrict__ xo = nullptr, long ldxo = 0) {
+                                                                uint16_t* xo = nullptr, long ldxo = 0) {
   __shared__ float part[4];
   const int tid = threadIdx.x, nc = H / 8;
   const uint16_t* xr = x + (long)blockIdx.x * ldx;

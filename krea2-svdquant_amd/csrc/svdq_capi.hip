@@ -559,6 +559,8 @@ int svdq_residual_rms_norm_modulate(const void* x, int64_t ldx, const void* v, i
       !aligned16(v) || !aligned16(g) || !aligned16(w) || !aligned16(shift) || !aligned16(xo) || !aligned16(y))
     return fail(SVDQ_ERR_ALIGN,
                 "residual_rms_norm_modulate: 16-byte aligned pointers, leading dimensions >= H and multiples of 8");
+  if (xo == x && ldxo != ldx && T > 1)   // a row would be written over another that is not read yet
+    return fail(SVDQ_ERR_SHAPE, "residual_rms_norm_modulate: ldx=%lld, ldxo=%lld in place", (long long)ldx, (long long)ldxo);
   return launched(svdq::launch_residual_rms_norm_modulate(
                       static_cast<const uint16_t*>(x), ldx, static_cast<const uint16_t*>(v), ldv,
                       static_cast<const uint16_t*>(g), static_cast<const uint16_t*>(w),
