@@ -17,8 +17,9 @@ class MXLinear(nn.Module):
     """``y = x w^T + bias`` with ``w`` held as E2M1 MX blocks and ``x`` quantised to ``activation`` MX blocks
     (``"e4m3"`` or ``"e2m1"``) by the call; bf16 in and out, sums in float32.
 
-    Buffers: ``weight_codes`` uint8 [out, kp / 2], ``weight_scales`` uint8 [out, sp] (the E8M0 bytes: a byte buffer
-    stays what it is under ``.to(dtype)``), ``bias`` bf16 [out] or None."""
+    Buffers: ``weight_codes`` uint8 [out, kp / 2], ``weight_scales`` uint8 [out, sp] (the E8M0 bytes), ``bias`` bf16 [out]
+    or None.  All keep their type under ``.to(dtype)``, ``.half()`` and ``.float()``: what the layer computes does not
+    follow the model's type."""
 
     def __init__(self, weight_codes: torch.Tensor, weight_scales: torch.Tensor, bias: torch.Tensor | None = None, *,
                  in_features: int, activation: str = "e4m3"):
@@ -69,6 +70,18 @@ class MXLinear(nn.Module):
         """The layer on MX blocks [..., in] of either format (``quantize``, or the output of
         ``ops.rms_norm_modulate_mx``, ``ops.residual_rms_norm_modulate_mx`` or ``ops.silu_mul_mx``)."""
         return ops.mx_gemm(codes, scales, self.weight_codes, self.weight_scales, self.bias)
+
+    def _apply(self, fn, *args, **kwargs):
+        bias = self.bias
+        super()._apply(fn, *args, **kwargs)
+        if bias is not None and self.bias.dtype != bias.dtype:   # moved, with the values it had
+            self.bias = bias.to(self.bias.device)
+        return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        if self.bias is not None:   # assigned from a checkpoint of another type
+            self.bias = self.bias.to(torch.bfloat16)
 
     def _check(self, x: torch.Tensor) -> None:
         if x.shape[-1] != self.in_features:

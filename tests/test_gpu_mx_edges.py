@@ -69,3 +69,29 @@ def test_norm_in_place(dev, fmt, m, h, ld):
     assert torch.equal(buf[:, :h], want[0]) and torch.equal(buf[:, h:], behind)
     assert torch.equal(codes.view(torch.uint8), want[1].view(torch.uint8))
     assert torch.equal(scales.view(torch.uint8), want[2].view(torch.uint8))
+
+
+# ---- layers ----
+@pytest.mark.parametrize("move", ["float", "half", "double", "bfloat16"])
+def test_layer_after_a_move_to_another_type(dev, move):
+    from krea2_svdquant_amd import MXLinear
+    bias = _randn(dev, 200, seed=2)
+    bias[:3] = torch.tensor([1e6, 1e-9, -3e38], device=dev)   # bf16 values that float16 does not hold
+    layer = MXLinear.from_dense(_randn(dev, 200, 300, seed=1, dtype=torch.float32) * 0.05, bias)
+    x = _randn(dev, 5, 300, seed=3)
+    want = layer(x)
+    getattr(layer, move)()
+    assert torch.equal(layer(x), want)
+    assert torch.equal(layer.forward_mx(*layer.quantize(x)), want)
+
+
+def test_inputs_that_ask_for_gradients(dev):
+    # forward works and gives the same bits; no gradient is defined
+    x, v, w = (_randn(dev, *s, seed=i) for i, s in enumerate(((4, 256), (4, 256), (256,))))
+    codes, scales = ops.mx_quantize(_randn(dev, 40, 256, seed=9))
+    calls = (lambda x: ops.mx_quantize(x), lambda x: ops.mx_quantize(x, "e4m3"), lambda x: (ops.mx_linear(x, codes, scales),),
+             lambda x: ops.silu_mul_mx(x, v), lambda x: ops.rms_norm_modulate_mx(x, w, w, 1e-6),
+             lambda x: ops.residual_rms_norm_modulate_mx(x, v, w, w, w, 1e-6))
+    for call in calls:
+        for got, want in zip(call(x.clone().requires_grad_()), call(x)):
+            assert torch.equal(got.detach().view(torch.uint8), want.view(torch.uint8))

@@ -29,3 +29,21 @@ def test_norm_refuses_rows_of_another_stride_in_place():
     with pytest.raises(lib.SVDQError, match="ldxo") as e:
         lib.call("svdq_residual_rms_norm_modulate_mx", *args(P, 72))
     assert e.value.status == -2
+
+
+@pytest.mark.parametrize("move", [lambda m: m.half(), lambda m: m.float(), lambda m: m.to(torch.float64),
+                                  lambda m: m.half().float().bfloat16(), lambda m: torch.nn.Sequential(m).half()[0]])
+def test_bias_stays_bf16(move):
+    bias = torch.tensor([1e6, 1e-9, -3e38, 0.1, 0, 7]).bfloat16()   # values that float16 does not hold among them
+    layer = MXLinear.from_dense(torch.randn(6, 40), bias)
+    moved = move(layer)
+    assert moved.bias.dtype == torch.bfloat16 and torch.equal(moved.bias, bias)
+    assert moved.weight_codes.dtype == torch.uint8
+    assert moved.to("meta").bias.device.type == "meta" and moved.bias.dtype == torch.bfloat16
+
+
+def test_bias_of_another_type_is_taken_as_bf16():
+    layer = MXLinear.from_dense(torch.randn(6, 40), torch.zeros(6))
+    state = {**layer.state_dict(), "bias": torch.full((6,), 0.3)}
+    layer.load_state_dict(state, assign=True)
+    assert layer.bias.dtype == torch.bfloat16 and torch.equal(layer.bias, torch.full((6,), 0.3).bfloat16())
