@@ -35,7 +35,9 @@ the stores of to_gate, ff.up, to_out.0 and ff.down instead.  The linears that re
 
 ``random(..., linears="mx")`` builds the blocks on ``MXLinear`` layers instead.  Their norms and SwiGLU products then
 come as MX blocks in the layers' format (E4M3) (``svdq::rms_norm_modulate_mx``, ``svdq::residual_rms_norm_modulate_mx``,
-``svdq::silu_mul_mx``), one quantised activation for all layers that read it and no bf16 copy of it.
+``svdq::silu_mul_mx``), one quantised activation for all layers that read it and no bf16 copy of it.  Blocks with other
+layers among them, with subclasses of ``MXLinear``, forward hooks or a replaced ``forward``, or with ``NORMS`` or ``GATES``
+set to "torch", call their layers on bf16 activations, each of which quantises its own.
 """
 from __future__ import annotations
 
@@ -47,6 +49,7 @@ from typing import Callable, Optional
 import torch
 import torch.nn.functional as F
 from torch import Tensor, nn
+from torch.nn.modules import module as _module
 
 from ..kernels.hip import ops as hip_ops
 from ..quant.state import SVDQuantLinearState
@@ -244,7 +247,8 @@ class Krea2StandInBlock(nn.Module):
         same input (to_q, to_k, to_v, to_gate; ff.gate, ff.up): ``"grouped"`` (default) runs their
         GEMMs as one launch (``run_grouped``; with the default ``linear`` only), ``True`` or
         ``"concurrent"`` issues them concurrently on side streams (``run_concurrent``), ``False``
-        one after another; all three give bit-identical outputs."""
+        one after another; all three give bit-identical outputs.  Blocks on ``MXLinear`` layers run those
+        linears one after another on one quantised activation, whatever ``siblings`` says."""
         mod = self.modulation if modulation is None else modulation
         if fused:
             if any(isinstance(m, MXLinear) for m in self.linears().values()):
@@ -254,9 +258,13 @@ class Krea2StandInBlock(nn.Module):
         return torch.addcmul(x, g_f, y_f)
 
     def _on_mx(self) -> bool:
-        """All layers are ``MXLinear``, those that read one activation in one format."""
-        a, f = self.attn, self.ff
-        return (all(isinstance(m, MXLinear) for m in self.linears().values())
+        """All layers are ``MXLinear`` as they come (no subclass, hooks or ``forward`` of their own, which
+        ``forward_mx`` would pass by), those that read one activation in one format, and no torch ops selected."""
+        a, f, layers = self.attn, self.ff, self.linears().values()
+        return (all(type(m) is MXLinear for m in layers)
+                and not any(m._forward_hooks or m._forward_pre_hooks or "forward" in vars(m) for m in layers)
+                and not (_module._global_forward_hooks or _module._global_forward_pre_hooks)
+                and NORMS == "hip" and GATES == "hip"
                 and len({m.activation for m in (a.to_q, a.to_k, a.to_v, a.to_gate)}) == 1
                 and f.gate.activation == f.up.activation)
 

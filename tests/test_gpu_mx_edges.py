@@ -95,3 +95,47 @@ def test_inputs_that_ask_for_gradients(dev):
     for call in calls:
         for got, want in zip(call(x.clone().requires_grad_()), call(x)):
             assert torch.equal(got.detach().view(torch.uint8), want.view(torch.uint8))
+
+
+# ---- blocks ----
+def _block_model(dev):
+    from krea2_svdquant_amd.runtime import krea2_standin as ks
+    dims = ks.Krea2Dims(layers=1, hidden=256, heads=2, kv_heads=1, head_dim=128, mlp=520)
+    return ks, ks.Krea2StandInTransformer.random(dims, linears="mx", device=dev, seed=5), _randn(dev, 70, 256, seed=1)
+
+
+def test_block_runs_the_hooks_of_its_layers(dev):
+    ks, model, x = _block_model(dev)
+    lin = model.transformer_blocks[0].linears()
+    want = model(x)
+    one_by_one = model(x, linear=lambda name, mod, z: mod(z))   # bf16 activations between the layers
+    seen = []
+    handles = [m.register_forward_hook(lambda mod, args, out, n=n: seen.append((n, args[0].dtype, out.shape[-1])))
+               for n, m in lin.items()]
+    assert torch.equal(model(x), one_by_one)
+    assert sorted(seen) == sorted(((n, torch.bfloat16, m.out_features) for n, m in lin.items()), key=lambda t: t[0])
+    for h in handles:
+        h.remove()
+    assert torch.equal(model(x), want)
+    for siblings in ("grouped", "concurrent", True, False):
+        assert torch.equal(model(x, siblings=siblings), want)
+
+
+def test_block_calls_the_forward_of_a_subclass(dev):
+    ks, model, x = _block_model(dev)
+    blk = model.transformer_blocks[0]
+
+    class Doubled(ks.MXLinear):
+        def forward(self, z):
+            return 2 * super().forward(z)
+    up = blk.ff.up
+    blk.ff.up = Doubled(up.weight_codes, up.weight_scales, None, in_features=256, activation=up.activation)
+    want = model(x, linear=lambda name, mod, z: mod(z))
+    assert torch.equal(model(x), want)
+
+
+@pytest.mark.parametrize("switch", ["NORMS", "GATES"])
+def test_block_follows_the_switches(dev, switch, monkeypatch):
+    ks, model, x = _block_model(dev)
+    monkeypatch.setattr(ks, switch, "torch")
+    assert torch.equal(model(x), model(x, linear=lambda name, mod, z: mod(z)))

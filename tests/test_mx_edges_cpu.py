@@ -47,3 +47,37 @@ def test_bias_of_another_type_is_taken_as_bf16():
     state = {**layer.state_dict(), "bias": torch.full((6,), 0.3)}
     layer.load_state_dict(state, assign=True)
     assert layer.bias.dtype == torch.bfloat16 and torch.equal(layer.bias, torch.full((6,), 0.3).bfloat16())
+
+
+def test_block_takes_microscaled_outputs_only_where_nothing_is_passed_by():
+    from krea2_svdquant_amd.runtime import krea2_standin as ks
+    dims = ks.Krea2Dims(layers=1, hidden=64, heads=2, kv_heads=1, head_dim=32, mlp=96)
+    blk = ks.Krea2StandInTransformer.random(dims, linears="mx", device="cpu", seed=5).transformer_blocks[0]
+    assert blk._on_mx()
+    for register in ("register_forward_hook", "register_forward_pre_hook"):
+        for m in blk.linears().values():
+            handle = getattr(m, register)(lambda *args: None)
+            assert not blk._on_mx()
+            handle.remove()
+        handle = getattr(torch.nn.modules.module, register.replace("register_", "register_module_"))(lambda *args: None)
+        assert not blk._on_mx()
+        handle.remove()
+    up = blk.ff.up
+    up.forward = lambda x: x   # replaced on the instance
+    assert not blk._on_mx()
+    del up.forward
+    assert blk._on_mx()
+
+    class Other(MXLinear):
+        pass
+    blk.ff.up = Other(up.weight_codes, up.weight_scales, in_features=64, activation=up.activation)
+    assert not blk._on_mx()
+    blk.ff.up = up
+    for switch in ("NORMS", "GATES"):
+        before = getattr(ks, switch)
+        setattr(ks, switch, "torch")
+        try:
+            assert not blk._on_mx()
+        finally:
+            setattr(ks, switch, before)
+    assert blk._on_mx()
