@@ -139,3 +139,54 @@ def test_block_follows_the_switches(dev, switch, monkeypatch):
     ks, model, x = _block_model(dev)
     monkeypatch.setattr(ks, switch, "torch")
     assert torch.equal(model(x), model(x, linear=lambda name, mod, z: mod(z)))
+
+
+# ---- products ----
+def _narrow(dev, m, k, seed):
+    """bf16 values with magnitudes of 0.026 to 0.99: E4M3 codes of 8 and more under a scale of 2^-9, whose products with
+    E2M1 codes are multiples of 1/2 of at most 2688, so the matrix instruction drops nothing."""
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    x = torch.rand(m, k, device=dev, generator=gen) * 0.964 + 0.026
+    return (x * torch.where(torch.rand(m, k, device=dev, generator=gen) < 0.5, -1.0, 1.0)).to(torch.bfloat16)
+
+
+# rows and columns that each kernel is chosen for, as lib.mx_tile names it
+E4M3_TILES = {(2, 8, 16): (7, 1000), (1, 64, 64): (70, 3000), (1, 64, 128): (250, 6100), (1, 128, 128): (500, 8100),
+              (1, 256, 256): (1990, 8100)}
+
+
+def _check_narrow(dev, tile, m, n, k):
+    assert lib.mx_tile(m, n, k, lib.SVDQ_MX_E4M3) == tile
+    a, b = ops.mx_quantize(_narrow(dev, m, k, 1), "e4m3"), ops.mx_quantize(_randn(dev, n, k, seed=2))
+    assert (a[1].view(torch.uint8)[:, :k // 32] == 127 - 9).all()
+    bias = _randn(dev, n, seed=3)
+    av, bv = (torch.from_numpy(values(*t)).to(dev) for t in (a, b))
+    y, mag = av @ bv.T + bias.double(), av.abs() @ bv.abs().T + bias.double().abs()
+    bound = 1.01 * (av.shape[1] + 1) * 2.0 ** -24 * mag   # as mx_util.product_bound; then one rounding to bf16
+    assert ((ops.mx_gemm(*a, *b, bias).double() - y).abs() <= bound + 2.0 ** -8 * (y.abs() + bound)).all()
+
+
+@pytest.mark.parametrize("k", [128, 384, 1000, 2432])
+@pytest.mark.parametrize("tile", E4M3_TILES)
+def test_every_e4m3_tile_where_nothing_is_dropped(dev, tile, k):
+    _check_narrow(dev, tile, *E4M3_TILES[tile], k)
+
+
+def test_last_rows_on_smaller_e4m3_tiles_where_nothing_is_dropped(dev):
+    _check_narrow(dev, (3, 256, 256), 2200, 8100, 3000)
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("k", [384, 1000, 2432])
+def test_bits_do_not_depend_on_the_tile(dev, fmt, f32, k):
+    # every output sums K in one order, whichever block tile holds it
+    sizes = [(70, 3000), (250, 6100), (500, 8100), (1990, 8100), (2200, 8100)]
+    a, b = ops.mx_quantize(_randn(dev, 2200, k, seed=1), fmt), ops.mx_quantize(_randn(dev, 8100, k, seed=2))
+    bias = _randn(dev, 8100, seed=3)
+    kinds = {lib.mx_tile(m, n, k, ops.MX_FORMATS[fmt]) for m, n in sizes}
+    assert len(kinds) >= 4 and all(kind != 2 for kind, _, _ in kinds)
+    whole = ops.mx_gemm(*a, *b, bias, f32)
+    for m, n in sizes[:-1]:
+        part = ops.mx_gemm(a[0][:m], a[1][:m], b[0][:n], b[1][:n], bias[:n].clone(), f32)
+        assert torch.equal(part, whole[:m, :n])
