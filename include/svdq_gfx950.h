@@ -407,9 +407,10 @@ int svdq_mx_dequantize(const void* codes, const void* scales, int M, int K, int 
 int svdq_mx_gemm(const void* a, const void* a_scales, int fmt, const void* w, const void* w_scales, const void* bias,
                  int M, int N, int K, void* y, int64_t ldy, int out_f32, hipStream_t stream);
 
-/* Block tile (*rows of a by *cols of w; either may be null) of the kernel that svdq_mx_gemm runs for these sizes;
- * returns 1, 2 for the kernel for few rows, 3 where a second launch of smaller tiles takes the last rows, 0 for
- * other arguments.  For callers that report which kernel ran (tests). */
+/* Block tile (*rows of a by *cols of w; either may be null) of the kernel that svdq_mx_gemm runs for these sizes with
+ * bf16 output (E4M3 with float32 output takes 128 rows of the 256); returns 1, 2 for the kernel for few rows, 3 where
+ * a second launch of smaller tiles takes the last rows, 0 for arguments that svdq_mx_gemm refuses.  For callers that
+ * report which kernel ran (tests). */
 int svdq_mx_gemm_tile(int M, int N, int K, int fmt, int* rows, int* cols);
 
 /* The SwiGLU product silu(g) * u of bf16 g, u [M, K] (row strides ldg, ldu) in float32, into MX blocks

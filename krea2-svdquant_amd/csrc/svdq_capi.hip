@@ -733,6 +733,9 @@ int mx_checks(const char* fn, int M, int K, int fmt, const void* codes, const vo
 
 bool aligned2(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1u) == 0; }
 
+// a product's launch in the smallest tiles
+bool mx_gemm_fits(int64_t M, int64_t N) { return (M + 63) / 64 * ((N + 63) / 64) <= UINT32_MAX / 256; }
+
 // A launch holds less than 2^32 threads, in whole workgroups of four waves.  per_wave: the units of 512 columns of a row
 // that a wave takes at these sizes (quantising and reading back 2, the SwiGLU product 1).
 int mx_launch_checks(const char* fn, int64_t M, int64_t K, int per_wave) {
@@ -775,8 +778,7 @@ int svdq_mx_gemm(const void* a, const void* a_scales, int fmt, const void* w, co
   if (N <= 0 || ldy < N) return fail(SVDQ_ERR_SHAPE, "mx_gemm: N=%d, ldy=%lld", N, (long long)ldy);
   if (K > 1 << 22) return fail(SVDQ_ERR_SHAPE, "mx_gemm: K=%d exceeds 2^22 (a tile's offsets are 32 bits)", K);
   if (out_f32 != 0 && out_f32 != 1) return fail(SVDQ_ERR_ARG, "mx_gemm: out_f32=%d", out_f32);
-  if (((int64_t)M + 63) / 64 * (((int64_t)N + 63) / 64) > UINT32_MAX / 256)   // in the smallest tiles
-    return fail(SVDQ_ERR_SHAPE, "mx_gemm: M=%d, N=%d are too many for a launch", M, N);
+  if (!mx_gemm_fits(M, N)) return fail(SVDQ_ERR_SHAPE, "mx_gemm: M=%d, N=%d are too many for a launch", M, N);
   if (M == 0) return ok();
   if (!w || !w_scales || !y) return fail(SVDQ_ERR_ARG, "mx_gemm: null pointer");
   if (!aligned16(w) || !aligned16(w_scales))
@@ -798,7 +800,8 @@ int svdq_mx_gemm(const void* a, const void* a_scales, int fmt, const void* w, co
 }
 
 int svdq_mx_gemm_tile(int M, int N, int K, int fmt, int* rows, int* cols) {
-  if (M <= 0 || N <= 0 || K <= 0 || K > 1 << 22 || (fmt != SVDQ_MX_E2M1 && fmt != SVDQ_MX_E4M3)) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || K > 1 << 22 || (fmt != SVDQ_MX_E2M1 && fmt != SVDQ_MX_E4M3) || !mx_gemm_fits(M, N))
+    return 0;
   int r = 0, c = 0;
   bool split = false;
   const int tile = svdq::mx_gemm_tile(M, N, K, fmt, r, c, split);

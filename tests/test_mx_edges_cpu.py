@@ -81,3 +81,11 @@ def test_block_takes_microscaled_outputs_only_where_nothing_is_passed_by():
         finally:
             setattr(ks, switch, before)
     assert blk._on_mx()
+
+
+@pytest.mark.skipif(not lib.LIB_PATH.exists(), reason="library not built")
+def test_no_tile_is_named_for_a_product_that_is_refused():
+    assert lib.mx_tile(2 ** 30, 2 ** 14, 64, 0)[0] == 0
+    with pytest.raises(lib.SVDQError, match="too many"):
+        lib.call("svdq_mx_gemm", P, P, 0, P, P, None, 2 ** 30, 2 ** 14, 64, P, 2 ** 14, 0, None)
+    assert lib.mx_tile(2 ** 16, 2 ** 14, 64, 0)[0] != 0
