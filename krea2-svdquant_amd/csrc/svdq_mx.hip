@@ -197,10 +197,10 @@ __device__ __forceinline__ double wave_sum(double v) {
 // mean: the mean is summed in 64 bits, its root's reciprocal kept as r0 + r1, xo w (with a power of two) is exact (but for
 // values under 2^-126 of the row's root mean square), and y = (xo w) r0 + shift + (xo w) r1 by two fused products.
 // Thread t takes chunks t, t + 256, ...: the first NR stay in registers between the passes, those beyond are read
-// again (RES: from xo, written by the same thread).  HBM-bound: 4.03 (E4M3) or 3.53 bytes a value beside x and v.  NR is
-// the row's own count, so that short rows keep few registers, and stores of what is not read again here go past the L2:
-// M = 4352, H = 6144, E4M3, through the operator 39.7 -> 30.8 us (6.1 TB/s; a copy of 107 MB 11.8 us, from the cache in
-// front of HBM).
+// again (RES: from xo, written by the same thread).  HBM-bound: RES, 3.03 (E4M3) or 2.53 bytes a value beside x and v.
+// NR is the row's own count, so that short rows keep few registers, and stores of what is not read again here go past
+// the L2: M = 4352, H = 6144, RES, E4M3, on inputs that the cache in front of HBM holds 39.7 -> 30.8 us; on inputs from
+// HBM (eight sets in turn) it takes 39.4 us, 4.8 TB/s.
 // xo may be x, so neither is restrict: each thread reads a chunk of x before it writes that chunk of xo.
 template <int FMT, int NR, bool RES>
 __global__ void __launch_bounds__(256) rms_norm_mx_kernel(const uint16_t* x, long ldx, const uint16_t* __restrict__ v,
@@ -300,6 +300,8 @@ hipError_t quantize(const uint16_t* x, long ldx, const uint16_t* u, long ldu, lo
   const long units = M * (mx_sp(K) / 16);
   // Two units a wave where there are waves enough: M = 4352, K = 6144 and 16384, E4M3, 1 / 2 / 4 units: quantising 14.8 13.9
   // 14.8 and 40.6 35.3 38.8 us, the SwiGLU product (before it looked for the range's ends) 21.4 23.9 - and 62.0 66.1 -.
+  // Between 8000 and 25000 units one and two differ by 3% either way (K = 6144, E2M1, 1 / 2 units: 8196 units 3.54 3.59, 12288
+  // 4.55 4.42, 16392 5.24 5.33, 24576 7.09 7.09, 32772 10.59 10.31, 52224 15.91 14.93; reading back the same).
   if (!GATE && units >= 16384) return quantize_by<FMT, GATE, 2>(vec, x, ldx, u, ldu, units, K, codes, scales, st);
   return quantize_by<FMT, GATE, 1>(vec, x, ldx, u, ldu, units, K, codes, scales, st);
 }

@@ -10,11 +10,12 @@
 //
 // Precision.  E2M1 x E2M1: the instruction's sums over a block are exact.  E4M3 x E2M1: within each group of 8
 // consecutive k it drops what lies below 2^-13 of the largest product's power of two (measured: 2688 + 0.125 is
-// exact, 2688 + 0.0625 is 2688, a ninth k apart it is exact again), about 1.2e-5 of a result in the 2-norm.
-// Under a bf16 output's own 2^-8 that is left so.  With float32 output each E4M3 operand is split by the top bit
-// of its exponent into codes of magnitude 2 and more and codes below 2, and multiplied in two instructions: the
-// products of either half are multiples of 2^-3 up to 2^11, or of 2^-10 up to 2^4, so neither drops anything.
-#include <cstdlib>
+// exact, 2688 + 0.0625 is 2688, a ninth k apart it is exact again): less than 2^-12 of the largest product for each
+// of the other seven.  For normal operands that is about 1.2e-5 of the results in the 2-norm, for a result that its
+// products cancel to it can be any share.  Beside a bf16 output's own half step of 2^-8 that is left so.  With
+// float32 output each E4M3 operand is split by the top bit of its exponent into codes of magnitude 2 and more and
+// codes below 2, and multiplied in two instructions: the products of either half are multiples of 2^-3 up to 2^11, or
+// of 2^-10 up to 2^4, so neither drops anything.
 #include <type_traits>
 #include <utility>
 
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(64 * WM * WN, (MxTile<AF, F32, TM, TN, WM, WN,
   // Step J: its products, with a memory instruction or more behind each: a wave issues in order, and a block of them
   // ahead of the products leaves the matrix unit idle while their queues drain.  The READS reads of the next step go
   // first, so that they are over when they are needed, then ND DMA instructions.  The scales are in dword Q of sa and sw.
-  uint32_t cur = 0, nxt = NB == 1 ? 0 : T::BUF, free_ = (NB - 1) * T::BUF;
+  uint32_t cur = 0, nxt = T::BUF, free_ = (NB - 1) * T::BUF;
   uint32_t ca[TM], cw[TN];
   auto pick = [&](int q) {   // this lane's blocks of a pair of steps are h and 2 + h of dword q: bytes 0 and 2 after the shift
 #pragma unroll
@@ -556,12 +557,16 @@ struct MxChoice {
   int large;   // rows that go to the large tiles ahead of a launch of smaller ones for the others, 0: one launch
 };
 
-// Up to 8 rows of a (16 of E2M1), unless 64 x 64 tiles fill the CUs, run the rows kernel (M = 1, K = 6144: N = 6144 6.7 us
-// E2M1, 6.4 E4M3, the tiles 9.1, 9.9; N = 16384 11.9 and 11.3, the tiles 10.6, 11.2); else the tile that takes least
-// by its rounds.  A last round of large tiles that leaves most CUs idle costs nearly as much as a full one, so the
-// rows behind the whole rounds go to smaller tiles where that is less: M = 4352, N = 16384, K = 6144 is 4 rounds and 64
-// tiles more, 241 us in one launch, 228 with the last 256 rows on 128 x 128 tiles (E4M3 333, 314); M = 3000, N = K =
-// 6144 85, 67.
+// Up to 8 rows of a (16 of E2M1), unless 64 x 64 tiles fill the CUs, run the rows kernel (M = 1, K = 6144, E2M1 and
+// E4M3: N = 1536 3.6 and 3.5 us, the tiles 8.1, 7.2; N = 6144 6.6 and 6.3, the tiles 8.8, 9.4; N = 12288 9.8 and 9.4,
+// the tiles 9.5, 10.2; N = 16384 11.9 and 11.3, the tiles 10.7, 10.9); else the tile that takes least by its rounds.
+// 9 to 16 rows of E4M3 would hold twice the bytes of a in every ring and gain at some sizes only (16 rows, this
+// kernel and the tiles: N = 6144 with K = 1024 4.5 3.8, K = 6144 9.8 9.6, K = 16384 16.8 20.6; K = 6144 with N = 1536
+// 4.7 7.3, N = 12288 14.4 10.6): they take the tiles.  As the last rows of a split the rows kernel counts 10 us (it
+// takes 3.5 to 12.8 up to K = 16384).  A last round of large tiles that leaves most CUs idle costs nearly as much as
+// a full one, so the rows behind the whole rounds go to smaller tiles where that is less: M = 4352, N = 16384, K =
+// 6144 is 4 rounds and 64 tiles more, 241 us in one launch, 228 with the last 256 rows on 128 x 128 tiles (E4M3 333,
+// 314); M = 3000, N = K = 6144 85, 67.
 MxChoice choose(long M, long N, int K, int fmt) {
   const int e8 = fmt == MX_E4M3;
   if (M <= (e8 ? 8 : 16) && N < 64 * 256) return {MX_ROWS, 10.0f, 0};
