@@ -57,6 +57,11 @@ def dequantize_mx(codes: torch.Tensor, scales: torch.Tensor, k: int, dtype: torc
     kp = v.shape[-1]
     if not 0 < k <= kp or -(-k // 128) * 128 != kp:
         raise ValueError(f"k={k} does not pad to the codes' {kp} columns")
+    if scales.element_size() != 1:
+        raise TypeError(f"scales must be float8_e8m0fnu or their bytes, got {scales.dtype}")
+    want = (*codes.shape[:-1], -(-kp // 512) * 16)
+    if tuple(scales.shape) != want:
+        raise ValueError(f"scales must be {want}, got {tuple(scales.shape)}")
     s = scales.view(torch.uint8)[..., :kp // BLOCK].int()
     f = torch.where(s == 255, float("nan"), torch.ldexp(torch.ones((), device=codes.device), s - 127))
     return (v.unflatten(-1, (-1, BLOCK)) * f[..., None]).flatten(-2)[..., :k].to(dtype)

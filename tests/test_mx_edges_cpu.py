@@ -89,3 +89,14 @@ def test_no_tile_is_named_for_a_product_that_is_refused():
     with pytest.raises(lib.SVDQError, match="too many"):
         lib.call("svdq_mx_gemm", P, P, 0, P, P, None, 2 ** 30, 2 ** 14, 64, P, 2 ** 14, 0, None)
     assert lib.mx_tile(2 ** 16, 2 ** 14, 64, 0)[0] != 0
+
+
+def test_converter_refuses_scales_that_are_not_the_codes():
+    from krea2_svdquant_amd.quant.mx import dequantize_mx, quantize_mx
+    codes, scales = quantize_mx(torch.randn(3, 512))
+    with pytest.raises(TypeError, match="scales"):   # four bytes each: their bytes are no scales
+        dequantize_mx(codes, torch.ones(3, 4), 512)
+    for wrong in (scales[:, :1], scales[:1], scales[:2], torch.cat([scales, scales], 1)):   # the first two broadcast
+        with pytest.raises(ValueError, match="scales"):
+            dequantize_mx(codes, wrong, 512)
+    assert torch.equal(dequantize_mx(codes, scales, 512), dequantize_mx(codes, scales.view(torch.uint8), 512))
