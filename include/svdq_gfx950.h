@@ -421,7 +421,7 @@ int svdq_silu_mul_mx(const void* g, int64_t ldg, const void* u, int64_t ldu, int
                      void* scales, hipStream_t stream);
 
 /* svdq_rms_norm_modulate and svdq_residual_rms_norm_modulate with the normed row in MX blocks:
- *   y = x * rsqrt(mean(x^2) + eps) * w + shift   in float32, quantised (not rounded to bf16 first)
+ *   y = x * rsqrt(mean(x^2) + eps) * w + shift   quantised from the exact value (to 2^-46 of its terms)
  * of x, or of xo = bf16(x + g * v), which is stored.  H % 8 == 0, 16-byte aligned pointers and row
  * strides (multiples of 8); xo may equal x, with ldxo = ldx, and overlaps it in no other way. */
 int svdq_rms_norm_modulate_mx(const void* x, int64_t ldx, const void* w, const void* shift, int T, int H, float eps,

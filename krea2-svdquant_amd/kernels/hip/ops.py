@@ -602,7 +602,7 @@ def silu_mul_mx(gate: Tensor, up: Tensor, fmt: str = "e4m3") -> tuple[Tensor, Te
 def rms_norm_modulate_mx(x: Tensor, weight: Tensor, shift: Tensor, eps: float,
                          fmt: str = "e4m3") -> tuple[Tensor, Tensor]:
     """``svdq::rms_norm_modulate_mx``: ``x * rsqrt(mean(x^2) + eps) * weight + shift`` over the last dimension of a
-    bf16 ``x`` [..., H] (H % 8 == 0), in float32, into MX blocks ``(codes, scales)``."""
+    bf16 ``x`` [..., H] (H % 8 == 0) into MX blocks ``(codes, scales)`` of the exact value (to 2^-46 of its terms)."""
     return _mx("rms_norm_modulate_mx", x, x, weight, shift, eps, _mx_fmt(fmt))
 
 

@@ -7,7 +7,7 @@ import torch
 
 from krea2_svdquant_amd.kernels.hip import lib, ops
 from oracle import mx
-from tests.mx_util import check_blocks, f64, values
+from tests.mx_util import check_blocks, f64, to_oracle, values
 
 pytestmark = pytest.mark.gpu
 FMTS = list(mx.FORMATS)
@@ -190,3 +190,28 @@ def test_bits_do_not_depend_on_the_tile(dev, fmt, f32, k):
     for m, n in sizes[:-1]:
         part = ops.mx_gemm(a[0][:m], a[1][:m], b[0][:n], b[1][:n], bias[:n].clone(), f32)
         assert torch.equal(part, whole[:m, :n])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_norm_next_to_the_borders_of_codes(dev, fmt):
+    # shifts in the middle of two codes, at a code and at a power of two (a block's scale), and normed values of 2^-25 to
+    # 2^-38 of them on either side, which float32's sum does not hold: every code and scale is that of the sum itself
+    h = 640
+    x = torch.zeros(8, h, dtype=torch.float64)
+    sign = torch.where(torch.arange(h) % 3 == 0, -1.0, 1.0)
+    for r in range(8):
+        x[r] = sign * (1 if r % 2 else -1) * 2.0 ** (-25 - 2 * (r // 2)) * (1 + torch.arange(h) % 5 / 8)
+        x[r, 32 * r] = 25.0   # the root mean square is about 1
+    shift = torch.tensor([1.25, 1.75, 1.0625, 1.1875, 2.0, 1.0, 0.875, 0.15625, 1.9375, 0.4375, 0.3125, 2.0 ** -9 * 1.5, 1.5,
+                          0.625, -1.25, -2.0, -0.6875], dtype=torch.float64)[torch.arange(h) % 17]
+    shift[::64] *= 4   # blocks with a largest value of other scales
+    x, shift = x.to(torch.bfloat16), shift.to(torch.bfloat16)
+    w = torch.ones(h, dtype=torch.bfloat16)
+    w[::7] = 0.5
+    codes, scales = ops.rms_norm_modulate_mx(x.to(dev), w.to(dev), shift.to(dev), 1e-6, fmt)
+    y, _ = _norm64(f64(x), f64(w), f64(shift), float(np.float32(1e-6)))
+    want_c, want_s = mx.quantize(y, fmt)
+    as_f32 = mx.quantize(y.astype(np.float32).astype(np.float64), fmt)
+    assert (as_f32[0] != want_c).sum() > 100 and (as_f32[1] != want_s).any()   # what float32 alone would give
+    got_c, got_s, _ = to_oracle(codes, scales)
+    assert np.array_equal(got_s, want_s) and np.array_equal(got_c, want_c)
