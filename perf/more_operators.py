@@ -9,8 +9,8 @@
 * ``attend``:  attention over such a cache, for a batch of sequences of their own lengths.
 
 The quantisers' scale is the smallest power of two, 2^-126 at least, under which the largest magnitude is at most 448;
-codes are the nearest values, ties to even.  Rows are padded with zero codes to a multiple of 128 columns, an activation's
-scales with zeros to a multiple of 4.  A page's keys are [64, dim], its values [dim, 64]; a page that holds tokens
+codes are the nearest values, ties to even.  Rows are padded with zero codes to a multiple of 128 columns; an activation's
+scales are [blocks, rows].  A page's keys are [64, dim], its values [dim, 64]; a page that holds tokens
 already keeps its scale unless the new ones need a larger one, and then its older codes are rounded again under that.
 
 Layer sizes are those of the denoiser's linears (hidden 6144, MLP 16384) and of its attention (48 query heads over 12
@@ -126,12 +126,11 @@ def _pow2(amax):
 
 
 def _encode_rows(x):
-    """f32 [M, K] -> E4M3 codes [M, K padded to 128] and f32 scales [M, blocks padded to 4]."""
+    """f32 [M, K] -> E4M3 codes [M, K padded to 128] and f32 scales [blocks, M]."""
     x = torch.nn.functional.pad(x, (0, -x.shape[1] % 128))
     b = x.view(x.shape[0], -1, 128)
     s = _pow2(b.abs().amax(-1))
-    codes = (b / s[..., None]).to(torch.float8_e4m3fn).view(x.shape)
-    return codes, torch.nn.functional.pad(s, (0, -s.shape[1] % 4))
+    return (b / s[..., None]).to(torch.float8_e4m3fn).view(x.shape), s.T.contiguous()
 
 
 def _weight(n, k, gen):
@@ -208,7 +207,7 @@ def prepare(case, seed):
 def _product(a, a_scales, s):
     """The products and sums of a layer in float32, rounded once."""
     kb = a.shape[1] // 128
-    a = (a.float().view(a.shape[0], kb, 128) * a_scales[:, :kb, None]).view(a.shape)
+    a = (a.float().view(a.shape[0], kb, 128) * a_scales.T[..., None]).view(a.shape)
     ws = s["ws"].repeat_interleave(128, 0)[:s["n"]]
     w = (s["w"].float().view(s["n"], kb, 128) * ws[..., None]).view(s["w"].shape)
     y = a @ w.T
@@ -362,7 +361,7 @@ def exact(case, seed):
             scale = _scale64(x.abs().max(-1).values)[..., None]
             a = (_round64(x / scale) * scale).reshape(len(x), -1)
         else:
-            a = (s["a"].double().reshape(-1, kb, 128) * s["as"].double()[:, :kb, None]).reshape(s["a"].shape)
+            a = (s["a"].double().reshape(-1, kb, 128) * s["as"].double().T[..., None]).reshape(s["a"].shape)
         block = torch.arange(case["n"], device="cuda") // 128
         w = (s["w"].double().reshape(-1, kb, 128) * s["ws"].double()[block][..., None]).reshape(s["w"].shape)
         y = torch.cat([part @ w.T for part in a.split(1024)])
