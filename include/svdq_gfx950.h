@@ -430,6 +430,65 @@ int svdq_residual_rms_norm_modulate_mx(const void* x, int64_t ldx, const void* v
                                        const void* w, const void* shift, int T, int H, float eps, int fmt, void* xo,
                                        int64_t ldxo, void* codes, void* scales, hipStream_t stream);
 
+/* ---- 8-bit floating point with a scale per block -------------------------------------------------
+ * E4M3 codes (OCP: largest value 448, 0x7F and 0xFF not a number) and float32 scales, the form of 8-bit checkpoints: an
+ * activation row has a scale for each 128 columns, a weight one for each 128 x 128 block.  No counterpart in the
+ * reference.
+ *
+ * Rows hold kp = K rounded up to 128 codes (zero codes beyond K), contiguous and 16-byte aligned.  Activation scales are
+ * [kp / 128, M] (the M rows' scales of a block side by side), weight scales [ceil(N / 128), kp / 128]. */
+
+/* bf16 x [M, K] (row stride ldx >= K, any alignment; 16-byte aligned rows and K % 8 == 0 run fastest).  A block's scale is
+ * the smallest power of two, 2^-126 at least, under which its largest finite magnitude is at most 448; codes are the
+ * nearest values, ties to even; infinities and NaN become NaN codes.  Rows times units of 512 columns (rounded up) are limited to
+ * 2^26 - 1.  M = 0 does nothing. */
+int svdq_fp8_quantize(const void* x, int64_t ldx, int M, int K, void* codes, float* scales, hipStream_t stream);
+
+/* y [M, ldy] bf16 = a w^T + bias, block by block in float32: each block's sum over its 128 columns is scaled (any float32
+ * scales) and added.  bias [N] bf16 or null.  Within 8 consecutive k the matrix instruction drops what lies below
+ * 2^-13 of the power of two of the largest product.  K at most 2^22, M N / 4096 (each rounded up to 64) under
+ * 2^24.  M = 0 does nothing. */
+int svdq_fp8_gemm(const void* a, const float* a_scales, const void* w, const float* w_scales, const void* bias, int M,
+                  int N, int K, void* y, int64_t ldy, hipStream_t stream);
+
+/* RMS norm of every head of queries and keys with a learned weight, and the position rotation, in one launch:
+ *   n = x * rsqrt(mean(x^2) + eps) * w;   (a, b) -> (a cos - b sin, b cos + a sin)
+ * of the pairs (n[j], n[j + D / 2]) or, with pairs = 1, (n[2 j], n[2 j + 1]), j < D / 2; float32, one rounding to bf16.
+ *   q [T, H, D], k [T, Hkv, D]: strides ldq, ldk of tokens and hsq, hsk of heads in elements (multiples of 8; D dense)
+ *   qw, kw: [D] bf16 or null (1);   cos, sin: [P, ldcs] float32 (wide = 1) or bf16 tables, of which D / 2 columns are read
+ *   at: [T] rows of the tables (a token whose row is not below P gets NaN), or null: row t for token t, P >= T
+ *   qo, ko: contiguous, may not overlap the inputs.  D a multiple of 16 up to 256; pointers and table rows 16-byte aligned. */
+int svdq_qk_norm_rope(const void* q, int64_t ldq, int hsq, const void* k, int64_t ldk, int hsk, const void* qw,
+                      const void* kw, const void* cos, const void* sin, int64_t ldcs, int P, int wide, const int64_t* at,
+                      int T, int H, int Hkv, int D, float eps, int pairs, void* qo, void* ko, hipStream_t stream);
+
+/* ---- The 8-bit cache of keys and values -----------------------------------------------------------
+ * P pages of 64 tokens: k_codes [P, Hkv, 64, D], v_codes [P, Hkv, D, 64] (E4M3), scales [P, Hkv, 2] float32 (of the
+ * page's keys, of its values); D is 64 or 128.  table [B, W]: the page of each 64 tokens of a sequence.  offsets
+ * [B + 1]: sequence b's new tokens are rows offsets[b] .. offsets[b + 1] - 1 of N (ascending; offsets[0] counts as 0).
+ * Everything contiguous, codes 16-byte aligned.  What these arrays hold is not known on the host: values out of range are
+ * held to it, and a page that is not one of the P holds nothing and is not written.  No sequence may share a page that is written. */
+
+/* Puts new keys and values (bf16 [N, Hkv, D], rows ldk, ldv apart, multiples of 8, 16-byte aligned) behind the lengths[b] tokens
+ * that the sequences hold.  A page that begins with new tokens gets their scale (as svdq_fp8_quantize, over the page and
+ * head); one that holds older tokens keeps its scale, or gets theirs where that is larger: the older codes are then
+ * rounded again under it.  Slots behind the new tokens are left as they are, and so are the lengths. */
+int svdq_kv8_append(const void* k, int64_t ldk, const void* v, int64_t ldv, int N, const int* offsets,
+                    const int* lengths, const int* table, int B, int W, void* k_codes, void* v_codes, float* scales,
+                    int P, int Hkv, int D, hipStream_t stream);
+
+/* Attention of q (bf16 [N, H, D], rows ldq apart; H % Hkv == 0) over the lengths[b] tokens that the sequences hold now, the new
+ * ones among them, into o (bf16 [N, H, D], contiguous):
+ *   o = sum_j softmax_j(scale q . k_j) v_j,   j < lengths[b], with causal = 1 and for the i-th of n new tokens also
+ *   j <= lengths[b] - n + i
+ * and 0 for rows that see nothing and rows behind the last sequence.  Scores and softmax in float32, probabilities (times the
+ * page's scale) rounded to bf16.  workspace: svdq_kv8_attention_workspace(...) bytes, 16-byte aligned, no initial
+ * contents, not shared by calls that overlap; may be null where that is 0. */
+int64_t svdq_kv8_attention_workspace(int N, int B, int W, int H, int Hkv, int D);
+int svdq_kv8_attention(const void* q, int64_t ldq, int N, const int* offsets, const int* lengths, const int* table,
+                       int B, int W, const void* k_codes, const void* v_codes, const float* scales, int P, int H, int Hkv,
+                       int D, float scale, int causal, void* o, void* workspace, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,7 +20,7 @@ LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libsvdq_gfx950.so"
 TORCH_LIB_PATH = LIB_DIR / "libsvdq_torch.so"
 SOURCES = ["svdq_act.hip", "svdq_gemm.hip", "svdq_gemm_small.hip", "svdq_w4a16_direct.hip", "svdq_block.hip", "svdq_attn.hip",
-           "svdq_mx.hip", "svdq_mx_gemm.hip", "svdq_capi.hip"]
+           "svdq_mx.hip", "svdq_mx_gemm.hip", "svdq_fp8.hip", "svdq_fp8_gemm.hip", "svdq_kv8.hip", "svdq_capi.hip"]
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [

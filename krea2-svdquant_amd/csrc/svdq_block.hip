@@ -182,7 +182,102 @@ __global__ void __launch_bounds__(256) head_rms_rope_vec_kernel(const uint16_t* 
   *reinterpret_cast<u32x4*>(out + row * 128 + 64 + 8 * j) = o2;
 }
 
+// RMS norm of a head with a learned weight, and the position rotation, of queries and keys in one launch:
+//   n = x rsqrt(mean(x^2) + eps) w,   (a, b) -> (a c - b s, b c + a s)   for pairs (n[j], n[j + D / 2]) or (n[2 j], n[2 j + 1])
+// in float32, rounded once.  L lanes (a power of two, 16 channels each) share a head: lane j holds eight pairs, of which the tables'
+// entries are 8 j .. 8 j + 7 in either order, so every access is 16 bytes.  HBM-bound: one read, one write.
+template <int L, bool WIDE, bool PAIRS>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkNormRopeParams p) {
+  const int heads = p.H + p.Hkv;
+  const long row = (long)blockIdx.x * (256 / L) + threadIdx.x / L;
+  if (row >= (long)p.T * heads) return;   // a row's lanes leave together
+  const int j = threadIdx.x % L;
+  const long tok = row / heads;
+  const int h = (int)(row - tok * heads);
+  const bool isq = h < p.H, live = 16 * j < p.D;
+  const int c0 = PAIRS ? 16 * j : 8 * j, c1 = PAIRS ? 16 * j + 8 : p.D / 2 + 8 * j;
+  const uint16_t* src = isq ? p.q + tok * p.ldq + (long)h * p.hsq : p.k + tok * p.ldk + (long)(h - p.H) * p.hsk;
+  float x[16] = {};
+  auto unpack = [](u32x4 r, float* v) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      v[2 * d] = bf16lo(r[d]);
+      v[2 * d + 1] = bf16hi(r[d]);
+    }
+  };
+  if (live) {
+    unpack(ld16(src + c0), x);
+    unpack(ld16(src + c1), x + 8);
+  }
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
+#pragma unroll
+  for (int off = L / 2; off > 0; off >>= 1) ss += __shfl_xor(ss, off, 64);
+  if (!live) return;
+  const float r = rsqrtf(ss / (float)p.D + p.eps);
+  const uint16_t* wt = isq ? p.qw : p.kw;
+  float w[16];
+  if (wt) {
+    unpack(ld16(wt + c0), w);
+    unpack(ld16(wt + c1), w + 8);
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = wt ? x[i] * r * w[i] : x[i] * r;
+  float c[8], s[8];
+  const long at = p.at ? p.at[tok] : tok;
+  if (at < 0 || at >= p.P) {   // no such position
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = s[i] = __builtin_nanf("");
+  } else if (WIDE) {
+    const f32x4* cs = reinterpret_cast<const f32x4*>(static_cast<const float*>(p.cs) + at * p.ldcs + 8 * j);
+    const f32x4* sn = reinterpret_cast<const f32x4*>(static_cast<const float*>(p.sn) + at * p.ldcs + 8 * j);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      c[i] = cs[i / 4][i % 4];
+      s[i] = sn[i / 4][i % 4];
+    }
+  } else {
+    unpack(ld16(static_cast<const uint16_t*>(p.cs) + at * p.ldcs + 8 * j), c);
+    unpack(ld16(static_cast<const uint16_t*>(p.sn) + at * p.ldcs + 8 * j), s);
+  }
+  float y[16];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int a = PAIRS ? 2 * i : i, b = PAIRS ? 2 * i + 1 : i + 8;
+    y[a] = __builtin_fmaf(x[a], c[i], -x[b] * s[i]);
+    y[b] = __builtin_fmaf(x[b], c[i], x[a] * s[i]);
+  }
+  uint16_t* dst = isq ? p.qo + (tok * p.H + h) * p.D : p.ko + (tok * p.Hkv + h - p.H) * p.D;
+  u32x4 o[2];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i / 4][i % 4] = pack_bf16x2(y[2 * i], y[2 * i + 1]);
+  *reinterpret_cast<u32x4*>(dst + c0) = o[0];
+  *reinterpret_cast<u32x4*>(dst + c1) = o[1];
+}
+
 }  // namespace
+
+template <int L>
+static hipError_t launch_qk(const QkNormRopeParams& p, hipStream_t st) {
+  const unsigned grid = (unsigned)(((long)p.T * (p.H + p.Hkv) + 256 / L - 1) / (256 / L));
+  if (p.wide) {
+    if (p.pairs) qk_norm_rope_kernel<L, true, true><<<grid, 256, 0, st>>>(p);
+    else qk_norm_rope_kernel<L, true, false><<<grid, 256, 0, st>>>(p);
+  } else {
+    if (p.pairs) qk_norm_rope_kernel<L, false, true><<<grid, 256, 0, st>>>(p);
+    else qk_norm_rope_kernel<L, false, false><<<grid, 256, 0, st>>>(p);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_qk_norm_rope(const QkNormRopeParams& p, hipStream_t st) {
+  if (p.D <= 16) return launch_qk<1>(p, st);
+  if (p.D <= 32) return launch_qk<2>(p, st);
+  if (p.D <= 64) return launch_qk<4>(p, st);
+  if (p.D <= 128) return launch_qk<8>(p, st);
+  return launch_qk<16>(p, st);
+}
 
 // rows of up to 4 * 256 chunks (H <= 8192) stay in registers between the passes
 template <bool RES, class... A>

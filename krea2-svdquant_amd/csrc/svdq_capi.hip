@@ -876,3 +876,137 @@ int svdq_residual_rms_norm_modulate_mx(const void* x, int64_t ldx, const void* v
 }
 
 }  // extern "C"
+
+extern "C" {
+
+int svdq_fp8_quantize(const void* x, int64_t ldx, int M, int K, void* codes, float* scales, hipStream_t stream) {
+  if (M < 0 || K <= 0 || K > 1 << 30) return fail(SVDQ_ERR_SHAPE, "fp8_quantize: M=%d, K=%d (0 < K <= 2^30)", M, K);
+  if (M == 0) return ok();
+  if (!x || !codes || !scales) return fail(SVDQ_ERR_ARG, "fp8_quantize: null pointer");
+  if (ldx < K) return fail(SVDQ_ERR_SHAPE, "fp8_quantize: M=%d, K=%d, ldx=%lld", M, K, (long long)ldx);
+  if (int e = mx_launch_checks("fp8_quantize", M, K, 1)) return e;
+  if (!aligned2(x) || !aligned16(codes) || reinterpret_cast<uintptr_t>(scales) % 4)
+    return fail(SVDQ_ERR_ALIGN, "fp8_quantize: codes must be 16-byte aligned, x and scales to their elements");
+  return launched(svdq::launch_fp8_quantize(static_cast<const uint16_t*>(x), ldx, M, K, static_cast<uint8_t*>(codes),
+                                            scales, stream),
+                  "fp8_quantize");
+}
+
+int svdq_fp8_gemm(const void* a, const float* a_scales, const void* w, const float* w_scales, const void* bias, int M,
+                  int N, int K, void* y, int64_t ldy, hipStream_t stream) {
+  if (M < 0 || N <= 0 || K <= 0 || ldy < N)
+    return fail(SVDQ_ERR_SHAPE, "fp8_gemm: M=%d, N=%d, K=%d, ldy=%lld", M, N, K, (long long)ldy);
+  if (K > 1 << 22) return fail(SVDQ_ERR_SHAPE, "fp8_gemm: K=%d exceeds 2^22 (a tile's offsets are 32 bits)", K);
+  if (!mx_gemm_fits(M, N)) return fail(SVDQ_ERR_SHAPE, "fp8_gemm: M=%d, N=%d are too many for a launch", M, N);
+  if (M == 0) return ok();
+  if (!a || !a_scales || !w || !w_scales || !y) return fail(SVDQ_ERR_ARG, "fp8_gemm: null pointer");
+  if (!aligned16(a) || !aligned16(w)) return fail(SVDQ_ERR_ALIGN, "fp8_gemm: codes must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(a_scales) % 4 || reinterpret_cast<uintptr_t>(w_scales) % 4 || !aligned2(bias) ||
+      !aligned2(y))
+    return fail(SVDQ_ERR_ALIGN, "fp8_gemm: scales, bias and y must be aligned to their elements");
+  const svdq::Fp8GemmParams p{static_cast<const uint8_t*>(a), a_scales, static_cast<const uint8_t*>(w), w_scales,
+                              static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(y), ldy, M, N, K};
+  return launched(svdq::launch_fp8_gemm(p, stream), "fp8_gemm");
+}
+
+int svdq_qk_norm_rope(const void* q, int64_t ldq, int hsq, const void* k, int64_t ldk, int hsk, const void* qw,
+                      const void* kw, const void* cos, const void* sin, int64_t ldcs, int P, int wide, const int64_t* at,
+                      int T, int H, int Hkv, int D, float eps, int pairs, void* qo, void* ko, hipStream_t stream) {
+  if (T < 0 || H <= 0 || Hkv <= 0 || D <= 0 || D > 256 || D % 16)
+    return fail(SVDQ_ERR_SHAPE, "qk_norm_rope: T=%d, H=%d, Hkv=%d, D=%d (a multiple of 16 up to 256)", T, H, Hkv, D);
+  if (P <= 0 || ldcs < D / 2 || (!at && P < T))
+    return fail(SVDQ_ERR_SHAPE, "qk_norm_rope: %d table rows, ldcs=%lld for T=%d, D=%d", P, (long long)ldcs, T, D);
+  if ((wide != 0 && wide != 1) || (pairs != 0 && pairs != 1) || !(eps >= 0.0f))
+    return fail(SVDQ_ERR_ARG, "qk_norm_rope: wide=%d, pairs=%d, eps=%g", wide, pairs, eps);
+  if (((int64_t)H + Hkv) * T > (int64_t)(UINT32_MAX / 32))
+    return fail(SVDQ_ERR_SHAPE, "qk_norm_rope: T=%d, H=%d, Hkv=%d are too many for a launch", T, H, Hkv);
+  if (T == 0) return ok();
+  if (!q || !k || !cos || !sin || !qo || !ko) return fail(SVDQ_ERR_ARG, "qk_norm_rope: null pointer");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(qw) || !aligned16(kw) || !aligned16(cos) || !aligned16(sin) ||
+      !aligned16(qo) || !aligned16(ko) || ldq % 8 || ldk % 8 || hsq % 8 || hsk % 8 || ldcs % (wide ? 4 : 8) ||
+      reinterpret_cast<uintptr_t>(at) % 8)
+    return fail(SVDQ_ERR_ALIGN, "qk_norm_rope: 16-byte aligned pointers, strides and table rows");
+  const svdq::QkNormRopeParams p{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), ldq, ldk, hsq, hsk,
+                                 static_cast<const uint16_t*>(qw), static_cast<const uint16_t*>(kw), cos, sin, ldcs, P,
+                                 at, T, H, Hkv, D, eps, wide, pairs, static_cast<uint16_t*>(qo),
+                                 static_cast<uint16_t*>(ko)};
+  return launched(svdq::launch_qk_norm_rope(p, stream), "qk_norm_rope");
+}
+
+}  // extern "C"
+
+namespace {
+
+// what holds for every call on a cache; pointers are looked at where there are rows
+int kv8_checks(const char* fn, int N, const int* offsets, const int* lengths, const int* table, int B, int W,
+               const void* k_codes, const void* v_codes, const float* scales, int P, int Hkv, int D) {
+  if (D != 64 && D != 128) return fail(SVDQ_ERR_UNSUPPORTED, "%s: D=%d has no kernel (64, 128)", fn, D);
+  if (N < 0 || B <= 0 || W <= 0 || W > 1 << 24 || P <= 0 || Hkv <= 0)
+    return fail(SVDQ_ERR_SHAPE, "%s: N=%d, B=%d, W=%d (at most 2^24), P=%d, Hkv=%d", fn, N, B, W, P, Hkv);
+  if (N && (!offsets || !lengths || !table || !k_codes || !v_codes || !scales))
+    return fail(SVDQ_ERR_ARG, "%s: null pointer", fn);
+  if (!aligned16(k_codes) || !aligned16(v_codes)) return fail(SVDQ_ERR_ALIGN, "%s: codes must be 16-byte aligned", fn);
+  if ((reinterpret_cast<uintptr_t>(offsets) | reinterpret_cast<uintptr_t>(lengths) |
+       reinterpret_cast<uintptr_t>(table) | reinterpret_cast<uintptr_t>(scales)) % 4)
+    return fail(SVDQ_ERR_ALIGN, "%s: offsets, lengths, table and scales must be aligned to their elements", fn);
+  return SVDQ_OK;
+}
+
+svdq::Kv8Cache kv8_cache(int N, const int* offsets, const int* lengths, const int* table, int B, int W,
+                         const void* k_codes, const void* v_codes, const float* scales, int P, int Hkv, int D) {
+  return {offsets, lengths, table, static_cast<uint8_t*>(const_cast<void*>(k_codes)),
+          static_cast<uint8_t*>(const_cast<void*>(v_codes)), const_cast<float*>(scales), N, B, W, P, Hkv, D};
+}
+
+// rows of heads, and tiles times splits (128 at most) of a launch of 256 threads each
+bool kv8_fits(int64_t N, int64_t B, int64_t H, int64_t Hkv) {
+  return N * (H / Hkv) <= INT32_MAX && (N * (H / Hkv) / 16 + B + 1) * Hkv <= (int64_t)(UINT32_MAX / 256);
+}
+
+}  // namespace
+
+extern "C" {
+
+int svdq_kv8_append(const void* k, int64_t ldk, const void* v, int64_t ldv, int N, const int* offsets,
+                    const int* lengths, const int* table, int B, int W, void* k_codes, void* v_codes, float* scales,
+                    int P, int Hkv, int D, hipStream_t stream) {
+  if (int e = kv8_checks("kv8_append", N, offsets, lengths, table, B, W, k_codes, v_codes, scales, P, Hkv, D)) return e;
+  if ((N / 64 + 2 * (int64_t)B) * Hkv > (int64_t)(UINT32_MAX / 256))
+    return fail(SVDQ_ERR_SHAPE, "kv8_append: N=%d, B=%d, Hkv=%d are too many for a launch", N, B, Hkv);
+  if (N == 0) return ok();
+  if (!k || !v) return fail(SVDQ_ERR_ARG, "kv8_append: null pointer");
+  if (ldk % 8 || ldv % 8 || !aligned16(k) || !aligned16(v))
+    return fail(SVDQ_ERR_ALIGN, "kv8_append: 16-byte aligned keys and values, row strides multiples of 8");
+  return launched(svdq::launch_kv8_append(kv8_cache(N, offsets, lengths, table, B, W, k_codes, v_codes, scales, P, Hkv, D),
+                                          static_cast<const uint16_t*>(k), ldk, static_cast<const uint16_t*>(v), ldv,
+                                          stream),
+                  "kv8_append");
+}
+
+int64_t svdq_kv8_attention_workspace(int N, int B, int W, int H, int Hkv, int D) {
+  if (N <= 0 || B <= 0 || W <= 0 || Hkv <= 0 || H <= 0 || H % Hkv || (D != 64 && D != 128) || !kv8_fits(N, B, H, Hkv))
+    return 0;
+  return svdq::kv8_attention_workspace_bytes(kv8_cache(N, nullptr, nullptr, nullptr, B, W, nullptr, nullptr, nullptr, 1, Hkv, D), H);
+}
+
+int svdq_kv8_attention(const void* q, int64_t ldq, int N, const int* offsets, const int* lengths, const int* table,
+                       int B, int W, const void* k_codes, const void* v_codes, const float* scales, int P, int H, int Hkv,
+                       int D, float scale, int causal, void* o, void* workspace, hipStream_t stream) {
+  const char* fn = "kv8_attention";
+  if (int e = kv8_checks(fn, N, offsets, lengths, table, B, W, k_codes, v_codes, scales, P, Hkv, D)) return e;
+  if (H <= 0 || H % Hkv) return fail(SVDQ_ERR_SHAPE, "%s: H=%d, Hkv=%d", fn, H, Hkv);
+  if (causal != 0 && causal != 1) return fail(SVDQ_ERR_ARG, "%s: causal=%d", fn, causal);
+  if (!kv8_fits(N, B, H, Hkv))
+    return fail(SVDQ_ERR_SHAPE, "%s: N=%d, B=%d, H=%d, Hkv=%d are too many for a launch", fn, N, B, H, Hkv);
+  if (N == 0) return ok();
+  if (!q || !o) return fail(SVDQ_ERR_ARG, "%s: null pointer", fn);
+  if (ldq % 8 || !aligned16(q) || !aligned16(o) || !aligned16(workspace))
+    return fail(SVDQ_ERR_ALIGN, "%s: 16-byte aligned q, o and workspace, a row stride multiple of 8", fn);
+  const svdq::Kv8Cache c = kv8_cache(N, offsets, lengths, table, B, W, k_codes, v_codes, scales, P, Hkv, D);
+  if (!workspace && svdq::kv8_attention_workspace_bytes(c, H) > 0) return fail(SVDQ_ERR_ARG, "%s: no workspace", fn);
+  return launched(svdq::launch_kv8_attention(c, {static_cast<const uint16_t*>(q), ldq, static_cast<uint16_t*>(o), H, scale,
+                                                 causal}, workspace, stream),
+                  fn);
+}
+
+}  // extern "C"

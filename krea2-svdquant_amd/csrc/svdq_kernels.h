@@ -201,4 +201,58 @@ hipError_t launch_mx_gemm(const MxGemmParams& p, int fmt, bool out_f32, hipStrea
 constexpr int MX_TILES = 4, MX_ROWS = -1;
 int mx_gemm_tile(int M, int N, int K, int fmt, int& rows, int& cols, bool& split);
 
+
+// 8-bit floating point with a scale per block (svdq_fp8.hip, svdq_fp8_gemm.hip); storage as in svdq_fp8_gemm.hip
+hipError_t launch_fp8_quantize(const uint16_t* x, long ldx, int M, int K, uint8_t* codes, float* scales, hipStream_t st);
+struct Fp8GemmParams {
+  const uint8_t* a;         // [M, kp] E4M3 codes
+  const float* as;          // [kp / 128, M]
+  const uint8_t* w;         // [N, kp] E4M3 codes
+  const float* ws;          // [ceil(N / 128), kp / 128]
+  const uint16_t* bias;     // [N] bf16 or null
+  uint16_t* y;              // [M, ldy] bf16
+  long ldy;
+  int M, N, K;
+};
+hipError_t launch_fp8_gemm(const Fp8GemmParams& p, hipStream_t st);
+
+// Norms of q's and k's heads with the position rotation (svdq_block.hip)
+struct QkNormRopeParams {
+  const uint16_t *q, *k;    // bf16 [T] rows of H (Hkv) heads of D; strides of tokens and heads in elements
+  long ldq, ldk;
+  int hsq, hsk;
+  const uint16_t *qw, *kw;  // [D] bf16 or null
+  const void *cs, *sn;      // [P, ldcs] tables of float32 or bf16, columns 0 .. D / 2 - 1
+  long ldcs;
+  int P;
+  const int64_t* at;        // [T] rows of the tables, or null: token t's is t
+  int T, H, Hkv, D;
+  float eps;
+  int wide, pairs;          // float32 tables; pairs (2 j, 2 j + 1) and not (j, j + D / 2)
+  uint16_t *qo, *ko;        // contiguous [T, H, D], [T, Hkv, D]
+};
+hipError_t launch_qk_norm_rope(const QkNormRopeParams& p, hipStream_t st);
+
+// The 8-bit cache of keys and values (svdq_kv8.hip): pages of 64 tokens
+struct Kv8Cache {
+  const int* offsets;       // [B + 1]: sequence b's new tokens are rows offsets[b] .. offsets[b + 1] - 1 (offsets[0] counts as 0)
+  const int* lengths;       // [B] tokens held
+  const int* table;         // [B, W] page of each 64 tokens
+  uint8_t *kc, *vc;         // [P, Hkv, 64, D], [P, Hkv, D, 64] E4M3 codes
+  float* scales;            // [P, Hkv, 2]: keys', values'
+  int N, B, W, P, Hkv, D;   // N: rows of all new tokens
+};
+hipError_t launch_kv8_append(const Kv8Cache& c, const uint16_t* k, long ldk, const uint16_t* v, long ldv,
+                             hipStream_t st);
+struct Kv8Attention {
+  const uint16_t* q;        // [N, H, D] bf16, rows ldq apart
+  long ldq;
+  uint16_t* o;              // [N, H, D], contiguous
+  int H;
+  float scale;
+  int causal;
+};
+long kv8_attention_workspace_bytes(const Kv8Cache& c, int H);
+hipError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Attention& a, void* workspace, hipStream_t st);
+
 }  // namespace svdq

@@ -456,6 +456,201 @@ std::tuple<Tensor, Tensor, Tensor> residual_rms_norm_modulate_mx(const Tensor& x
   return {xo, codes, scales};
 }
 
+// ---- 8-bit floating point with a scale per block ---------------------------------------------------
+// Codes are float8_e4m3fn [..., kp], scales float32: an activation's [kp / 128, rows], a weight's [ceil(N / 128), kp / 128].
+
+std::tuple<Tensor, Tensor> fp8_quantize(const Tensor& x) {
+  const c10::DeviceGuard guard(x.device());
+  const Rows r("x", x);
+  std::vector<int64_t> cs = r.lead;
+  cs.push_back(mx_kp(r.k));
+  Tensor codes = at::empty(cs, r.t.options().dtype(at::kFloat8_e4m3fn));
+  Tensor scales = at::empty({mx_kp(r.k) / 128, r.m}, r.t.options().dtype(at::kFloat));
+  check_status("svdq_fp8_quantize", svdq_fp8_quantize(ptr(r.t), r.ld, (int)r.m, (int)r.k, ptr(codes), ptr<float>(scales),
+                                                      stream_of(x.device())));
+  return {codes, scales};
+}
+
+// y [lead..., N] of rows of kp codes at a, their scales at as
+Tensor fp8_product(const void* a, const float* as, int64_t m, int64_t kp, std::vector<int64_t> lead, const Tensor& w,
+                   const Tensor& w_scales, const OptTensor& bias) {
+  const c10::Device dev = w.device();
+  check_tensor("w", w, dev, at::kFloat8_e4m3fn);
+  TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) > 0 && w.size(0) <= INT32_MAX, "w must be [N, K] codes, got ", w.sizes());
+  TORCH_CHECK_VALUE(w.size(1) == kp, "rows of ", kp, " values (padded to 128) against a weight of ", w.size(1));
+  const int64_t n = w.size(0);
+  check_tensor("w_scales", w_scales, dev, at::kFloat);
+  const std::vector<int64_t> want{(n + 127) / 128, kp / 128};
+  TORCH_CHECK_VALUE(w_scales.sizes() == at::IntArrayRef(want), "w_scales must be ", at::IntArrayRef(want), ", got ",
+                    w_scales.sizes());
+  if (bias.has_value()) {
+    check_tensor("bias", *bias, dev, at::kBFloat16);
+    TORCH_CHECK_VALUE(bias->numel() == n, "bias must have ", n, " entries, got ", bias->numel());
+  }
+  lead.push_back(n);
+  Tensor y = at::empty(lead, w.options().dtype(at::kBFloat16));
+  check_status("svdq_fp8_gemm", svdq_fp8_gemm(a, as, ptr(w), ptr<float>(w_scales), ptr(bias), (int)m, (int)n, (int)kp,
+                                              ptr(y), n, stream_of(dev)));
+  return y;
+}
+
+Tensor fp8_gemm(const Tensor& a, const Tensor& a_scales, const Tensor& w, const Tensor& w_scales, const OptTensor& bias) {
+  const c10::DeviceGuard guard(w.device());
+  check_tensor("a", a, w.device(), at::kFloat8_e4m3fn);
+  TORCH_CHECK_VALUE(a.dim() >= 1 && a.size(-1) > 0 && a.size(-1) % 128 == 0 && a.size(-1) <= 1 << 30, "a must be [..., K] "
+                    "codes, K a multiple of 128, got ", a.sizes());
+  std::vector<int64_t> lead = a.sizes().vec();
+  const int64_t kp = lead.back(), m = a.numel() / kp;
+  lead.pop_back();
+  TORCH_CHECK_VALUE(m <= INT32_MAX, "a: ", m, " rows are too many");
+  check_tensor("a_scales", a_scales, w.device(), at::kFloat);
+  const std::vector<int64_t> want{kp / 128, m};
+  TORCH_CHECK_VALUE(a_scales.sizes() == at::IntArrayRef(want), "a_scales must be ", at::IntArrayRef(want), ", got ",
+                    a_scales.sizes());
+  return fp8_product(ptr(a), ptr<float>(a_scales), m, kp, lead, w, w_scales, bias);
+}
+
+Tensor fp8_linear(const Tensor& x, const Tensor& w, const Tensor& w_scales, const OptTensor& bias) {
+  const c10::DeviceGuard guard(w.device());
+  TORCH_CHECK_VALUE(x.device() == w.device(), "x is on ", x.device(), ", expected ", w.device());
+  const Rows r("x", x);
+  const int64_t kp = mx_kp(r.k), codes = r.m * kp;
+  const Tensor work = at::empty({codes + r.m * kp / 32}, r.t.options().dtype(at::kByte));
+  uint8_t* base = ptr<uint8_t>(work);
+  float* scales = reinterpret_cast<float*>(base + codes);
+  check_status("svdq_fp8_quantize", svdq_fp8_quantize(ptr(r.t), r.ld, (int)r.m, (int)r.k, base, scales,
+                                                      stream_of(w.device())));
+  return fp8_product(base, scales, r.m, kp, r.lead, w, w_scales, bias);
+}
+
+// [T, heads, D] with dense heads on 16 bytes; `packed`: heads one behind another
+Tensor heads_of(const char* name, const Tensor& t, c10::Device dev, bool packed) {
+  TORCH_CHECK_VALUE(t.device() == dev, name, " is on ", t.device(), ", expected ", dev);
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kBFloat16, name, " must be bfloat16, got ", t.scalar_type());
+  TORCH_CHECK_VALUE(t.dim() == 3 && t.size(1) > 0 && t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX, name,
+                    " must be [tokens, heads, dim], got ", t.sizes());
+  const bool fits = t.stride(2) == 1 && (packed ? t.stride(1) == t.size(2) : t.stride(1) % 8 == 0 && t.stride(1) <= INT32_MAX) &&
+                    t.stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  return fits ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const OptTensor& q_weight,
+                                        const OptTensor& k_weight, const Tensor& cos, const Tensor& sin, double eps,
+                                        const OptTensor& positions, bool interleaved) {
+  const c10::Device dev = q.device();
+  const c10::DeviceGuard guard(dev);
+  const Tensor qh = heads_of("q", q, dev, false), kh = heads_of("k", k, dev, false);
+  const int64_t t = q.size(0), d = q.size(2);
+  TORCH_CHECK_VALUE(k.size(0) == t && k.size(2) == d, "k ", k.sizes(), " must have q's tokens and channels ", q.sizes());
+  TORCH_CHECK_VALUE(d > 0 && d <= 256 && d % 16 == 0, "heads must have a multiple of 16 channels up to 256, got ", d);
+  auto weight = [&](const char* name, const OptTensor& w) -> OptTensor {
+    if (!w.has_value()) return w;
+    return norm_vector(name, *w, d, dev);
+  };
+  const OptTensor qw = weight("q_weight", q_weight), kw = weight("k_weight", k_weight);
+  const bool wide = cos.scalar_type() == at::kFloat;
+  auto table = [&](const char* name, const Tensor& x) {
+    TORCH_CHECK_VALUE(x.device() == dev, name, " is on ", x.device(), ", expected ", dev);
+    TORCH_CHECK_TYPE(x.scalar_type() == (wide ? at::kFloat : at::kBFloat16), "cos and sin must both be float32 or bfloat16, got ",
+                     cos.scalar_type(), " and ", sin.scalar_type());
+    TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) > 0 && x.size(0) <= INT32_MAX && x.size(1) >= d / 2, name,
+                      " must be [positions, >= ", d / 2, "], got ", x.sizes());
+    const bool fits = x.stride(1) == 1 && x.stride(0) >= d / 2 && x.stride(0) * (wide ? 4 : 2) % 16 == 0 &&
+                      reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+    return fits ? x : x.narrow(1, 0, d / 2).clone(at::MemoryFormat::Contiguous);
+  };
+  Tensor c = table("cos", cos), s = table("sin", sin);
+  TORCH_CHECK_VALUE(c.size(0) == s.size(0), "cos ", cos.sizes(), " and sin ", sin.sizes(), " differ");
+  if (c.stride(0) != s.stride(0)) {
+    c = c.narrow(1, 0, d / 2).clone(at::MemoryFormat::Contiguous);
+    s = s.narrow(1, 0, d / 2).clone(at::MemoryFormat::Contiguous);
+  }
+  OptTensor at_;
+  if (positions.has_value()) {
+    TORCH_CHECK_VALUE(positions->device() == dev, "positions are on ", positions->device(), ", expected ", dev);
+    TORCH_CHECK_TYPE(positions->scalar_type() == at::kLong || positions->scalar_type() == at::kInt,
+                     "positions must be int64 or int32, got ", positions->scalar_type());
+    TORCH_CHECK_VALUE(positions->dim() == 1 && positions->size(0) == t, "positions must be [", t, "], got ", positions->sizes());
+    at_ = positions->to(at::kLong).contiguous();
+  } else {
+    TORCH_CHECK_VALUE(c.size(0) >= t, "tables of ", c.size(0), " positions for ", t, " tokens");
+  }
+  Tensor qo = at::empty(q.sizes(), qh.options()), ko = at::empty(k.sizes(), kh.options());
+  check_status("svdq_qk_norm_rope",
+               svdq_qk_norm_rope(ptr(qh), qh.stride(0), (int)qh.stride(1), ptr(kh), kh.stride(0), (int)kh.stride(1), ptr(qw),
+                                 ptr(kw), ptr(c), ptr(s), c.stride(0), (int)c.size(0), wide, ptr<int64_t>(at_), (int)t,
+                                 (int)q.size(1), (int)k.size(1), (int)d, (float)eps, interleaved, ptr(qo), ptr(ko),
+                                 stream_of(dev)));
+  return {qo, ko};
+}
+
+// ---- The 8-bit cache of keys and values ---------------------------------------------------------------
+
+struct Kv8 {
+  int n, b, w, p, hkv, d;
+
+  Kv8(int64_t tokens, const Tensor& offsets, const Tensor& lengths, const Tensor& table, const Tensor& k_codes,
+      const Tensor& v_codes, const Tensor& scales, c10::Device dev) {
+    check_tensor("k_codes", k_codes, dev, at::kFloat8_e4m3fn);
+    check_tensor("v_codes", v_codes, dev, at::kFloat8_e4m3fn);
+    check_tensor("scales", scales, dev, at::kFloat);
+    check_tensor("cu_seqlens", offsets, dev, at::kInt);
+    check_tensor("lengths", lengths, dev, at::kInt);
+    check_tensor("block_table", table, dev, at::kInt);
+    TORCH_CHECK_VALUE(k_codes.dim() == 4 && k_codes.size(2) == 64, "k_codes must be [pages, heads, 64, dim], got ", k_codes.sizes());
+    const int64_t pages = k_codes.size(0), heads = k_codes.size(1), dim = k_codes.size(3);
+    TORCH_CHECK_VALUE(dim == 64 || dim == 128, "heads must have 64 or 128 channels, got ", dim);
+    const std::vector<int64_t> vs{pages, heads, dim, 64}, ss{pages, heads, 2};
+    TORCH_CHECK_VALUE(v_codes.sizes() == at::IntArrayRef(vs), "v_codes must be ", at::IntArrayRef(vs), ", got ", v_codes.sizes());
+    TORCH_CHECK_VALUE(scales.sizes() == at::IntArrayRef(ss), "scales must be ", at::IntArrayRef(ss), ", got ", scales.sizes());
+    TORCH_CHECK_VALUE(table.dim() == 2, "block_table must be [sequences, pages], got ", table.sizes());
+    const int64_t batch = table.size(0), width = table.size(1);
+    TORCH_CHECK_VALUE(lengths.dim() == 1 && lengths.size(0) == batch && offsets.dim() == 1 && offsets.size(0) == batch + 1,
+                      "lengths must be [", batch, "] and cu_seqlens [", batch + 1, "], got ", lengths.sizes(), " and ", offsets.sizes());
+    TORCH_CHECK_VALUE(tokens <= INT32_MAX && pages > 0 && heads > 0 && batch > 0 && width > 0 && pages <= INT32_MAX &&
+                      heads <= INT32_MAX && batch < INT32_MAX && width <= 1 << 24, "a cache of ", pages, " pages of ", heads,
+                      " heads, a table of ", table.sizes(), ", ", tokens, " tokens");
+    n = (int)tokens, b = (int)batch, w = (int)width, p = (int)pages, hkv = (int)heads, d = (int)dim;
+  }
+};
+
+void kv8_append(const Tensor& k, const Tensor& v, const Tensor& cu_seqlens, const Tensor& lengths, const Tensor& block_table,
+                const Tensor& k_codes, const Tensor& v_codes, const Tensor& scales) {
+  const c10::Device dev = k_codes.device();
+  const c10::DeviceGuard guard(dev);
+  TORCH_CHECK(!(at::GradMode::is_enabled() && (k.requires_grad() || v.requires_grad())),
+              "svdq::kv8_append has no gradient: its inputs may not require one");
+  const Tensor kh = heads_of("k", k, dev, true), vh = heads_of("v", v, dev, true);
+  const Kv8 c(k.size(0), cu_seqlens, lengths, block_table, k_codes, v_codes, scales, dev);
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.size(1) == c.hkv && k.size(2) == c.d, "k and v must be [tokens, ", c.hkv, ", ",
+                    c.d, "], got ", k.sizes(), " and ", v.sizes());
+  check_status("svdq_kv8_append",
+               svdq_kv8_append(ptr(kh), kh.stride(0), ptr(vh), vh.stride(0), c.n, ptr<int>(cu_seqlens), ptr<int>(lengths),
+                               ptr<int>(block_table), c.b, c.w, ptr(k_codes), ptr(v_codes), ptr<float>(scales), c.p, c.hkv,
+                               c.d, stream_of(dev)));
+  for (const Tensor* t : {&k_codes, &v_codes, &scales})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+Tensor kv8_attention(const Tensor& q, const Tensor& cu_seqlens, const Tensor& lengths, const Tensor& block_table,
+                     const Tensor& k_codes, const Tensor& v_codes, const Tensor& scales, double scale, bool causal) {
+  const c10::Device dev = q.device();
+  const c10::DeviceGuard guard(dev);
+  const Tensor qh = heads_of("q", q, dev, true);
+  const Kv8 c(q.size(0), cu_seqlens, lengths, block_table, k_codes, v_codes, scales, dev);
+  TORCH_CHECK_VALUE(q.size(2) == c.d && q.size(1) % c.hkv == 0, "q must be [tokens, a multiple of ", c.hkv, ", ", c.d, "], got ",
+                    q.sizes());
+  const int h = (int)q.size(1);
+  Tensor out = at::empty(q.sizes(), qh.options());
+  const int64_t bytes = svdq_kv8_attention_workspace(c.n, c.b, c.w, h, c.hkv, c.d);
+  const Tensor work = bytes ? at::empty({bytes}, qh.options().dtype(at::kByte)) : Tensor();
+  check_status("svdq_kv8_attention",
+               svdq_kv8_attention(ptr(qh), qh.stride(0), c.n, ptr<int>(cu_seqlens), ptr<int>(lengths), ptr<int>(block_table),
+                                  c.b, c.w, ptr(k_codes), ptr(v_codes), ptr<float>(scales), c.p, h, c.hkv, c.d, (float)scale,
+                                  causal, ptr(out), bytes ? ptr(work) : nullptr, stream_of(dev)));
+  return out;
+}
+
 }  // namespace
 
 // The torch that this file was compiled against, found in the file by kernels/hip/lib.py ahead of
@@ -480,6 +675,18 @@ TORCH_LIBRARY_FRAGMENT(svdq, m) {
   m.def(
       "residual_rms_norm_modulate_mx(Tensor x, Tensor v, Tensor gate, Tensor weight, Tensor shift, float eps, int fmt) "
       "-> (Tensor, Tensor, Tensor)");
+  m.def("fp8_quantize(Tensor x) -> (Tensor, Tensor)");
+  m.def("fp8_gemm(Tensor a, Tensor a_scales, Tensor w, Tensor w_scales, Tensor? bias) -> Tensor");
+  m.def("fp8_linear(Tensor x, Tensor w, Tensor w_scales, Tensor? bias) -> Tensor");
+  m.def(
+      "qk_norm_rope(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor cos, Tensor sin, float eps, "
+      "Tensor? positions, bool interleaved) -> (Tensor, Tensor)");
+  m.def(
+      "kv8_append(Tensor k, Tensor v, Tensor cu_seqlens, Tensor lengths, Tensor block_table, Tensor(a!) k_codes, "
+      "Tensor(b!) v_codes, Tensor(c!) scales) -> ()");
+  m.def(
+      "kv8_attention(Tensor q, Tensor cu_seqlens, Tensor lengths, Tensor block_table, Tensor k_codes, Tensor v_codes, "
+      "Tensor scales, float scale, bool causal) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(svdq, CUDA, m) {
   m.impl("linear", TORCH_FN(linear));
@@ -491,6 +698,12 @@ TORCH_LIBRARY_IMPL(svdq, CUDA, m) {
   m.impl("silu_mul_mx", TORCH_FN(silu_mul_mx));
   m.impl("rms_norm_modulate_mx", TORCH_FN(rms_norm_modulate_mx));
   m.impl("residual_rms_norm_modulate_mx", TORCH_FN(residual_rms_norm_modulate_mx));
+  m.impl("fp8_quantize", TORCH_FN(fp8_quantize));
+  m.impl("fp8_gemm", TORCH_FN(fp8_gemm));
+  m.impl("fp8_linear", TORCH_FN(fp8_linear));
+  m.impl("qk_norm_rope", TORCH_FN(qk_norm_rope));
+  m.impl("kv8_append", TORCH_FN(kv8_append));
+  m.impl("kv8_attention", TORCH_FN(kv8_attention));
 }
 TORCH_LIBRARY_IMPL(svdq, Autograd, m) {
   m.impl("linear", torch::autograd::autogradNotImplementedFallback());
@@ -502,4 +715,10 @@ TORCH_LIBRARY_IMPL(svdq, Autograd, m) {
   m.impl("silu_mul_mx", torch::autograd::autogradNotImplementedFallback());
   m.impl("rms_norm_modulate_mx", torch::autograd::autogradNotImplementedFallback());
   m.impl("residual_rms_norm_modulate_mx", torch::autograd::autogradNotImplementedFallback());
+  m.impl("fp8_quantize", torch::autograd::autogradNotImplementedFallback());
+  m.impl("fp8_gemm", torch::autograd::autogradNotImplementedFallback());
+  m.impl("fp8_linear", torch::autograd::autogradNotImplementedFallback());
+  m.impl("qk_norm_rope", torch::autograd::autogradNotImplementedFallback());
+  m.impl("kv8_append", torch::autograd::autogradNotImplementedFallback());
+  m.impl("kv8_attention", torch::autograd::autogradNotImplementedFallback());
 }

@@ -480,10 +480,11 @@ def load_native() -> dict:
             lib.load_torch_ops()
             torch.library.register_fake("svdq::linear", _linear_fake)
             torch.library.register_fake("svdq::linear_siblings", _linear_siblings_fake)
-            for name, fake in _MX_FAKES.items():
+            fakes = {**_MX_FAKES, **_FP8_FAKES}
+            for name, fake in fakes.items():
                 torch.library.register_fake(f"svdq::{name}", fake)
             _native_ops.update({name: getattr(torch.ops.svdq, name).default
-                                for name in ("linear", "linear_siblings", *_MX_FAKES)})
+                                for name in ("linear", "linear_siblings", *fakes)})
     return _native_ops
 
 
@@ -611,6 +612,85 @@ def residual_rms_norm_modulate_mx(x: Tensor, v: Tensor, gate: Tensor, weight: Te
     """``svdq::residual_rms_norm_modulate_mx``: ``xo = torch.addcmul(x, gate, v)`` (bf16, one rounding) and
     ``rms_norm_modulate_mx(xo, weight, shift, eps, fmt)`` in one pass; ``(xo, codes, scales)``."""
     return _mx("residual_rms_norm_modulate_mx", x, x, v, gate, weight, shift, eps, _mx_fmt(fmt))
+
+
+# ---- 8-bit floating point with a scale per block --------------------------------------------------
+# E4M3 codes (float8_e4m3fn) and float32 scales.  Rows of K values hold kp codes, K rounded up to 128 (zero codes).
+# An activation [..., K] has scales [kp / 128, rows], a weight [N, K] scales [ceil(N / 128), kp / 128] of its 128 x 128 blocks.
+FP8_BLOCK = 128
+
+
+def _fp8_quantize_fake(x):
+    kp = (x.shape[-1] + 127) // 128 * 128
+    rows = 1
+    for n in x.shape[:-1]:
+        rows = rows * n
+    return x.new_empty((*x.shape[:-1], kp), dtype=torch.float8_e4m3fn), x.new_empty((kp // 128, rows), dtype=torch.float32)
+
+
+_FP8_FAKES = {
+    "fp8_quantize": _fp8_quantize_fake,
+    "fp8_gemm": lambda a, a_scales, w, w_scales, bias: _mx_out_fake(a, w, False),
+    "fp8_linear": lambda x, w, w_scales, bias: _mx_out_fake(x, w, False),
+    "qk_norm_rope": lambda q, k, q_weight, k_weight, cos, sin, eps, positions, interleaved: (
+        q.new_empty(q.shape), k.new_empty(k.shape)),
+    "kv8_append": lambda k, v, cu_seqlens, lengths, block_table, k_codes, v_codes, scales: None,
+    "kv8_attention": lambda q, cu_seqlens, lengths, block_table, k_codes, v_codes, scales, scale, causal: (
+        q.new_empty(q.shape)),
+}
+
+
+def fp8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
+    """``svdq::fp8_quantize``: bf16 ``x`` [..., K] as E4M3, ``(codes [..., kp], scales [kp / 128, rows])``.
+
+    The scale of 128 columns of a row is the smallest power of two (2^-126 at least) under which their largest finite
+    magnitude is at most 448, their codes the nearest values, ties to even.  Infinities and NaN become NaN."""
+    return _mx("fp8_quantize", x, x)
+
+
+def fp8_gemm(a: Tensor, a_scales: Tensor, w: Tensor, w_scales: Tensor, bias: Optional[Tensor] = None) -> Tensor:
+    """``svdq::fp8_gemm``: ``a w^T + bias`` of an E4M3 activation (as ``fp8_quantize`` gives it) and an E4M3 weight ``w``
+    [N, kp] with a float32 scale for each 128 x 128 block (any values); bf16 [..., N], sums in float32."""
+    return _mx("fp8_gemm", a, a, a_scales, w, w_scales, bias)
+
+
+def fp8_linear(x: Tensor, w: Tensor, w_scales: Tensor, bias: Optional[Tensor] = None) -> Tensor:
+    """``svdq::fp8_linear``: ``fp8_gemm(*fp8_quantize(x), w, w_scales, bias)`` in one call."""
+    return _mx("fp8_linear", x, x, w, w_scales, bias)
+
+
+def qk_norm_rope(q: Tensor, k: Tensor, q_weight: Optional[Tensor], k_weight: Optional[Tensor], cos: Tensor, sin: Tensor,
+                 eps: float, positions: Optional[Tensor] = None, interleaved: bool = False) -> tuple[Tensor, Tensor]:
+    """``svdq::qk_norm_rope``: the RMS norm of every head of bf16 ``q`` [T, H, D] and ``k`` [T, Hkv, D] with weights [D]
+    (or None), and the position rotation, in one launch: float32 throughout, one rounding.
+
+    ``cos`` and ``sin`` are tables [positions, >= D / 2], float32 or bf16; token t takes row ``positions[t]`` (NaN where
+    there is no such row), or row t.  Rotated pairs are channels (j, j + D / 2), with ``interleaved`` (2 j, 2 j + 1).
+    D is a multiple of 16 up to 256.  q and k may be slices of one wider projection."""
+    return _mx("qk_norm_rope", q, q, k, q_weight, k_weight, cos, sin, eps, positions, interleaved)
+
+
+def kv8_append(k: Tensor, v: Tensor, cu_seqlens: Tensor, lengths: Tensor, block_table: Tensor, k_codes: Tensor,
+               v_codes: Tensor, scales: Tensor) -> None:
+    """``svdq::kv8_append``: new keys and values (bf16 [tokens, Hkv, D]) into an 8-bit cache, in place.
+
+    The cache is pages of 64 tokens: ``k_codes`` [pages, Hkv, 64, D] and ``v_codes`` [pages, Hkv, D, 64] E4M3 with a scale
+    each for a page and head in ``scales`` [pages, Hkv, 2] (float32); D is 64 or 128.  ``block_table`` [B, W] (int32) names the pages of
+    each sequence, ``lengths`` [B] (int32) how many tokens it holds before the call, ``cu_seqlens`` [B + 1] (int32) which of the
+    new tokens are its own: rows ``cu_seqlens[b]`` to ``cu_seqlens[b + 1]``, ascending from 0.  A page that begins with new
+    tokens gets their scale (``fp8_quantize``'s, over the page and head); one that holds older tokens keeps its own or takes
+    theirs where that is larger, and the older codes are rounded again under it.  Tokens beyond the table, or whose page
+    is not in the cache, are dropped; sequences may not share a page that is written."""
+    return _mx("kv8_append", k_codes, k, v, cu_seqlens, lengths, block_table, k_codes, v_codes, scales)
+
+
+def kv8_attention(q: Tensor, cu_seqlens: Tensor, lengths: Tensor, block_table: Tensor, k_codes: Tensor, v_codes: Tensor,
+                  scales: Tensor, scale: float, causal: bool = True) -> Tensor:
+    """``svdq::kv8_attention``: softmax attention of bf16 ``q`` [tokens, H, D] over an 8-bit cache (``kv8_append``), H a
+    multiple of Hkv: ``sum_j softmax_j(scale q . k_j) v_j`` over the ``lengths[b]`` tokens that a sequence holds, its new ones
+    among them; with ``causal`` the i-th of n new tokens sees ``lengths[b] - n + i + 1`` of them.  bf16 [tokens, H, D]; rows
+    that see nothing, and rows behind the last sequence, are 0."""
+    return _mx("kv8_attention", q, q, cu_seqlens, lengths, block_table, k_codes, v_codes, scales, scale, causal)
 
 
 # ---- stand-in block normalizations -------------------------------------------------------------
