@@ -37,18 +37,31 @@ __device__ __forceinline__ void dma4_at(const void* at, uint32_t lds) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(at), "{m0}"(lds) : "memory");
 }
 
+template <class F, int... I>
+__device__ __forceinline__ void for_each_index(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+
 // Block tile BM x BN (BM = 16 TM WM rows of a, BN = 16 TN WN rows of w, a wave's 16 TN within one block of 128), WM x WN
 // waves, a ring of NB stages of 128 columns in LDS filled by DMA.  Rows of 128 bytes lie in chunks of 16, chunk c at slot
 // c ^ (row / 2 mod 8).
+//
+// A stage's products go by pairs of tiles of w, TM tiles of a within a pair, so that the operands of a have time to be
+// replaced: those of the next stage are read behind their last use in the last pair, the operands of w a pair ahead.  Each product is
+// followed by the scaling of the one two before it and by a memory instruction or two; a block of them would leave the
+// matrix unit idle while their queues drain.  Ahead of the last pair everything of the stage has been read: there the wave
+// waits for the next stage's bytes and for the other waves, and the buffer takes stage s + NB.
 template <int TM, int TN, int WM, int WN, int NB>
 struct Fp8Tile {
   static constexpr int NW = WM * WN, BM = 16 * TM * WM, BN = 16 * TN * WN;
   static constexpr int TA = BM / 8, TB = BN / 8;                            // DMA instructions of 1024 bytes
-  static constexpr int DA = TA / NW, D = DA + TB / NW;                      // per wave and stage, and one of scales
+  static constexpr int DA = TA / NW, D = DA + TB / NW + 1;                  // per wave and stage, the last one of scales
   static constexpr int BUF = (TA + TB) * 1024, OS = NB * BUF, LDS = OS + NB * NW * 256;
-  static_assert(LDS <= 160 * 1024, "LDS");
-  static_assert(TA % NW == 0 && TB % NW == 0 && 128 % (16 * TN) == 0 && TM <= 4 && NB >= 2, "whole instructions");
-  static_assert(NB * (D + 1) <= 63, "vmcnt counts to 63");
+  static constexpr int GROUPS = 160 * 1024 / LDS;                           // workgroups that a CU's LDS holds
+  static constexpr int PITCH = 32 * TN + 16;                                // of 16 rows of the output in LDS
+  static_assert(LDS <= 160 * 1024 && NW * 16 * PITCH <= LDS, "LDS");
+  static_assert(TA % NW == 0 && TB % NW == 0 && 128 % (16 * TN) == 0 && TN % 4 == 0 && TM <= 4 && NB >= 2, "whole instructions");
+  static_assert(NB * D <= 63, "vmcnt counts to 63");
 };
 
 template <int TM, int TN, int WM, int WN, int NB>
@@ -61,91 +74,258 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) fp8_gemm_tile_kernel(Fp8GemmP
   tile_coords(blockIdx.x, nbm, nbn, group_m, bm, bn);
   const int m0 = bm * T::BM, n0 = bn * T::BN, kp = (int)fp8_kp(p.K), nst = kp / 128;
   const uint32_t lds0 = lds_offset(sm);
-  const int chunk = lane % 8 ^ (lane / 8 >> 1 & 3), turned = 4;   // row / 2 mod 8 of row 8 i + lane / 8: 4 (i & 1) more
-  uint32_t off[T::D];
+  const int chunk = lane % 8 ^ (lane / 8 >> 1 & 3);   // row / 2 mod 8 of row 8 i + lane / 8: 4 (i & 1) more
+  uint32_t off[T::D - 1];
 #pragma unroll
-  for (int d = 0; d < T::D; ++d) {
+  for (int d = 0; d < T::D - 1; ++d) {
     const bool a = d < T::DA;
     const int i = wave + T::NW * (a ? d : d - T::DA), row = 8 * i + lane / 8;
-    off[d] = (uint32_t)((long)min(row, (a ? p.M - m0 : p.N - n0) - 1) * kp + 16 * (chunk ^ (i & 1 ? turned : 0)));
+    off[d] = (uint32_t)((long)min(row, (a ? p.M - m0 : p.N - n0) - 1) * kp + 16 * (chunk ^ (i & 1 ? 4 : 0)));
   }
   const uint8_t *src_a = p.a + (long)m0 * kp, *src_w = p.w + (long)n0 * kp;
   const int mw = m0 + 16 * TM * wm, nw = n0 + 16 * TN * wn;
   const float* src_s = p.as + min(mw + min(lane, 16 * TM - 1), p.M - 1);
   int ahead = 0;
-  // the stage `ahead`; past the last one that again, so that the waits count the same loads throughout
-  auto fetch = [&](int buf) {
-#pragma unroll
-    for (int d = 0; d < T::D; ++d)
+  // this wave's d-th instruction of the stage `ahead`; past the last one that again, so that the waits count the same
+  // loads throughout
+  auto fetch = [&](int buf, int d) {
+    if (d == T::D - 1) {
+      dma4_at(src_s, lds0 + T::OS + 256 * (buf * T::NW + wave));
+      if (++ahead < nst) {
+        src_a += 128;
+        src_w += 128;
+        src_s += p.M;
+      }
+    } else {
       dma16(d < T::DA ? src_a : src_w, off[d],
             lds0 + buf * T::BUF + 1024 * (d < T::DA ? wave + T::NW * d : T::TA + wave + T::NW * (d - T::DA)));
-    dma4_at(src_s, lds0 + T::OS + 256 * (buf * T::NW + wave));
-    if (++ahead < nst) {
-      src_a += 128;
-      src_w += 128;
-      src_s += p.M;
     }
   };
   const float* wsrow = p.ws + (long)min(nw / 128, (p.N - 1) / 128) * nst;
-  float wscales = wsrow[min(lane, nst - 1)];
+  float wscales = wsrow[min(lane, nst - 1)];   // of stages s .. s + 63
   asm volatile("s_waitcnt vmcnt(0)" : "+v"(wscales)::"memory");
 
-  f32x4 acc[TN][TM] = {};
+  constexpr int P = TN / 2, S = 2 * TM, READS = 4 + 2 * TM;
+  constexpr int D0 = T::D / 2;   // instructions issued in a last pair, the others in the first pair that follows
+  Fp8Frag fa[TM], fw[2][2];
+  f32x4 acc[TN][TM] = {}, v[4] = {};
+  float sc[TM], sraw[TM], scl = 0.0f;
+  const uint32_t turn = 16 * (b ^ (lr >> 1 & 7));
+  const uint8_t *pa = nullptr, *pw = nullptr;   // this lane's chunk in its row of the first tiles
+  const float* ps = nullptr;
+  auto at_buffer = [&](int buf) {
+    pa = sm + buf * T::BUF + (16 * TM * wm + lr) * 128 + turn;
+    pw = sm + buf * T::BUF + T::TA * 1024 + (16 * TN * wn + lr) * 128 + turn;
+    ps = reinterpret_cast<const float*>(sm + T::OS + 256 * (buf * T::NW + wave)) + lr;
+  };
+  const int other = 64 - 2 * (turn & 64);   // chunk c ^ 4
+  auto read_w = [&](int pair, int i) {      // i-th of the four reads of a pair
+    fw[pair & 1][i / 2].q[i % 2] = *reinterpret_cast<const u32x4*>(pw + 2048 * (2 * pair + i / 2) + (i % 2 ? other : 0));
+  };
+  auto read_a = [&](int i) { fa[i / 2].q[i % 2] = *reinterpret_cast<const u32x4*>(pa + 2048 * (i / 2) + (i % 2 ? other : 0)); };
+  auto scaled = [&](int slot, float s) {    // the product of a slot into its accumulator
+    const int pair = slot / S, j = slot % S;
 #pragma unroll
-  for (int i = 0; i < NB - 1; ++i) fetch(i);
-  int cur = 0, nxt = NB - 1;
-#pragma unroll 1
-  for (int s = 0; s < nst; ++s) {
-    landed_and_met<(NB - 2) * (T::D + 1)>();
-    if ((s & 63) == 0 && s) {   // waited for in here: a wait behind it would be for every stage's loads
-      wscales = wsrow[min(s + lane, nst - 1)];
-      asm volatile("s_waitcnt vmcnt(0)" : "+v"(wscales)::"memory");
-    }
-    fetch(nxt);
-    const uint8_t* ba = sm + cur * T::BUF + (16 * TM * wm + lr) * 128;
-    const uint8_t* bw = sm + cur * T::BUF + T::TA * 1024 + (16 * TN * wn + lr) * 128;
-    const float* bs = reinterpret_cast<const float*>(sm + T::OS + 256 * (cur * T::NW + wave)) + lr;
-    const float sw = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wscales), s & 63));
-    const int o0 = 16 * (b ^ (lr >> 1 & 7)), o1 = 16 * ((4 + b) ^ (lr >> 1 & 7));
-    Fp8Frag fa[TM];
-    float sc[TM];
+    for (int r = 0; r < 4; ++r) acc[2 * pair + j % 2][j / 2][r] = __builtin_fmaf(v[slot & 3][r], s, acc[2 * pair + j % 2][j / 2][r]);
+  };
+
 #pragma unroll
-    for (int t = 0; t < TM; ++t) {
-      fa[t].q[0] = *reinterpret_cast<const u32x4*>(ba + 2048 * t + o0);
-      fa[t].q[1] = *reinterpret_cast<const u32x4*>(ba + 2048 * t + o1);
-      sc[t] = bs[16 * t] * sw;
-    }
+  for (int i = 0; i < NB; ++i)
 #pragma unroll
-    for (int x = 0; x < TN; ++x) {
-      Fp8Frag fw;
-      fw.q[0] = *reinterpret_cast<const u32x4*>(bw + 2048 * x + o0);
-      fw.q[1] = *reinterpret_cast<const u32x4*>(bw + 2048 * x + o1);
+    for (int d = 0; d < (i == NB - 1 ? D0 : T::D); ++d) fetch(i, d);
+  landed_and_met<(NB - 2) * T::D + D0>();
+  at_buffer(0);
 #pragma unroll
-      for (int t = 0; t < TM; ++t) {
-        const f32x4 v = fp8_mfma16(fw, fa[t]);
+  for (int i = 0; i < 4; ++i) read_w(0, i);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[x][t][r] = __builtin_fmaf(v[r], sc[t], acc[x][t][r]);
-      }
-    }
-    cur = cur + 1 == NB ? 0 : cur + 1;
-    nxt = nxt + 1 == NB ? 0 : nxt + 1;
-  }
-  // nothing of the DMA may be under way when the next workgroup takes this LDS
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  // register r of lane (lr, b): row lr of a, column 4 b + r of w
+  for (int i = 0; i < 2 * TM; ++i) read_a(i);
 #pragma unroll
   for (int t = 0; t < TM; ++t) {
-    const int m = mw + 16 * t + lr;
+    sraw[t] = ps[16 * t];
+    sc[t] = sraw[t] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wscales), 0));
+  }
+  int cur = 0, last = NB - 1;   // the buffer of this stage, and the one that is being filled
+#pragma unroll 1
+  for (int s = 0; s < nst; ++s) {
+    if ((s + 1) % 64 == 0) {   // waited for in here: a wait behind it would be for every stage's loads
+      wscales = wsrow[min(s + 1 + lane, nst - 1)];
+      asm volatile("s_waitcnt vmcnt(0)" : "+v"(wscales)::"memory");
+    }
+    const float sw = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(wscales), (s + 1) & 63));
+    const int nxt = cur + 1 == NB ? 0 : cur + 1;
+    for_each_index([&](auto pp) {
+      constexpr int pair = decltype(pp)::value;
+      constexpr bool final = pair == P - 1;
+      if (final) {
+        landed_and_met<(NB - 2) * T::D>();
+        at_buffer(nxt);
+      }
+      // the memory instructions of this pair, those of slot j behind its product
+      constexpr int ND = final ? D0 : pair == 0 ? T::D - D0 : 0;
+      constexpr int PER = (READS + S - 1) / S;
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        constexpr int slots = P * S;
+        const int slot = pair * S + j;
+        __builtin_amdgcn_s_setprio(1);   // a wave that has a product to issue goes first: 359 -> 353 us at 4096 x 16384 x 6144
+        v[slot & 3] = fp8_mfma16(fw[pair & 1][j % 2], fa[j / 2]);
+        __builtin_amdgcn_s_setprio(0);
+        if (slot < 2) scaled(slots - 2 + slot, scl);
+        else scaled(slot - 2, sc[(slot - 2) % S / 2]);
+        if (final) {
+          // four of w's, then a's behind their last use
+#pragma unroll
+          for (int i = 0; i < READS; ++i) {
+            const int at_ = i < 4 ? i / PER : (i - 4) / 2 * 2 + 1 > i / PER ? (i - 4) / 2 * 2 + 1 : i / PER;
+            if ((at_ < S ? at_ : S - 1) == j) {
+              if (i < 4) read_w(0, i);   // pair P is even: the next stage's pair 0 goes to buffer 0
+              else read_a(i - 4);
+            }
+          }
+          if (j < TM) sraw[j] = ps[16 * j];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i * (S < 4 ? S : 4) / 4 == j) read_w(pair + 1, i);
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+          if (d * S / (ND ? ND : 1) == j) fetch(final ? cur : last, final ? d : D0 + d);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }, std::make_integer_sequence<int, P>{});
+    scl = sc[TM - 1];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) sc[t] = sraw[t] * sw;
+    last = cur;
+    cur = nxt;
+  }
+  scaled(P * S - 2, scl);
+  scaled(P * S - 1, scl);
+  // Register r of lane (lr, b): row lr of a, column 4 b + r of w.  16 rows at a time go through LDS, each wave in a part of
+  // its own, and out as whole rows of its tile past the L2, whose lines the operands need.  Nothing of the DMA may be under way when
+  // LDS is used again, here or by the next workgroup.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  uint8_t* stage_out = sm + wave * 16 * T::PITCH;
+  constexpr int COLS = 16 * TN, LPR = COLS / 8;   // lanes a row
+  const bool wide = p.ldy % 8 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
+  f32x4 bias[TN];
+#pragma unroll
+  for (int x = 0; x < TN; ++x)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int n = nw + 16 * x + 4 * b + r;
+      bias[x][r] = p.bias && n < p.N ? bf16f(p.bias[n]) : 0.0f;
+    }
+  const int cols = min(COLS, p.N - nw);
+#pragma unroll
+  for (int t = 0; t < TM; ++t) {
 #pragma unroll
     for (int x = 0; x < TN; ++x) {
-      const int n = nw + 16 * x + 4 * b;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (m < p.M && n + r < p.N)
-          p.y[(long)m * p.ldy + n + r] =
-              (uint16_t)pack_bf16x2(acc[x][t][r] + (p.bias ? bf16f(p.bias[n + r]) : 0.0f), 0.0f);
+      const f32x4 y = acc[x][t] + bias[x];
+      *reinterpret_cast<u32x2*>(stage_out + lr * T::PITCH + 32 * x + 8 * b) = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own writes, read by its other lanes
+    const int rows = min(16, p.M - (mw + 16 * t));
+    uint16_t* out = p.y + (long)(mw + 16 * t) * p.ldy + nw;
+    if (wide && cols % 8 == 0) {
+#pragma unroll
+      for (int k = 0; k < 16 * LPR / 64; ++k) {
+        const int row = (64 * k + lane) / LPR, c = (64 * k + lane) % LPR;
+        const u32x4 y = *reinterpret_cast<const u32x4*>(stage_out + row * T::PITCH + 16 * c);
+        if (row < rows && 8 * c < cols) __builtin_nontemporal_store(y, reinterpret_cast<u32x4*>(out + (long)row * p.ldy + 8 * c));
+      }
+    } else {
+#pragma unroll 4
+      for (int k = 0; k < 16 * COLS / 64; ++k) {
+        const int row = (64 * k + lane) / COLS, c = (64 * k + lane) % COLS;
+        if (row < rows && c < cols) out[(long)row * p.ldy + c] = *reinterpret_cast<const uint16_t*>(stage_out + row * T::PITCH + 2 * c);
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
+}
+
+// Few rows of a (16 at most): what counts is reading w once, from as many places at once as possible.  A workgroup of
+// 8 waves takes 16 columns of the output and all of K; the waves take blocks of 128 columns of K in turn (whole cache
+// lines of w) and add their sums through LDS in wave order.  Each wave has a ring of U blocks in LDS to itself, filled
+// by DMA, so the waves need no barrier before the sums.  MR = 8 or 16 rows of a are held; rows beyond M repeat the last.
+template <int MR, int U>
+struct Fp8Rows {
+  static constexpr int NW = 8, OA = 2048, OSC = OA + 128 * MR, UNIT = OSC + 256;
+  static constexpr int DA = MR / 8, D = 2 + DA + 1;   // DMA instructions of a block: w, a, scales
+  static constexpr int LDS = NW * U * UNIT;
+  static_assert(LDS <= 80 * 1024 && NW * 1024 <= LDS, "two workgroups share a CU's LDS");
+};
+
+template <int MR, int U>
+__global__ void __launch_bounds__(512) fp8_gemm_rows_kernel(Fp8GemmParams p) {
+  using T = Fp8Rows<MR, U>;
+  __shared__ __attribute__((aligned(1024))) uint8_t sm[T::LDS];
+  const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, b = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = blockIdx.x * 16, kp = (int)fp8_kp(p.K), nst = kp / 128;
+  const uint32_t lds0 = lds_offset(sm) + wave * U * T::UNIT;
+  const uint8_t* mine = sm + wave * U * T::UNIT;
+  const int chunk = lane % 8 ^ (lane / 8 >> 1 & 3);   // as in the tiles
+  uint32_t off_w[2], off_a[T::DA];
+#pragma unroll
+  for (int d = 0; d < 2; ++d) off_w[d] = (uint32_t)(min(8 * d + lane / 8, p.N - n0 - 1) * (long)kp + 16 * (chunk ^ 4 * d));
+#pragma unroll
+  for (int d = 0; d < T::DA; ++d) off_a[d] = (uint32_t)(min(8 * d + lane / 8, p.M - 1) * (long)kp + 16 * (chunk ^ 4 * d));
+  const uint8_t* src_w = p.w + (long)n0 * kp;
+  // scales of a block: lanes 0..15 the rows', lane 16 the weight's
+  const float* ssrc = lane < 16 ? p.as + min(lane, p.M - 1) : p.ws + (long)(n0 / 128) * nst;
+  const long sstep = lane < 16 ? p.M : 1;
+  auto fetch = [&](int block, int buf) {
+    const uint32_t to = lds0 + buf * T::UNIT;
+#pragma unroll
+    for (int d = 0; d < 2; ++d) dma16(src_w, off_w[d] + 128 * block, to + 1024 * d);
+#pragma unroll
+    for (int d = 0; d < T::DA; ++d) dma16(p.a, off_a[d] + 128 * block, to + T::OA + 1024 * d);
+    dma4_at(ssrc + sstep * block, to + T::OSC);
+  };
+  const int count = wave < nst ? (nst - wave + T::NW - 1) / T::NW : 0;
+  f32x4 acc = {};
+  const int ma = min(lr, MR - 1), o0 = 16 * (b ^ (lr >> 1 & 7)), oa = 16 * (b ^ (ma >> 1 & 7));
+  if (count) {
+    // blocks past the last are the last again, into a buffer that is not read: the waits count the same loads throughout
+    auto block_of = [&](int i) { return wave + T::NW * min(i, count - 1); };
+#pragma unroll
+    for (int i = 0; i < U; ++i) fetch(block_of(i), i);
+    int buf = 0;
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((U - 1) * T::D) : "memory");
+      const uint8_t* u = mine + buf * T::UNIT;
+      Fp8Frag fw, fa;
+      fw.q[0] = *reinterpret_cast<const u32x4*>(u + 128 * lr + o0);
+      fw.q[1] = *reinterpret_cast<const u32x4*>(u + 128 * lr + (o0 ^ 64));
+      fa.q[0] = *reinterpret_cast<const u32x4*>(u + T::OA + 128 * ma + oa);
+      fa.q[1] = *reinterpret_cast<const u32x4*>(u + T::OA + 128 * ma + (oa ^ 64));
+      const float* sc = reinterpret_cast<const float*>(u + T::OSC);
+      const float s = sc[lr] * sc[16];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // all of the block is in registers
+      fetch(block_of(i + U), buf);
+      buf = buf + 1 == U ? 0 : buf + 1;
+      const f32x4 v = fp8_mfma16(fw, fa);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(v[r], s, acc[r]);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+  __syncthreads();   // every ring is done with; their memory takes the sums
+  reinterpret_cast<f32x4*>(sm)[64 * wave + lane] = acc;
+  __syncthreads();
+  // register r of lane (lr, b): row lr of a, column 4 b + r of w
+  const int m = tid >> 4, n = tid & 15;
+  if (m >= p.M || m >= 16 || n0 + n >= p.N) return;
+  float y = 0.0f;
+#pragma unroll
+  for (int k = 0; k < T::NW; ++k) y += reinterpret_cast<const float*>(sm)[4 * (64 * k + 16 * (n / 4) + m) + n % 4];
+  if (p.bias) y += bf16f(p.bias[n0 + n]);
+  p.y[(long)m * p.ldy + n0 + n] = (uint16_t)pack_bf16x2(y, 0.0f);
 }
 
 template <int TM, int TN, int WM, int WN, int NB>
@@ -156,11 +336,27 @@ hipError_t launch_tile(const Fp8GemmParams& p, hipStream_t st) {
   return hipGetLastError();
 }
 
+constexpr int FP8_TILES = 5, FP8_ROWS = -1;
+
+hipError_t launch_kernel(int tile, const Fp8GemmParams& p, hipStream_t st) {
+  switch (tile) {
+    case FP8_ROWS:
+      if (p.M > 8) fp8_gemm_rows_kernel<16, 2><<<(unsigned)((p.N + 15) / 16), 512, 0, st>>>(p);
+      else fp8_gemm_rows_kernel<8, 3><<<(unsigned)((p.N + 15) / 16), 512, 0, st>>>(p);
+      return hipGetLastError();
+    case 0: return launch_tile<1, 4, 4, 1, 3>(p, st);
+    case 1: return launch_tile<2, 4, 2, 2, 3>(p, st);
+    case 2: return launch_tile<4, 4, 2, 2, 2>(p, st);
+    case 3: return launch_tile<4, 4, 4, 2, 3>(p, st);
+    default: return launch_tile<4, 8, 4, 2, 2>(p, st);
+  }
+}
+
 }  // namespace
 
 hipError_t launch_fp8_gemm(const Fp8GemmParams& p, hipStream_t st) {
   const long large = (p.M + 255L) / 256 * ((p.N + 255L) / 256);
-  return large >= 256 ? launch_tile<4, 8, 4, 2, 2>(p, st) : launch_tile<2, 2, 2, 2, 4>(p, st);
+  return launch_kernel(p.M <= 16 ? FP8_ROWS : large >= 256 ? 4 : 0, p, st);
 }
 
 }  // namespace svdq
