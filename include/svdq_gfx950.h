@@ -484,7 +484,7 @@ int svdq_kv8_append(const void* k, int64_t ldk, const void* v, int64_t ldv, int 
  * and 0 for rows that see nothing and rows behind the last sequence.  Scores and softmax in float32, probabilities (times the
  * page's scale) rounded to bf16.  workspace: svdq_kv8_attention_workspace(...) bytes, 16-byte aligned, no initial
  * contents, not shared by calls that overlap; may be null where that is 0. */
-int64_t svdq_kv8_attention_workspace(int N, int B, int W, int H, int Hkv, int D);
+int64_t svdq_kv8_attention_workspace(int N, int B, int W, int H, int Hkv, int D, int causal);
 int svdq_kv8_attention(const void* q, int64_t ldq, int N, const int* offsets, const int* lengths, const int* table,
                        int B, int W, const void* k_codes, const void* v_codes, const float* scales, int P, int H, int Hkv,
                        int D, float scale, int causal, void* o, void* workspace, hipStream_t stream);

@@ -958,9 +958,9 @@ svdq::Kv8Cache kv8_cache(int N, const int* offsets, const int* lengths, const in
           static_cast<uint8_t*>(const_cast<void*>(v_codes)), const_cast<float*>(scales), N, B, W, P, Hkv, D};
 }
 
-// rows of heads, and tiles times splits (128 at most) of a launch of 256 threads each
+// rows of heads, and the workgroups of a launch: 16 rows each, and up to 8 numbers of no tile a sequence
 bool kv8_fits(int64_t N, int64_t B, int64_t H, int64_t Hkv) {
-  return N * (H / Hkv) <= INT32_MAX && (N * (H / Hkv) / 16 + B + 1) * Hkv <= (int64_t)(UINT32_MAX / 256);
+  return N * (H / Hkv) <= INT32_MAX && (N * (H / Hkv) / 16 + 8 * (B + 2)) * Hkv <= (int64_t)(UINT32_MAX / 256);
 }
 
 }  // namespace
@@ -983,10 +983,10 @@ int svdq_kv8_append(const void* k, int64_t ldk, const void* v, int64_t ldv, int 
                   "kv8_append");
 }
 
-int64_t svdq_kv8_attention_workspace(int N, int B, int W, int H, int Hkv, int D) {
+int64_t svdq_kv8_attention_workspace(int N, int B, int W, int H, int Hkv, int D, int causal) {
   if (N <= 0 || B <= 0 || W <= 0 || Hkv <= 0 || H <= 0 || H % Hkv || (D != 64 && D != 128) || !kv8_fits(N, B, H, Hkv))
     return 0;
-  return svdq::kv8_attention_workspace_bytes(kv8_cache(N, nullptr, nullptr, nullptr, B, W, nullptr, nullptr, nullptr, 1, Hkv, D), H);
+  return svdq::kv8_attention_workspace_bytes(kv8_cache(N, nullptr, nullptr, nullptr, B, W, nullptr, nullptr, nullptr, 1, Hkv, D), H, causal);
 }
 
 int svdq_kv8_attention(const void* q, int64_t ldq, int N, const int* offsets, const int* lengths, const int* table,
@@ -1003,7 +1003,7 @@ int svdq_kv8_attention(const void* q, int64_t ldq, int N, const int* offsets, co
   if (ldq % 8 || !aligned16(q) || !aligned16(o) || !aligned16(workspace))
     return fail(SVDQ_ERR_ALIGN, "%s: 16-byte aligned q, o and workspace, a row stride multiple of 8", fn);
   const svdq::Kv8Cache c = kv8_cache(N, offsets, lengths, table, B, W, k_codes, v_codes, scales, P, Hkv, D);
-  if (!workspace && svdq::kv8_attention_workspace_bytes(c, H) > 0) return fail(SVDQ_ERR_ARG, "%s: no workspace", fn);
+  if (!workspace && svdq::kv8_attention_workspace_bytes(c, H, causal) > 0) return fail(SVDQ_ERR_ARG, "%s: no workspace", fn);
   return launched(svdq::launch_kv8_attention(c, {static_cast<const uint16_t*>(q), ldq, static_cast<uint16_t*>(o), H, scale,
                                                  causal}, workspace, stream),
                   fn);

@@ -252,7 +252,7 @@ struct Kv8Attention {
   float scale;
   int causal;
 };
-long kv8_attention_workspace_bytes(const Kv8Cache& c, int H);
+long kv8_attention_workspace_bytes(const Kv8Cache& c, int H, int causal);
 hipError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Attention& a, void* workspace, hipStream_t st);
 
 }  // namespace svdq

@@ -12,6 +12,9 @@
 //          tokens already; those are then rounded again under the new scale.
 // attend:  o = sum over visible j of softmax_j(scale q . k_j) v_j,  j < length, and with a causal mask, for the i-th of n new
 //          tokens, j <= length - n + i; 0 where nothing is visible.
+#include <cstdlib>
+#include <type_traits>
+
 #include "svdq_fp8.h"
 #include "svdq_kernels.h"
 
@@ -183,6 +186,8 @@ struct Kv8Args {
   long ldq;
   uint16_t* o;
   int H, G, causal, splits;
+  int numbers;      // of tiles, those of no tile among them
+  int whole;        // many rows: an XCD's tiles that are not split
   float scale_log2;
   float* part_o;    // [tile, split, rows, D]
   float* part_ml;   // [tile, split, rows, 2]: maximum (log2 units), sum
@@ -208,19 +213,64 @@ __device__ __forceinline__ int kv8_visible(const Kv8Args& p, const Kv8Tile& t, i
   return p.causal ? max(t.len - t.n + row / p.G + 1, 0) : t.len;
 }
 
+// Many rows: workgroups go round the 8 XCDs, each with an L2 of its own.  With g the largest power of two, 8 at most, that
+// divides the key / value heads, XCD x takes heads x mod g, x mod g + g, ... one after another, and every (8 / g)-th of their
+// tiles: an L2 holds the pages of a head or two at a time.  The last tiles, which see most under a causal mask, go first.
+// An XCD's first `whole` tiles run in one piece, the others in `splits` along the keys.
+__host__ __device__ inline int kv8_shared(int Hkv) { return Hkv % 8 == 0 ? 8 : Hkv % 4 == 0 ? 4 : Hkv % 2 == 0 ? 2 : 1; }
+__host__ __device__ inline long kv8_each(long numbers, int Hkv) {   // an XCD's tiles of a head
+  const int per = 8 / kv8_shared(Hkv);
+  return (numbers + per - 1) / per;
+}
+__device__ __forceinline__ bool kv8_tile_of(const Kv8Args& p, uint32_t x, uint32_t j, int& number, int& hk) {
+  const uint32_t g = kv8_shared(p.c.Hkv), per = 8 / g, each = (uint32_t)kv8_each(p.numbers, p.c.Hkv), head = j / each;
+  const uint32_t s = (j - head * each) * per + x / g;
+  hk = x % g + g * head;
+  number = p.numbers - 1 - s;
+  return s < (uint32_t)p.numbers && head < p.c.Hkv / g;
+}
+// the tile of a workgroup, its piece and where that goes (-1: a whole tile)
+__device__ __forceinline__ bool kv8_piece(const Kv8Args& p, int& number, int& hk, int& split, int& piece) {
+  const uint32_t x = blockIdx.x % 8, j = blockIdx.x / 8;
+  if (j < (uint32_t)p.whole) {
+    split = 0;
+    piece = -1;
+    return kv8_tile_of(p, x, j, number, hk);
+  }
+  const uint32_t k = (j - p.whole) / p.splits;
+  split = (j - p.whole) - k * p.splits;
+  piece = (k * 8 + x) * p.splits + split;
+  return kv8_tile_of(p, x, p.whole + k, number, hk);
+}
+
 __device__ __forceinline__ f32x4 mfma_bf16_16x16x32(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Masked keys have probability 0, but 0 times a code that is not a number is not: where masked keys may hold such codes,
-// they are taken out of the values, and the rows that do see them get them from a product of their own.
-__device__ __forceinline__ uint32_t bf16x2_nan(uint32_t x) {   // 0xFFFF in the halves that are not a number
-  const uint32_t lo = (x & 0x7FFFu) > 0x7F80u ? 0xFFFFu : 0u, hi = (x & 0x7FFF0000u) > 0x7F800000u ? 0xFFFF0000u : 0u;
-  return lo | hi;
+// Masked keys have probability 0, but 0 times a code that is not a number is not.  In pages of which rows see different parts
+// such codes are taken out of the values, and the rows that do see them get them from a product of their own: of ones where
+// the codes are and ones where the row sees the key.
+__device__ __forceinline__ uint32_t fp8x4_nan(uint32_t x) {   // 0x80 in the bytes that are not a number
+  return ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
 }
-__device__ __forceinline__ u32x4 bf16x8_nan(u32x4 x) {
-  return u32x4{bf16x2_nan(x[0]), bf16x2_nan(x[1]), bf16x2_nan(x[2]), bf16x2_nan(x[3])};
+__device__ __forceinline__ uint32_t bytes_of(uint32_t high) {   // 0xFF where a byte's top bit is set, other bits being clear
+  return (high << 1) - (high >> 7);
 }
+// ones (bf16) for the low four, then the high four of eight bits
+__device__ __forceinline__ u32x4 ones_of(uint32_t bits) {
+  u32x4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = (bits >> 2 * e & 1 ? 0x3F80u : 0u) | (bits >> 2 * e & 2 ? 0x3F800000u : 0u);
+  return o;
+}
+// the bits of eight keys from key `from` that lie below `end`
+__device__ __forceinline__ uint32_t bits_below(int from, int end) {
+  const int n = end - from;
+  return n >= 8 ? 0xFFu : n <= 0 ? 0u : (1u << n) - 1u;
+}
+// four bits of bytes that hold 0x80 or 0
+__device__ __forceinline__ uint32_t bits_of(uint32_t high) { return high * 0x00204081u >> 28; }
+
 // bytes of 16 keys from key `from` that lie below `end`
 __device__ __forceinline__ u32x4 keys_below(u32x4 x, int from, int end) {
 #pragma unroll
@@ -231,27 +281,64 @@ __device__ __forceinline__ u32x4 keys_below(u32x4 x, int from, int end) {
   return x;
 }
 
+// The offset of a softmax's exponent follows the maximum only where that is more than 2^KV8_LAZY above it, so the output is
+// hardly ever rescaled; probabilities up to 2^KV8_LAZY are as exact as those below 1.
+constexpr float KV8_LAZY = 8.0f;
+constexpr int KV8_SPLITS = 128;   // at most
+
+__device__ __forceinline__ float other_half_max(float v) {   // over lanes l and l ^ 32
+  uint32_t a = __float_as_uint(v), b = a;
+  permlane32_swap(a, b);
+  return fmaxf(__uint_as_float(a), __uint_as_float(b));
+}
+
 // Few rows: 16 of them a workgroup, whose four waves take the split's pages in turn, each with a softmax of its own; they are
-// joined in LDS at the end.  Pages go from memory straight into the operands of the matrix instructions: a lane's 16 bytes of
-// keys are 16 channels of the key in its row of K, its 16 bytes of values 16 keys of one channel.
+// joined in LDS at the end.  Each wave has a page in LDS to itself, filled by DMA while it computes on the one before, which is
+// in registers by then; the waves need no barrier before the end.
+// A lane reads 16 channels of the key in its row of K, and 16 keys of one channel of V:
 //   S^T = K Q^T: row 4 g + i of tile t stands for key 16 g + 4 t + i, so lane group g gets the probabilities of the 16 keys that
-//   it holds values of; O^T += V^T P^T takes them as they are, tiles 2 u and 2 u + 1 in step u.
+//   it reads values of; O^T += V^T P^T takes them as they are, tiles 2 u and 2 u + 1 in step u.
+// Chunks of 16 bytes lie at slots that spread sixteen lanes' reads over the 64 banks: chunk c of key row r at
+// c ^ (2 (r / 16) + r / 2 mod 2) (rows of 128 bytes; of 64: c ^ (r / 16)), of channel row r of V at c ^ (r / 4 mod 4).
+template <bool NT>
+__device__ __forceinline__ void dma16_page(const void* base, uint32_t off, uint32_t lds) {
+  if (NT) asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+  else dma16(base, off, lds);
+}
+
 template <int D>
-__global__ void __launch_bounds__(256) kv8_rows_kernel(Kv8Args p) {
-  constexpr int R = 16, SP = D / 64, DT = D / 16, PITCH = D + 4;
-  __shared__ __attribute__((aligned(16))) float so[4][R * PITCH];
-  __shared__ float sml[4][R][2];
+struct Kv8Few {
+  static constexpr int R = 16, PITCH = D + 4, HALF = PAGE * D, RING = 2 * HALF, DMA = 2 * HALF / 1024;
+  static_assert(8 * RING <= 160 * 1024 && 4 * R * PITCH * 4 + 4 * R * 8 <= 4 * RING, "LDS");
+  __device__ static int key_turn(int row) { return D == 128 ? row >> 4 << 1 | (row >> 1 & 1) : row >> 4; }
+  // an instruction moves 1024 bytes of a page as they lie, chunks exchanged within their rows
+  template <bool NT>
+  __device__ static void fetch(const uint8_t* kc, const uint8_t* vc, uint32_t koff, uint32_t voff, uint32_t lds) {
+#pragma unroll
+    for (int d = 0; d < DMA / 2; ++d)   // its first key row is d * 1024 / D: what that adds to the turn
+      dma16_page<NT>(kc + 1024 * d, koff ^ 16 * key_turn(d * (1024 / D)), lds + 1024 * d);
+#pragma unroll
+    for (int d = 0; d < DMA / 2; ++d) dma16_page<NT>(vc + 1024 * d, voff, lds + HALF + 1024 * d);
+  }
+};
+
+template <int D>
+__global__ void __launch_bounds__(256, 2) kv8_rows_kernel(Kv8Args p) {
+  using T = Kv8Few<D>;
+  constexpr int R = T::R, SP = D / 64, DT = D / 16, KC = D / 16;
+  __shared__ __attribute__((aligned(1024))) uint8_t sm[4 * T::RING];
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int split = blockIdx.x % p.splits;
-  const int tile = blockIdx.x / p.splits, hk = tile % p.c.Hkv;
+  // heads one after another: a page's heads lie side by side, and the card reads them together from all of its memory (a
+  // head to an XCD reads parts of it: 131072 tokens 99 us, so 75)
+  const uint32_t hk = blockIdx.x % p.c.Hkv, rest = blockIdx.x / p.c.Hkv, split = rest % p.splits, number = rest / p.splits;
   Kv8Tile t;
-  if (!kv8_tile<R>(p, tile / p.c.Hkv, t)) return;
+  if (!kv8_tile<R>(p, number, t)) return;
   const int row = min(t.r0 + lr, t.rows - 1);
   const int vis = kv8_visible(p, t, row);
   const int vmin = kv8_visible(p, t, t.r0), vmax = kv8_visible(p, t, min(t.r0 + R, t.rows) - 1);
   const int pages = (vmax + PAGE - 1) / PAGE, per = (pages + p.splits - 1) / p.splits;
-  const int p0 = split * per, p1 = min(p0 + per, pages);
+  const int p0 = (int)split * per, p1 = min(p0 + per, pages);
 
   u32x4 qf[2 * SP];
   const uint16_t* qr = p.q + (long)(t.row0 + row / p.G) * p.ldq + (hk * p.G + row % p.G) * D + 16 * g;
@@ -260,118 +347,174 @@ __global__ void __launch_bounds__(256) kv8_rows_kernel(Kv8Args p) {
 
   f32x4 O[DT] = {};
   float m = -INFINITY, l = 0.0f;
-  const int* table = p.c.table + (long)t.b * p.c.W;
-  for (int pg = p0 + wave; pg < p1; pg += 4) {
-    const int id = table[pg];
-    if (id < 0 || id >= p.c.P) continue;
-    const long at = (long)id * p.c.Hkv + hk;
-    const uint8_t *kc = p.c.kc + at * PAGE * D + (16 * (lr >> 2) + (lr & 3)) * D + 16 * g, *vc = p.c.vc + at * PAGE * D + lr * PAGE + 16 * g;
-    const float ks = p.c.scales[2 * at] * p.scale_log2, vs = p.c.scales[2 * at + 1];
-    u32x4 kq[4][SP], vq[DT];
+  const int count = p0 + wave < p1 ? (p1 - p0 - wave + 3) / 4 : 0;   // this wave's pages: p0 + wave + 4 i
+  if (count) {
+    const uint32_t lds0 = lds_offset(sm) + wave * T::RING;
+    const uint32_t koff = (lane / KC) * D + 16 * (lane % KC ^ (D == 128 ? lane / KC >> 1 & 1 : 0));
+    const uint32_t voff = (lane / 4) * PAGE + 16 * (lane % 4 ^ (lane / 16 & 3));
+    const int* table = p.c.table + (long)t.b * p.c.W;
+    int id = 0;
+    float ks = 0.0f, vs = 0.0f;
+    auto look_up = [&](int i0) {   // lane i: page i0 + i of this wave; a page that is not there holds nothing
+      const int i = i0 + lane;
+      id = i < count ? table[p0 + wave + 4 * i] : -1;
+      if (id < 0 || id >= p.c.P) id = -1;
+      const long at = (long)max(id, 0) * p.c.Hkv + hk;
+      ks = p.c.scales[2 * at] * p.scale_log2;
+      vs = p.c.scales[2 * at + 1];
+      asm volatile("s_waitcnt vmcnt(0)" : "+v"(id), "+v"(ks), "+v"(vs)::"memory");   // ahead of the DMA, which is not counted
+    };
+    look_up(0);
+    int first = 0;   // the page that lane 0 holds
+    // past the caches where no other tile reads the page (131072 tokens 75 us, so 66)
+    const bool once = t.rows <= R;
+    auto fetch = [&](int i) {   // page i of this wave, past the last one that again
+      const int pid = max(__builtin_amdgcn_readlane(id, max(min(i, count - 1) - first, 0)), 0);
+      const long at = (long)pid * p.c.Hkv + hk;
+      const uint8_t *kc = p.c.kc + at * T::HALF, *vc = p.c.vc + at * T::HALF;
+      if (once) T::template fetch<true>(kc, vc, koff, voff, lds0);
+      else T::template fetch<false>(kc, vc, koff, voff, lds0);
+    };
+    fetch(0);
+    auto rescale = [&](float top) {
+      const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn;
+      const float alpha = __builtin_amdgcn_exp2f(m - base);
+      m = mn;
+      l *= alpha;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int d = 0; d < DT; ++d) O[d] *= alpha;
+    };
+    auto rows_max = [](float v) {   // over the four lanes of a row
+      v = fmaxf(v, __shfl_xor(v, 16, 64));
+      return other_half_max(v);
+    };
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) {
+      const int pg = p0 + wave + 4 * i;
+      const bool have = __builtin_amdgcn_readlane(id, i - first) >= 0;
+      const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), i - first));
+      const float pv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), i - first));
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      const uint8_t *sk = sm + wave * T::RING, *sv = sk + T::HALF;
+      u32x4 kq[4][SP], vq[DT];
 #pragma unroll
-      for (int s = 0; s < SP; ++s) kq[i][s] = ld16(kc + 4 * i * D + 64 * s);
+      for (int k = 0; k < 4; ++k) {
+        const int r = 16 * (lr >> 2) + 4 * k + (lr & 3);
 #pragma unroll
-    for (int d = 0; d < DT; ++d) vq[d] = ld16(vc + 16 * d * PAGE);
-    f32x4 S[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      S[i] = f32x4{};
-#pragma unroll
-      for (int s = 0; s < SP; ++s) {
-        S[i] = mfma_bf16_16x16x32(fp8_to_bf16x8(kq[i][s][0], kq[i][s][1]), qf[2 * s], S[i]);
-        S[i] = mfma_bf16_16x16x32(fp8_to_bf16x8(kq[i][s][2], kq[i][s][3]), qf[2 * s + 1], S[i]);
+        for (int s = 0; s < SP; ++s) kq[k][s] = ld16(sk + r * D + 16 * ((4 * s + g) ^ T::key_turn(r)));
       }
-    }
-    const int key0 = pg * PAGE + 16 * g;
-    const bool edge = pg * PAGE + PAGE > vmin;   // some row does not see all of the page
-    if (edge) {
 #pragma unroll
-      for (int d = 0; d < DT; ++d) vq[d] = keys_below(vq[d], key0, vmax);
-    }
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        S[i][r] = edge && key0 + 4 * i + r >= vis ? -INFINITY : S[i][r] * ks;
-        top = fmaxf(top, S[i][r]);
+      for (int d = 0; d < DT; ++d) vq[d] = ld16(sv + (16 * d + lr) * PAGE + 16 * (g ^ (lr >> 2)));
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // all of the page is in registers
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + 1 - first >= 64) {   // its next page is not among those looked up
+        first = i + 1;
+        look_up(first);
       }
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn;
-    const float alpha = __builtin_amdgcn_exp2f(m - base);
-    m = mn;
-    l *= alpha;
-    u32x4 pf[2];
+      fetch(i + 1);
+      if (!have) continue;
+      f32x4 S[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+      for (int k = 0; k < 4; ++k) {
+        S[k] = f32x4{};
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        S[i][r] = __builtin_amdgcn_exp2f(S[i][r] - base);
-        l += S[i][r];
-      }
-      pf[i / 2][2 * (i % 2)] = pack_bf16x2(S[i][0] * vs, S[i][1] * vs);
-      pf[i / 2][2 * (i % 2) + 1] = pack_bf16x2(S[i][2] * vs, S[i][3] * vs);
-    }
-    uint32_t odd = 0;   // codes that are not a number, in a page of which rows see different parts
-#pragma unroll
-    for (int d = 0; d < DT; ++d) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) O[d][r] *= alpha;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        u32x4 vf = fp8_to_bf16x8(vq[d][2 * u], vq[d][2 * u + 1]);
-        if (edge) {
-          const u32x4 bad = bf16x8_nan(vf);
-          vf &= ~bad;
-          odd |= bad[0] | bad[1] | bad[2] | bad[3];
+        for (int s = 0; s < SP; ++s) {
+          S[k] = mfma_bf16_16x16x32(fp8_to_bf16x8(kq[k][s][0], kq[k][s][1]), qf[2 * s], S[k]);
+          S[k] = mfma_bf16_16x16x32(fp8_to_bf16x8(kq[k][s][2], kq[k][s][3]), qf[2 * s + 1], S[k]);
         }
-        O[d] = mfma_bf16_16x16x32(vf, pf[u], O[d]);
       }
-    }
-    if (edge && __any(odd != 0)) {
-      u32x4 seen[2];
+      u32x4 pf[2];
+      if (pg * PAGE + PAGE <= vmin && f >= 0.0f && pv > 0x1p-60f && pv < 0x1p60f) {
+        const float lv = __builtin_amdgcn_logf(pv);   // log2
+        float hi = S[0][0];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+        for (int k = 0; k < 16; ++k) hi = fmaxf(hi, S[k / 4][k % 4]);
+        const float top = rows_max(hi * f);
+        if (__any(top > m + KV8_LAZY)) rescale(top);
+        const float off = (m == -INFINITY ? 0.0f : m) - lv;
+        float sum = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          seen[u][e] = (key0 + 8 * u + 2 * e < vis ? 0x3F80u : 0u) | (key0 + 8 * u + 2 * e + 1 < vis ? 0x3F800000u : 0u);
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        f32x4 hit = {};
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const u32x4 bad = bf16x8_nan(fp8_to_bf16x8(vq[d][2 * u], vq[d][2 * u + 1])) & 0x3F803F80u;
-          hit = mfma_bf16_16x16x32(bad, seen[u], hit);
+        for (int k = 0; k < 16; k += 2) {
+          const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(S[k / 4][k % 4], f, -off));
+          const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(S[k / 4][k % 4 + 1], f, -off));
+          const uint32_t w = pack_bf16x2(a, b);
+          pf[k / 8][k % 8 / 2] = w;
+          sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3F803F80u), sum, false);
         }
+        l = __builtin_fmaf(sum, 1.0f / pv, l);
+      } else {   // masks, values that are not numbers behind them, any scales
+        const int key0 = pg * PAGE + 16 * g;
+        float hi = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) O[d][r] = hit[r] > 0.0f ? __builtin_nanf("") : O[d][r];
+        for (int k = 0; k < 16; ++k) {
+          S[k / 4][k % 4] = key0 + k >= vis ? -INFINITY : S[k / 4][k % 4] * f;
+          hi = fmaxf(hi, S[k / 4][k % 4]);
+        }
+        const float top = rows_max(hi);
+        if (__any(top > m + KV8_LAZY)) rescale(top);
+        const float off = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int k = 0; k < 16; k += 2) {
+          const float a = __builtin_amdgcn_exp2f(S[k / 4][k % 4] - off), b = __builtin_amdgcn_exp2f(S[k / 4][k % 4 + 1] - off);
+          l += a + b;
+          pf[k / 8][k % 8 / 2] = pack_bf16x2(a * pv, b * pv);
+        }
+        uint32_t odd = 0;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          vq[d] = keys_below(vq[d], key0, vmax);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd |= fp8x4_nan(vq[d][e]);
+        }
+        if (__any(odd != 0)) {
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            f32x4 hit = {};
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t lo = fp8x4_nan(vq[d][2 * u]), hi4 = fp8x4_nan(vq[d][2 * u + 1]);
+              hit = mfma_bf16_16x16x32(ones_of(bits_of(lo) | bits_of(hi4) << 4), ones_of(bits_below(key0 + 8 * u, vis)), hit);
+              vq[d][2 * u] &= ~bytes_of(lo);
+              vq[d][2 * u + 1] &= ~bytes_of(hi4);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) O[d][r] = hit[r] > 0.0f ? __builtin_nanf("") : O[d][r];
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);   // the values are not converted ahead of the softmax: there are no registers for them
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) O[d] = mfma_bf16_16x16x32(fp8_to_bf16x8(vq[d][2 * u], vq[d][2 * u + 1]), pf[u], O[d]);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
+  __syncthreads();   // every ring is done with; their memory takes the waves' sums
+  float* so = reinterpret_cast<float*>(sm);
+  float* sml = so + 4 * R * T::PITCH;
 #pragma unroll
-  for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(&so[wave][lr * PITCH + 16 * d + 4 * g]) = O[d];
+  for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(so + (wave * R + lr) * T::PITCH + 16 * d + 4 * g) = O[d];
   if (g == 0) {
-    sml[wave][lr][0] = m;
-    sml[wave][lr][1] = l;
+    sml[2 * (wave * R + lr)] = m;
+    sml[2 * (wave * R + lr) + 1] = l;
   }
   __syncthreads();
   // 16 threads a row
   const int r = tid >> 4, c0 = (tid & 15) * (D / 16);
   float mm = -INFINITY, ll = 0.0f, o[D / 16] = {};
 #pragma unroll
-  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sml[w][r][0]);
+  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, sml[2 * (w * R + r)]);
   const float base = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    const float f = __builtin_amdgcn_exp2f(sml[w][r][0] - base);
-    ll += f * sml[w][r][1];
+    const float f = __builtin_amdgcn_exp2f(sml[2 * (w * R + r)] - base);
+    ll += f * sml[2 * (w * R + r) + 1];
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) o[i] += f * so[w][r * PITCH + c0 + i];
+    for (int i = 0; i < D / 16; ++i) o[i] += f * so[(w * R + r) * T::PITCH + c0 + i];
   }
   if (t.r0 + r >= t.rows) return;
   if (p.splits == 1) {
@@ -382,7 +525,7 @@ __global__ void __launch_bounds__(256) kv8_rows_kernel(Kv8Args p) {
       *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(o[i] * inv, o[i + 1] * inv);
     return;
   }
-  const long at = (long)blockIdx.x * R + r;
+  const long at = (((long)number * p.c.Hkv + hk) * p.splits + split) * R + r;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) p.part_o[at * D + c0 + i] = o[i];
   if ((tid & 15) == 0) {
@@ -391,178 +534,353 @@ __global__ void __launch_bounds__(256) kv8_rows_kernel(Kv8Args p) {
   }
 }
 
-// Joins the splits of 16 rows of a tile of R.
+// Joins the splits of two rows of a tile of R: a wave finds the weights of a row's splits, a split a lane; then 32 lanes take a
+// row's columns, four of them each, and four such groups every fourth split.
 template <int D, int R>
 __global__ void __launch_bounds__(256) kv8_join_kernel(Kv8Args p) {
-  const int tile = blockIdx.x / (R / 16), part = blockIdx.x % (R / 16), hk = tile % p.c.Hkv;
+  constexpr int C = D / 32;   // columns of a lane
+  __shared__ float weight[2][KV8_SPLITS], total[2];
+  __shared__ float part[2][4][D];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t tile = blockIdx.x / (R / 2);
+  const int r0 = 2 * (blockIdx.x % (R / 2));
+  int number = tile / p.c.Hkv, hk = tile % p.c.Hkv;
+  if (R > 16 && !kv8_tile_of(p, tile % 8, p.whole + tile / 8, number, hk)) return;
   Kv8Tile t;
-  if (!kv8_tile<R>(p, tile / p.c.Hkv, t)) return;
-  const int r = 16 * part + (threadIdx.x >> 4), c0 = (threadIdx.x & 15) * (D / 16);
-  if (t.r0 + r >= t.rows) return;
-  const long first = (long)tile * p.splits * R + r;
-  float mm = -INFINITY, ll = 0.0f, o[D / 16] = {};
-  for (int s = 0; s < p.splits; ++s) mm = fmaxf(mm, p.part_ml[2 * (first + (long)s * R)]);
-  const float base = mm == -INFINITY ? 0.0f : mm;
-  for (int s = 0; s < p.splits; ++s) {
-    const long at = first + (long)s * R;
-    const float f = __builtin_amdgcn_exp2f(p.part_ml[2 * at] - base);
-    ll += f * p.part_ml[2 * at + 1];
+  if (!kv8_tile<R>(p, number, t)) return;
+  if (t.r0 + r0 >= t.rows) return;
+  const long first = (long)tile * p.splits * R + r0;
+  if (wave < 2) {
+    float m[KV8_SPLITS / 64], l[KV8_SPLITS / 64], top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) o[i] += f * p.part_o[at * D + c0 + i];
+    for (int i = 0; i < KV8_SPLITS / 64; ++i) {
+      const int s = 64 * i + lane;
+      const long at = first + wave + (long)min(s, p.splits - 1) * R;
+      m[i] = s < p.splits ? p.part_ml[2 * at] : -INFINITY;
+      l[i] = p.part_ml[2 * at + 1];
+      top = fmaxf(top, m[i]);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int i = 0; i < KV8_SPLITS / 64; ++i) {
+      const float f = __builtin_amdgcn_exp2f(m[i] - base);
+      weight[wave][64 * i + lane] = f;
+      if (64 * i + lane < p.splits) sum += f * l[i];
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) total[wave] = sum;
   }
-  const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-  uint16_t* out = p.o + ((long)(t.row0 + (t.r0 + r) / p.G) * p.H + hk * p.G + (t.r0 + r) % p.G) * D + c0;
+  __syncthreads();
+  const int r = tid >> 7, g = tid >> 5 & 3, c0 = (tid & 31) * C;
+  float o[C] = {};
+#pragma unroll 4
+  for (int s = g; s < p.splits; s += 4) {
+    const float f = weight[r][s];
+    const float* from = p.part_o + (first + r + (long)s * R) * D + c0;
 #pragma unroll
-  for (int i = 0; i < D / 16; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack_bf16x2(o[i] * inv, o[i + 1] * inv);
+    for (int i = 0; i < C; ++i) o[i] += f * from[i];
+  }
+#pragma unroll
+  for (int i = 0; i < C; ++i) part[r][g][c0 + i] = o[i];
+  __syncthreads();
+  const int row = t.r0 + r0 + (tid >> 7), c = tid & 127;
+  if (row >= t.rows || 2 * c >= D) return;
+  const float sum = total[tid >> 7], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  float y[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float(&q)[4][D] = part[tid >> 7];
+    y[i] = ((q[0][2 * c + i] + q[1][2 * c + i]) + (q[2][2 * c + i] + q[3][2 * c + i])) * inv;
+  }
+  uint16_t* out = p.o + ((long)(t.row0 + row / p.G) * p.H + hk * p.G + row % p.G) * D;
+  *reinterpret_cast<uint32_t*>(out + 2 * c) = pack_bf16x2(y[0], y[1]);
 }
 
-// Many rows: 32 a wave, 128 a workgroup; pages go through LDS, as bf16, for its four waves.  A lane holds one row's scores of half of
-// the keys.  Row 16 s + 8 a + 4 h + i of K in LDS order is key 16 s + 8 h + 4 a + i of the page (bits 2 and 3 exchanged), so that the
-// probabilities leave the softmax in the values' order.
+// Many rows: 32 a wave, 128 a workgroup; pages go through LDS, as bf16, for its four waves.  Two workgroups share a CU, so that
+// one's softmax runs under the other's products.  A lane holds one row's scores of half of the keys.  Row
+// 16 s + 8 a + 4 h + i of K in LDS is key 16 s + 8 h + 4 a + i of the page (bits 2 and 3 exchanged), so that the probabilities
+// leave the softmax in the values' order.
+//
+// The scale of the keys is part of the exponent's factor, that of the values (vs) of its offset:
+// exp2(f s - (m - log2 vs)) = vs p, which is what the product needs; the row's sum takes the rounded values over vs, two in an
+// instruction.  The offset is a row's maximum over the first page and stays, so the output is touched by the matrix unit
+// alone; later probabilities may exceed 1, which float32 and bf16 hold as exactly.  Where a sum passes 2^64, anything is
+// not finite, or a page of which rows see different parts holds values that are no numbers, the tile is done again with an
+// offset that follows the maximum.
+// Scales that are no ordinary positive numbers are dealt with as the pages come in: a factor below 0 turns the keys' signs, other
+// scales of values are multiplied into them.  Pages that are not there count as -infinity.
+//
+// Rows in LDS are not padded: chunks of 16 bytes lie at slots exchanged by the row, c ^ (row mod 16) in rows of 256 bytes, c ^
+// (row / 2 mod 8) in rows of 128, which spreads sixteen lanes' reads of a chunk, and sixteen lanes' writes of two chunks each, over the 64
+// banks.
 template <int D>
 struct Kv8Many {
-  static constexpr int R = 128, KP = 2 * D + 16, VP = 2 * PAGE + 16, CH = PAGE * D / 16 / 256;
+  static constexpr int R = 128, CH = PAGE * D / 16 / 256, DB = D / 32, KS = D / 16, KB = PAGE * D * 2;   // bytes of a buffer
+  __device__ static int key_turn(int row) { return D == 128 ? row & 15 : row >> 1 & 7; }
+  __device__ static int value_turn(int row) { return row >> 1 & 7; }
+};
+
+struct Kv8Scale {
+  float f, lv, inv, at;   // the exponent's factor, log2 of the values' scale and its reciprocal, 0 or (no page) -infinity
 };
 
 template <int D>
 __global__ void __launch_bounds__(256, 2) kv8_many_kernel(Kv8Args p) {
   using T = Kv8Many<D>;
-  __shared__ __attribute__((aligned(16))) uint8_t sk[2][PAGE * T::KP];
-  __shared__ __attribute__((aligned(16))) uint8_t sv[2][D * T::VP];
+  constexpr int DB = T::DB, KS = T::KS, KB = T::KB;
+  __shared__ __attribute__((aligned(1024))) uint8_t sk[2 * KB], sv[2 * KB];
+  __shared__ uint16_t odd_keys[D][4];   // bits of the codes that are not numbers, of a page that some row sees a part of
+  __shared__ int odd_any[4];            // whether a wave found any
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int split = blockIdx.x % p.splits;
-  const int tile = blockIdx.x / p.splits, hk = tile % p.c.Hkv;
+  int number, hk, split, piece;
+  if (!kv8_piece(p, number, hk, split, piece)) return;
   Kv8Tile t;
-  if (!kv8_tile<T::R>(p, tile / p.c.Hkv, t)) return;
-  const int row = min(t.r0 + 32 * wave + lr, t.rows - 1);
-  const int vis = kv8_visible(p, t, row);
+  if (!kv8_tile<T::R>(p, number, t)) return;
   const int vmin = kv8_visible(p, t, t.r0), vmax = kv8_visible(p, t, min(t.r0 + T::R, t.rows) - 1);
-  const int pages = (vmax + PAGE - 1) / PAGE, per = (pages + p.splits - 1) / p.splits;
-  const int p0 = split * per, p1 = min(p0 + per, pages);
+  const int pages = (vmax + PAGE - 1) / PAGE, pieces = piece < 0 ? 1 : p.splits, per = (pages + pieces - 1) / pieces;
+  const int p0 = split * per, p1 = min(p0 + per, pages), pe = vmin / PAGE;   // pages from pe on: some row sees a part of them
 
-  u32x4 qf[D / 16];
+  const int row = min(t.r0 + 32 * wave + lr, t.rows - 1), vis = kv8_visible(p, t, row);
+  u32x4 qf[KS];
   const uint16_t* qr = p.q + (long)(t.row0 + row / p.G) * p.ldq + (hk * p.G + row % p.G) * D + 8 * h;
 #pragma unroll
-  for (int s = 0; s < D / 16; ++s) qf[s] = ld16(qr + 16 * s);
+  for (int s = 0; s < KS; ++s) qf[s] = ld16(qr + 16 * s);
 
+  // Pages, their scales and what follows from those are looked up 64 at a time, one a lane.
   const int* table = p.c.table + (long)t.b * p.c.W;
+  int ids = -1, first = p0;   // the page that lane 0 holds
+  float kss = 0.0f, vss = 0.0f, lvs = 0.0f, invs = 1.0f;
+  uint64_t odd_scales = 0;    // pages that are not there or whose scales are no ordinary numbers
+  auto ordinary = [](float vs) { return vs > 0x1p-60f && vs < 0x1p60f; };
+  auto look_up = [&](int from) __attribute__((always_inline)) {
+    first = from;
+    ids = from + lane < p1 ? table[from + lane] : -1;
+    if (ids < 0 || ids >= p.c.P) ids = -1;
+    const long at = (long)max(ids, 0) * p.c.Hkv + hk;
+    kss = p.c.scales[2 * at] * p.scale_log2;
+    vss = p.c.scales[2 * at + 1];
+    lvs = ordinary(vss) ? __builtin_amdgcn_logf(vss) : 0.0f;   // log2
+    invs = ordinary(vss) ? 1.0f / vss : 1.0f;
+    odd_scales = __ballot(ids < 0 || !ordinary(vss) || !(kss > 0.0f));
+  };
+  auto lane_of = [](float v, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i)); };
   u32x4 kr[T::CH], vr[T::CH];
-  float ks_next = 0.0f, vs_next = 0.0f;
-  bool have_next = false;
-  auto load = [&](int pg) {
-    const int id = table[pg];
-    have_next = id >= 0 && id < p.c.P;
-    const long at = (long)(have_next ? id : 0) * p.c.Hkv + hk;
-    ks_next = p.c.scales[2 * at] * p.scale_log2;
-    vs_next = p.c.scales[2 * at + 1];
+  auto load = [&](int pg) __attribute__((always_inline)) {
+    const int id = max(__builtin_amdgcn_readlane(ids, pg - first), 0);
+    const long at = ((long)id * p.c.Hkv + hk) * PAGE * D;
+    const __amdgpu_buffer_rsrc_t k = __builtin_amdgcn_make_buffer_rsrc(p.c.kc + at, (short)0, PAGE * D, 0x00020000);
+    const __amdgpu_buffer_rsrc_t v = __builtin_amdgcn_make_buffer_rsrc(p.c.vc + at, (short)0, PAGE * D, 0x00020000);
 #pragma unroll
     for (int i = 0; i < T::CH; ++i) {
-      kr[i] = ld16(p.c.kc + at * PAGE * D + 16 * (tid + 256 * i));
-      vr[i] = ld16(p.c.vc + at * PAGE * D + 16 * (tid + 256 * i));
+      kr[i] = __builtin_amdgcn_raw_buffer_load_b128(k, 16 * tid + 4096 * i, 0, 0);
+      vr[i] = __builtin_amdgcn_raw_buffer_load_b128(v, 16 * tid + 4096 * i, 0, 0);
     }
   };
-  auto store = [&](int pg, int buf) {
+  auto scale_in = [&](int pg) __attribute__((always_inline)) {
+    const int i = pg - first;
+    Kv8Scale s{lane_of(kss, i), lane_of(lvs, i), lane_of(invs, i), 0.0f};
+    if (odd_scales >> i & 1) {
+      // a factor of 0 is the smallest there is: times -infinity that is no NaN
+      s.f = s.f == 0.0f ? 0x1p-126f : fabsf(s.f);
+      if (__builtin_amdgcn_readlane(ids, i) < 0) s = {0x1p-126f, -INFINITY, 1.0f, -INFINITY};
+    }
+    return s;
+  };
+  // The tile is to be done again: offsets that are too low for a later score, nothing there of the first page, values that
+  // are no numbers behind a mask.
+  bool again = false;
+  auto store = [&](int pg, int buf) __attribute__((always_inline)) {
+    const int i0 = pg - first;
+    const bool odd = odd_scales >> i0 & 1, here = __builtin_amdgcn_readlane(ids, i0) >= 0;
+    const float vs = odd && here ? lane_of(vss, i0) : 1.0f;
+    if (odd) {
+      const uint32_t turn = here && lane_of(kss, i0) < 0.0f ? 0x80808080u : 0u, keep = here ? ~0u : 0u;
+#pragma unroll
+      for (int i = 0; i < T::CH; ++i) {
+        kr[i] = (kr[i] & keep) ^ turn;
+        vr[i] &= keep;
+      }
+    }
+    if (pg >= pe) {
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < T::CH; ++i) {
+        const int c = tid + 256 * i;
+        vr[i] = keys_below(vr[i], pg * PAGE + 16 * (c % 4), vmax);
+        uint32_t bits = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t high = fp8x4_nan(vr[i][e]);
+          bits |= bits_of(high) << 4 * e;
+          vr[i][e] &= ~bytes_of(high);
+        }
+        odd_keys[c / 4][c % 4] = (uint16_t)bits;
+        any |= bits;
+      }
+      const int found = __any(any != 0);
+      if (lane == 0) odd_any[wave] = found;
+      again |= found != 0;
+    }
 #pragma unroll
     for (int i = 0; i < T::CH; ++i) {
-      const int c = tid + 256 * i, key = c / (D / 16), kd = c % (D / 16), d = c / 4, vk = 16 * (c % 4);
-      // key's row: bits 2 and 3 exchanged
-      const int kro = (key & ~12) | (key & 4) << 1 | (key & 8) >> 1;
-      *reinterpret_cast<u32x4*>(&sk[buf][kro * T::KP + 32 * kd]) = fp8_to_bf16x8(kr[i][0], kr[i][1]);
-      *reinterpret_cast<u32x4*>(&sk[buf][kro * T::KP + 32 * kd + 16]) = fp8_to_bf16x8(kr[i][2], kr[i][3]);
-      const u32x4 x = pg * PAGE + PAGE > vmax ? keys_below(vr[i], pg * PAGE + vk, vmax) : vr[i];
-      *reinterpret_cast<u32x4*>(&sv[buf][d * T::VP + 2 * vk]) = fp8_to_bf16x8(x[0], x[1]);
-      *reinterpret_cast<u32x4*>(&sv[buf][d * T::VP + 2 * vk + 16]) = fp8_to_bf16x8(x[2], x[3]);
-    }
-  };
-
-  f32x16 O[D / 32] = {};
-  float m = -INFINITY, l = 0.0f;
-  if (p0 < p1) {
-    load(p0);
-    store(p0, 0);
-  }
-  float ks = ks_next, vs = vs_next;
-  bool have = have_next;
-  __syncthreads();
-  for (int pg = p0; pg < p1; ++pg) {
-    const int buf = (pg - p0) & 1;
-    if (pg + 1 < p1) load(pg + 1);
-    const bool edge = pg * PAGE + PAGE > vmin || !have;
-    const int sees = have ? vis : 0;
+      const int c = tid + 256 * i, key = c / KS, kd = c % KS, d = c / 4, j = c % 4;
+      const int kro = (key & ~12) | (key & 4) << 1 | (key & 8) >> 1;   // key's row: bits 2 and 3 exchanged
+      uint8_t* kt = sk + buf * KB + kro * 2 * D + 16 * (2 * kd ^ T::key_turn(kro));
+      uint8_t* vt = sv + buf * KB + d * 2 * PAGE + 16 * (2 * j ^ T::value_turn(d));
+      const int ko = T::key_turn(kro) & 1 ? -16 : 16, vo = T::value_turn(d) & 1 ? -16 : 16;   // to chunk c ^ 1
+      *reinterpret_cast<u32x4*>(kt) = fp8_to_bf16x8(kr[i][0], kr[i][1]);
+      *reinterpret_cast<u32x4*>(kt + ko) = fp8_to_bf16x8(kr[i][2], kr[i][3]);
+      u32x4 lo = fp8_to_bf16x8(vr[i][0], vr[i][1]), hi = fp8_to_bf16x8(vr[i][2], vr[i][3]);
+      if (odd && !ordinary(vs)) {
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      f32x16 S = {};
-      const uint8_t* ka = &sk[buf][(32 * hf + lr) * T::KP + 16 * h];
-#pragma unroll
-      for (int s = 0; s < D / 16; ++s) S = mfma_bf16_32x32x16(ld16(ka + 32 * s), qf[s], S);
-      const int key0 = pg * PAGE + 32 * hf + 8 * h;   // register 8 s + 4 a + i: key 16 s + 4 a + i further
-      float top = -INFINITY;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        S[r] = edge && key0 + 16 * (r / 8) + r % 8 >= sees ? -INFINITY : S[r] * ks;
-        top = fmaxf(top, S[r]);
-      }
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn;
-      const float alpha = __builtin_amdgcn_exp2f(m - base);
-      m = mn;
-      l *= alpha;
-      u32x4 pf[2];
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        const float a = __builtin_amdgcn_exp2f(S[r] - base), b = __builtin_amdgcn_exp2f(S[r + 1] - base);
-        l += a + b;
-        pf[r / 8][r % 8 / 2] = pack_bf16x2(a * vs, b * vs);
-      }
-      if (!have) pf[0] = pf[1] = u32x4{};   // 0 times a scale that is not there
-#pragma unroll
-      for (int db = 0; db < D / 32; ++db) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) O[db][r] *= alpha;
-        const uint8_t* va = &sv[buf][(32 * db + lr) * T::VP + 16 * h + 64 * hf];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          u32x4 vf = ld16(va + 32 * s);
-          if (edge) {
-            const u32x4 bad = bf16x8_nan(vf);
-            vf &= ~bad;
-            if (have && __any((bad[0] | bad[1] | bad[2] | bad[3]) != 0)) {
-              u32x4 seen;
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                seen[e] = (key0 + 16 * s + 2 * e < vis ? 0x3F80u : 0u) | (key0 + 16 * s + 2 * e + 1 < vis ? 0x3F800000u : 0u);
-              const f32x16 hit = mfma_bf16_32x32x16(bad & 0x3F803F80u, seen, f32x16{});
-#pragma unroll
-              for (int r = 0; r < 16; ++r) O[db][r] = hit[r] > 0.0f ? __builtin_nanf("") : O[db][r];
-            }
-          }
-          O[db] = mfma_bf16_32x32x16(vf, pf[s], O[db]);
+        for (int e = 0; e < 4; ++e) {
+          lo[e] = pack_bf16x2(bf16lo(lo[e]) * vs, bf16hi(lo[e]) * vs);
+          hi[e] = pack_bf16x2(bf16lo(hi[e]) * vs, bf16hi(hi[e]) * vs);
         }
       }
+      *reinterpret_cast<u32x4*>(vt) = lo;
+      *reinterpret_cast<u32x4*>(vt + vo) = hi;
     }
-    if (pg + 1 < p1) store(pg + 1, buf ^ 1);
-    ks = ks_next;
-    vs = vs_next;
-    have = have_next;
+  };
+
+  f32x16 O[DB], S[2];
+  u32x4 pf[2][2];
+  float m, l;   // the exponent's offset (log2 units), this lane's part of the sum
+  // This lane's chunk 2 g + h of its row of K, 2 s + h of its row of V: 32 g or 32 s exchanged into the address of the first.
+  const uint32_t kl = lr * 2 * D + 16 * (h ^ T::key_turn(lr)), vl = lr * 2 * PAGE + 16 * (h ^ T::value_turn(lr));
+  auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db) O[db] = f32x16{};
+    m = -INFINITY;
+    l = 0.0f;
+  };
+  auto scores = [&](int buf) __attribute__((always_inline)) {
+    S[0] = S[1] = f32x16{};
+#pragma unroll
+    for (int g = 0; g < KS; ++g)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) S[hf] = mfma_bf16_32x32x16(ld16(sk + (kl ^ 32 * g) + buf * KB + hf * 64 * D), qf[g], S[hf]);
+  };
+  auto masked = [&](int pg) __attribute__((always_inline)) {   // register 8 s + 4 a + i: key 16 s + 4 a + i of the lane's
+    const int key0 = pg * PAGE + 8 * h;
+#pragma unroll
+    for (int r = 0; r < 32; ++r)
+      if (key0 + 16 * (r / 8) + r % 8 >= vis) S[r / 16][r % 16] = -INFINITY;
+  };
+  auto top_of = [&](const Kv8Scale& w) __attribute__((always_inline)) {   // the row's largest score
+    float hi = S[0][0];
+#pragma unroll
+    for (int r = 1; r < 32; ++r) hi = fmaxf(hi, S[r / 16][r % 16]);
+    return other_half_max(__builtin_fmaf(hi, w.f, w.at));
+  };
+  auto softmax = [&](const Kv8Scale& w) __attribute__((always_inline)) {
+    const float off = (m == -INFINITY ? 0.0f : m) - w.lv;
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int r = 0; r < 32; r += 2) {
+      const int hf = r / 16, q = r % 16;
+      const uint32_t x = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(S[hf][q], w.f, -off)),
+                                     __builtin_amdgcn_exp2f(__builtin_fmaf(S[hf][q + 1], w.f, -off)));
+      pf[hf][q / 8][q % 8 / 2] = x;
+      sum[hf] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), __builtin_bit_cast(bf16x2, 0x3F803F80u), sum[hf], false);
+    }
+    l = __builtin_fmaf(sum[0] + sum[1], w.inv, l);
+  };
+  auto values = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+        O[db] = mfma_bf16_32x32x16(ld16(sv + (vl ^ 32 * s) + buf * KB + db * 64 * PAGE), pf[s / 2][s % 2], O[db]);
+  };
+  clear();
+  if (p0 < p1) {
+    look_up(p0);
+    load(p0);
+    store(p0, 0);
+    Kv8Scale now = scale_in(p0);
+    again |= __builtin_amdgcn_readlane(ids, 0) < 0;
     __syncthreads();
+    auto stage = [&](int pg, int buf) __attribute__((always_inline)) {
+      const int next = min(pg + 1, p1 - 1);
+      if (next - first >= 64) look_up(next);
+      load(next);
+      scores(buf);
+      if (pg >= pe) masked(pg);
+      if (pg == p0) m = top_of(now);
+      softmax(now);
+      values(buf);
+      store(next, buf ^ 1);
+      now = scale_in(next);
+      __syncthreads();
+    };
+    for (int pg = p0; pg < p1; pg += 2) {
+      stage(pg, 0);
+      if (pg + 1 < p1) stage(pg + 1, 1);
+    }
+  }
+  again |= !(l <= 0x1p64f);   // infinities and NaN among them
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) again |= !(fabsf(O[db][r]) < INFINITY);
+  if (__syncthreads_or(again)) {
+    clear();
+    for (int pg = p0; pg < p1; ++pg) {
+      if ((pg - p0) % 64 == 0) look_up(pg);
+      load(pg);
+      __syncthreads();
+      store(pg, 0);
+      const Kv8Scale w = scale_in(pg);
+      __syncthreads();
+      scores(0);
+      if (pg >= pe) {
+        masked(pg);
+        // rows that see a key whose value is not a number
+        if (odd_any[0] | odd_any[1] | odd_any[2] | odd_any[3]) {
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            f32x16 hit = {};
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              hit = mfma_bf16_32x32x16(ones_of(odd_keys[32 * db + lr][s] >> 8 * h & 0xFFu),
+                                       ones_of(bits_below(pg * PAGE + 16 * s + 8 * h, vis)), hit);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) O[db][r] = hit[r] > 0.0f ? __builtin_nanf("") : O[db][r];
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+      const float mn = fmaxf(m, top_of(w)), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.0f : mn));
+      m = mn;
+      l *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db) O[db] *= alpha;
+      softmax(w);
+      values(0);
+    }
   }
   l += __shfl_xor(l, 32, 64);
-  if (t.r0 + 32 * wave + lr >= t.rows) return;
-  if (p.splits == 1) {
+  const int r = t.r0 + 32 * wave + lr;
+  if (r >= t.rows) return;
+  if (piece < 0) {
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* out = p.o + ((long)(t.row0 + row / p.G) * p.H + hk * p.G + row % p.G) * D + 4 * h;
+    uint16_t* out = p.o + ((long)(t.row0 + r / p.G) * p.H + hk * p.G + r % p.G) * D + 4 * h;
 #pragma unroll
-    for (int db = 0; db < D / 32; ++db)
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         *reinterpret_cast<u32x2*>(out + 32 * db + 8 * q) = u32x2{pack_bf16x2(O[db][4 * q] * inv, O[db][4 * q + 1] * inv),
                                                                  pack_bf16x2(O[db][4 * q + 2] * inv, O[db][4 * q + 3] * inv)};
     return;
   }
-  const long at = (long)blockIdx.x * T::R + 32 * wave + lr;
+  const long at = (long)piece * T::R + r - t.r0;
 #pragma unroll
-  for (int db = 0; db < D / 32; ++db)
+  for (int db = 0; db < DB; ++db)
 #pragma unroll
     for (int q = 0; q < 4; ++q)
       *reinterpret_cast<f32x4*>(p.part_o + at * D + 32 * db + 8 * q + 4 * h) =
@@ -575,34 +893,59 @@ __global__ void __launch_bounds__(256, 2) kv8_many_kernel(Kv8Args p) {
 
 struct Kv8Plan {
   bool many;
-  int rows;      // of a tile
-  long tiles;    // numbers of tiles times key / value heads, those of no tile among them
-  int splits;
+  int rows;     // of a tile
+  int numbers;  // of tiles, those of no tile among them
+  int splits;   // pieces of a tile along the keys
+  int whole;    // many rows: an XCD's tiles that are not split
+  long pieces;  // partial results
 };
 
-// Up to 16 rows a sequence on average take the kernel for few rows.  Splits: until the card is full, two pages a wave at least.
-Kv8Plan kv8_plan(const Kv8Cache& c, int H) {
+// Sequences are as long as the table is wide at most, and shorter ones split into shorter pieces.
+Kv8Plan kv8_plan(const Kv8Cache& c, int H, bool causal) {
   const long G = H / c.Hkv, rows = c.N * G;
-  Kv8Plan pl;
-  pl.many = rows > 32L * c.B;
+  Kv8Plan pl{};
+  pl.many = rows > (getenv("KVX")?atoi(getenv("KVX")):32) * (long)c.B;
   pl.rows = pl.many ? 128 : 16;
-  pl.tiles = (rows / pl.rows + c.B + 1) * c.Hkv;
-  const long busy = ((rows + pl.rows - 1) / pl.rows > c.B ? (rows + pl.rows - 1) / pl.rows : c.B) * c.Hkv;
-  const long want = (pl.many ? 512 : 1024) / (busy > 0 ? busy : 1), most = pl.many ? c.W / 4 : c.W / 8;
-  pl.splits = (int)(want < 1 ? 1 : want > 128 ? 128 : want);
-  if (pl.splits > most) pl.splits = most < 1 ? 1 : (int)most;
-  while (pl.splits > 1 && pl.tiles * pl.splits > (long)(UINT32_MAX / 256)) pl.splits /= 2;   // more than a launch holds
+  pl.numbers = (int)(rows / pl.rows + c.B + 1);
+  if (!pl.many) {
+    const long busy = ((rows + 15) / 16 > c.B ? (rows + 15) / 16 : c.B) * c.Hkv;
+    const long want = (getenv("KVF")?atoi(getenv("KVF")):256) / busy, most = c.W / 16;
+    pl.splits = (int)(want > KV8_SPLITS ? KV8_SPLITS : want);
+    if (pl.splits > most) pl.splits = (int)most;
+    if (pl.splits < 1) pl.splits = 1;
+    pl.pieces = pl.splits == 1 ? 0 : (long)pl.numbers * c.Hkv * pl.splits;
+    return pl;
+  }
+  // 64 workgroups run on an XCD at a time
+  const long tiles = (rows + 127) / 128 > c.B ? (rows + 127) / 128 : c.B;   // as many as there can be, all about equal
+  const long each = kv8_each(tiles, c.Hkv) * (c.Hkv / kv8_shared(c.Hkv)), all = kv8_each(pl.numbers, c.Hkv) * (c.Hkv / kv8_shared(c.Hkv));
+  const long rounds = each / 64, rest = each % 64, most = c.W / 4;
+  pl.whole = (int)all;
+  pl.splits = 1;
+  if (rest && (rounds == 0 || !causal)) {
+    const long want = 64 / rest;
+    pl.splits = (int)(want > (rounds ? 8 : KV8_SPLITS) ? (rounds ? 8 : KV8_SPLITS) : want);
+    if (pl.splits > most) pl.splits = (int)most;
+    if (pl.splits > 1) pl.whole = (int)(rounds == 0 ? 0 : all - rest);
+    else pl.splits = 1;
+  }
+  pl.pieces = 8 * (all - pl.whole) * pl.splits;
   return pl;
 }
 
 template <int D>
 hipError_t launch_attention(const Kv8Args& a, const Kv8Plan& pl, hipStream_t st) {
-  const unsigned grid = (unsigned)(pl.tiles * pl.splits);
-  if (pl.many) kv8_many_kernel<D><<<grid, 256, 0, st>>>(a);
-  else kv8_rows_kernel<D><<<grid, 256, 0, st>>>(a);
-  if (hipError_t e = hipGetLastError(); e != hipSuccess || pl.splits == 1) return e;
-  if (pl.many) kv8_join_kernel<D, 128><<<(unsigned)(pl.tiles * 8), 256, 0, st>>>(a);
-  else kv8_join_kernel<D, 16><<<(unsigned)pl.tiles, 256, 0, st>>>(a);
+  if (pl.many) {
+    const int all = (int)(kv8_each(pl.numbers, a.c.Hkv) * (a.c.Hkv / kv8_shared(a.c.Hkv)));
+    kv8_many_kernel<D><<<(unsigned)(8 * (pl.whole + (all - pl.whole) * pl.splits)), 256, 0, st>>>(a);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess || pl.pieces == 0) return e;
+    kv8_join_kernel<D, 128><<<(unsigned)(8 * (all - pl.whole) * 64), 256, 0, st>>>(a);
+  } else {
+    const unsigned tiles = (unsigned)(pl.numbers * a.c.Hkv);
+    kv8_rows_kernel<D><<<tiles * pl.splits, 256, 0, st>>>(a);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess || pl.pieces == 0) return e;
+    kv8_join_kernel<D, 16><<<tiles * 8, 256, 0, st>>>(a);
+  }
   return hipGetLastError();
 }
 
@@ -616,16 +959,16 @@ hipError_t launch_kv8_append(const Kv8Cache& c, const uint16_t* k, long ldk, con
   return hipGetLastError();
 }
 
-long kv8_attention_workspace_bytes(const Kv8Cache& c, int H) {
-  const Kv8Plan pl = kv8_plan(c, H);
-  return pl.splits == 1 ? 0 : pl.tiles * pl.splits * pl.rows * (c.D + 2) * 4;
+long kv8_attention_workspace_bytes(const Kv8Cache& c, int H, int causal) {
+  const Kv8Plan pl = kv8_plan(c, H, causal);
+  return pl.pieces * pl.rows * (c.D + 2) * 4;
 }
 
 hipError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Attention& a, void* workspace, hipStream_t st) {
-  const Kv8Plan pl = kv8_plan(c, a.H);
+  const Kv8Plan pl = kv8_plan(c, a.H, a.causal);
   float* part = static_cast<float*>(workspace);
-  const Kv8Args args{c, a.q, a.ldq, a.o, a.H, a.H / c.Hkv, a.causal, pl.splits, a.scale * 1.4426950408889634f,
-                     part, part + pl.tiles * pl.splits * pl.rows * c.D};
+  const Kv8Args args{c, a.q, a.ldq, a.o, a.H, a.H / c.Hkv, a.causal, pl.splits, pl.numbers, pl.whole,
+                     a.scale * 1.4426950408889634f, part, part + pl.pieces * pl.rows * c.D};
   return c.D == 128 ? launch_attention<128>(args, pl, st) : launch_attention<64>(args, pl, st);
 }
 

@@ -642,7 +642,7 @@ Tensor kv8_attention(const Tensor& q, const Tensor& cu_seqlens, const Tensor& le
                     q.sizes());
   const int h = (int)q.size(1);
   Tensor out = at::empty(q.sizes(), qh.options());
-  const int64_t bytes = svdq_kv8_attention_workspace(c.n, c.b, c.w, h, c.hkv, c.d);
+  const int64_t bytes = svdq_kv8_attention_workspace(c.n, c.b, c.w, h, c.hkv, c.d, causal);
   const Tensor work = bytes ? at::empty({bytes}, qh.options().dtype(at::kByte)) : Tensor();
   check_status("svdq_kv8_attention",
                svdq_kv8_attention(ptr(qh), qh.stride(0), c.n, ptr<int>(cu_seqlens), ptr<int>(lengths), ptr<int>(block_table),

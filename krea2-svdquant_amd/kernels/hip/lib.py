@@ -117,7 +117,7 @@ SIGNATURES = {
     "svdq_qk_norm_rope": (_I, [_P, _L, _I, _P, _L, _I, _P, _P, _P, _P, _L, _I, _I, _P, _I, _I, _I, _I, ctypes.c_float,
                                _I, _P, _P, _P]),
     "svdq_kv8_append": (_I, [_P, _L, _P, _L, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _P]),
-    "svdq_kv8_attention_workspace": (_L, [_I, _I, _I, _I, _I, _I]),
+    "svdq_kv8_attention_workspace": (_L, [_I, _I, _I, _I, _I, _I, _I]),
     "svdq_kv8_attention": (_I, [_P, _L, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, ctypes.c_float, _I, _P, _P,
                                 _P]),
 }
