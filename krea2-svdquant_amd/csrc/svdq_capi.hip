@@ -892,21 +892,28 @@ int svdq_fp8_quantize(const void* x, int64_t ldx, int M, int K, void* codes, flo
                   "fp8_quantize");
 }
 
+int64_t svdq_fp8_gemm_workspace(int M, int N, int K) {
+  if (M <= 0 || N <= 0 || K <= 0 || K > 1 << 22 || !mx_gemm_fits(M, N)) return 0;
+  return svdq::fp8_gemm_workspace_bytes(M, N, K);
+}
+
 int svdq_fp8_gemm(const void* a, const float* a_scales, const void* w, const float* w_scales, const void* bias, int M,
-                  int N, int K, void* y, int64_t ldy, hipStream_t stream) {
+                  int N, int K, void* y, int64_t ldy, void* workspace, hipStream_t stream) {
   if (M < 0 || N <= 0 || K <= 0 || ldy < N)
     return fail(SVDQ_ERR_SHAPE, "fp8_gemm: M=%d, N=%d, K=%d, ldy=%lld", M, N, K, (long long)ldy);
   if (K > 1 << 22) return fail(SVDQ_ERR_SHAPE, "fp8_gemm: K=%d exceeds 2^22 (a tile's offsets are 32 bits)", K);
   if (!mx_gemm_fits(M, N)) return fail(SVDQ_ERR_SHAPE, "fp8_gemm: M=%d, N=%d are too many for a launch", M, N);
   if (M == 0) return ok();
   if (!a || !a_scales || !w || !w_scales || !y) return fail(SVDQ_ERR_ARG, "fp8_gemm: null pointer");
-  if (!aligned16(a) || !aligned16(w)) return fail(SVDQ_ERR_ALIGN, "fp8_gemm: codes must be 16-byte aligned");
+  if (!aligned16(a) || !aligned16(w) || !aligned16(workspace))
+    return fail(SVDQ_ERR_ALIGN, "fp8_gemm: codes and workspace must be 16-byte aligned");
+  if (!workspace && svdq::fp8_gemm_workspace_bytes(M, N, K) > 0) return fail(SVDQ_ERR_ARG, "fp8_gemm: no workspace");
   if (reinterpret_cast<uintptr_t>(a_scales) % 4 || reinterpret_cast<uintptr_t>(w_scales) % 4 || !aligned2(bias) ||
       !aligned2(y))
     return fail(SVDQ_ERR_ALIGN, "fp8_gemm: scales, bias and y must be aligned to their elements");
   const svdq::Fp8GemmParams p{static_cast<const uint8_t*>(a), a_scales, static_cast<const uint8_t*>(w), w_scales,
                               static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(y), ldy, M, N, K};
-  return launched(svdq::launch_fp8_gemm(p, stream), "fp8_gemm");
+  return launched(svdq::launch_fp8_gemm(p, workspace, stream), "fp8_gemm");
 }
 
 int svdq_qk_norm_rope(const void* q, int64_t ldq, int hsq, const void* k, int64_t ldk, int hsk, const void* qw,

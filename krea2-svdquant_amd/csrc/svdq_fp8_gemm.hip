@@ -65,14 +65,16 @@ struct Fp8Tile {
 };
 
 template <int TM, int TN, int WM, int WN, int NB>
-__global__ void __launch_bounds__(64 * WM * WN, 2) fp8_gemm_tile_kernel(Fp8GemmParams p, int nbm, int nbn, int group_m) {
+__global__ void __launch_bounds__(64 * WM * WN, 2)
+    fp8_gemm_tile_kernel(Fp8GemmParams p, int nbm, int nbn, int group_m, int per, float* part) {
   using T = Fp8Tile<TM, TN, WM, WN, NB>;
   __shared__ __attribute__((aligned(1024))) uint8_t sm[T::LDS];
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, b = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
   int bm, bn;
+  // pieces of `per` blocks of K, one after another in blockIdx.y
   tile_coords(blockIdx.x, nbm, nbn, group_m, bm, bn);
-  const int m0 = bm * T::BM, n0 = bn * T::BN, kp = (int)fp8_kp(p.K), nst = kp / 128;
+  const int m0 = bm * T::BM, n0 = bn * T::BN, kp = (int)fp8_kp(p.K), k0 = blockIdx.y * per, nst = min(per, kp / 128 - k0);
   const uint32_t lds0 = lds_offset(sm);
   const int chunk = lane % 8 ^ (lane / 8 >> 1 & 3);   // row / 2 mod 8 of row 8 i + lane / 8: 4 (i & 1) more
   uint32_t off[T::D - 1];
@@ -82,9 +84,9 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) fp8_gemm_tile_kernel(Fp8GemmP
     const int i = wave + T::NW * (a ? d : d - T::DA), row = 8 * i + lane / 8;
     off[d] = (uint32_t)((long)min(row, (a ? p.M - m0 : p.N - n0) - 1) * kp + 16 * (chunk ^ (i & 1 ? 4 : 0)));
   }
-  const uint8_t *src_a = p.a + (long)m0 * kp, *src_w = p.w + (long)n0 * kp;
+  const uint8_t *src_a = p.a + (long)m0 * kp + 128 * k0, *src_w = p.w + (long)n0 * kp + 128 * k0;
   const int mw = m0 + 16 * TM * wm, nw = n0 + 16 * TN * wn;
-  const float* src_s = p.as + min(mw + min(lane, 16 * TM - 1), p.M - 1);
+  const float* src_s = p.as + (long)k0 * p.M + min(mw + min(lane, 16 * TM - 1), p.M - 1);
   int ahead = 0;
   // this wave's d-th instruction of the stage `ahead`; past the last one that again, so that the waits count the same
   // loads throughout
@@ -101,7 +103,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) fp8_gemm_tile_kernel(Fp8GemmP
             lds0 + buf * T::BUF + 1024 * (d < T::DA ? wave + T::NW * d : T::TA + wave + T::NW * (d - T::DA)));
     }
   };
-  const float* wsrow = p.ws + (long)min(nw / 128, (p.N - 1) / 128) * nst;
+  const float* wsrow = p.ws + (long)min(nw / 128, (p.N - 1) / 128) * (kp / 128) + k0;
   float wscales = wsrow[min(lane, nst - 1)];   // of stages s .. s + 63
   asm volatile("s_waitcnt vmcnt(0)" : "+v"(wscales)::"memory");
 
@@ -207,6 +209,17 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) fp8_gemm_tile_kernel(Fp8GemmP
   // LDS is used again, here or by the next workgroup.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
+  if (part) {   // sums of this piece, rows of N rounded up to 4
+    const int np = (p.N + 3) & ~3;
+#pragma unroll
+    for (int t = 0; t < TM; ++t)
+#pragma unroll
+      for (int x = 0; x < TN; ++x) {
+        const int m = mw + 16 * t + lr, n = nw + 16 * x + 4 * b;
+        if (m < p.M && n < np) *reinterpret_cast<f32x4*>(part + ((long)blockIdx.y * p.M + m) * np + n) = acc[x][t];
+      }
+    return;
+  }
   uint8_t* stage_out = sm + wave * 16 * T::PITCH;
   constexpr int COLS = 16 * TN, LPR = COLS / 8;   // lanes a row
   const bool wide = p.ldy % 8 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
@@ -328,35 +341,110 @@ __global__ void __launch_bounds__(512) fp8_gemm_rows_kernel(Fp8GemmParams p) {
   p.y[(long)m * p.ldy + n0 + n] = (uint16_t)pack_bf16x2(y, 0.0f);
 }
 
+// y = the pieces' sums, in their order, and the bias; four columns a thread
+__global__ void __launch_bounds__(256) fp8_gemm_join_kernel(Fp8GemmParams p, const float* __restrict__ part, int pieces) {
+  const int np = (p.N + 3) & ~3, quads = np / 4;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x, m = i / quads;
+  if (m >= p.M) return;
+  const int n = 4 * (int)(i - m * quads);
+  f32x4 y = {};
+#pragma unroll 4
+  for (int s = 0; s < pieces; ++s) y += *reinterpret_cast<const f32x4*>(part + ((long)s * p.M + m) * np + n);
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (p.bias && n + r < p.N) y[r] += bf16f(p.bias[n + r]);
+  uint16_t* out = p.y + m * p.ldy + n;
+  const u32x2 o = {pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+  if (n + 3 < p.N && p.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % 8 == 0) {
+    *reinterpret_cast<u32x2*>(out) = o;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < p.N) out[r] = (uint16_t)(o[r / 2] >> 16 * (r % 2));
+  }
+}
+
 template <int TM, int TN, int WM, int WN, int NB>
-hipError_t launch_tile(const Fp8GemmParams& p, hipStream_t st) {
+hipError_t launch_tile(const Fp8GemmParams& p, int per, float* part, hipStream_t st) {
   using T = Fp8Tile<TM, TN, WM, WN, NB>;
   const long nbm = (p.M + T::BM - 1) / T::BM, nbn = (p.N + T::BN - 1) / T::BN;
-  fp8_gemm_tile_kernel<TM, TN, WM, WN, NB><<<(unsigned)(nbm * nbn), 64 * WM * WN, 0, st>>>(p, (int)nbm, (int)nbn, 4);
+  const int blocks = (int)(fp8_kp(p.K) / 128);
+  fp8_gemm_tile_kernel<TM, TN, WM, WN, NB><<<dim3((unsigned)(nbm * nbn), (unsigned)((blocks + per - 1) / per)), 64 * WM * WN, 0, st>>>(
+      p, (int)nbm, (int)nbn, 4, per, part);
   return hipGetLastError();
 }
 
+// Block tiles: rows of a, of w, workgroups that share a CU, and microseconds for a block of K with n of them on a CU
+// (us[n - 1]).  As measured at K = 6144 (48 blocks; M x N and us of the tiles in order: 77 x 6144 17.3 21.6 40 39 60, 256 x
+// 6144 23 22 41 40 61, 1024 x 6144 74 56 50 45 64, 4352 x 1536 84 66 51 46 65, 2381 x 6144 167 133 110 102 86, 4096 x
+// 16384 660 540 447 411 345); a launch takes 4 us besides, a further round 1.
+struct Fp8TileCost {
+  int rows, cols, slots;
+  float us[3];
+};
 constexpr int FP8_TILES = 5, FP8_ROWS = -1;
+const Fp8TileCost kTiles[FP8_TILES] = {{64, 64, 3, {0.28f, 0.42f, 0.66f}}, {64, 128, 2, {0.38f, 0.66f}}, {128, 128, 2, {0.78f, 1.10f}},
+                                       {256, 128, 1, {0.98f}}, {256, 256, 1, {1.75f}}};
 
-hipError_t launch_kernel(int tile, const Fp8GemmParams& p, hipStream_t st) {
-  switch (tile) {
+struct Fp8Choice {
+  int tile, per;   // blocks of K in a piece
+  float us;
+};
+
+// Few tiles leave most CUs idle for all of K, so K is cut into pieces where that is less with what joining them takes (a
+// launch, and a write and a read of every piece's sums at 4 TB/s).  In one piece and in several: 77 x 1536, K = 6144 15.8
+// and 9.5 us, 32 x 6144, K = 16384 38 and 20; 512 x 1536, K = 6144 17.3 in one, 17.7 in two.  Up to 16 rows the rows
+// kernel runs (16 x 6144, K = 6144 8.6 us, tiles 16.7; K = 16384 16.8 and 19.7).
+Fp8Choice choose(long M, long N, int K) {
+  const int blocks = (int)(fp8_kp(K) / 128);
+  if (M <= 16) return {FP8_ROWS, blocks, 0.0f};
+  Fp8Choice best{-2, 0, 0.0f};
+  for (int i = 0; i < FP8_TILES; ++i) {
+    const Fp8TileCost& t = kTiles[i];
+    const long tiles = ((M + t.rows - 1) / t.rows) * ((N + t.cols - 1) / t.cols);
+    for (int n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+      const int per = (blocks + n - 1) / n, pieces = (blocks + per - 1) / per;
+      const long all = tiles * pieces, whole = all / (256 * t.slots), rest = (all % (256 * t.slots) + 255) / 256;
+      if (n > 1 && (per < 4 || all > 512)) break;
+      float us = 4.0f + whole * (1.0f + per * t.us[t.slots - 1]) + (rest ? per * t.us[rest - 1] : 0.0f);
+      if (pieces > 1) us += 2.0f + 2.0f * pieces * M * N * 4.0f / 4e6f;
+      if (best.tile < -1 || us < best.us) best = {i, per, us};
+    }
+  }
+  return best;
+}
+
+hipError_t launch_kernel(const Fp8Choice& c, const Fp8GemmParams& p, float* part, hipStream_t st) {
+  switch (c.tile) {
     case FP8_ROWS:
       if (p.M > 8) fp8_gemm_rows_kernel<16, 2><<<(unsigned)((p.N + 15) / 16), 512, 0, st>>>(p);
       else fp8_gemm_rows_kernel<8, 3><<<(unsigned)((p.N + 15) / 16), 512, 0, st>>>(p);
       return hipGetLastError();
-    case 0: return launch_tile<1, 4, 4, 1, 3>(p, st);
-    case 1: return launch_tile<2, 4, 2, 2, 3>(p, st);
-    case 2: return launch_tile<4, 4, 2, 2, 2>(p, st);
-    case 3: return launch_tile<4, 4, 4, 2, 3>(p, st);
-    default: return launch_tile<4, 8, 4, 2, 2>(p, st);
+    case 0: return launch_tile<1, 4, 4, 1, 3>(p, c.per, part, st);
+    case 1: return launch_tile<2, 4, 2, 2, 3>(p, c.per, part, st);
+    case 2: return launch_tile<4, 4, 2, 2, 2>(p, c.per, part, st);
+    case 3: return launch_tile<4, 4, 4, 2, 3>(p, c.per, part, st);
+    default: return launch_tile<4, 8, 4, 2, 2>(p, c.per, part, st);
   }
 }
 
+int pieces_of(const Fp8Choice& c, int K) { return (int)((fp8_kp(K) / 128 + c.per - 1) / c.per); }
+
 }  // namespace
 
-hipError_t launch_fp8_gemm(const Fp8GemmParams& p, hipStream_t st) {
-  const long large = (p.M + 255L) / 256 * ((p.N + 255L) / 256);
-  return launch_kernel(p.M <= 16 ? FP8_ROWS : large >= 256 ? 4 : 0, p, st);
+long fp8_gemm_workspace_bytes(int M, int N, int K) {
+  const int pieces = pieces_of(choose(M, N, K), K);
+  return pieces == 1 ? 0 : 4L * pieces * M * ((N + 3) & ~3);
+}
+
+hipError_t launch_fp8_gemm(const Fp8GemmParams& p, void* workspace, hipStream_t st) {
+  const Fp8Choice c = choose(p.M, p.N, p.K);
+  const int pieces = pieces_of(c, p.K);
+  float* part = pieces == 1 ? nullptr : static_cast<float*>(workspace);
+  if (hipError_t e = launch_kernel(c, p, part, st); e != hipSuccess || !part) return e;
+  const long quads = (long)p.M * ((p.N + 3) / 4);
+  fp8_gemm_join_kernel<<<(unsigned)((quads + 255) / 256), 256, 0, st>>>(p, part, pieces);
+  return hipGetLastError();
 }
 
 }  // namespace svdq

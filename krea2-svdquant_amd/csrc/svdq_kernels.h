@@ -214,7 +214,8 @@ struct Fp8GemmParams {
   long ldy;
   int M, N, K;
 };
-hipError_t launch_fp8_gemm(const Fp8GemmParams& p, hipStream_t st);
+long fp8_gemm_workspace_bytes(int M, int N, int K);
+hipError_t launch_fp8_gemm(const Fp8GemmParams& p, void* workspace, hipStream_t st);
 
 // Norms of q's and k's heads with the position rotation (svdq_block.hip)
 struct QkNormRopeParams {

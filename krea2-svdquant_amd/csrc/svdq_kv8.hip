@@ -12,7 +12,6 @@
 //          tokens already; those are then rounded again under the new scale.
 // attend:  o = sum over visible j of softmax_j(scale q . k_j) v_j,  j < length, and with a causal mask, for the i-th of n new
 //          tokens, j <= length - n + i; 0 where nothing is visible.
-#include <cstdlib>
 #include <type_traits>
 
 #include "svdq_fp8.h"
@@ -36,13 +35,32 @@ __device__ __forceinline__ int first_row(const Kv8Cache& c, int b) {
 __device__ __forceinline__ long first_unit(const Kv8Cache& c, int b, int mult, int unit, int extra) {
   return (long)first_row(c, b) * mult / unit + (long)extra * b;
 }
-__device__ __forceinline__ int find_sequence(const Kv8Cache& c, long number, int mult, int unit, int extra) {
-  int before = 0;
-  for (int b0 = 1; b0 <= c.B; b0 += 64) {
-    const int b = b0 + (threadIdx.x & 63);
-    before += __popcll(__ballot(b <= c.B && first_unit(c, b, mult, unit, extra) <= number));
+struct Kv8Sequence {
+  int b, row0, n, len;   // sequence, its first row and new tokens, tokens held
+  long unit0;            // its first unit
+};
+__device__ __forceinline__ Kv8Sequence find_sequence(const Kv8Cache& c, long number, int mult, int unit, int extra) {
+  const int lane = threadIdx.x & 63;
+  Kv8Sequence s;
+  if (c.B < 63) {   // a lane each: one latency for all of it
+    const int row = first_row(c, lane), len = c.lengths[min(lane, c.B - 1)];
+    s.b = __popcll(__ballot(lane > 0 && lane <= c.B && (long)row * mult / unit + (long)extra * lane <= number));
+    s.row0 = __builtin_amdgcn_readlane(row, s.b);
+    s.n = __builtin_amdgcn_readlane(row, s.b + 1) - s.row0;
+    s.len = __builtin_amdgcn_readlane(len, s.b);
+  } else {
+    int before = 0;
+    for (int b0 = 1; b0 <= c.B; b0 += 64)
+      before += __popcll(__ballot(b0 + lane <= c.B && first_unit(c, b0 + lane, mult, unit, extra) <= number));
+    s.b = __builtin_amdgcn_readfirstlane(before);
+    s.row0 = first_row(c, s.b);
+    s.n = first_row(c, s.b + 1) - s.row0;
+    s.len = c.lengths[min(s.b, c.B - 1)];
   }
-  return __builtin_amdgcn_readfirstlane(before);
+  s.n = max(s.n, 0);
+  s.len = s.b == c.B ? 0 : min(max(s.len, 0), c.W * PAGE);
+  s.unit0 = (long)s.row0 * mult / unit + (long)extra * s.b;
+  return s;
 }
 
 // ---- append -------------------------------------------------------------------------------------
@@ -65,12 +83,10 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8Cache c, const uint1
   __shared__ __attribute__((aligned(16))) uint8_t turn[D * PAGE];
   const int tid = threadIdx.x, head = blockIdx.x % c.Hkv;
   const long number = blockIdx.x / c.Hkv;
-  const int b = find_sequence(c, number, 1, PAGE, 2);
-  if (b >= c.B) return;
-  const int row0 = first_row(c, b), n = first_row(c, b + 1) - row0;
-  if (n <= 0) return;
-  const long start = min(max(c.lengths[b], 0), c.W * PAGE);
-  const long page = start / PAGE + (number - first_unit(c, b, 1, PAGE, 2));
+  const Kv8Sequence q = find_sequence(c, number, 1, PAGE, 2);
+  if (q.b >= c.B || q.n == 0) return;
+  const int b = q.b, row0 = q.row0, n = q.n;
+  const long start = q.len, page = start / PAGE + (number - q.unit0);
   if (page >= c.W || page * PAGE >= start + n) return;
   const int id = c.table[(long)b * c.W + page];
   if (id < 0 || id >= c.P) return;
@@ -185,7 +201,8 @@ struct Kv8Args {
   const uint16_t* q;
   long ldq;
   uint16_t* o;
-  int H, G, causal, splits;
+  int H, G, causal;
+  int splits;       // of a tile along the keys
   int numbers;      // of tiles, those of no tile among them
   int whole;        // many rows: an XCD's tiles that are not split
   float scale_log2;
@@ -198,15 +215,15 @@ struct Kv8Tile {
 };
 template <int R>
 __device__ __forceinline__ bool kv8_tile(const Kv8Args& p, long number, Kv8Tile& t) {
-  t.b = find_sequence(p.c, number, p.G, R, 1);
-  t.row0 = first_row(p.c, t.b);
-  t.n = max(first_row(p.c, t.b + 1) - t.row0, 0);
-  t.rows = t.n * p.G;
-  const long r0 = (number - first_unit(p.c, t.b, p.G, R, 1)) * R;
-  if (r0 >= t.rows) return false;
+  const Kv8Sequence q = find_sequence(p.c, number, p.G, R, 1);
+  t.b = q.b;
+  t.row0 = q.row0;
+  t.n = q.n;
+  t.len = q.len;
+  t.rows = q.n * p.G;
+  const long r0 = (number - q.unit0) * R;
   t.r0 = (int)r0;
-  t.len = t.b == p.c.B ? 0 : min(max(p.c.lengths[t.b], 0), p.c.W * PAGE);
-  return true;
+  return r0 < t.rows;
 }
 // keys that the row's token sees
 __device__ __forceinline__ int kv8_visible(const Kv8Args& p, const Kv8Tile& t, int row) {
@@ -359,10 +376,13 @@ __global__ void __launch_bounds__(256, 2) kv8_rows_kernel(Kv8Args p) {
       const int i = i0 + lane;
       id = i < count ? table[p0 + wave + 4 * i] : -1;
       if (id < 0 || id >= p.c.P) id = -1;
+      asm volatile("" : "+v"(id)::"memory");   // ahead of the DMA, which the compiler does not count
+    };
+    auto look_scales_up = [&] {
       const long at = (long)max(id, 0) * p.c.Hkv + hk;
       ks = p.c.scales[2 * at] * p.scale_log2;
       vs = p.c.scales[2 * at + 1];
-      asm volatile("s_waitcnt vmcnt(0)" : "+v"(id), "+v"(ks), "+v"(vs)::"memory");   // ahead of the DMA, which is not counted
+      asm volatile("s_waitcnt vmcnt(0)" : "+v"(ks), "+v"(vs)::"memory");
     };
     look_up(0);
     int first = 0;   // the page that lane 0 holds
@@ -376,6 +396,7 @@ __global__ void __launch_bounds__(256, 2) kv8_rows_kernel(Kv8Args p) {
       else T::template fetch<false>(kc, vc, koff, voff, lds0);
     };
     fetch(0);
+    look_scales_up();
     auto rescale = [&](float top) {
       const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn;
       const float alpha = __builtin_amdgcn_exp2f(m - base);
@@ -410,6 +431,7 @@ __global__ void __launch_bounds__(256, 2) kv8_rows_kernel(Kv8Args p) {
       if (i + 1 - first >= 64) {   // its next page is not among those looked up
         first = i + 1;
         look_up(first);
+        look_scales_up();
       }
       fetch(i + 1);
       if (!have) continue;
@@ -534,69 +556,71 @@ __global__ void __launch_bounds__(256, 2) kv8_rows_kernel(Kv8Args p) {
   }
 }
 
-// Joins the splits of two rows of a tile of R: a wave finds the weights of a row's splits, a split a lane; then 32 lanes take a
-// row's columns, four of them each, and four such groups every fourth split.
-template <int D, int R>
+// Joins the splits of the rows of a tile of R, 8 / GROUPS of them a workgroup: half a wave finds the weights of a row's splits;
+// then 32 lanes take a row's columns, and GROUPS such groups every GROUPS-th split.
+template <int D, int R, int GROUPS>
 __global__ void __launch_bounds__(256) kv8_join_kernel(Kv8Args p) {
-  constexpr int C = D / 32;   // columns of a lane
-  __shared__ float weight[2][KV8_SPLITS], total[2];
-  __shared__ float part[2][4][D];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t tile = blockIdx.x / (R / 2);
-  const int r0 = 2 * (blockIdx.x % (R / 2));
+  constexpr int C = D / 32, ROWS = 8 / GROUPS;   // columns of a lane, rows of a workgroup
+  __shared__ float weight[ROWS][KV8_SPLITS], total[ROWS];
+  __shared__ __attribute__((aligned(16))) float part[GROUPS][ROWS][D];
+  const int tid = threadIdx.x, hl = tid & 31, hw = tid >> 5;
+  const uint32_t tile = blockIdx.x / (R / ROWS);
+  const int r0 = ROWS * (blockIdx.x % (R / ROWS));
   int number = tile / p.c.Hkv, hk = tile % p.c.Hkv;
   if (R > 16 && !kv8_tile_of(p, tile % 8, p.whole + tile / 8, number, hk)) return;
   Kv8Tile t;
   if (!kv8_tile<R>(p, number, t)) return;
   if (t.r0 + r0 >= t.rows) return;
   const long first = (long)tile * p.splits * R + r0;
-  if (wave < 2) {
-    float m[KV8_SPLITS / 64], l[KV8_SPLITS / 64], top = -INFINITY, sum = 0.0f;
+  if (hw < ROWS) {
+    float m[KV8_SPLITS / 32], l[KV8_SPLITS / 32], top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < KV8_SPLITS / 64; ++i) {
-      const int s = 64 * i + lane;
-      const long at = first + wave + (long)min(s, p.splits - 1) * R;
+    for (int i = 0; i < KV8_SPLITS / 32; ++i) {
+      const int s = 32 * i + hl;
+      const long at = first + hw + (long)min(s, p.splits - 1) * R;
       m[i] = s < p.splits ? p.part_ml[2 * at] : -INFINITY;
-      l[i] = p.part_ml[2 * at + 1];
+      l[i] = s < p.splits ? p.part_ml[2 * at + 1] : 0.0f;
       top = fmaxf(top, m[i]);
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
     const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-    for (int i = 0; i < KV8_SPLITS / 64; ++i) {
+    for (int i = 0; i < KV8_SPLITS / 32; ++i) {
       const float f = __builtin_amdgcn_exp2f(m[i] - base);
-      weight[wave][64 * i + lane] = f;
-      if (64 * i + lane < p.splits) sum += f * l[i];
+      weight[hw][32 * i + hl] = f;
+      sum += f * l[i];
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) total[wave] = sum;
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (hl == 0) total[hw] = sum;
   }
   __syncthreads();
-  const int r = tid >> 7, g = tid >> 5 & 3, c0 = (tid & 31) * C;
+  const int r = hw % ROWS, g = hw / ROWS;
   float o[C] = {};
 #pragma unroll 4
-  for (int s = g; s < p.splits; s += 4) {
+  for (int s = g; s < p.splits; s += GROUPS) {
     const float f = weight[r][s];
-    const float* from = p.part_o + (first + r + (long)s * R) * D + c0;
+    const float* from = p.part_o + (first + r + (long)s * R) * D + C * hl;
 #pragma unroll
     for (int i = 0; i < C; ++i) o[i] += f * from[i];
   }
+  if (GROUPS > 1) {
 #pragma unroll
-  for (int i = 0; i < C; ++i) part[r][g][c0 + i] = o[i];
-  __syncthreads();
-  const int row = t.r0 + r0 + (tid >> 7), c = tid & 127;
-  if (row >= t.rows || 2 * c >= D) return;
-  const float sum = total[tid >> 7], inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  float y[2];
+    for (int i = 0; i < C; ++i) part[g][r][C * hl + i] = o[i];
+    __syncthreads();
+    if (g) return;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const float(&q)[4][D] = part[tid >> 7];
-    y[i] = ((q[0][2 * c + i] + q[1][2 * c + i]) + (q[2][2 * c + i] + q[3][2 * c + i])) * inv;
+    for (int k = 1; k < GROUPS; ++k)
+#pragma unroll
+      for (int i = 0; i < C; ++i) o[i] += part[k][r][C * hl + i];
   }
-  uint16_t* out = p.o + ((long)(t.row0 + row / p.G) * p.H + hk * p.G + row % p.G) * D;
-  *reinterpret_cast<uint32_t*>(out + 2 * c) = pack_bf16x2(y[0], y[1]);
+  const int row = t.r0 + r0 + r;
+  if (row >= t.rows) return;
+  const float inv = total[r] == 0.0f ? 0.0f : 1.0f / total[r];
+  uint32_t* out = reinterpret_cast<uint32_t*>(p.o + ((long)(t.row0 + row / p.G) * p.H + hk * p.G + row % p.G) * D + C * hl);
+#pragma unroll
+  for (int i = 0; i < C / 2; ++i) out[i] = pack_bf16x2(o[2 * i] * inv, o[2 * i + 1] * inv);
 }
 
 // Many rows: 32 a wave, 128 a workgroup; pages go through LDS, as bf16, for its four waves.  Two workgroups share a CU, so that
@@ -660,6 +684,8 @@ __global__ void __launch_bounds__(256, 2) kv8_many_kernel(Kv8Args p) {
     first = from;
     ids = from + lane < p1 ? table[from + lane] : -1;
     if (ids < 0 || ids >= p.c.P) ids = -1;
+  };
+  auto look_scales_up = [&]() __attribute__((always_inline)) {
     const long at = (long)max(ids, 0) * p.c.Hkv + hk;
     kss = p.c.scales[2 * at] * p.scale_log2;
     vss = p.c.scales[2 * at + 1];
@@ -801,13 +827,17 @@ __global__ void __launch_bounds__(256, 2) kv8_many_kernel(Kv8Args p) {
   if (p0 < p1) {
     look_up(p0);
     load(p0);
+    look_scales_up();
     store(p0, 0);
     Kv8Scale now = scale_in(p0);
     again |= __builtin_amdgcn_readlane(ids, 0) < 0;
     __syncthreads();
     auto stage = [&](int pg, int buf) __attribute__((always_inline)) {
       const int next = min(pg + 1, p1 - 1);
-      if (next - first >= 64) look_up(next);
+      if (next - first >= 64) {
+        look_up(next);
+        look_scales_up();
+      }
       load(next);
       scores(buf);
       if (pg >= pe) masked(pg);
@@ -831,7 +861,10 @@ __global__ void __launch_bounds__(256, 2) kv8_many_kernel(Kv8Args p) {
   if (__syncthreads_or(again)) {
     clear();
     for (int pg = p0; pg < p1; ++pg) {
-      if ((pg - p0) % 64 == 0) look_up(pg);
+      if ((pg - p0) % 64 == 0) {
+        look_up(pg);
+        look_scales_up();
+      }
       load(pg);
       __syncthreads();
       store(pg, 0);
@@ -904,12 +937,19 @@ struct Kv8Plan {
 Kv8Plan kv8_plan(const Kv8Cache& c, int H, bool causal) {
   const long G = H / c.Hkv, rows = c.N * G;
   Kv8Plan pl{};
-  pl.many = rows > (getenv("KVX")?atoi(getenv("KVX")):32) * (long)c.B;
+  // A page that is read for 16 rows takes the few-rows kernel's 16 x 16 products through all of it again for the next 16; the
+  // other kernel reads it once for 128 rows, but a workgroup of it that is not full takes as long as a full one.  Rows
+  // (of heads) a sequence, few / many rows kernel: 8 x 128 of 4096 keys 30 / 48 us, 8 x 256 48 / 54, 32 x 64 74 / 107,
+  // 1 x 308 of 65536 (two and a half tiles) 330 / 223.
+  pl.many = rows > 256L * c.B;
   pl.rows = pl.many ? 128 : 16;
   pl.numbers = (int)(rows / pl.rows + c.B + 1);
   if (!pl.many) {
     const long busy = ((rows + 15) / 16 > c.B ? (rows + 15) / 16 : c.B) * c.Hkv;
-    const long want = (getenv("KVF")?atoi(getenv("KVF")):256) / busy, most = c.W / 16;
+    // One workgroup a CU reads fastest where there are no more (131072 tokens, 12 heads, in 252 pieces 64 us, 320 80, 512 68).
+    // Up to 512 tiles in two pieces each fill the last round better (32 sequences of 1000 to 8000 tokens, 12 heads: 88 us, in
+    // one piece 98; pieces of each by its length 92), longer tables alone (64 of 2048 in one piece 21, two 24).
+    const long want = busy <= 256 ? 256 / busy : busy <= 512 ? 2 : 1, most = c.W / (busy <= 256 ? 16 : 64);
     pl.splits = (int)(want > KV8_SPLITS ? KV8_SPLITS : want);
     if (pl.splits > most) pl.splits = (int)most;
     if (pl.splits < 1) pl.splits = 1;
@@ -939,12 +979,12 @@ hipError_t launch_attention(const Kv8Args& a, const Kv8Plan& pl, hipStream_t st)
     const int all = (int)(kv8_each(pl.numbers, a.c.Hkv) * (a.c.Hkv / kv8_shared(a.c.Hkv)));
     kv8_many_kernel<D><<<(unsigned)(8 * (pl.whole + (all - pl.whole) * pl.splits)), 256, 0, st>>>(a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess || pl.pieces == 0) return e;
-    kv8_join_kernel<D, 128><<<(unsigned)(8 * (all - pl.whole) * 64), 256, 0, st>>>(a);
+    kv8_join_kernel<D, 128, 1><<<(unsigned)(8 * (all - pl.whole) * 16), 256, 0, st>>>(a);
   } else {
     const unsigned tiles = (unsigned)(pl.numbers * a.c.Hkv);
     kv8_rows_kernel<D><<<tiles * pl.splits, 256, 0, st>>>(a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess || pl.pieces == 0) return e;
-    kv8_join_kernel<D, 16><<<tiles * 8, 256, 0, st>>>(a);
+    kv8_join_kernel<D, 16, 4><<<tiles * 8, 256, 0, st>>>(a);
   }
   return hipGetLastError();
 }

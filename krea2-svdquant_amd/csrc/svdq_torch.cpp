@@ -489,8 +489,10 @@ Tensor fp8_product(const void* a, const float* as, int64_t m, int64_t kp, std::v
   }
   lead.push_back(n);
   Tensor y = at::empty(lead, w.options().dtype(at::kBFloat16));
+  const int64_t bytes = svdq_fp8_gemm_workspace((int)m, (int)n, (int)kp);
+  const Tensor work = bytes ? at::empty({bytes}, w.options().dtype(at::kByte)) : Tensor();
   check_status("svdq_fp8_gemm", svdq_fp8_gemm(a, as, ptr(w), ptr<float>(w_scales), ptr(bias), (int)m, (int)n, (int)kp,
-                                              ptr(y), n, stream_of(dev)));
+                                              ptr(y), n, bytes ? ptr(work) : nullptr, stream_of(dev)));
   return y;
 }
 
