@@ -453,6 +453,12 @@ int64_t svdq_fp8_gemm_workspace(int M, int N, int K);
 int svdq_fp8_gemm(const void* a, const float* a_scales, const void* w, const float* w_scales, const void* bias, int M,
                   int N, int K, void* y, int64_t ldy, void* workspace, hipStream_t stream);
 
+/* y = svdq_fp8_quantize(x) times w as above, for bf16 x [M, ldx >= K].  workspace: svdq_fp8_linear_workspace(M, N, K) bytes,
+ * as above.  M = 0 does nothing. */
+int64_t svdq_fp8_linear_workspace(int M, int N, int K);
+int svdq_fp8_linear(const void* x, int64_t ldx, const void* w, const float* w_scales, const void* bias, int M, int N,
+                    int K, void* y, int64_t ldy, void* workspace, hipStream_t stream);
+
 /* RMS norm of every head of queries and keys with a learned weight, and the position rotation, in one launch:
  *   n = x * rsqrt(mean(x^2) + eps) * w;   (a, b) -> (a cos - b sin, b cos + a sin)
  * of the pairs (n[j], n[j + D / 2]) or, with pairs = 1, (n[2 j], n[2 j + 1]), j < D / 2; float32, one rounding to bf16.

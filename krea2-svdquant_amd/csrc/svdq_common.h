@@ -144,6 +144,13 @@ __device__ __forceinline__ void permlane32_swap(uint32_t& a, uint32_t& b) {
   b = r[1];
 }
 
+// v_permlane16_swap: exchange lanes 16..31 (48..63) of `a` with lanes 0..15 (32..47) of `b`.
+__device__ __forceinline__ void permlane16_swap(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+
 // VGPR banks of the rescale FMA acc += P * S.  The FMA reads three VGPRs; the register file
 // has four banks (register index mod 4) and three operands in one bank issue at about half
 // rate (measured: 1.85x the time of three distinct banks).  The allocator starts the MFMA result

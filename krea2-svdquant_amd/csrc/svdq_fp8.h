@@ -32,6 +32,16 @@ __device__ __forceinline__ uint32_t fp8_encode4(float a, float b, float c, float
   return __builtin_bit_cast(uint32_t, r);
 }
 
+// Four bf16 values of two registers as E4M3 codes under a power-of-two scale, to nearest even.
+__device__ __forceinline__ uint32_t fp8_encode_bf16x4(uint32_t lo, uint32_t hi, float scale) {
+  typedef short i16x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  i16x2 r = {0, 0};
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, lo), scale, false);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(bf16x2_t, hi), scale, true);
+  return __builtin_bit_cast(uint32_t, r);
+}
+
 // Eight codes as bf16 (exact).
 __device__ __forceinline__ u32x4 fp8_to_bf16x8(uint32_t lo, uint32_t hi) {
   u32x4 o;

@@ -37,6 +37,10 @@ __device__ __forceinline__ void dma4_at(const void* at, uint32_t lds) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(at), "{m0}"(lds) : "memory");
 }
 
+__device__ __forceinline__ void dma16_at(const void* at, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(at), "{m0}"(lds) : "memory");
+}
+
 template <class F, int... I>
 __device__ __forceinline__ void for_each_index(F&& f, std::integer_sequence<int, I...>) {
   (f(std::integral_constant<int, I>{}), ...);
@@ -260,6 +264,22 @@ __global__ void __launch_bounds__(64 * WM * WN, 2)
   }
 }
 
+// Adds 8 waves' sums of 16 rows and 16 columns in wave order; memory: 8 KB of LDS that the waves have done with.
+__device__ __forceinline__ void fp8_rows_sum(const Fp8GemmParams& p, uint8_t* sm, const f32x4& acc, int n0) {
+  const int tid = threadIdx.x;
+  __syncthreads();   // every ring is done with; their memory takes the sums
+  reinterpret_cast<f32x4*>(sm)[tid] = acc;
+  __syncthreads();
+  // register r of lane (lr, b): row lr of a, column 4 b + r of w
+  const int m = tid >> 4, n = tid & 15;
+  if (m >= p.M || m >= 16 || n0 + n >= p.N) return;
+  float y = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) y += reinterpret_cast<const float*>(sm)[4 * (64 * k + 16 * (n / 4) + m) + n % 4];
+  if (p.bias) y += bf16f(p.bias[n0 + n]);
+  p.y[(long)m * p.ldy + n0 + n] = (uint16_t)pack_bf16x2(y, 0.0f);
+}
+
 // Few rows of a (16 at most): what counts is reading w once, from as many places at once as possible.  A workgroup of
 // 8 waves takes 16 columns of the output and all of K; the waves take blocks of 128 columns of K in turn (whole cache
 // lines of w) and add their sums through LDS in wave order.  Each wave has a ring of U blocks in LDS to itself, filled
@@ -328,17 +348,104 @@ __global__ void __launch_bounds__(512) fp8_gemm_rows_kernel(Fp8GemmParams p) {
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
-  __syncthreads();   // every ring is done with; their memory takes the sums
-  reinterpret_cast<f32x4*>(sm)[64 * wave + lane] = acc;
-  __syncthreads();
-  // register r of lane (lr, b): row lr of a, column 4 b + r of w
-  const int m = tid >> 4, n = tid & 15;
-  if (m >= p.M || m >= 16 || n0 + n >= p.N) return;
-  float y = 0.0f;
+  fp8_rows_sum(p, sm, acc, n0);
+}
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+// The scale of a row's block that lanes l, l ^ 16, l ^ 32, l ^ 48 hold 32 bf16 values each of.
+__device__ __forceinline__ float row4_scale(const u32x4 (&v)[4]) {
+  u16x2 part[4] = {};
 #pragma unroll
-  for (int k = 0; k < T::NW; ++k) y += reinterpret_cast<const float*>(sm)[4 * (64 * k + 16 * (n / 4) + m) + n % 4];
-  if (p.bias) y += bf16f(p.bias[n0 + n]);
-  p.y[(long)m * p.ldy + n0 + n] = (uint16_t)pack_bf16x2(y, 0.0f);
+  for (int j = 0; j < 16; ++j)
+    part[j % 4] = __builtin_elementwise_max(part[j % 4], __builtin_bit_cast(u16x2, v[j / 4][j % 4] & 0x7FFF7FFFu));
+  const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(part[0], part[1]), __builtin_elementwise_max(part[2], part[3]));
+  uint32_t top = max((uint32_t)m[0], (uint32_t)m[1]);
+  if (__any(top >= 0x7F80u)) {   // values that are not finite: they say nothing about the scale
+    top = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const uint32_t d = v[j / 4][j % 4];
+      top = max(top, max(fp8_magnitude(bf16lo(d)), fp8_magnitude(bf16hi(d))) >> 16);
+    }
+  }
+  uint32_t other = top;
+  permlane16_swap(top, other);
+  top = other = max(top, other);
+  permlane32_swap(top, other);
+  return fp8_scale(max(top, other) << 16);
+}
+
+// The same of up to four rows of a bf16 activation, encoded by every workgroup for itself: K % 128 = 0, rows of x on 16 bytes.
+// A lane holds 32 of a block's 128 values of its row, and four lanes agree on the scale.  The conversion rounds as that of the
+// quantising kernel, so the sums are the same.  The encoding takes longer than the product's wait for w leaves, but less
+// than a launch: one row, K = 6144, N = 6144 9.8 us and (two launches) 10.2, N = 1536 5.5 and 8.1; with eight rows, N = 16384
+// it took 24.6 and 23.3, so more than four go the other way.
+struct Fp8RowsOf {
+  static constexpr int MR = 4, NW = 8, U = 3, OA = 2048, OSC = OA + 256 * MR, UNIT = OSC + 256;
+  static constexpr int D = 2 + 1 + 1;   // DMA instructions of a block: w, x, the weight's scale
+  static constexpr int LDS = NW * U * UNIT;
+  static_assert(LDS <= 80 * 1024 && NW * 1024 <= LDS, "two workgroups share a CU's LDS");
+};
+
+__global__ void __launch_bounds__(512) fp8_linear_rows_kernel(Fp8GemmParams p, const uint16_t* __restrict__ x, long ldx) {
+  using T = Fp8RowsOf;
+  constexpr int U = T::U;
+  __shared__ __attribute__((aligned(1024))) uint8_t sm[T::LDS];
+  const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, b = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = blockIdx.x * 16, kp = p.K, nst = kp / 128;
+  const uint32_t lds0 = lds_offset(sm) + wave * U * T::UNIT;
+  const uint8_t* mine = sm + wave * U * T::UNIT;
+  const int chunk = lane % 8 ^ (lane / 8 >> 1 & 3);
+  uint32_t off_w[2];
+#pragma unroll
+  for (int d = 0; d < 2; ++d) off_w[d] = (uint32_t)(min(8 * d + lane / 8, p.N - n0 - 1) * (long)kp + 16 * (chunk ^ 4 * d));
+  const uint16_t* src_x = x + min(lane / 16, p.M - 1) * ldx + 8 * (lane % 16);
+  const uint8_t* src_w = p.w + (long)n0 * kp;
+  const float* src_s = p.ws + (long)(n0 / 128) * nst;
+  auto fetch = [&](int block, int buf) __attribute__((always_inline)) {
+    const uint32_t to = lds0 + buf * T::UNIT;
+#pragma unroll
+    for (int d = 0; d < 2; ++d) dma16(src_w, off_w[d] + 128 * block, to + 1024 * d);
+    dma16_at(src_x + 128 * block, to + T::OA);
+    dma4_at(src_s + block, to + T::OSC);
+  };
+  const int count = wave < nst ? (nst - wave + T::NW - 1) / T::NW : 0;
+  f32x4 acc = {};
+  const int o0 = 16 * (b ^ (lr >> 1 & 7)), ox = 256 * (lr % T::MR) + 32 * b;
+  if (count) {
+    auto block_of = [&](int i) { return wave + T::NW * min(i, count - 1); };
+#pragma unroll
+    for (int i = 0; i < U; ++i) fetch(block_of(i), i);
+    int buf = 0;
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((U - 1) * T::D) : "memory");
+      const uint8_t* u = mine + buf * T::UNIT;
+      Fp8Frag fw, fa;
+      fw.q[0] = *reinterpret_cast<const u32x4*>(u + 128 * lr + o0);
+      fw.q[1] = *reinterpret_cast<const u32x4*>(u + 128 * lr + (o0 ^ 64));
+      u32x4 v[4];   // values 16 b .. 16 b + 15, 64 + 16 b .. 64 + 16 b + 15
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const u32x4*>(u + T::OA + ox + 128 * (j / 2) + 16 * (j % 2));
+      const float ws = *reinterpret_cast<const float*>(u + T::OSC);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // all of the block is in registers
+      fetch(block_of(i + U), buf);
+      buf = buf + 1 == U ? 0 : buf + 1;
+      const float s = row4_scale(v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        fa.q[j / 2][2 * (j % 2)] = fp8_encode_bf16x4(v[j][0], v[j][1], s);
+        fa.q[j / 2][2 * (j % 2) + 1] = fp8_encode_bf16x4(v[j][2], v[j][3], s);
+      }
+      const f32x4 y = fp8_mfma16(fw, fa);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(y[r], s * ws, acc[r]);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+  fp8_rows_sum(p, sm, acc, n0);
 }
 
 // y = the pieces' sums, in their order, and the bias; four columns a thread
@@ -445,6 +552,25 @@ hipError_t launch_fp8_gemm(const Fp8GemmParams& p, void* workspace, hipStream_t 
   const long quads = (long)p.M * ((p.N + 3) / 4);
   fp8_gemm_join_kernel<<<(unsigned)((quads + 255) / 256), 256, 0, st>>>(p, part, pieces);
   return hipGetLastError();
+}
+
+long fp8_linear_workspace_bytes(int M, int N, int K) {
+  const long kp = fp8_kp(K), codes = M * kp, scales = (M * (kp / 32) + 15) & ~15L;
+  return codes + scales + fp8_gemm_workspace_bytes(M, N, K);
+}
+
+hipError_t launch_fp8_linear(Fp8GemmParams p, const uint16_t* x, long ldx, void* workspace, hipStream_t st) {
+  if (p.M <= Fp8RowsOf::MR && p.K % 128 == 0 && ldx % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0) {
+    fp8_linear_rows_kernel<<<(unsigned)((p.N + 15) / 16), 512, 0, st>>>(p, x, ldx);
+    return hipGetLastError();
+  }
+  const long kp = fp8_kp(p.K), codes = p.M * kp, scales = (p.M * (kp / 32) + 15) & ~15L;
+  uint8_t* work = static_cast<uint8_t*>(workspace);
+  p.a = work;
+  float* at = reinterpret_cast<float*>(work + codes);
+  if (hipError_t e = launch_fp8_quantize(x, ldx, p.M, p.K, work, at, st); e != hipSuccess) return e;
+  p.as = at;
+  return launch_fp8_gemm(p, work + codes + scales, st);
 }
 
 }  // namespace svdq

@@ -323,6 +323,10 @@ __device__ __forceinline__ void dma16_page(const void* base, uint32_t off, uint3
   else dma16(base, off, lds);
 }
 
+// A page's scale that is not finite makes all of its keys (values) NaN.
+constexpr uint32_t FP8_NAN4 = 0x7F7F7F7Fu;
+__device__ __forceinline__ float finite_or_nan(float f) { return fabsf(f) < INFINITY ? f : __builtin_nanf(""); }
+
 template <int D>
 struct Kv8Few {
   static constexpr int R = 16, PITCH = D + 4, HALF = PAGE * D, RING = 2 * HALF, DMA = 2 * HALF / 1024;
@@ -380,7 +384,7 @@ __global__ void __launch_bounds__(256, 2) kv8_rows_kernel(Kv8Args p) {
     };
     auto look_scales_up = [&] {
       const long at = (long)max(id, 0) * p.c.Hkv + hk;
-      ks = p.c.scales[2 * at] * p.scale_log2;
+      ks = finite_or_nan(p.c.scales[2 * at] * p.scale_log2);
       vs = p.c.scales[2 * at + 1];
       asm volatile("s_waitcnt vmcnt(0)" : "+v"(ks), "+v"(vs)::"memory");
     };
@@ -414,7 +418,7 @@ __global__ void __launch_bounds__(256, 2) kv8_rows_kernel(Kv8Args p) {
       const int pg = p0 + wave + 4 * i;
       const bool have = __builtin_amdgcn_readlane(id, i - first) >= 0;
       const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks), i - first));
-      const float pv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), i - first));
+      float pv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs), i - first));
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       const uint8_t *sk = sm + wave * T::RING, *sv = sk + T::HALF;
       u32x4 kq[4][SP], vq[DT];
@@ -467,6 +471,11 @@ __global__ void __launch_bounds__(256, 2) kv8_rows_kernel(Kv8Args p) {
       } else {   // masks, values that are not numbers behind them, any scales
         const int key0 = pg * PAGE + 16 * g;
         float hi = -INFINITY;
+        if (!(fabsf(pv) < INFINITY)) {   // values that are not numbers, which the masks below take out
+          pv = 1.0f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) vq[d] = u32x4{} | FP8_NAN4;
+        }
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           S[k / 4][k % 4] = key0 + k >= vis ? -INFINITY : S[k / 4][k % 4] * f;
@@ -635,7 +644,7 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(Kv8Args p) {
 // not finite, or a page of which rows see different parts holds values that are no numbers, the tile is done again with an
 // offset that follows the maximum.
 // Scales that are no ordinary positive numbers are dealt with as the pages come in: a factor below 0 turns the keys' signs, other
-// scales of values are multiplied into them.  Pages that are not there count as -infinity.
+// scales of values are multiplied into them, those that are not finite make the codes NaN.  Pages that are not there count as -infinity.
 //
 // Rows in LDS are not padded: chunks of 16 bytes lie at slots exchanged by the row, c ^ (row mod 16) in rows of 256 bytes, c ^
 // (row / 2 mod 8) in rows of 128, which spreads sixteen lanes' reads of a chunk, and sixteen lanes' writes of two chunks each, over the 64
@@ -691,7 +700,7 @@ __global__ void __launch_bounds__(256, 2) kv8_many_kernel(Kv8Args p) {
     vss = p.c.scales[2 * at + 1];
     lvs = ordinary(vss) ? __builtin_amdgcn_logf(vss) : 0.0f;   // log2
     invs = ordinary(vss) ? 1.0f / vss : 1.0f;
-    odd_scales = __ballot(ids < 0 || !ordinary(vss) || !(kss > 0.0f));
+    odd_scales = __ballot(ids < 0 || !ordinary(vss) || !(kss > 0.0f && kss < INFINITY));
   };
   auto lane_of = [](float v, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i)); };
   u32x4 kr[T::CH], vr[T::CH];
@@ -711,7 +720,7 @@ __global__ void __launch_bounds__(256, 2) kv8_many_kernel(Kv8Args p) {
     Kv8Scale s{lane_of(kss, i), lane_of(lvs, i), lane_of(invs, i), 0.0f};
     if (odd_scales >> i & 1) {
       // a factor of 0 is the smallest there is: times -infinity that is no NaN
-      s.f = s.f == 0.0f ? 0x1p-126f : fabsf(s.f);
+      s.f = s.f == 0.0f ? 0x1p-126f : fabsf(s.f) < INFINITY ? fabsf(s.f) : 1.0f;
       if (__builtin_amdgcn_readlane(ids, i) < 0) s = {0x1p-126f, -INFINITY, 1.0f, -INFINITY};
     }
     return s;
@@ -722,14 +731,17 @@ __global__ void __launch_bounds__(256, 2) kv8_many_kernel(Kv8Args p) {
   auto store = [&](int pg, int buf) __attribute__((always_inline)) {
     const int i0 = pg - first;
     const bool odd = odd_scales >> i0 & 1, here = __builtin_amdgcn_readlane(ids, i0) >= 0;
-    const float vs = odd && here ? lane_of(vss, i0) : 1.0f;
+    float vs = odd && here ? lane_of(vss, i0) : 1.0f;
     if (odd) {
-      const uint32_t turn = here && lane_of(kss, i0) < 0.0f ? 0x80808080u : 0u, keep = here ? ~0u : 0u;
+      const float ks = lane_of(kss, i0);
+      const uint32_t turn = here && ks < 0.0f ? 0x80808080u : 0u, keep = here ? ~0u : 0u;
+      const uint32_t kn = here && !(fabsf(ks) < INFINITY) ? FP8_NAN4 : 0u, vn = fabsf(vs) < INFINITY ? 0u : FP8_NAN4;
 #pragma unroll
       for (int i = 0; i < T::CH; ++i) {
-        kr[i] = (kr[i] & keep) ^ turn;
-        vr[i] &= keep;
+        kr[i] = ((kr[i] & keep) ^ turn) | kn;
+        vr[i] = (vr[i] & keep) | vn;
       }
+      if (vn) vs = 1.0f;
     }
     if (pg >= pe) {
       uint32_t any = 0;

@@ -471,9 +471,8 @@ std::tuple<Tensor, Tensor> fp8_quantize(const Tensor& x) {
   return {codes, scales};
 }
 
-// y [lead..., N] of rows of kp codes at a, their scales at as
-Tensor fp8_product(const void* a, const float* as, int64_t m, int64_t kp, std::vector<int64_t> lead, const Tensor& w,
-                   const Tensor& w_scales, const OptTensor& bias) {
+// w, w_scales and bias for rows of kp codes; y [lead..., N]
+Tensor fp8_output(int64_t kp, std::vector<int64_t> lead, const Tensor& w, const Tensor& w_scales, const OptTensor& bias) {
   const c10::Device dev = w.device();
   check_tensor("w", w, dev, at::kFloat8_e4m3fn);
   TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) > 0 && w.size(0) <= INT32_MAX, "w must be [N, K] codes, got ", w.sizes());
@@ -488,41 +487,46 @@ Tensor fp8_product(const void* a, const float* as, int64_t m, int64_t kp, std::v
     TORCH_CHECK_VALUE(bias->numel() == n, "bias must have ", n, " entries, got ", bias->numel());
   }
   lead.push_back(n);
-  Tensor y = at::empty(lead, w.options().dtype(at::kBFloat16));
-  const int64_t bytes = svdq_fp8_gemm_workspace((int)m, (int)n, (int)kp);
-  const Tensor work = bytes ? at::empty({bytes}, w.options().dtype(at::kByte)) : Tensor();
-  check_status("svdq_fp8_gemm", svdq_fp8_gemm(a, as, ptr(w), ptr<float>(w_scales), ptr(bias), (int)m, (int)n, (int)kp,
-                                              ptr(y), n, bytes ? ptr(work) : nullptr, stream_of(dev)));
-  return y;
+  return at::empty(lead, w.options().dtype(at::kBFloat16));
+}
+
+Tensor workspace_of(int64_t bytes, const Tensor& like) {
+  return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
 
 Tensor fp8_gemm(const Tensor& a, const Tensor& a_scales, const Tensor& w, const Tensor& w_scales, const OptTensor& bias) {
-  const c10::DeviceGuard guard(w.device());
-  check_tensor("a", a, w.device(), at::kFloat8_e4m3fn);
+  const c10::Device dev = w.device();
+  const c10::DeviceGuard guard(dev);
+  check_tensor("a", a, dev, at::kFloat8_e4m3fn);
   TORCH_CHECK_VALUE(a.dim() >= 1 && a.size(-1) > 0 && a.size(-1) % 128 == 0 && a.size(-1) <= 1 << 30, "a must be [..., K] "
                     "codes, K a multiple of 128, got ", a.sizes());
   std::vector<int64_t> lead = a.sizes().vec();
   const int64_t kp = lead.back(), m = a.numel() / kp;
   lead.pop_back();
   TORCH_CHECK_VALUE(m <= INT32_MAX, "a: ", m, " rows are too many");
-  check_tensor("a_scales", a_scales, w.device(), at::kFloat);
+  check_tensor("a_scales", a_scales, dev, at::kFloat);
   const std::vector<int64_t> want{kp / 128, m};
   TORCH_CHECK_VALUE(a_scales.sizes() == at::IntArrayRef(want), "a_scales must be ", at::IntArrayRef(want), ", got ",
                     a_scales.sizes());
-  return fp8_product(ptr(a), ptr<float>(a_scales), m, kp, lead, w, w_scales, bias);
+  const Tensor y = fp8_output(kp, lead, w, w_scales, bias);
+  const int n = (int)w.size(0);
+  const Tensor work = workspace_of(svdq_fp8_gemm_workspace((int)m, n, (int)kp), w);
+  check_status("svdq_fp8_gemm", svdq_fp8_gemm(ptr(a), ptr<float>(a_scales), ptr(w), ptr<float>(w_scales), ptr(bias), (int)m,
+                                              n, (int)kp, ptr(y), n, work.defined() ? ptr(work) : nullptr, stream_of(dev)));
+  return y;
 }
 
 Tensor fp8_linear(const Tensor& x, const Tensor& w, const Tensor& w_scales, const OptTensor& bias) {
-  const c10::DeviceGuard guard(w.device());
-  TORCH_CHECK_VALUE(x.device() == w.device(), "x is on ", x.device(), ", expected ", w.device());
+  const c10::Device dev = w.device();
+  const c10::DeviceGuard guard(dev);
+  TORCH_CHECK_VALUE(x.device() == dev, "x is on ", x.device(), ", expected ", dev);
   const Rows r("x", x);
-  const int64_t kp = mx_kp(r.k), codes = r.m * kp;
-  const Tensor work = at::empty({codes + r.m * kp / 32}, r.t.options().dtype(at::kByte));
-  uint8_t* base = ptr<uint8_t>(work);
-  float* scales = reinterpret_cast<float*>(base + codes);
-  check_status("svdq_fp8_quantize", svdq_fp8_quantize(ptr(r.t), r.ld, (int)r.m, (int)r.k, base, scales,
-                                                      stream_of(w.device())));
-  return fp8_product(base, scales, r.m, kp, r.lead, w, w_scales, bias);
+  const Tensor y = fp8_output(mx_kp(r.k), r.lead, w, w_scales, bias);
+  const int n = (int)w.size(0);
+  const Tensor work = workspace_of(svdq_fp8_linear_workspace((int)r.m, n, (int)r.k), w);
+  check_status("svdq_fp8_linear", svdq_fp8_linear(ptr(r.t), r.ld, ptr(w), ptr<float>(w_scales), ptr(bias), (int)r.m, n,
+                                                  (int)r.k, ptr(y), n, work.defined() ? ptr(work) : nullptr, stream_of(dev)));
+  return y;
 }
 
 // [T, heads, D] with dense heads on 16 bytes; `packed`: heads one behind another

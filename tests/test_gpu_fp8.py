@@ -96,6 +96,40 @@ def test_product_of_small_whole_numbers_is_exact(dev, m, n):
     assert torch.equal(y, (ab @ wb.T).to(torch.bfloat16))
 
 
+@pytest.mark.parametrize("m,n,k,bias", [(20, 130, 4096, True), (33, 1001, 2048, True), (77, 256, 6144, False), (17, 3, 16384, False)])
+def test_product_in_pieces_of_k(dev, m, n, k, bias):
+    """Few tiles: K is cut into pieces, whose sums are joined."""
+    test_product(dev, m, n, k, bias)
+
+
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 8, 9])
+@pytest.mark.parametrize("n,k", [(1, 128), (100, 640), (1000, 6144)])
+def test_linear_of_few_rows_is_the_product_of_the_quantized_ones(dev, m, n, k):
+    """Bit for bit, whichever kernel encodes: rows on 16 bytes and off them, of all magnitudes, zeros, infinities and NaN."""
+    g = gen(m + n)
+    x = normal((m, k + 8), g) * torch.exp2(torch.randint(-130, 100, (m, k + 8), generator=g).float()).to(torch.bfloat16)
+    x[m - 1, :130] = 0
+    x[m // 2, 64] = math.inf
+    x[0, k - 1] = math.nan
+    w, ws = (t.to(dev) for t in weight(n, k, g))
+    b = normal((n,), g).to(dev)
+    for z in (x.to(dev)[:, :k], x.to(dev)[:, 3:3 + k], x.to(dev)[:, 8:].contiguous()):
+        y = ops.fp8_linear(z, w, ws, b)
+        want = ops.fp8_gemm(*ops.fp8_quantize(z), w, ws, b)
+        assert torch.equal(torch.isnan(y), torch.isnan(want))
+        assert torch.equal(y.nan_to_num(), want.nan_to_num())
+
+
+def test_product_whose_output_passes_32_bits(dev):
+    m, n = 140000, 16384   # one block of K: a value is one product, whatever the tile
+    g = torch.Generator(device=dev).manual_seed(0)
+    a, w = (torch.randint(-3, 4, (r, 128), device=dev, generator=g).float().to(torch.float8_e4m3fn) for r in (m, n))
+    sa, sw = torch.rand(1, m, device=dev, generator=g), torch.rand(n // 128, 1, device=dev, generator=g)
+    y = ops.fp8_gemm(a, sa, w, sw)
+    for at in (0, 131071, m - 300):
+        assert torch.equal(y[at:at + 300], ops.fp8_gemm(a[at:at + 300], sa[:, at:at + 300].contiguous(), w, sw))
+
+
 def test_product_passes_nan_and_zero_scales(dev):
     x = normal((5, 256), gen(3))
     x[1, 40], x[2, 200] = math.nan, math.inf
@@ -227,6 +261,11 @@ def attend(c, heads, causal, scale=None, q=None):
     return got
 
 
+def attend_gpu(c, heads, causal):
+    q = normal((c.offsets[-1], heads, c.d), c.g)
+    return ops.kv8_attention(q.to(c.dev), *c.device(), c.d ** -0.5, causal)
+
+
 @pytest.mark.parametrize("name", SEQS)
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("heads,kv", [(1, 1), (6, 2), (12, 3), (40, 2)])
@@ -294,6 +333,213 @@ def test_attention_queries_sliced_from_a_projection(dev):
     c = Cache(dev, [(30, 100)], 2, 64, 9)
     wide = normal((30, 12, 64), c.g)
     assert torch.equal(attend(c, 8, True, q=wide[:, 2:10]), attend(c, 8, True, q=wide[:, 2:10].contiguous()))
+
+
+def shared(dev, n, held, heads, kv, d, count, seed):
+    """`count` sequences of the same tokens that read the same pages: one of them against the definition, all alike."""
+    c = Cache(dev, [(n, held)], kv, d, seed)
+    q = normal((n, heads, d), c.g)
+    want, bound = u.attention(q, c.offsets, c.lengths(), c.table, *c.oracle(), d ** -0.5, True)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)   # noqa: E731
+    _, _, _, k, v, s = c.device()
+    got = ops.kv8_attention(q.to(dev).repeat(count, 1, 1), i32([n * b for b in range(count + 1)]), i32([held] * count),
+                            i32(c.table * count), k, v, s, d ** -0.5)
+    u.check(got, want.repeat(count, 1, 1), bound.repeat(count, 1, 1))
+
+
+@pytest.mark.parametrize("n,heads,count", [(1, 1, 129), (9, 32, 100)])
+def test_attention_of_many_sequences_over_more_pages_than_a_look_up(dev, n, heads, count):
+    """More sequences than lanes, and each piece longer than the 64 pages that are looked up at a time."""
+    shared(dev, n, 17000, heads, 1, 64, count, 20)
+
+
+@pytest.mark.parametrize("n", [1, 100])
+def test_many_sequences(dev, n):
+    """64 and more sequences, some empty; few rows and many."""
+    seqs = [(0, 3) if b % 7 == 3 else (n + b % 3, n + 3 * b) for b in range(75)]
+    attend(Cache(dev, seqs, 2, 64, 21, stale=False), 8, True)
+    c = Cache(dev, seqs, 2, 64, 22)
+    k, v = normal((c.offsets[-1], 2, 64), c.g), normal((c.offsets[-1], 2, 64), c.g)
+    c.s = torch.exp2(torch.randint(-9, 3, c.s.shape, generator=c.g).float())
+    want = c.oracle()
+    u.append(k, v, c.offsets, c.lengths(True), c.table, *want)
+    args = c.device(before=True)
+    ops.kv8_append(k.to(dev), v.to(dev), *args)
+    same_codes(args[3], want[0])
+    same_codes(args[4], want[1])
+    assert torch.equal(args[5].cpu().double(), want[2])
+
+
+@pytest.mark.parametrize("n", [3, 130])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_page_scales_of_any_kind(dev, n, d):
+    """Negative, zero, far from 1, and not a number in a page that only the last tokens see."""
+    c = Cache(dev, [(n, 700)], 2, d, 30)
+    t = c.table[0]
+    c.s[t[0], 0, 0], c.s[t[1], 1, 0] = 0.0, -0.003
+    c.s[t[2], 0, 1], c.s[t[3], 1, 1], c.s[t[4], 0, 1], c.s[t[5], 1, 1] = 0.0, -0.01, 2.0 ** -100, 2.0 ** 100
+    attend(c, 8, True)
+    c.s[t[10], 0, 0], c.s[t[10], 1, 1] = math.nan, math.nan   # tokens 640 ..
+    attend(c, 8, True)
+    c.s[t[10]] = 0.01
+    c.s[t[3], 1, 1], c.s[t[10], 1, 0] = math.inf, -math.inf   # head 1: NaN throughout
+    c.s[t[10], 0, 1] = math.nan
+    got = attend_gpu(c, 8, True)
+    assert torch.isnan(got[:, 4:]).all()
+    seen = max(0, n - 60)   # rows that see token 640
+    assert torch.isnan(got[n - min(n, 60):, :4]).all() and torch.isfinite(got[:seen, :4]).all()
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("n", [12, 130])
+def test_attention_scale_that_is_no_number_reaches_only_rows_that_see_it(dev, n, bad, which):
+    c = Cache(dev, [(n, 136)], 1, 64, 33)   # the last page: tokens 128 to 135, seen by the last 8 rows
+    c.s[c.table[0][2], 0, which] = bad
+    got = attend_gpu(c, 4, True).cpu()
+    assert torch.isnan(got[n - 8:]).all() and torch.isfinite(got[:n - 8]).all()
+    c.s[c.table[0][2], 0, which] = math.nan   # as the definition has it
+    attend(c, 4, True)
+
+
+@pytest.mark.parametrize("n", [3, 130])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_scores_far_apart_and_a_missing_first_page(dev, n, d):
+    """Scores whose exponents are hundreds apart, in any order; then without the first page, or the first four."""
+    c = Cache(dev, [(n, 700)], 2, d, 31)
+    attend(c, 8, True, scale=4.0)
+    c.table[0][0] = -1
+    attend(c, 8, True, scale=4.0)
+    attend(c, 8, False)
+    c.table[0][:4] = [-1, 10 ** 6, -5, -1]
+    attend(c, 8, True)
+    c.table[0][:] = [-1] * len(c.table[0])
+    assert not attend(c, 8, True).any()
+
+
+@pytest.mark.parametrize("n", [1, 130])
+def test_attention_of_infinite_queries_stays_in_its_rows(dev, n):
+    c = Cache(dev, [(n, 300)], 1, 64, 32)
+    q = normal((n, 4, 64), c.g)
+    want = ops.kv8_attention(q.to(dev), *c.device(), 0.125)
+    q[0, 1, 5], q[n - 1, 2, 0] = math.inf, math.nan
+    got = ops.kv8_attention(q.to(dev), *c.device(), 0.125)
+    hit = torch.zeros(n, 4, dtype=torch.bool)
+    hit[0, 1] = hit[n - 1, 2] = True
+    # a matrix tile of which some row is not finite may be summed in another order
+    assert torch.isnan(got.cpu()[hit]).all() and torch.isfinite(got.cpu()[~hit]).all()
+    wanted, bound = u.attention(q[:, [0, 3]], c.offsets, c.lengths(), c.table, *c.oracle(), 0.125, True)
+    u.check(got[:, [0, 3]], wanted, bound)
+    assert torch.isfinite(want).all()
+
+
+@pytest.mark.parametrize("n", [1, 80])
+def test_cache_that_passes_32_bits(dev, n):
+    """Pages at the end of a cache of more than 2^32 codes: as those of a small one."""
+    c = Cache(dev, [(n, 400)], 4, 128, 40)
+    count, kv, d = 140000, 4, 128
+    used = torch.tensor(c.table[0], device=dev)
+    cu, before, table, k, v, s = c.device(before=True)
+    big_k = torch.empty((count, kv, u.PAGE, d), dtype=torch.float8_e4m3fn, device=dev)
+    big_v = torch.empty((count, kv, d, u.PAGE), dtype=torch.float8_e4m3fn, device=dev)
+    big_s = torch.zeros((count, kv, 2), device=dev)
+    far = count - 1 - 2 * torch.arange(len(used), device=dev)
+    for big, small in ((big_k.view(torch.uint8), k.view(torch.uint8)), (big_v.view(torch.uint8), v.view(torch.uint8)), (big_s, s)):
+        for i, j in zip(far.tolist(), used.tolist()):
+            big[i] = small[j]
+    x = normal((n, 2 * kv, d), c.g).to(dev)
+    q = normal((n, 8, d), c.g).to(dev)
+    outs = []
+    for tab, cache in ((table, (k, v, s)), (far.int()[None], (big_k, big_v, big_s))):
+        ops.kv8_append(x[:, :kv], x[:, kv:], cu, before, tab, *cache)
+        outs.append(ops.kv8_attention(q, cu, before + n, tab, *cache, d ** -0.5))
+    assert torch.equal(*outs) and outs[0].any()
+    for i, j in zip(far.tolist(), used.tolist()):
+        assert torch.equal(big_k[i].view(torch.uint8), k[j].view(torch.uint8)) and torch.equal(big_s[i], s[j])
+        assert torch.equal(big_v[i].view(torch.uint8), v[j].view(torch.uint8))
+
+
+def test_strides_that_pass_32_bits(dev):
+    """Two tokens 2^31 + 64 values apart."""
+    far = torch.zeros(2 ** 31 + 4096, dtype=torch.bfloat16, device=dev)
+    x = far.as_strided((2, 4, 64), (2 ** 31 + 64, 64, 1))
+    dense = normal((2, 4, 64), gen(41)).to(dev)
+    x.copy_(dense)
+    rows, drows = x.as_strided((2, 256), (2 ** 31 + 64, 1)), dense.view(2, 256)
+    for a, b in zip(ops.fp8_quantize(rows), ops.fp8_quantize(drows)):
+        assert torch.equal(a.float(), b.float())
+    w, ws = (t.to(dev) for t in weight(130, 256, gen(42)))
+    assert torch.equal(ops.fp8_linear(rows, w, ws), ops.fp8_linear(drows, w, ws))
+    tab = torch.rand(2, 32, device=dev)
+    for a, b in zip(ops.qk_norm_rope(x[:, :2], x[:, 2:], None, None, tab, tab, 1e-6),
+                    ops.qk_norm_rope(dense[:, :2], dense[:, 2:], None, None, tab, tab, 1e-6)):
+        assert torch.equal(a, b)
+    c = Cache(dev, [(2, 30)], 2, 64, 43)
+    outs = []
+    for t in (x, dense):
+        args = c.device(before=True)
+        ops.kv8_append(t[:, :2], t[:, 2:], *args)
+        outs.append((args[3].float(), args[4].float(), args[5], ops.kv8_attention(t, args[0], args[1] + 2, *args[2:], 0.125)))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+def test_calls_on_two_streams_at_once(dev):
+    """Split along the keys and along K, so that each call has partial results of its own."""
+    c = Cache(dev, [(1, 9000)], 2, 64, 44)
+    args = c.device()
+    q = [normal((1, 8, 64), c.g).to(dev) for _ in range(2)]
+    w, ws = (t.to(dev) for t in weight(256, 6144, gen(45)))
+    x = [normal((40, 6144), c.g).to(dev) for _ in range(2)]
+    want = [(ops.kv8_attention(a, *args, 0.125), ops.fp8_linear(b, w, ws)) for a, b in zip(q, x)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append((ops.kv8_attention(q[i], *args, 0.125), ops.fp8_linear(x[i], w, ws)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o, y in got[i]:
+            assert torch.equal(o, want[i][0]) and torch.equal(y, want[i][1])
+
+
+def test_graph_of_split_calls_replayed(dev):
+    c = Cache(dev, [(1, 9000), (1, 400)], 2, 64, 46)
+    args = c.device()
+    q = normal((2, 8, 64), c.g).to(dev)
+    w, ws = (t.to(dev) for t in weight(256, 6144, gen(47)))
+    x = normal((40, 6144), c.g).to(dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.kv8_attention(q, *args, 0.125), ops.fp8_linear(x, w, ws)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, y = ops.kv8_attention(q, *args, 0.125), ops.fp8_linear(x, w, ws)
+    for i in range(5):
+        q.copy_(normal(q.shape, c.g))
+        x.copy_(normal(x.shape, c.g))
+        args[1].copy_(torch.tensor([9000 - 700 * i, 1 + 90 * i]))
+        want = ops.kv8_attention(q, *args, 0.125), ops.fp8_linear(x, w, ws)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want[0]) and torch.equal(y, want[1])
+
+
+def test_nothing_to_do(dev):
+    c = Cache(dev, [(0, 5), (0, 0)], 2, 64, 48)
+    args = c.device()
+    none = torch.zeros((0, 2, 64), dtype=torch.bfloat16, device=dev)
+    assert ops.kv8_attention(none, *args, 0.125).shape == (0, 2, 64)
+    before = [t.float().clone() for t in args[3:]]
+    ops.kv8_append(none, none, *args)
+    assert all(torch.equal(a.float().nan_to_num(), b.nan_to_num()) for a, b in zip(args[3:], before))
+    tab = torch.zeros(1, 32, device=dev)
+    assert [t.shape for t in ops.qk_norm_rope(none, none, None, None, tab, tab, 1e-6)] == [(0, 2, 64)] * 2
 
 
 # ---- together ------------------------------------------------------------------------------------------------------
