@@ -80,7 +80,8 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8Cache c, const uint1
                                                          const uint16_t* __restrict__ v, long ldv) {
   constexpr int CH = D / 8, ROUNDS = PAGE * CH / 256;   // chunks of 8 channels of a token
   __shared__ uint32_t tops[2][4];
-  __shared__ __attribute__((aligned(16))) uint8_t turn[D * PAGE];
+  constexpr int PITCH = PAGE + 4;   // bytes of a channel: one word over, which spreads the lanes over the banks
+  __shared__ __attribute__((aligned(16))) uint8_t turn[D * PITCH];
   const int tid = threadIdx.x, head = blockIdx.x % c.Hkv;
   const long number = blockIdx.x / c.Hkv;
   const Kv8Sequence q = find_sequence(c, number, 1, PAGE, 2);
@@ -89,23 +90,23 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8Cache c, const uint1
   const long start = q.len, page = start / PAGE + (number - q.unit0);
   if (page >= c.W || page * PAGE >= start + n) return;
   const int id = c.table[(long)b * c.W + page];
-  if (id < 0 || id >= c.P) return;
   const int lo = (int)max(start - page * PAGE, 0L), hi = (int)min(start + n - page * PAGE, (long)PAGE);
   const long base = row0 + page * PAGE - start;   // row of the page's slot 0
-  const long at = (long)id * c.Hkv + head;
-  uint8_t *kc = c.kc + at * PAGE * D, *vc = c.vc + at * PAGE * D;
 
-  u32x4 x[2][ROUNDS];
+  u32x4 x[2][ROUNDS];   // on their way while the page is looked up
   uint32_t top[2] = {0, 0};
 #pragma unroll
   for (int i = 0; i < ROUNDS; ++i) {
-    const int slot = (tid + 256 * i) / CH, ch = (tid + 256 * i) % CH;
+    const int slot = ROUNDS * (tid / CH) + i, ch = tid % CH;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       x[w][i] = u32x4{};
       if (slot >= lo && slot < hi) x[w][i] = ld16((w ? v + (base + slot) * ldv : k + (base + slot) * ldk) + head * D + 8 * ch);
     }
   }
+  if (id < 0 || id >= c.P) return;
+  const long at = (long)id * c.Hkv + head;
+  uint8_t *kc = c.kc + at * PAGE * D, *vc = c.vc + at * PAGE * D;
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
 #pragma unroll
@@ -117,6 +118,7 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8Cache c, const uint1
     for (int o = 32; o > 0; o >>= 1) top[w] = max(top[w], (uint32_t)__shfl_xor((int)top[w], o, 64));
     if ((tid & 63) == 0) tops[w][tid >> 6] = top[w];
   }
+  const float had[2] = {c.scales[2 * at], c.scales[2 * at + 1]};
   __syncthreads();
   float s[2], again[2];   // the page's scales, and what its older codes are multiplied by
 #pragma unroll
@@ -124,15 +126,10 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8Cache c, const uint1
     s[w] = fp8_scale(max(max(tops[w][0], tops[w][1]), max(tops[w][2], tops[w][3])));
     again[w] = 1.0f;
     if (lo > 0) {
-      const float before = c.scales[2 * at + w];
-      if (before >= s[w]) {
-        s[w] = before;
-      } else {
-        again[w] = before / s[w];
-      }
+      if (had[w] >= s[w]) s[w] = had[w];
+      else again[w] = had[w] / s[w];
     }
   }
-  __syncthreads();   // the scales have been read
   if (tid < 2) c.scales[2 * at + tid] = tid ? s[1] : s[0];
   auto encode = [](u32x4 r, float s) {
     if (__float_as_uint(s) & 0x7FFFFFu) {   // a scale of the caller's, no power of two: the conversion takes only those
@@ -154,30 +151,38 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8Cache c, const uint1
   const bool whole = lo == 0 && hi == PAGE;
 #pragma unroll
   for (int i = 0; i < ROUNDS; ++i) {
-    const int slot = (tid + 256 * i) / CH, ch = (tid + 256 * i) % CH;
+    const int slot = ROUNDS * (tid / CH) + i, ch = tid % CH;
     u32x2* kd = reinterpret_cast<u32x2*>(kc + slot * D + 8 * ch);
     if (slot >= lo && slot < hi) {
       *kd = encode(x[0][i], s[0]);
-      const u32x2 o = encode(x[1][i], s[1]);
+      if (!whole) {
+        const u32x2 o = encode(x[1][i], s[1]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint8_t q = (uint8_t)(o[e / 4] >> (8 * (e % 4)));
-        if (whole) turn[(8 * ch + e) * PAGE + (slot ^ (ch % 16 * 4))] = q;   // spread over the banks
-        else vc[(8 * ch + e) * PAGE + slot] = q;
+        for (int e = 0; e < 8; ++e) vc[(8 * ch + e) * PAGE + slot] = (uint8_t)(o[e / 4] >> (8 * (e % 4)));
       }
     } else if (slot < lo && again[0] != 1.0f) {
       const u32x2 old = *kd;
       *kd = u32x2{scaled(old[0], again[0]), scaled(old[1], again[0])};
     }
   }
-  if (whole) {
+  if (whole) {   // values through LDS: a thread holds ROUNDS tokens of 8 channels, a line of the page is 64 of one
+    const int ch = tid % CH;
+    u32x2 o[ROUNDS];
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) o[i] = encode(x[1][i], s[1]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < ROUNDS; ++i) w |= (o[i][e / 4] >> 8 * (e % 4) & 0xFFu) << 8 * i;
+      uint8_t* to = turn + (8 * ch + e) * PITCH + ROUNDS * (tid / CH);
+      if (ROUNDS == 4) *reinterpret_cast<uint32_t*>(to) = w;
+      else *reinterpret_cast<uint16_t*>(to) = (uint16_t)w;
+    }
     __syncthreads();
     for (int i = tid; i < D * PAGE / 16; i += 256) {
-      const int d = i / 4, key = 16 * (i % 4), f = d / 8 % 16 * 4;
-      u32x4 o;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = *reinterpret_cast<const uint32_t*>(turn + d * PAGE + ((key + 4 * e) ^ f));
-      *reinterpret_cast<u32x4*>(vc + d * PAGE + key) = o;
+      const uint32_t* from = reinterpret_cast<const uint32_t*>(turn + i / 4 * PITCH + 16 * (i % 4));
+      *reinterpret_cast<u32x4*>(vc + 16 * i) = u32x4{from[0], from[1], from[2], from[3]};
     }
   } else if (lo > 0 && again[1] != 1.0f) {
     // whole words of older values; in the last one the new tokens' bytes, which other threads write, are not touched
