@@ -37,7 +37,8 @@ the stores of to_gate, ff.up, to_out.0 and ff.down instead.  The linears that re
 come as MX blocks in the layers' format (E4M3) (``svdq::rms_norm_modulate_mx``, ``svdq::residual_rms_norm_modulate_mx``,
 ``svdq::silu_mul_mx``), one quantised activation for all layers that read it and no bf16 copy of it.  Blocks with other
 layers among them, with subclasses of ``MXLinear``, forward hooks or a replaced ``forward``, or with ``NORMS`` or ``GATES``
-set to "torch", call their layers on bf16 activations, each of which quantises its own.
+set to "torch", call their layers on bf16 activations, each of which quantises its own.  ``linears="fp8"`` builds them on
+``FP8Linear`` layers, those that read the same input on one quantised activation (``run_grouped``).
 """
 from __future__ import annotations
 
@@ -54,6 +55,7 @@ from torch.nn.modules import module as _module
 from ..kernels.hip import ops as hip_ops
 from ..quant.state import SVDQuantLinearState
 from .linear import SVDQuantLinear
+from .fp8_linear import FP8Linear
 from .mx_linear import MXLinear
 from .siblings import run_concurrent, run_grouped
 
@@ -110,6 +112,13 @@ def random_mx_linear(n: int, k: int, *, device: torch.device | str = "cuda", gen
     """A random-init ``MXLinear`` of a N(0, 1 / k) weight."""
     w = torch.randn(n, k, device=torch.device(device), generator=generator) / math.sqrt(k)
     return MXLinear.from_dense(w, activation=activation)
+
+
+def random_fp8_linear(n: int, k: int, *, device: torch.device | str = "cuda", generator: torch.Generator | None = None
+                      ) -> FP8Linear:
+    """A random-init ``FP8Linear`` of a N(0, 1 / k) weight."""
+    w = torch.randn(n, k, device=torch.device(device), generator=generator) / math.sqrt(k)
+    return FP8Linear.from_dense(w)
 
 
 def rms_norm(x: Tensor, eps: float = 1e-6, weight: Optional[Tensor] = None) -> Tensor:
@@ -251,8 +260,9 @@ class Krea2StandInBlock(nn.Module):
         linears one after another on one quantised activation, whatever ``siblings`` says."""
         mod = self.modulation if modulation is None else modulation
         if fused:
-            if any(isinstance(m, MXLinear) for m in self.linears().values()):
-                raise NotImplementedError("MXLinear layers have no fused store ops")
+            for m in self.linears().values():
+                if isinstance(m, (MXLinear, FP8Linear)):
+                    raise NotImplementedError(f"{type(m).__name__} layers have no fused store ops")
             return self._forward_fused(x, cos, sin, self.linears(), tuple(m.to(x.dtype) for m in mod), siblings)
         x, (g_f, y_f) = self._forward_deferred(x, cos, sin, linear, mod, siblings, None)
         return torch.addcmul(x, g_f, y_f)
@@ -400,14 +410,15 @@ class Krea2StandInTransformer(nn.Module):
                backend: str = "hip_gfx950", device: torch.device | str = "cuda", seed: int = 0,
                linears: str = "svdquant") -> "Krea2StandInTransformer":
         """Random-init model with every quantized linear resident on ``device``: ``linears`` "svdquant"
-        (``SVDQuantLinear`` of ``rank``, ``group_size`` and ``backend``) or "mx" (``MXLinear``)."""
-        if linears not in ("svdquant", "mx"):
-            raise ValueError(f"linears must be 'svdquant' or 'mx', got {linears!r}")
+        (``SVDQuantLinear`` of ``rank``, ``group_size`` and ``backend``), "mx" (``MXLinear``) or "fp8" (``FP8Linear``)."""
+        dense = {"mx": random_mx_linear, "fp8": random_fp8_linear}
+        if linears != "svdquant" and linears not in dense:
+            raise ValueError(f"linears must be 'svdquant', 'mx' or 'fp8', got {linears!r}")
         dev = torch.device(device)
         gen = torch.Generator(device=dev).manual_seed(seed)
         blocks = []
         for _ in range(dims.layers):
-            layers = {name: random_mx_linear(n, k, device=dev, generator=gen) if linears == "mx" else
+            layers = {name: dense[linears](n, k, device=dev, generator=gen) if linears in dense else
                       SVDQuantLinear(random_quantized_state(n, k, rank=rank, group_size=group_size,
                                                             device=dev, generator=gen), backend=backend)
                       for name, (n, k) in dims.linear_shapes().items()}

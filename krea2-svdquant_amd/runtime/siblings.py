@@ -87,11 +87,25 @@ def _groupable(x: Tensor, layers: Sequence[nn.Module]) -> bool:
                for m in layers)
 
 
+def _share_fp8(x: Tensor, layers: Sequence[nn.Module]) -> bool:
+    """All are ``FP8Linear`` as they come: no subclass, hooks or ``forward`` of their own, which ``forward_fp8`` would pass by."""
+    from torch.nn.modules import module
+    from .fp8_linear import FP8Linear
+    return (x.is_cuda and len(layers) > 1
+            and all(type(m) is FP8Linear and m.in_features == layers[0].in_features for m in layers)
+            and not any(m._forward_hooks or m._forward_pre_hooks or "forward" in vars(m) for m in layers)
+            and not (module._global_forward_hooks or module._global_forward_pre_hooks))
+
+
 def run_grouped(x: Tensor, layers: Sequence[nn.Module]) -> list[Tensor]:
     """``[layer(x) for layer in layers]``; when every layer is an ``SVDQuantLinear`` of one mode
     (W4A4 or W4A16) with group size 64 or 128 and the same in_features (2 to 4 layers, on the
     GPU), their GEMMs run as one launch (``forward_prepared_siblings``; W4A16 where the grouped
-    tiles pay), each with its layer's LoRA adapters.  Other layer sets run one after another."""
+    tiles pay), each with its layer's LoRA adapters.  ``FP8Linear`` layers run one after another on one quantised
+    activation, with the same results.  Other layer sets run one after another."""
+    if _share_fp8(x, layers):
+        h = layers[0].quantize(x)
+        return [m.forward_fp8(*h) for m in layers]
     if not _groupable(x, layers):
         return [m(x) for m in layers]
     from ..kernels.hip.backend import forward_prepared_siblings

@@ -607,3 +607,142 @@ def test_a_layer_step_by_step(dev):
         assert torch.equal(a, b)
     for a, b in zip(cache_a, cache_b):
         assert torch.equal(a.view(torch.uint8) if a.element_size() == 1 else a, b.view(torch.uint8) if b.element_size() == 1 else b)
+
+
+# ---- modules -----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("m", [1, 5, 40])
+def test_module(dev, m):
+    from krea2_svdquant_amd import FP8Linear
+    from krea2_svdquant_amd.quant.fp8 import quantize_fp8
+    g = gen(50 + m)
+    dense, bias = normal((200, 300), g, 0.05), normal((200,), g)
+    layer = FP8Linear.from_dense(dense.to(dev), bias.to(dev))
+    x = normal((2, m, 300), g).to(dev)
+    y = layer(x)
+    codes, scales = quantize_fp8(dense)
+    assert torch.equal(layer.weight_codes.cpu(), codes.view(torch.uint8)) and torch.equal(layer.weight_scales.cpu(), scales)
+    assert y.shape == (2, m, 200) and torch.equal(y, ops.fp8_linear(x, codes.to(dev), scales.to(dev), bias.to(dev)))
+    assert torch.equal(y, layer.forward_fp8(*layer.quantize(x)))
+    a, sa = ops.fp8_quantize(x)
+    want, bound = u.product(a.cpu().float().view(2 * m, -1), sa.cpu(), codes.float(), scales, bias)
+    u.check(y.view(2 * m, -1), want, bound)
+    moved = FP8Linear.from_dense(torch.zeros(200, 300), torch.zeros(200))
+    moved.load_state_dict(layer.cpu().state_dict())
+    assert torch.equal(moved.to(dev, torch.bfloat16)(x), y)
+
+
+def test_block_on_fp8_layers(dev):
+    from krea2_svdquant_amd.runtime import krea2_standin as ks
+    dims = ks.Krea2Dims(layers=2, hidden=256, heads=2, kv_heads=1, head_dim=128, mlp=520)
+    model = ks.Krea2StandInTransformer.random(dims, linears="fp8", device=dev, seed=5)
+    x = normal((70, 256), gen(60)).to(dev)
+    y = model(x)
+    assert torch.isfinite(y).all() and y.shape == x.shape
+    # each layer called by itself: the quantised activation that they share changes nothing
+    calls = []
+    assert torch.equal(model(x, linear=lambda name, mod, z: calls.append(name) or mod(z)), y) and len(calls) == 16
+    assert torch.equal(model(x, siblings=True), y)
+    layer = model.transformer_blocks[0].attn.to_k
+    seen = []
+    hook = layer.register_forward_hook(lambda mod, args, out: seen.append(out))
+    assert torch.equal(model(x), y) and len(seen) == 1
+    hook.remove()
+    with pytest.raises(NotImplementedError, match="FP8Linear"):
+        model(x, fused=True)
+
+
+def test_block_on_fp8_layers_captured(dev):
+    from krea2_svdquant_amd.runtime import krea2_standin as ks
+    dims = ks.Krea2Dims(layers=1, hidden=256, heads=2, kv_heads=1, head_dim=128, mlp=520)
+    model = ks.Krea2StandInTransformer.random(dims, linears="fp8", device=dev, seed=6)
+    x = normal((33, 256), gen(61)).to(dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        model(x)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = model(x)
+    for i in range(3):
+        x.copy_(normal(x.shape, gen(62 + i)))
+        want = model(x)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
+# ---- refusals -----------------------------------------------------------------------------------------------------------
+def test_refusals_of_the_linear(dev):
+    x = normal((4, 256), gen(0)).to(dev)
+    w, ws = (t.to(dev) for t in weight(130, 256, gen(1)))
+    a, sa = ops.fp8_quantize(x)
+    with pytest.raises(TypeError):
+        ops.fp8_quantize(x.float())
+    for kind, call in ((TypeError, lambda: ops.fp8_linear(x.half(), w, ws)), (TypeError, lambda: ops.fp8_linear(x, w.view(torch.uint8), ws)),
+                       (TypeError, lambda: ops.fp8_linear(x, w, ws.half())), (ValueError, lambda: ops.fp8_linear(x[:, :100], w, ws)),
+                       (ValueError, lambda: ops.fp8_linear(x, w, ws[:1])), (ValueError, lambda: ops.fp8_linear(x, w, ws, x[0, :129])),
+                       (TypeError, lambda: ops.fp8_linear(x, w, ws, torch.zeros(130, device=dev))),
+                       (ValueError, lambda: ops.fp8_linear(x, w, ws.cpu())), (ValueError, lambda: ops.fp8_linear(x, w[:, :128], ws)),
+                       (ValueError, lambda: ops.fp8_gemm(a, sa[:1], w, ws)), (TypeError, lambda: ops.fp8_gemm(a, sa.half(), w, ws)),
+                       (ValueError, lambda: ops.fp8_gemm(a[:, :100].contiguous(), sa, w, ws)),
+                       (TypeError, lambda: ops.fp8_gemm(x, sa, w, ws))):
+        with pytest.raises(kind):
+            call()
+
+
+def test_refusals_of_the_norms(dev):
+    q, k = normal((4, 2, 64), gen(0)).to(dev), normal((4, 1, 64), gen(1)).to(dev)
+    tab = torch.rand(4, 32, device=dev)
+    i = torch.arange(4, device=dev)
+    for kind, args in ((TypeError, (q.half(), k, None, None, tab, tab, 1e-6)), (ValueError, (q, k[:3], None, None, tab, tab, 1e-6)),
+                       (ValueError, (q[0], k, None, None, tab, tab, 1e-6)), (ValueError, (q, k, q[0, 0, :60], None, tab, tab, 1e-6)),
+                       (TypeError, (q, k, None, None, tab, tab.bfloat16(), 1e-6)), (ValueError, (q, k, None, None, tab[:3], tab[:3], 1e-6)),
+                       (ValueError, (q, k, None, None, tab[:, :31], tab[:, :31], 1e-6)), (ValueError, (q, k, None, None, tab, tab[:3], 1e-6)),
+                       (ValueError, (q, k, None, None, tab, tab, 1e-6, i[:3])), (TypeError, (q, k, None, None, tab, tab, 1e-6, i.float())),
+                       (ValueError, (q, k, None, None, tab, tab, 1e-6, i.cpu())), (ValueError, (q[..., :60], k[..., :60], None, None, tab, tab, 1e-6))):
+        with pytest.raises(kind):
+            ops.qk_norm_rope(*args)
+    with pytest.raises(Exception, match="eps"):
+        ops.qk_norm_rope(q, k, None, None, tab, tab, -1.0)
+
+
+def test_refusals_of_the_cache(dev):
+    c = Cache(dev, [(3, 100)], 2, 64, 0)
+    good = c.device()
+    x, q = normal((3, 2, 64), c.g).to(dev), normal((3, 4, 64), c.g).to(dev)
+    before = good[3].float().clone()
+    names = ("cu_seqlens", "lengths", "block_table", "k_codes", "v_codes", "scales")
+    bad = [(TypeError, 0, good[0].long()), (ValueError, 0, good[0][:1]), (TypeError, 1, good[1].float()), (ValueError, 1, good[1].cpu()),
+           (ValueError, 2, good[2][0]), (ValueError, 2, good[2][:0]), (TypeError, 3, good[3].view(torch.uint8)),
+           (ValueError, 3, good[3][..., :32].contiguous()), (ValueError, 3, good[3].transpose(0, 1)), (ValueError, 4, good[4][:1]),
+           (TypeError, 5, good[5].half()), (ValueError, 5, good[5][..., 0])]
+    for kind, at, t in bad:
+        args = [*good[:at], t, *good[at + 1:]]
+        for call in (lambda: ops.kv8_append(x, x, *args), lambda: ops.kv8_attention(q, *args, 0.125)):
+            with pytest.raises(kind):
+                call()
+                raise AssertionError(names[at])
+    for kind, k, v in ((ValueError, x, x[:2]), (ValueError, x[:, :1], x[:, :1]), (TypeError, x.float(), x.float()),
+                       (ValueError, x.cpu(), x), (ValueError, x[..., :32], x[..., :32])):
+        with pytest.raises(kind):
+            ops.kv8_append(k, v, *good)
+    with pytest.raises(RuntimeError, match="gradient"):
+        ops.kv8_append(x.clone().requires_grad_(), x, *good)
+    for kind, z in ((ValueError, q[:, :3]), (TypeError, q.float()), (ValueError, q[0])):
+        with pytest.raises(kind):
+            ops.kv8_attention(z, *good, 0.125)
+    assert torch.equal(good[3].float().nan_to_num(), before.nan_to_num())
+
+
+def test_append_marks_the_cache_as_changed(dev):
+    c = Cache(dev, [(3, 100)], 2, 64, 0)
+    args = c.device(before=True)
+    versions = [t._version for t in args[3:]]
+    ops.kv8_append(*(normal((3, 2, 64), c.g).to(dev) for _ in range(2)), *args)
+    assert all(t._version > v for t, v in zip(args[3:], versions))
+    x = normal((3, 2, 64), c.g).to(dev).requires_grad_()
+    y = ops.kv8_attention(x, *args, 0.125)
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
