@@ -900,40 +900,30 @@ static int fp8_product_checks(const char* fn, int M, int N, int K, int64_t ldy) 
   return 0;
 }
 
-static int fp8_operand_checks(const char* fn, const void* w, const float* w_scales, const void* bias, const void* y,
-                              const void* workspace, int64_t bytes) {
+static int fp8_operand_checks(const char* fn, const void* w, const float* w_scales, const void* bias, const void* y) {
   if (!w || !w_scales || !y) return fail(SVDQ_ERR_ARG, "%s: null pointer", fn);
-  if (!workspace && bytes > 0) return fail(SVDQ_ERR_ARG, "%s: no workspace", fn);
-  if (!aligned16(w) || !aligned16(workspace))
-    return fail(SVDQ_ERR_ALIGN, "%s: codes and workspace must be 16-byte aligned", fn);
+  if (!aligned16(w)) return fail(SVDQ_ERR_ALIGN, "%s: codes must be 16-byte aligned", fn);
   if (reinterpret_cast<uintptr_t>(w_scales) % 4 || !aligned2(bias) || !aligned2(y))
     return fail(SVDQ_ERR_ALIGN, "%s: scales, bias and y must be aligned to their elements", fn);
   return 0;
 }
 
-int64_t svdq_fp8_gemm_workspace(int M, int N, int K) {
-  if (M <= 0 || N <= 0 || K <= 0 || K > 1 << 22 || !mx_gemm_fits(M, N)) return 0;
-  return svdq::fp8_gemm_workspace_bytes(M, N, K);
-}
-
 int svdq_fp8_gemm(const void* a, const float* a_scales, const void* w, const float* w_scales, const void* bias, int M,
-                  int N, int K, void* y, int64_t ldy, void* workspace, hipStream_t stream) {
+                  int N, int K, void* y, int64_t ldy, hipStream_t stream) {
   if (int e = fp8_product_checks("fp8_gemm", M, N, K, ldy)) return e;
   if (M == 0) return ok();
   if (!a || !a_scales) return fail(SVDQ_ERR_ARG, "fp8_gemm: null pointer");
-  if (!aligned16(a)) return fail(SVDQ_ERR_ALIGN, "fp8_gemm: codes and workspace must be 16-byte aligned");
+  if (!aligned16(a)) return fail(SVDQ_ERR_ALIGN, "fp8_gemm: codes must be 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(a_scales) % 4)
     return fail(SVDQ_ERR_ALIGN, "fp8_gemm: scales, bias and y must be aligned to their elements");
-  if (int e = fp8_operand_checks("fp8_gemm", w, w_scales, bias, y, workspace, svdq::fp8_gemm_workspace_bytes(M, N, K)))
-    return e;
+  if (int e = fp8_operand_checks("fp8_gemm", w, w_scales, bias, y)) return e;
   const svdq::Fp8GemmParams p{static_cast<const uint8_t*>(a), a_scales, static_cast<const uint8_t*>(w), w_scales,
                               static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(y), ldy, M, N, K};
-  return launched(svdq::launch_fp8_gemm(p, workspace, stream), "fp8_gemm");
+  return launched(svdq::launch_fp8_gemm(p, stream), "fp8_gemm");
 }
 
-int64_t svdq_fp8_linear_workspace(int M, int N, int K) {
-  if (M <= 0 || N <= 0 || K <= 0 || K > 1 << 22 || !mx_gemm_fits(M, N)) return 0;
-  return svdq::fp8_linear_workspace_bytes(M, N, K);
+int64_t svdq_fp8_linear_workspace(int M, int K) {
+  return M <= 0 || K <= 0 || K > 1 << 22 ? 0 : svdq::fp8_linear_workspace_bytes(M, K);
 }
 
 int svdq_fp8_linear(const void* x, int64_t ldx, const void* w, const float* w_scales, const void* bias, int M, int N,
@@ -944,7 +934,9 @@ int svdq_fp8_linear(const void* x, int64_t ldx, const void* w, const float* w_sc
   if (ldx < K) return fail(SVDQ_ERR_SHAPE, "fp8_linear: K=%d, ldx=%lld", K, (long long)ldx);
   if (!aligned2(x)) return fail(SVDQ_ERR_ALIGN, "fp8_linear: x must be aligned to its elements");
   if (int e = mx_launch_checks("fp8_linear", M, K, 1)) return e;
-  if (int e = fp8_operand_checks("fp8_linear", w, w_scales, bias, y, workspace, 1)) return e;
+  if (!workspace) return fail(SVDQ_ERR_ARG, "fp8_linear: no workspace");
+  if (!aligned16(workspace)) return fail(SVDQ_ERR_ALIGN, "fp8_linear: the workspace must be 16-byte aligned");
+  if (int e = fp8_operand_checks("fp8_linear", w, w_scales, bias, y)) return e;
   const svdq::Fp8GemmParams p{nullptr, nullptr, static_cast<const uint8_t*>(w), w_scales,
                               static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(y), ldy, M, N, K};
   return launched(svdq::launch_fp8_linear(p, static_cast<const uint16_t*>(x), ldx, workspace, stream), "fp8_linear");

@@ -69,16 +69,14 @@ struct Fp8Tile {
 };
 
 template <int TM, int TN, int WM, int WN, int NB>
-__global__ void __launch_bounds__(64 * WM * WN, 2)
-    fp8_gemm_tile_kernel(Fp8GemmParams p, int nbm, int nbn, int group_m, int per, float* part) {
+__global__ void __launch_bounds__(64 * WM * WN, 2) fp8_gemm_tile_kernel(Fp8GemmParams p, int nbm, int nbn, int group_m) {
   using T = Fp8Tile<TM, TN, WM, WN, NB>;
   __shared__ __attribute__((aligned(1024))) uint8_t sm[T::LDS];
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, b = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave % WM, wn = wave / WM;
   int bm, bn;
-  // pieces of `per` blocks of K, one after another in blockIdx.y
   tile_coords(blockIdx.x, nbm, nbn, group_m, bm, bn);
-  const int m0 = bm * T::BM, n0 = bn * T::BN, kp = (int)fp8_kp(p.K), k0 = blockIdx.y * per, nst = min(per, kp / 128 - k0);
+  const int m0 = bm * T::BM, n0 = bn * T::BN, kp = (int)fp8_kp(p.K), nst = kp / 128;
   const uint32_t lds0 = lds_offset(sm);
   const int chunk = lane % 8 ^ (lane / 8 >> 1 & 3);   // row / 2 mod 8 of row 8 i + lane / 8: 4 (i & 1) more
   uint32_t off[T::D - 1];
@@ -88,9 +86,9 @@ __global__ void __launch_bounds__(64 * WM * WN, 2)
     const int i = wave + T::NW * (a ? d : d - T::DA), row = 8 * i + lane / 8;
     off[d] = (uint32_t)((long)min(row, (a ? p.M - m0 : p.N - n0) - 1) * kp + 16 * (chunk ^ (i & 1 ? 4 : 0)));
   }
-  const uint8_t *src_a = p.a + (long)m0 * kp + 128 * k0, *src_w = p.w + (long)n0 * kp + 128 * k0;
+  const uint8_t *src_a = p.a + (long)m0 * kp, *src_w = p.w + (long)n0 * kp;
   const int mw = m0 + 16 * TM * wm, nw = n0 + 16 * TN * wn;
-  const float* src_s = p.as + (long)k0 * p.M + min(mw + min(lane, 16 * TM - 1), p.M - 1);
+  const float* src_s = p.as + min(mw + min(lane, 16 * TM - 1), p.M - 1);
   int ahead = 0;
   // this wave's d-th instruction of the stage `ahead`; past the last one that again, so that the waits count the same
   // loads throughout
@@ -107,7 +105,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2)
             lds0 + buf * T::BUF + 1024 * (d < T::DA ? wave + T::NW * d : T::TA + wave + T::NW * (d - T::DA)));
     }
   };
-  const float* wsrow = p.ws + (long)min(nw / 128, (p.N - 1) / 128) * (kp / 128) + k0;
+  const float* wsrow = p.ws + (long)min(nw / 128, (p.N - 1) / 128) * nst;
   float wscales = wsrow[min(lane, nst - 1)];   // of stages s .. s + 63
   asm volatile("s_waitcnt vmcnt(0)" : "+v"(wscales)::"memory");
 
@@ -213,17 +211,6 @@ __global__ void __launch_bounds__(64 * WM * WN, 2)
   // LDS is used again, here or by the next workgroup.
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (part) {   // sums of this piece, rows of N rounded up to 4
-    const int np = (p.N + 3) & ~3;
-#pragma unroll
-    for (int t = 0; t < TM; ++t)
-#pragma unroll
-      for (int x = 0; x < TN; ++x) {
-        const int m = mw + 16 * t + lr, n = nw + 16 * x + 4 * b;
-        if (m < p.M && n < np) *reinterpret_cast<f32x4*>(part + ((long)blockIdx.y * p.M + m) * np + n) = acc[x][t];
-      }
-    return;
-  }
   uint8_t* stage_out = sm + wave * 16 * T::PITCH;
   constexpr int COLS = 16 * TN, LPR = COLS / 8;   // lanes a row
   const bool wide = p.ldy % 8 == 0 && reinterpret_cast<uintptr_t>(p.y) % 16 == 0;
@@ -261,6 +248,22 @@ __global__ void __launch_bounds__(64 * WM * WN, 2)
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+}
+
+// Four columns of a row, with the bias.
+__device__ __forceinline__ void fp8_store4(const Fp8GemmParams& p, long m, int n, f32x4 y) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (p.bias && n + r < p.N) y[r] += bf16f(p.bias[n + r]);
+  uint16_t* out = p.y + m * p.ldy + n;
+  const u32x2 o = {pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+  if (n + 3 < p.N && p.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % 8 == 0) {
+    *reinterpret_cast<u32x2*>(out) = o;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < p.N) out[r] = (uint16_t)(o[r / 2] >> 16 * (r % 2));
   }
 }
 
@@ -349,6 +352,109 @@ __global__ void __launch_bounds__(512) fp8_gemm_rows_kernel(Fp8GemmParams p) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
   fp8_rows_sum(p, sm, acc, n0);
+}
+
+// Strips, for outputs of few tiles (16 TM rows a workgroup, 16 TN columns): as with few rows, NW waves take blocks of all of K
+// in turn, each with a ring of two in LDS to itself, and add their sums in wave order.  A lone tile spends 0.27 us on a
+// block of K, most of it waiting at one point or another for DMA, LDS, the matrix unit and the other waves; here NW such
+// chains run side by side without a barrier.  77 x 6144, K = 6144: 12.3 us, as 64 x 64 tiles 17.1, as those in pieces of K that
+// a second launch joins 16.5 (w alone takes 7.3 to read).
+template <int TM, int TN, int NW>
+struct Fp8Strip {
+  static constexpr int OA = 2048 * TN, OSC = OA + 2048 * TM, UNIT = OSC + 512;   // w, a, scales of 16 TM rows and w's
+  static constexpr int D = 2 * TN + 2 * TM + 2;                                // DMA instructions of a block
+  static constexpr int LDS = 2 * NW * UNIT;
+  static_assert(LDS <= 160 * 1024 && TM * TN * 1024 <= 2 * UNIT && 16 * TM <= 128 && 128 % (16 * TN) == 0, "LDS");
+};
+
+template <int TM, int TN, int NW>
+__global__ void __launch_bounds__(64 * NW) fp8_gemm_strip_kernel(Fp8GemmParams p) {
+  using T = Fp8Strip<TM, TN, NW>;
+  __shared__ __attribute__((aligned(1024))) uint8_t sm[T::LDS];
+  const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, b = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n0 = blockIdx.x * 16 * TN, m0 = blockIdx.y * 16 * TM, kp = (int)fp8_kp(p.K), nst = kp / 128;
+  const uint32_t lds0 = lds_offset(sm) + wave * 2 * T::UNIT;
+  const uint8_t* mine = sm + wave * 2 * T::UNIT;
+  const int chunk = lane % 8 ^ (lane / 8 >> 1 & 3);   // as in the tiles
+  uint32_t off_w[2 * TN], off_a[2 * TM];
+#pragma unroll
+  for (int d = 0; d < 2 * TN; ++d)
+    off_w[d] = (uint32_t)(min(8 * d + lane / 8, p.N - n0 - 1) * (long)kp + 16 * (chunk ^ 4 * (d & 1)));
+#pragma unroll
+  for (int d = 0; d < 2 * TM; ++d)
+    off_a[d] = (uint32_t)(min(8 * d + lane / 8, p.M - m0 - 1) * (long)kp + 16 * (chunk ^ 4 * (d & 1)));
+  const uint8_t *src_w = p.w + (long)n0 * kp, *src_a = p.a + (long)m0 * kp;
+  // scales of a block: the rows', and behind the last of them the weight's
+  auto scale_at = [&](int i) { return i < 16 * TM ? p.as + min(m0 + i, p.M - 1) : p.ws + (long)(n0 / 128) * nst; };
+  const float *src_s = scale_at(lane), *src_t = scale_at(64 + lane);
+  const long step_s = lane < 16 * TM ? p.M : 1, step_t = 64 + lane < 16 * TM ? p.M : 1;
+  auto fetch = [&](int block, int buf) __attribute__((always_inline)) {
+    const uint32_t to = lds0 + buf * T::UNIT;
+#pragma unroll
+    for (int d = 0; d < 2 * TN; ++d) dma16(src_w, off_w[d] + 128 * block, to + 1024 * d);
+#pragma unroll
+    for (int d = 0; d < 2 * TM; ++d) dma16(src_a, off_a[d] + 128 * block, to + T::OA + 1024 * d);
+    dma4_at(src_s + step_s * block, to + T::OSC);
+    dma4_at(src_t + step_t * block, to + T::OSC + 256);
+  };
+  const int count = wave < nst ? (nst - wave + NW - 1) / NW : 0;
+  f32x4 acc[TN][TM] = {};
+  const uint32_t o0 = 128 * lr + 16 * (b ^ (lr >> 1 & 7));
+  if (count) {
+    // blocks past the last are the last again, into a buffer that is not read: the waits count the same loads throughout
+    auto block_of = [&](int i) { return wave + NW * min(i, count - 1); };
+    fetch(block_of(0), 0);
+    fetch(block_of(1), 1);
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::D) : "memory");
+      const uint8_t* u = mine + (i & 1) * T::UNIT;
+      Fp8Frag fw[TN], fa[TM];
+      float s[TM];
+#pragma unroll
+      for (int x = 0; x < TN; ++x) {
+        fw[x].q[0] = *reinterpret_cast<const u32x4*>(u + 2048 * x + o0);
+        fw[x].q[1] = *reinterpret_cast<const u32x4*>(u + 2048 * x + (o0 ^ 64));
+      }
+      const float* sc = reinterpret_cast<const float*>(u + T::OSC);
+      const float ws = sc[16 * TM];
+#pragma unroll
+      for (int t = 0; t < TM; ++t) {
+        fa[t].q[0] = *reinterpret_cast<const u32x4*>(u + T::OA + 2048 * t + o0);
+        fa[t].q[1] = *reinterpret_cast<const u32x4*>(u + T::OA + 2048 * t + (o0 ^ 64));
+        s[t] = sc[16 * t + lr] * ws;
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // all of the block is in registers
+      __builtin_amdgcn_sched_barrier(0);
+      fetch(block_of(i + 2), i & 1);
+#pragma unroll
+      for (int t = 0; t < TM; ++t)
+#pragma unroll
+        for (int x = 0; x < TN; ++x) {
+          const f32x4 v = fp8_mfma16(fw[x], fa[t]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[x][t][r] = __builtin_fmaf(v[r], s[t], acc[x][t][r]);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
+  __syncthreads();   // every ring is done with; their memory takes the sums
+  f32x4* sums = reinterpret_cast<f32x4*>(sm);
+#pragma unroll
+  for (int t = 0; t < TM; ++t)
+#pragma unroll
+    for (int x = 0; x < TN; ++x) sums[64 * (TM * TN * wave + TN * t + x) + lane] = acc[x][t];
+  __syncthreads();
+  // register r of lane (lr, b): row lr of a, column 4 b + r of w
+#pragma unroll
+  for (int q = wave; q < TM * TN; q += NW) {
+    const int m = m0 + 16 * (q / TN) + lr, n = n0 + 16 * (q % TN) + 4 * b;
+    f32x4 y = {};
+#pragma unroll
+    for (int k = 0; k < NW; ++k) y += sums[64 * (TM * TN * k + q) + lane];
+    if (m < p.M) fp8_store4(p, m, n, y);
+  }
 }
 
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -448,115 +554,87 @@ __global__ void __launch_bounds__(512) fp8_linear_rows_kernel(Fp8GemmParams p, c
   fp8_rows_sum(p, sm, acc, n0);
 }
 
-// y = the pieces' sums, in their order, and the bias; four columns a thread
-__global__ void __launch_bounds__(256) fp8_gemm_join_kernel(Fp8GemmParams p, const float* __restrict__ part, int pieces) {
-  const int np = (p.N + 3) & ~3, quads = np / 4;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x, m = i / quads;
-  if (m >= p.M) return;
-  const int n = 4 * (int)(i - m * quads);
-  f32x4 y = {};
-#pragma unroll 4
-  for (int s = 0; s < pieces; ++s) y += *reinterpret_cast<const f32x4*>(part + ((long)s * p.M + m) * np + n);
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (p.bias && n + r < p.N) y[r] += bf16f(p.bias[n + r]);
-  uint16_t* out = p.y + m * p.ldy + n;
-  const u32x2 o = {pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-  if (n + 3 < p.N && p.ldy % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % 8 == 0) {
-    *reinterpret_cast<u32x2*>(out) = o;
-  } else {
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (n + r < p.N) out[r] = (uint16_t)(o[r / 2] >> 16 * (r % 2));
-  }
-}
-
 template <int TM, int TN, int WM, int WN, int NB>
-hipError_t launch_tile(const Fp8GemmParams& p, int per, float* part, hipStream_t st) {
+hipError_t launch_tile(const Fp8GemmParams& p, hipStream_t st) {
   using T = Fp8Tile<TM, TN, WM, WN, NB>;
   const long nbm = (p.M + T::BM - 1) / T::BM, nbn = (p.N + T::BN - 1) / T::BN;
-  const int blocks = (int)(fp8_kp(p.K) / 128);
-  fp8_gemm_tile_kernel<TM, TN, WM, WN, NB><<<dim3((unsigned)(nbm * nbn), (unsigned)((blocks + per - 1) / per)), 64 * WM * WN, 0, st>>>(
-      p, (int)nbm, (int)nbn, 4, per, part);
+  fp8_gemm_tile_kernel<TM, TN, WM, WN, NB><<<(unsigned)(nbm * nbn), 64 * WM * WN, 0, st>>>(p, (int)nbm, (int)nbn, 4);
   return hipGetLastError();
 }
 
-// Block tiles: rows of a, of w, workgroups that share a CU, and microseconds for a block of K with n of them on a CU
-// (us[n - 1]).  As measured at K = 6144 (48 blocks; M x N and us of the tiles in order: 77 x 6144 17.3 21.6 40 39 60, 256 x
-// 6144 23 22 41 40 61, 1024 x 6144 74 56 50 45 64, 4352 x 1536 84 66 51 46 65, 2381 x 6144 167 133 110 102 86, 4096 x
-// 16384 660 540 447 411 345); a launch takes 4 us besides, a further round 1.
-struct Fp8TileCost {
+template <int TM, int TN, int NW>
+hipError_t launch_strip(const Fp8GemmParams& p, hipStream_t st) {
+  const dim3 grid((unsigned)((p.N + 16 * TN - 1) / (16 * TN)), (unsigned)((p.M + 16 * TM - 1) / (16 * TM)));
+  fp8_gemm_strip_kernel<TM, TN, NW><<<grid, 64 * NW, 0, st>>>(p);
+  return hipGetLastError();
+}
+
+// What a kernel's workgroups take: rows of a, of w, how many share a CU, and microseconds for a block of K with n of them
+// on a CU (us[n - 1]); a launch takes 3.5 us besides, a further round 1, and w is read from memory at 5.2 TB/s at most.
+// Measured (us, K = 6144; strips of 32 x 16, 32 x 32, 64 x 32, 48 x 64 and 64 x 64, then the tiles):
+//     32 x  1536     5.4   6.6   8.6  10.5  12.4 |  16.1  21.6  30.1  37.8  59.2
+//     77 x  1536     9.5   6.9   9.0  10.8  13.0 |  16.1  21.7  30.5  38.0  59.7
+//     32 x  6144    12.2   8.9   9.7  11.4  13.5 |  16.5  21.6  40.2  39.1  59.6
+//     64 x  6144    17.4  15.5  10.9  12.3  14.3 |  16.8  21.7  40.5  39.6  59.9
+//     77 x  6144       -  21.2  17.6  12.3  14.5 |  17.1  21.9  40.2  39.3  59.9
+//    128 x  6144       -     -  19.5  21.5  14.8 |  17.0  21.7  40.3  39.5  60.1
+//    320 x  6144       -     -  39.5  36.0  28.6 |  24.1  25.0  40.6  41.0  61.2
+//   1024 x  6144       -     -     -     -  81.1 |  64.9  57.3  51.7  45.6  63.1
+//   2381 x  6144       -     -     -     - 201   | 156   132   109   101    86.1
+struct Fp8Cost {
   int rows, cols, slots;
   float us[3];
 };
-constexpr int FP8_TILES = 5, FP8_ROWS = -1;
-const Fp8TileCost kTiles[FP8_TILES] = {{64, 64, 3, {0.28f, 0.42f, 0.66f}}, {64, 128, 2, {0.38f, 0.66f}}, {128, 128, 2, {0.78f, 1.10f}},
-                                       {256, 128, 1, {0.98f}}, {256, 256, 1, {1.75f}}};
+constexpr int FP8_STRIPS = 5, FP8_KERNELS = FP8_STRIPS + 5;
+const Fp8Cost kCosts[FP8_KERNELS] = {
+    {32, 16, 1, {0.075f}}, {32, 32, 1, {0.105f}}, {64, 32, 1, {0.15f}}, {48, 64, 1, {0.185f}}, {64, 64, 1, {0.235f}},
+    {64, 64, 3, {0.27f, 0.42f, 0.64f}}, {64, 128, 2, {0.38f, 0.62f}}, {128, 128, 2, {0.78f, 1.10f}}, {256, 128, 1, {1.00f}},
+    {256, 256, 1, {1.75f}}};
 
-struct Fp8Choice {
-  int tile, per;   // blocks of K in a piece
-  float us;
-};
-
-// Few tiles leave most CUs idle for all of K, so K is cut into pieces where that is less with what joining them takes (a
-// launch, and a write and a read of every piece's sums at 4 TB/s).  In one piece and in several: 77 x 1536, K = 6144 15.8
-// and 9.5 us, 32 x 6144, K = 16384 38 and 20; 512 x 1536, K = 6144 17.3 in one, 17.7 in two.  Up to 16 rows the rows
-// kernel runs (16 x 6144, K = 6144 8.6 us, tiles 16.7; K = 16384 16.8 and 19.7).
-Fp8Choice choose(long M, long N, int K) {
-  const int blocks = (int)(fp8_kp(K) / 128);
-  if (M <= 16) return {FP8_ROWS, blocks, 0.0f};
-  Fp8Choice best{-2, 0, 0.0f};
-  for (int i = 0; i < FP8_TILES; ++i) {
-    const Fp8TileCost& t = kTiles[i];
-    const long tiles = ((M + t.rows - 1) / t.rows) * ((N + t.cols - 1) / t.cols);
-    for (int n : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-      const int per = (blocks + n - 1) / n, pieces = (blocks + per - 1) / per;
-      const long all = tiles * pieces, whole = all / (256 * t.slots), rest = (all % (256 * t.slots) + 255) / 256;
-      if (n > 1 && (per < 4 || all > 512)) break;
-      float us = 4.0f + whole * (1.0f + per * t.us[t.slots - 1]) + (rest ? per * t.us[rest - 1] : 0.0f);
-      if (pieces > 1) us += 2.0f + 2.0f * pieces * M * N * 4.0f / 4e6f;
-      if (best.tile < -1 || us < best.us) best = {i, per, us};
-    }
+int choose(long M, long N, int K) {
+  const long blocks = fp8_kp(K) / 128;
+  const float read = 3.5f + N * blocks * 128 / 5.2e6f;   // of w, from memory
+  int best = 0;
+  float least = 0.0f;
+  for (int i = 0; i < FP8_KERNELS; ++i) {
+    const Fp8Cost& t = kCosts[i];
+    const long nbm = (M + t.rows - 1) / t.rows, nbn = (N + t.cols - 1) / t.cols, all = nbm * nbn;
+    if (i < FP8_STRIPS && nbm > 65535) continue;
+    const long whole = all / (256 * t.slots), rest = (all % (256 * t.slots) + 255) / 256;
+    float us = 2.5f + whole * (1.0f + blocks * t.us[t.slots - 1]) + (rest ? 1.0f + blocks * t.us[rest - 1] : 0.0f);
+    if (us < read) us = 0.9f * read + 0.1f * us;   // where reading w takes longest, what takes least besides
+    if (i == 0 || us < least) best = i, least = us;
   }
   return best;
 }
 
-hipError_t launch_kernel(const Fp8Choice& c, const Fp8GemmParams& p, float* part, hipStream_t st) {
-  switch (c.tile) {
-    case FP8_ROWS:
-      if (p.M > 8) fp8_gemm_rows_kernel<16, 2><<<(unsigned)((p.N + 15) / 16), 512, 0, st>>>(p);
-      else fp8_gemm_rows_kernel<8, 3><<<(unsigned)((p.N + 15) / 16), 512, 0, st>>>(p);
-      return hipGetLastError();
-    case 0: return launch_tile<1, 4, 4, 1, 3>(p, c.per, part, st);
-    case 1: return launch_tile<2, 4, 2, 2, 3>(p, c.per, part, st);
-    case 2: return launch_tile<4, 4, 2, 2, 2>(p, c.per, part, st);
-    case 3: return launch_tile<4, 4, 4, 2, 3>(p, c.per, part, st);
-    default: return launch_tile<4, 8, 4, 2, 2>(p, c.per, part, st);
+hipError_t launch_kernel(int kernel, const Fp8GemmParams& p, hipStream_t st) {
+  switch (kernel) {
+    case 0: return launch_strip<2, 1, 8>(p, st);
+    case 1: return launch_strip<2, 2, 8>(p, st);
+    case 2: return launch_strip<4, 2, 4>(p, st);
+    case 3: return launch_strip<3, 4, 4>(p, st);
+    case 4: return launch_strip<4, 4, 4>(p, st);
+    case 5: return launch_tile<1, 4, 4, 1, 3>(p, st);
+    case 6: return launch_tile<2, 4, 2, 2, 3>(p, st);
+    case 7: return launch_tile<4, 4, 2, 2, 2>(p, st);
+    case 8: return launch_tile<4, 4, 4, 2, 3>(p, st);
+    default: return launch_tile<4, 8, 4, 2, 2>(p, st);
   }
 }
 
-int pieces_of(const Fp8Choice& c, int K) { return (int)((fp8_kp(K) / 128 + c.per - 1) / c.per); }
-
 }  // namespace
 
-long fp8_gemm_workspace_bytes(int M, int N, int K) {
-  const int pieces = pieces_of(choose(M, N, K), K);
-  return pieces == 1 ? 0 : 4L * pieces * M * ((N + 3) & ~3);
-}
-
-hipError_t launch_fp8_gemm(const Fp8GemmParams& p, void* workspace, hipStream_t st) {
-  const Fp8Choice c = choose(p.M, p.N, p.K);
-  const int pieces = pieces_of(c, p.K);
-  float* part = pieces == 1 ? nullptr : static_cast<float*>(workspace);
-  if (hipError_t e = launch_kernel(c, p, part, st); e != hipSuccess || !part) return e;
-  const long quads = (long)p.M * ((p.N + 3) / 4);
-  fp8_gemm_join_kernel<<<(unsigned)((quads + 255) / 256), 256, 0, st>>>(p, part, pieces);
+hipError_t launch_fp8_gemm(const Fp8GemmParams& p, hipStream_t st) {
+  if (p.M > 16) return launch_kernel(choose(p.M, p.N, p.K), p, st);
+  if (p.M > 8) fp8_gemm_rows_kernel<16, 2><<<(unsigned)((p.N + 15) / 16), 512, 0, st>>>(p);
+  else fp8_gemm_rows_kernel<8, 3><<<(unsigned)((p.N + 15) / 16), 512, 0, st>>>(p);
   return hipGetLastError();
 }
 
-long fp8_linear_workspace_bytes(int M, int N, int K) {
-  const long kp = fp8_kp(K), codes = M * kp, scales = (M * (kp / 32) + 15) & ~15L;
-  return codes + scales + fp8_gemm_workspace_bytes(M, N, K);
+long fp8_linear_workspace_bytes(int M, int K) {
+  const long kp = fp8_kp(K);
+  return M * kp + M * (kp / 32);   // codes, scales
 }
 
 hipError_t launch_fp8_linear(Fp8GemmParams p, const uint16_t* x, long ldx, void* workspace, hipStream_t st) {
@@ -564,13 +642,12 @@ hipError_t launch_fp8_linear(Fp8GemmParams p, const uint16_t* x, long ldx, void*
     fp8_linear_rows_kernel<<<(unsigned)((p.N + 15) / 16), 512, 0, st>>>(p, x, ldx);
     return hipGetLastError();
   }
-  const long kp = fp8_kp(p.K), codes = p.M * kp, scales = (p.M * (kp / 32) + 15) & ~15L;
-  uint8_t* work = static_cast<uint8_t*>(workspace);
-  p.a = work;
-  float* at = reinterpret_cast<float*>(work + codes);
-  if (hipError_t e = launch_fp8_quantize(x, ldx, p.M, p.K, work, at, st); e != hipSuccess) return e;
-  p.as = at;
-  return launch_fp8_gemm(p, work + codes + scales, st);
+  uint8_t* codes = static_cast<uint8_t*>(workspace);
+  float* scales = reinterpret_cast<float*>(codes + p.M * fp8_kp(p.K));
+  p.a = codes;
+  p.as = scales;
+  if (hipError_t e = launch_fp8_quantize(x, ldx, p.M, p.K, codes, scales, st); e != hipSuccess) return e;
+  return launch_fp8_gemm(p, st);
 }
 
 }  // namespace svdq

@@ -214,10 +214,9 @@ struct Fp8GemmParams {
   long ldy;
   int M, N, K;
 };
-long fp8_gemm_workspace_bytes(int M, int N, int K);
-hipError_t launch_fp8_gemm(const Fp8GemmParams& p, void* workspace, hipStream_t st);
+hipError_t launch_fp8_gemm(const Fp8GemmParams& p, hipStream_t st);
 // p.a and p.as are not looked at: they are made of x [M, ldx]
-long fp8_linear_workspace_bytes(int M, int N, int K);
+long fp8_linear_workspace_bytes(int M, int K);
 hipError_t launch_fp8_linear(Fp8GemmParams p, const uint16_t* x, long ldx, void* workspace, hipStream_t st);
 
 // Norms of q's and k's heads with the position rotation (svdq_block.hip)

@@ -490,10 +490,6 @@ Tensor fp8_output(int64_t kp, std::vector<int64_t> lead, const Tensor& w, const 
   return at::empty(lead, w.options().dtype(at::kBFloat16));
 }
 
-Tensor workspace_of(int64_t bytes, const Tensor& like) {
-  return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
-}
-
 Tensor fp8_gemm(const Tensor& a, const Tensor& a_scales, const Tensor& w, const Tensor& w_scales, const OptTensor& bias) {
   const c10::Device dev = w.device();
   const c10::DeviceGuard guard(dev);
@@ -509,10 +505,8 @@ Tensor fp8_gemm(const Tensor& a, const Tensor& a_scales, const Tensor& w, const 
   TORCH_CHECK_VALUE(a_scales.sizes() == at::IntArrayRef(want), "a_scales must be ", at::IntArrayRef(want), ", got ",
                     a_scales.sizes());
   const Tensor y = fp8_output(kp, lead, w, w_scales, bias);
-  const int n = (int)w.size(0);
-  const Tensor work = workspace_of(svdq_fp8_gemm_workspace((int)m, n, (int)kp), w);
   check_status("svdq_fp8_gemm", svdq_fp8_gemm(ptr(a), ptr<float>(a_scales), ptr(w), ptr<float>(w_scales), ptr(bias), (int)m,
-                                              n, (int)kp, ptr(y), n, work.defined() ? ptr(work) : nullptr, stream_of(dev)));
+                                              (int)w.size(0), (int)kp, ptr(y), w.size(0), stream_of(dev)));
   return y;
 }
 
@@ -523,9 +517,9 @@ Tensor fp8_linear(const Tensor& x, const Tensor& w, const Tensor& w_scales, cons
   const Rows r("x", x);
   const Tensor y = fp8_output(mx_kp(r.k), r.lead, w, w_scales, bias);
   const int n = (int)w.size(0);
-  const Tensor work = workspace_of(svdq_fp8_linear_workspace((int)r.m, n, (int)r.k), w);
+  const Tensor work = at::empty({svdq_fp8_linear_workspace((int)r.m, (int)r.k)}, w.options().dtype(at::kByte));
   check_status("svdq_fp8_linear", svdq_fp8_linear(ptr(r.t), r.ld, ptr(w), ptr<float>(w_scales), ptr(bias), (int)r.m, n,
-                                                  (int)r.k, ptr(y), n, work.defined() ? ptr(work) : nullptr, stream_of(dev)));
+                                                  (int)r.k, ptr(y), n, ptr(work), stream_of(dev)));
   return y;
 }
 

@@ -113,9 +113,8 @@ SIGNATURES = {
     "svdq_residual_rms_norm_modulate_mx": (_I, [_P, _L, _P, _L, _P, _P, _P, _I, _I, ctypes.c_float, _I, _P, _L, _P,
                                                 _P, _P]),
     "svdq_fp8_quantize": (_I, [_P, _L, _I, _I, _P, _P, _P]),
-    "svdq_fp8_gemm_workspace": (_L, [_I, _I, _I]),
-    "svdq_fp8_gemm": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P]),
-    "svdq_fp8_linear_workspace": (_L, [_I, _I, _I]),
+    "svdq_fp8_gemm": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P, _L, _P]),
+    "svdq_fp8_linear_workspace": (_L, [_I, _I]),
     "svdq_fp8_linear": (_I, [_P, _L, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P]),
     "svdq_qk_norm_rope": (_I, [_P, _L, _I, _P, _L, _I, _P, _P, _P, _P, _L, _I, _I, _P, _I, _I, _I, _I, ctypes.c_float,
                                _I, _P, _P, _P]),
