@@ -917,7 +917,7 @@ int svdq_fp8_gemm(const void* a, const float* a_scales, const void* w, const flo
   if (reinterpret_cast<uintptr_t>(a_scales) % 4)
     return fail(SVDQ_ERR_ALIGN, "fp8_gemm: scales, bias and y must be aligned to their elements");
   if (int e = fp8_operand_checks("fp8_gemm", w, w_scales, bias, y)) return e;
-  const svdq::Fp8GemmParams p{static_cast<const uint8_t*>(a), a_scales, static_cast<const uint8_t*>(w), w_scales,
+  const svdq::Fp8GemmParams p{static_cast<const uint8_t*>(a), a_scales, M, static_cast<const uint8_t*>(w), w_scales,
                               static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(y), ldy, M, N, K};
   return launched(svdq::launch_fp8_gemm(p, stream), "fp8_gemm");
 }
@@ -937,7 +937,7 @@ int svdq_fp8_linear(const void* x, int64_t ldx, const void* w, const float* w_sc
   if (!workspace) return fail(SVDQ_ERR_ARG, "fp8_linear: no workspace");
   if (!aligned16(workspace)) return fail(SVDQ_ERR_ALIGN, "fp8_linear: the workspace must be 16-byte aligned");
   if (int e = fp8_operand_checks("fp8_linear", w, w_scales, bias, y)) return e;
-  const svdq::Fp8GemmParams p{nullptr, nullptr, static_cast<const uint8_t*>(w), w_scales,
+  const svdq::Fp8GemmParams p{nullptr, nullptr, M, static_cast<const uint8_t*>(w), w_scales,
                               static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(y), ldy, M, N, K};
   return launched(svdq::launch_fp8_linear(p, static_cast<const uint16_t*>(x), ldx, workspace, stream), "fp8_linear");
 }

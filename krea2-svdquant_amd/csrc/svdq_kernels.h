@@ -206,7 +206,8 @@ int mx_gemm_tile(int M, int N, int K, int fmt, int& rows, int& cols, bool& split
 hipError_t launch_fp8_quantize(const uint16_t* x, long ldx, int M, int K, uint8_t* codes, float* scales, hipStream_t st);
 struct Fp8GemmParams {
   const uint8_t* a;         // [M, kp] E4M3 codes
-  const float* as;          // [kp / 128, M]
+  const float* as;          // [kp / 128, lds]: columns 0 to M - 1 are the rows'
+  long lds;
   const uint8_t* w;         // [N, kp] E4M3 codes
   const float* ws;          // [ceil(N / 128), kp / 128]
   const uint16_t* bias;     // [N] bf16 or null
