@@ -130,6 +130,16 @@ def test_product_whose_output_passes_32_bits(dev):
         assert torch.equal(y[at:at + 300], ops.fp8_gemm(a[at:at + 300], sa[:, at:at + 300].contiguous(), w, sw))
 
 
+def test_product_of_more_rows_than_a_grid_has_in_y(dev):
+    m, n = 2200000, 20   # one block of K, as above
+    g = torch.Generator(device=dev).manual_seed(1)
+    a, w = (torch.randint(-3, 4, (r, 128), device=dev, generator=g).float().to(torch.float8_e4m3fn) for r in (m, n))
+    sa, sw = torch.rand(1, m, device=dev, generator=g), torch.rand(1, 1, device=dev, generator=g)
+    y = ops.fp8_gemm(a, sa, w, sw)
+    for at in (0, 2097100, m - 300):
+        assert torch.equal(y[at:at + 300], ops.fp8_gemm(a[at:at + 300], sa[:, at:at + 300].contiguous(), w, sw))
+
+
 def test_product_passes_nan_and_zero_scales(dev):
     x = normal((5, 256), gen(3))
     x[1, 40], x[2, 200] = math.nan, math.inf
@@ -164,6 +174,19 @@ def test_qk_norm_rope(dev, d, pairs, wide):
                                None if pos is None else pos.to(dev), pairs)
         for y, z, w in zip(got, (q, k), weights):
             u.check(y, *u.qk(z.cpu(), w, cos, sin, 1e-6, pos, pairs))
+
+
+@pytest.mark.parametrize("d", [16, 64, 256])
+@pytest.mark.parametrize("eps", [0.0, 1e-6, 0.5])
+def test_qk_norm_rope_of_any_magnitude(dev, d, eps):
+    """Heads whose squares pass the ends of float32 beside ordinary ones."""
+    g = gen(d)
+    q, k = normal((12, 5, d), g), normal((12, 1, d), g)
+    for i, amp in enumerate((1e38, 1e25, 1e19, 1e-15, 1e-25, 1e-36)):
+        q[2 * i + 1, :3] = (torch.rand((3, d), generator=g) * 2 - 1).mul(amp).to(torch.bfloat16)
+    tab = torch.randn((12, d // 2), generator=g)
+    for y, z in zip(ops.qk_norm_rope(q.to(dev), k.to(dev), None, None, tab.to(dev), tab.to(dev), eps), (q, k)):
+        u.check(y, *u.qk(z, None, tab, tab, eps, None, False))
 
 
 def test_qk_norm_rope_positions_that_are_not_there(dev):
@@ -259,6 +282,22 @@ def attend(c, heads, causal, scale=None, q=None):
     want, bound = u.attention(q, c.offsets, c.lengths(), c.table, *c.oracle(), scale, causal)
     u.check(got, want, bound)
     return got
+
+
+@pytest.mark.parametrize("n", [3, 130])
+def test_offsets_that_do_not_ascend_stay_in_range(dev, n):
+    """What such a batch means is not defined; nothing is read or written out of range, and other sequences' pages stay."""
+    c = Cache(dev, [(n, 200), (n, 200), (n, 200)], 2, 64, 70)
+    args = c.device(before=True)
+    q, x = normal((3 * n, 8, 64), c.g).to(dev), normal((3 * n, 2, 64), c.g).to(dev)
+    before = args[3].view(torch.uint8).clone()
+    free = [p for p in range(len(before)) if not any(p in row for row in c.table)]
+    for offsets in ([0, 2 * n, n, 3 * n], [3 * n, 2 * n, n, 0], [-5, 10 ** 9, -7, 2 ** 31 - 1], [n, n, n, n]):
+        args = (torch.tensor(offsets, dtype=torch.int32, device=dev), *args[1:])
+        ops.kv8_append(x, x, *args)
+        ops.kv8_attention(q, *args, 0.125)
+        torch.cuda.synchronize()
+    assert torch.equal(args[3].view(torch.uint8)[free], before[free])
 
 
 def attend_gpu(c, heads, causal):
