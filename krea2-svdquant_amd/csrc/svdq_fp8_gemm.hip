@@ -516,9 +516,9 @@ __global__ void __launch_bounds__(512) fp8_linear_rows_kernel(Fp8GemmParams p, c
   const float* src_s = p.ws + (long)(n0 / 128) * nst;
   auto fetch = [&](int block, int buf) __attribute__((always_inline)) {
     const uint32_t to = lds0 + buf * T::UNIT;
+    dma16_at(src_x + 128 * block, to + T::OA);
 #pragma unroll
     for (int d = 0; d < 2; ++d) dma16(src_w, off_w[d] + 128 * block, to + 1024 * d);
-    dma16_at(src_x + 128 * block, to + T::OA);
     dma4_at(src_s + block, to + T::OSC);
   };
   const int count = wave < nst ? (nst - wave + T::NW - 1) / T::NW : 0;
@@ -531,24 +531,26 @@ __global__ void __launch_bounds__(512) fp8_linear_rows_kernel(Fp8GemmParams p, c
     int buf = 0;
 #pragma unroll 1
     for (int i = 0; i < count; ++i) {
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((U - 1) * T::D) : "memory");
       const uint8_t* u = mine + buf * T::UNIT;
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((U - 1) * T::D + 3) : "memory");   // x is there, w not yet
       Fp8Frag fw, fa;
-      fw.q[0] = *reinterpret_cast<const u32x4*>(u + 128 * lr + o0);
-      fw.q[1] = *reinterpret_cast<const u32x4*>(u + 128 * lr + (o0 ^ 64));
       u32x4 v[4];   // values 16 b .. 16 b + 15, 64 + 16 b .. 64 + 16 b + 15
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const u32x4*>(u + T::OA + ox + 128 * (j / 2) + 16 * (j % 2));
-      const float ws = *reinterpret_cast<const float*>(u + T::OSC);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // all of the block is in registers
-      fetch(block_of(i + U), buf);
-      buf = buf + 1 == U ? 0 : buf + 1;
       const float s = row4_scale(v);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         fa.q[j / 2][2 * (j % 2)] = fp8_encode_bf16x4(v[j][0], v[j][1], s);
         fa.q[j / 2][2 * (j % 2) + 1] = fp8_encode_bf16x4(v[j][2], v[j][3], s);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((U - 1) * T::D) : "memory");
+      fw.q[0] = *reinterpret_cast<const u32x4*>(u + 128 * lr + o0);
+      fw.q[1] = *reinterpret_cast<const u32x4*>(u + 128 * lr + (o0 ^ 64));
+      const float ws = *reinterpret_cast<const float*>(u + T::OSC);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // all of the block is in registers
+      fetch(block_of(i + U), buf);
+      buf = buf + 1 == U ? 0 : buf + 1;
       const f32x4 y = fp8_mfma16(fw, fa);
 #pragma unroll
       for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(y[r], s * ws, acc[r]);
