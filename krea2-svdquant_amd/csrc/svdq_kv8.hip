@@ -38,16 +38,26 @@ __device__ __forceinline__ long first_unit(const Kv8Cache& c, int b, int mult, i
 struct Kv8Sequence {
   int b, row0, n, len;   // sequence, its first row and new tokens, tokens held
   long unit0;            // its first unit
+  int share;             // SHARE: a `run`-th of all units' pages, rounded up
 };
-__device__ __forceinline__ Kv8Sequence find_sequence(const Kv8Cache& c, long number, int mult, int unit, int extra) {
+template <bool SHARE = false>
+__device__ __forceinline__ Kv8Sequence find_sequence(const Kv8Cache& c, long number, int mult, int unit, int extra, int run = 0) {
   const int lane = threadIdx.x & 63;
   Kv8Sequence s;
+  s.share = 0;
   if (c.B < 63) {   // a lane each: one latency for all of it
     const int row = first_row(c, lane), len = c.lengths[min(lane, c.B - 1)];
     s.b = __popcll(__ballot(lane > 0 && lane <= c.B && (long)row * mult / unit + (long)extra * lane <= number));
     s.row0 = __builtin_amdgcn_readlane(row, s.b);
     s.n = __builtin_amdgcn_readlane(row, s.b + 1) - s.row0;
     s.len = __builtin_amdgcn_readlane(len, s.b);
+    if (SHARE) {
+      const int n = __shfl_down(row, 1, 64) - row, pages = (min(max(len, 0), c.W * PAGE) + PAGE - 1) / PAGE;
+      float work = lane < c.B && n > 0 ? (float)pages * (float)(((long)n * mult + unit - 1) / unit) : 0.0f;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) work += __shfl_xor(work, o, 64);
+      s.share = (int)fminf(ceilf(work / (float)run), 1e6f);
+    }
   } else {
     int before = 0;
     for (int b0 = 1; b0 <= c.B; b0 += 64)
@@ -209,6 +219,7 @@ struct Kv8Args {
   uint16_t* o;
   int H, G, causal;
   int splits;       // of a tile along the keys
+  int run;          // many rows: pieces of a head's tiles that are to be about as long; 0: every tile has `splits`
   int numbers;      // of tiles, those of no tile among them
   int whole;        // many rows: an XCD's tiles that are not split
   float scale_log2;
@@ -218,15 +229,17 @@ struct Kv8Args {
 
 struct Kv8Tile {
   int b, row0, n, rows, r0, len;   // sequence, its first row of q and tokens, its rows of heads, the tile's first, tokens held
+  int share;
 };
 template <int R>
 __device__ __forceinline__ bool kv8_tile(const Kv8Args& p, long number, Kv8Tile& t) {
-  const Kv8Sequence q = find_sequence(p.c, number, p.G, R, 1);
+  const Kv8Sequence q = R > 16 && p.run ? find_sequence<(R > 16)>(p.c, number, p.G, R, 1, p.run) : find_sequence(p.c, number, p.G, R, 1);
   t.b = q.b;
   t.row0 = q.row0;
   t.n = q.n;
   t.len = q.len;
   t.rows = q.n * p.G;
+  t.share = q.share;
   const long r0 = (number - q.unit0) * R;
   t.r0 = (int)r0;
   return r0 >= 0 && r0 < t.rows;   // below 0: offsets that do not ascend
@@ -260,8 +273,17 @@ __device__ __forceinline__ bool kv8_piece(const Kv8Args& p, int& number, int& hk
     piece = -1;
     return kv8_tile_of(p, x, j, number, hk);
   }
-  const uint32_t k = (j - p.whole) / p.splits;
-  split = (j - p.whole) - k * p.splits;
+  uint32_t k;
+  if (p.run) {
+    // every tile's first piece, then their second, ...: those that a tile does not have come last.  Between others the dispatcher
+    // deals these out to few of the CUs (250 us, so 168).
+    const uint32_t tail = kv8_each(p.numbers, p.c.Hkv) * (p.c.Hkv / kv8_shared(p.c.Hkv)) - p.whole;
+    split = (j - p.whole) / tail;
+    k = (j - p.whole) - split * tail;
+  } else {
+    k = (j - p.whole) / p.splits;
+    split = (j - p.whole) - k * p.splits;
+  }
   piece = (k * 8 + x) * p.splits + split;
   return kv8_tile_of(p, x, p.whole + k, number, hk);
 }
@@ -302,6 +324,10 @@ __device__ __forceinline__ u32x4 keys_below(u32x4 x, int from, int end) {
     x[d] = n >= 4 ? x[d] : n <= 0 ? 0u : x[d] & ((1u << (8 * n)) - 1u);
   }
   return x;
+}
+// Pages of a piece of a tile that is split: an even part, or, for pieces of a batch that are about as long, no less than t.share.
+__device__ __forceinline__ int kv8_per(const Kv8Args& p, const Kv8Tile& t, int pages) {
+  return max((pages + p.splits - 1) / p.splits, t.share);
 }
 
 // The offset of a softmax's exponent follows the maximum only where that is more than 2^KV8_LAZY above it, so the output is
@@ -587,14 +613,19 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(Kv8Args p) {
   if (!kv8_tile<R>(p, number, t)) return;
   if (t.r0 + r0 >= t.rows) return;
   const long first = (long)tile * p.splits * R + r0;
+  int splits = p.splits;
+  if (R > 16) {   // those that the tile has
+    const int pages = (kv8_visible(p, t, min(t.r0 + R, t.rows) - 1) + PAGE - 1) / PAGE, per = kv8_per(p, t, pages);
+    splits = max((pages + per - 1) / per, 1);
+  }
   if (hw < ROWS) {
     float m[KV8_SPLITS / 32], l[KV8_SPLITS / 32], top = -INFINITY, sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < KV8_SPLITS / 32; ++i) {
       const int s = 32 * i + hl;
-      const long at = first + hw + (long)min(s, p.splits - 1) * R;
-      m[i] = s < p.splits ? p.part_ml[2 * at] : -INFINITY;
-      l[i] = s < p.splits ? p.part_ml[2 * at + 1] : 0.0f;
+      const long at = first + hw + (long)min(s, splits - 1) * R;
+      m[i] = s < splits ? p.part_ml[2 * at] : -INFINITY;
+      l[i] = s < splits ? p.part_ml[2 * at + 1] : 0.0f;
       top = fmaxf(top, m[i]);
     }
 #pragma unroll
@@ -614,7 +645,7 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(Kv8Args p) {
   const int r = hw % ROWS, g = hw / ROWS;
   float o[C] = {};
 #pragma unroll 4
-  for (int s = g; s < p.splits; s += GROUPS) {
+  for (int s = g; s < splits; s += GROUPS) {
     const float f = weight[r][s];
     const float* from = p.part_o + (first + r + (long)s * R) * D + C * hl;
 #pragma unroll
@@ -670,7 +701,7 @@ struct Kv8Scale {
 };
 
 template <int D>
-__global__ void __launch_bounds__(256, 2) kv8_many_kernel(Kv8Args p) {
+__global__ void __launch_bounds__(256, D == 64 ? 3 : 2) kv8_many_kernel(Kv8Args p) {   // of heads of 64 three share a CU
   using T = Kv8Many<D>;
   constexpr int DB = T::DB, KS = T::KS, KB = T::KB;
   __shared__ __attribute__((aligned(1024))) uint8_t sk[2 * KB], sv[2 * KB];
@@ -683,8 +714,9 @@ __global__ void __launch_bounds__(256, 2) kv8_many_kernel(Kv8Args p) {
   Kv8Tile t;
   if (!kv8_tile<T::R>(p, number, t)) return;
   const int vmin = kv8_visible(p, t, t.r0), vmax = kv8_visible(p, t, min(t.r0 + T::R, t.rows) - 1);
-  const int pages = (vmax + PAGE - 1) / PAGE, pieces = piece < 0 ? 1 : p.splits, per = (pages + pieces - 1) / pieces;
+  const int pages = (vmax + PAGE - 1) / PAGE, per = piece < 0 ? pages : kv8_per(p, t, pages);
   const int p0 = split * per, p1 = min(p0 + per, pages), pe = vmin / PAGE;   // pages from pe on: some row sees a part of them
+  if (split && p0 >= pages) return;   // a piece that the tile does not have
 
   const int row = min(t.r0 + 32 * wave + lr, t.rows - 1), vis = kv8_visible(p, t, row);
   u32x4 qf[KS];
@@ -950,6 +982,7 @@ struct Kv8Plan {
   int rows;     // of a tile
   int numbers;  // of tiles, those of no tile among them
   int splits;   // pieces of a tile along the keys
+  int run;      // Kv8Args::run
   int whole;    // many rows: an XCD's tiles that are not split
   long pieces;  // partial results
 };
@@ -984,7 +1017,15 @@ Kv8Plan kv8_plan(const Kv8Cache& c, int H, bool causal) {
   pl.whole = (int)all;
   pl.splits = 1;
   if (rest && (rounds == 0 || !causal)) {
-    const long want = 64 / rest;
+    long want = 64 / rest;
+    // Tiles that take more than half of the places are not split evenly, and the longest would run alone at the end: there a
+    // batch's longer sequences are cut into up to three pieces, about as long as a place's share of all (6 sequences of 900 to
+    // 9000 keys, 12 heads of 128: 251 us, so 168; 4 of 940 to 6000, 4 heads of 64, 117 and 85).  With fewer tiles it brings
+    // nothing, as two workgroups of a CU get done 1.2 times as much as one (three chunks over 5000 keys and less 44 us, so 50).
+    if (rounds == 0 && want == 1 && c.B > 1 && c.B < 63) {   // a lane for each sequence
+      want = 3;
+      pl.run = (int)(512 / c.Hkv > 1 ? 512 / c.Hkv : 1);
+    }
     pl.splits = (int)(want > (rounds ? 8 : KV8_SPLITS) ? (rounds ? 8 : KV8_SPLITS) : want);
     if (pl.splits > most) pl.splits = (int)most;
     if (pl.splits > 1) pl.whole = (int)(rounds == 0 ? 0 : all - rest);
@@ -1028,7 +1069,7 @@ long kv8_attention_workspace_bytes(const Kv8Cache& c, int H, int causal) {
 hipError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Attention& a, void* workspace, hipStream_t st) {
   const Kv8Plan pl = kv8_plan(c, a.H, a.causal);
   float* part = static_cast<float*>(workspace);
-  const Kv8Args args{c, a.q, a.ldq, a.o, a.H, a.H / c.Hkv, a.causal, pl.splits, pl.numbers, pl.whole,
+  const Kv8Args args{c, a.q, a.ldq, a.o, a.H, a.H / c.Hkv, a.causal, pl.splits, pl.splits > 1 ? pl.run : 0, pl.numbers, pl.whole,
                      a.scale * 1.4426950408889634f, part, part + pl.pieces * pl.rows * c.D};
   return c.D == 128 ? launch_attention<128>(args, pl, st) : launch_attention<64>(args, pl, st);
 }

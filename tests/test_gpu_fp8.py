@@ -392,6 +392,21 @@ def test_attention_of_many_sequences_over_more_pages_than_a_look_up(dev, n, head
     shared(dev, n, 17000, heads, 1, 64, count, 20)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("seqs", [[(300, 5000), (100, 640), (0, 300), (129, 2100), (200, 900)], [(400, 400), (330, 4700)]])
+def test_attention_of_a_ragged_batch(dev, seqs, d, causal):
+    """Long sequences in pieces about as long as the short ones; the last rows of each against the definition."""
+    c = Cache(dev, seqs, 8, d, 23)
+    q = normal((c.offsets[-1], 64, d), c.g)
+    got = ops.kv8_attention(q.to(dev), *c.device(), d ** -0.5, causal).cpu()
+    assert torch.isfinite(got).all()
+    last = [min(n, 5) for n, _ in seqs]
+    rows = torch.cat([torch.arange(end - n, end) for n, end in zip(last, c.offsets[1:])])
+    offsets = [0, *torch.tensor(last).cumsum(0).tolist()]
+    u.check(got[rows], *u.attention(q[rows], offsets, c.lengths(), c.table, *c.oracle(), d ** -0.5, causal))
+
+
 @pytest.mark.parametrize("n", [1, 100])
 def test_many_sequences(dev, n):
     """64 and more sequences, some empty; few rows and many."""
