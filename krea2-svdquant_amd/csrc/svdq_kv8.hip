@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(Kv8Args p) {
   if (t.r0 + r0 >= t.rows) return;
   const long first = (long)tile * p.splits * R + r0;
   int splits = p.splits;
-  if (R > 16) {   // those that the tile has
+  if (R > 16 && p.run) {   // those that the tile has
     const int pages = (kv8_visible(p, t, min(t.r0 + R, t.rows) - 1) + PAGE - 1) / PAGE, per = kv8_per(p, t, pages);
     splits = max((pages + per - 1) / per, 1);
   }
