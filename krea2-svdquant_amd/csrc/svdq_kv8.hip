@@ -327,7 +327,7 @@ __device__ __forceinline__ u32x4 keys_below(u32x4 x, int from, int end) {
 }
 // Pages of a piece of a tile that is split: an even part, or, for pieces of a batch that are about as long, no less than t.share.
 __device__ __forceinline__ int kv8_per(const Kv8Args& p, const Kv8Tile& t, int pages) {
-  return max((pages + p.splits - 1) / p.splits, t.share);
+  return max(max((pages + p.splits - 1) / p.splits, t.share), 1);   // of none: one that is empty
 }
 
 // The offset of a softmax's exponent follows the maximum only where that is more than 2^KV8_LAZY above it, so the output is
@@ -614,7 +614,7 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(Kv8Args p) {
   if (t.r0 + r0 >= t.rows) return;
   const long first = (long)tile * p.splits * R + r0;
   int splits = p.splits;
-  if (R > 16 && p.run) {   // those that the tile has
+  if (R > 16) {   // those that the tile has: the others have written nothing
     const int pages = (kv8_visible(p, t, min(t.r0 + R, t.rows) - 1) + PAGE - 1) / PAGE, per = kv8_per(p, t, pages);
     splits = max((pages + per - 1) / per, 1);
   }

@@ -89,7 +89,9 @@ def append(k, v, offsets, lengths, table, kc, vc, scales):
 
 def attention(q, offsets, lengths, table, kc, vc, scales, scale, causal):
     """(o, bound): a probability is off by its score's error (D + 4 roundings of the sum of magnitudes; exp2's argument and value)
-    and a bf16 rounding, in the numerator and (the former) in the sum; then the result's rounding."""
+    and a bf16 rounding e <= 2^-8, which the numerator and the sum share:
+        (sum p (1 + e) v) / (sum p (1 + e)) - o = (sum p e (v - o)) / (sum p (1 + e)),
+    at most 2^-8 / (1 - 2^-8) (sum p |v| + |o|), and less where the sum takes p itself; then the result's rounding."""
     q = q.double()
     heads, d, kv = q.shape[1], q.shape[2], kc.shape[1]
     out, bound = torch.zeros_like(q), torch.zeros_like(q)
@@ -118,7 +120,7 @@ def attention(q, offsets, lengths, table, kc, vc, scales, scale, causal):
         o = torch.stack([p[:, i, seen[i]].unsqueeze(1) @ v[:, seen[i]] for i in range(n)], 1).squeeze(2)
         size = p.nan_to_num() @ v.nan_to_num().abs()
         off = 2 * ((d + 8) * 2.0 ** -24 * 1.4427 * mag + 2.0 ** -20)
-        near = size * (HALF + 2 * off + 2.0 ** -18)
+        near = HALF / (1 - HALF) * (size + o.nan_to_num().abs()) + size * (2 * off + 2.0 ** -18)
         out[row:row + n] = o.transpose(0, 1)
         bound[row:row + n] = (near + HALF * (o.nan_to_num().abs() + near) + 2.0 ** -133).transpose(0, 1)
     return out, bound

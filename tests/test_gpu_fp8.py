@@ -351,6 +351,16 @@ def test_attention_nothing_visible(dev):
     assert not got[103:].any() and got[:10].any()
 
 
+@pytest.mark.parametrize("seqs", [[(300, 0), (200, 4)], [(500, 0)], [(0, 70), (300, 0), (100, 64), (60, 70)]])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_nothing_visible_in_pieces(dev, seqs, causal):
+    """Many rows over a wide table of which little or nothing is held."""
+    c = Cache(dev, seqs, 1, 64, 71, width=60)
+    got = attend(c, 8, causal)
+    if all(held == 0 for _, held in seqs):
+        assert not got.any()
+
+
 def test_attention_pages_and_lengths_out_of_range(dev):
     c = Cache(dev, [(5, 200), (1, 130)], 2, 64, 7)
     c.table[0][1], c.table[1][2] = 10 ** 6, -7
