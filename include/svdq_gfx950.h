@@ -451,6 +451,11 @@ int svdq_fp8_quantize(const void* x, int64_t ldx, int M, int K, void* codes, flo
 int svdq_fp8_gemm(const void* a, const float* a_scales, const void* w, const float* w_scales, const void* bias, int M,
                   int N, int K, void* y, int64_t ldy, hipStream_t stream);
 
+/* The kernel that svdq_fp8_gemm takes at these sizes: 1 tiles that a workgroup's waves share, 2 strips whose waves take blocks of K
+ * side by side, 3 the one for up to 16 rows; 0 where it refuses them.  rows and cols (may be null) are what a workgroup
+ * takes; *head rows (0: none) go ahead in a launch of 256 x 256 tiles, and the rest is what the others describe. */
+int svdq_fp8_gemm_kernel(int M, int N, int K, int* rows, int* cols, int* head);
+
 /* y = svdq_fp8_quantize(x) times w as above, for bf16 x [M, ldx >= K].  workspace: svdq_fp8_linear_workspace(M, K) bytes,
  * 16-byte aligned, no initial contents, not shared by calls that overlap.  M = 0 does nothing. */
 int64_t svdq_fp8_linear_workspace(int M, int K);

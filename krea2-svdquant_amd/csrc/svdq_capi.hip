@@ -922,6 +922,16 @@ int svdq_fp8_gemm(const void* a, const float* a_scales, const void* w, const flo
   return launched(svdq::launch_fp8_gemm(p, stream), "fp8_gemm");
 }
 
+int svdq_fp8_gemm_kernel(int M, int N, int K, int* rows, int* cols, int* head) {
+  if (M <= 0 || N <= 0 || K <= 0 || K > 1 << 22 || !mx_gemm_fits(M, N)) return 0;
+  int r = 0, c = 0, h = 0;
+  const int kernel = svdq::fp8_gemm_kernel(M, N, K, r, c, h);
+  if (rows) *rows = r;
+  if (cols) *cols = c;
+  if (head) *head = h;
+  return kernel;
+}
+
 int64_t svdq_fp8_linear_workspace(int M, int K) {
   return M <= 0 || K <= 0 || K > 1 << 22 ? 0 : svdq::fp8_linear_workspace_bytes(M, K);
 }

@@ -575,8 +575,8 @@ hipError_t launch_strip(const Fp8GemmParams& p, hipStream_t st) {
   return hipGetLastError();
 }
 
-// What a kernel's workgroups take: rows of a, of w, how many share a CU, and microseconds for a block of K with n of them
-// on a CU (us[n - 1]); a launch takes 3.5 us besides, a further round 1, and w is read from memory at 5.2 TB/s at most.
+// What a kernel's workgroups take: rows of a, of w, their threads, how many share a CU, and microseconds for a block of K with
+// n of them on a CU (us[n - 1]); a launch takes 3.5 us besides, a further round 1, and w is read from memory at 5.2 TB/s at most.
 // Measured (us, K = 6144; strips of 32 x 16, 32 x 32, 64 x 32, 48 x 64 and 64 x 64, then the tiles):
 //     32 x  1536     5.4   6.6   8.6  10.5  12.4 |  16.1  21.6  30.1  37.8  59.2
 //     77 x  1536     9.5   6.9   9.0  10.8  13.0 |  16.1  21.7  30.5  38.0  59.7
@@ -588,14 +588,15 @@ hipError_t launch_strip(const Fp8GemmParams& p, hipStream_t st) {
 //   1024 x  6144       -     -     -     -  81.1 |  64.9  57.3  51.7  45.6  63.1
 //   2381 x  6144       -     -     -     - 201   | 156   132   109   101    86.1
 struct Fp8Cost {
-  int rows, cols, slots;
+  int rows, cols, threads, slots;
   float us[3];
 };
 constexpr int FP8_STRIPS = 5, FP8_KERNELS = FP8_STRIPS + 5;
 const Fp8Cost kCosts[FP8_KERNELS] = {
-    {32, 16, 1, {0.075f}}, {32, 32, 1, {0.105f}}, {64, 32, 1, {0.15f}}, {48, 64, 1, {0.185f}}, {64, 64, 1, {0.235f}},
-    {64, 64, 3, {0.27f, 0.42f, 0.64f}}, {64, 128, 2, {0.38f, 0.62f}}, {128, 128, 2, {0.78f, 1.10f}}, {256, 128, 1, {1.00f}},
-    {256, 256, 1, {1.75f}}};
+    {32, 16, 512, 1, {0.075f}}, {32, 32, 512, 1, {0.105f}}, {64, 32, 256, 1, {0.15f}}, {48, 64, 256, 1, {0.185f}},
+    {64, 64, 256, 1, {0.235f}}, {64, 64, 256, 3, {0.27f, 0.42f, 0.64f}}, {64, 128, 256, 2, {0.38f, 0.62f}},
+    {128, 128, 256, 2, {0.78f, 1.10f}}, {256, 128, 512, 1, {1.00f}}, {256, 256, 512, 1, {1.75f}}};
+constexpr long FP8_THREADS = 1L << 32;   // a launch holds fewer
 
 struct Fp8Choice {
   int kernel;
@@ -608,7 +609,7 @@ Fp8Choice choose(long M, long N, int K) {
   for (int i = 0; i < FP8_KERNELS; ++i) {
     const Fp8Cost& t = kCosts[i];
     const long nbm = (M + t.rows - 1) / t.rows, nbn = (N + t.cols - 1) / t.cols, all = nbm * nbn;
-    if (i < FP8_STRIPS && nbm > 65535) continue;
+    if ((i < FP8_STRIPS && nbm > 65535) || all * t.threads >= FP8_THREADS) continue;   // tiles of 64 x 64 always fit
     const long whole = all / (256 * t.slots), rest = (all % (256 * t.slots) + 255) / 256;
     float us = 2.5f + whole * (1.0f + blocks * t.us[t.slots - 1]) + (rest ? 1.0f + blocks * t.us[rest - 1] : 0.0f);
     if (us < read) us = 0.9f * read + 0.1f * us;   // where reading w takes longest, what takes least besides
@@ -645,8 +646,25 @@ hipError_t launch_kernel(int kernel, const Fp8GemmParams& p, hipStream_t st) {
 
 }  // namespace
 
+// 16 columns a workgroup of 512 threads: wider outputs than a launch holds go to the other kernels
+static bool few_rows(int M, int N) { return M <= 16 && (N + 15L) / 16 * 512 < FP8_THREADS; }
+
+int fp8_gemm_kernel(int M, int N, int K, int& rows, int& cols, int& head) {
+  head = 0;
+  if (few_rows(M, N)) {
+    rows = 16;
+    cols = 16;
+    return FP8_ROWS_KERNEL;
+  }
+  head = (int)head_rows(M, N, K);
+  const int kernel = choose(M - head, N, K).kernel;
+  rows = kCosts[kernel].rows;
+  cols = kCosts[kernel].cols;
+  return kernel < FP8_STRIPS ? FP8_STRIP_KERNEL : FP8_TILE_KERNEL;
+}
+
 hipError_t launch_fp8_gemm(const Fp8GemmParams& p, hipStream_t st) {
-  if (p.M <= 16) {
+  if (few_rows(p.M, p.N)) {
     if (p.M > 8) fp8_gemm_rows_kernel<16, 2><<<(unsigned)((p.N + 15) / 16), 512, 0, st>>>(p);
     else fp8_gemm_rows_kernel<8, 3><<<(unsigned)((p.N + 15) / 16), 512, 0, st>>>(p);
     return hipGetLastError();
@@ -669,7 +687,7 @@ long fp8_linear_workspace_bytes(int M, int K) {
 }
 
 hipError_t launch_fp8_linear(Fp8GemmParams p, const uint16_t* x, long ldx, void* workspace, hipStream_t st) {
-  if (p.M <= Fp8RowsOf::MR && p.K % 128 == 0 && ldx % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0) {
+  if (p.M <= Fp8RowsOf::MR && few_rows(p.M, p.N) && p.K % 128 == 0 && ldx % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0) {
     fp8_linear_rows_kernel<<<(unsigned)((p.N + 15) / 16), 512, 0, st>>>(p, x, ldx);
     return hipGetLastError();
   }

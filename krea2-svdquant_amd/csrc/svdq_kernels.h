@@ -216,6 +216,9 @@ struct Fp8GemmParams {
   int M, N, K;
 };
 hipError_t launch_fp8_gemm(const Fp8GemmParams& p, hipStream_t st);
+// the kernel of a product, what its workgroups take, and rows that go ahead in the largest tiles (0: one launch)
+constexpr int FP8_TILE_KERNEL = 1, FP8_STRIP_KERNEL = 2, FP8_ROWS_KERNEL = 3;
+int fp8_gemm_kernel(int M, int N, int K, int& rows, int& cols, int& head);
 // p.a and p.as are not looked at: they are made of x [M, ldx]
 long fp8_linear_workspace_bytes(int M, int K);
 hipError_t launch_fp8_linear(Fp8GemmParams p, const uint16_t* x, long ldx, void* workspace, hipStream_t st);

@@ -114,6 +114,7 @@ SIGNATURES = {
                                                 _P, _P]),
     "svdq_fp8_quantize": (_I, [_P, _L, _I, _I, _P, _P, _P]),
     "svdq_fp8_gemm": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _P, _L, _P]),
+    "svdq_fp8_gemm_kernel": (_I, [_I, _I, _I, ctypes.POINTER(_I), ctypes.POINTER(_I), ctypes.POINTER(_I)]),
     "svdq_fp8_linear_workspace": (_L, [_I, _I]),
     "svdq_fp8_linear": (_I, [_P, _L, _P, _P, _P, _I, _I, _I, _P, _L, _P, _P]),
     "svdq_qk_norm_rope": (_I, [_P, _L, _I, _P, _L, _I, _P, _P, _P, _P, _L, _I, _I, _P, _I, _I, _I, _I, ctypes.c_float,
@@ -203,6 +204,14 @@ def mx_tile(m: int, n: int, k: int, fmt: int) -> tuple[int, int, int]:
     rows, cols = _I(), _I()
     kind = load().svdq_mx_gemm_tile(m, n, k, fmt, ctypes.byref(rows), ctypes.byref(cols))
     return int(kind), rows.value, cols.value
+
+
+def fp8_kernel(m: int, n: int, k: int) -> tuple[int, int, int, int]:
+    """(1: tiles, 2: strips, 3: the kernel for few rows; rows; columns; rows ahead in the largest tiles) of an 8-bit product
+    (``svdq_fp8_gemm_kernel``)."""
+    rows, cols, head = _I(), _I(), _I()
+    kind = load().svdq_fp8_gemm_kernel(m, n, k, ctypes.byref(rows), ctypes.byref(cols), ctypes.byref(head))
+    return int(kind), rows.value, cols.value, head.value
 
 
 def w4a4_tile_cols(m: int, n: int, k: int, group: int, operand: int) -> int:
