@@ -12,6 +12,8 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
+from .pow2 import pow2
+
 BLOCK = 128
 
 
@@ -27,9 +29,9 @@ def quantize_fp8(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     amax = torch.where(finite, b.abs(), 0.0).amax((1, 3))
     m, e = torch.frexp(amax)
     e = torch.where(amax > 0, torch.where(m <= 0.875, e - 9, e - 8), -126).clamp_min(-126)
-    v = torch.ldexp(torch.where(finite, b, float("nan")), -e[:, None, :, None])
+    v = torch.where(finite, b, float("nan")) * pow2(-e)[:, None, :, None]
     codes = v.flatten(2).flatten(0, 1)[:n].to(torch.float8_e4m3fn)
-    return codes.contiguous(), torch.ldexp(torch.ones_like(amax), e)
+    return codes.contiguous(), pow2(e)
 
 
 def dequantize_fp8(codes: torch.Tensor, scales: torch.Tensor, k: int, dtype: torch.dtype = torch.float32) -> torch.Tensor:

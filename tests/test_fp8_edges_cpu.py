@@ -1,7 +1,11 @@
 """Which kernels the 8-bit operators take, on the CPU: every size that the entry points accept has a launch that the card takes."""
 import pytest
+import torch
 
 from krea2_svdquant_amd.kernels.hip import lib
+from krea2_svdquant_amd.quant.fp8 import quantize_fp8
+from krea2_svdquant_amd.quant.pow2 import pow2
+from tests import fp8_util as u
 
 TILE, STRIP, ROWS = 1, 2, 3
 
@@ -23,3 +27,23 @@ def test_product_kernel_is_told_of_sizes_that_are_taken_alone():
     assert lib.fp8_kernel(5, 300, 640) == (ROWS, 16, 16, 0)
     assert lib.fp8_kernel(0, 300, 640)[0] == lib.fp8_kernel(5, 0, 640)[0] == lib.fp8_kernel(5, 300, 0)[0] == 0
     assert lib.fp8_kernel(5, 300, 2 ** 22 + 1)[0] == 0 and lib.fp8_kernel(2 ** 30, 2 ** 14, 128)[0] == 0
+
+
+# ---- the converter ---------------------------------------------------------------------------------------
+def test_powers_of_two():
+    e = torch.arange(-149, 128)
+    assert torch.equal(pow2(e).double(), torch.tensor([2.0 ** i for i in range(-149, 128)], dtype=torch.float64))
+
+
+def every_exponent(g):
+    """A weight of one column of blocks, a magnitude each: [257 blocks, 128, 40]."""
+    amp = torch.exp2(torch.arange(-140, 117).double())[:, None, None]
+    return (torch.randn(257, 128, 40, generator=g).double().clamp(-3.9, 3.9) * amp).float().flatten(0, 1)
+
+
+def test_converter_at_every_exponent():
+    w = every_exponent(torch.Generator().manual_seed(0))
+    codes, scales = quantize_fp8(w)
+    s = u.scale_of(w.double().view(257, 128, 40).abs().amax((1, 2)))
+    assert torch.equal(scales[:, 0].double(), s)
+    assert torch.equal(codes[:, :40].double(), u.e4m3(w.double() / s.repeat_interleave(128)[:, None]))

@@ -36,3 +36,12 @@ def test_product_of_more_columns_than_a_launch_of_few_rows_holds(dev, m):
             s = ws[torch.arange(p.start, p.stop, device=dev) // 128].double()
             assert torch.equal(y[:, p], (x.double() @ (w[p].double() * s).T).to(torch.bfloat16))
         assert not y[:, 300:400].any() and not y[:, 2 ** 26 + 200:2 ** 26 + 300].any()
+
+
+# ---- the converter -------------------------------------------------------------------------------------------
+def test_converter_on_the_gpu_is_the_one_on_the_cpu(dev):
+    from krea2_svdquant_amd.quant.fp8 import quantize_fp8
+    from tests.test_fp8_edges_cpu import every_exponent
+    w = every_exponent(gen(0))
+    (codes, scales), (c, s) = quantize_fp8(w), quantize_fp8(w.to(dev))
+    assert torch.equal(s.cpu(), scales) and torch.equal(c.cpu().view(torch.uint8), codes.view(torch.uint8))
