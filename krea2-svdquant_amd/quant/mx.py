@@ -11,6 +11,8 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
+from .pow2 import pow2
+
 BLOCK = 32
 EMAX = {"e2m1": 2, "e4m3": 8}
 
@@ -31,7 +33,7 @@ def quantize_mx(x: torch.Tensor, fmt: str = "e2m1") -> tuple[torch.Tensor, torch
     b = torch.where(finite[..., None], b, 0.0)
     e = torch.frexp(torch.where(finite, amax, 1.0)).exponent - 1 - EMAX[fmt]
     e = torch.where(amax > 0, e, -127).clamp(-127, 127)
-    v = torch.ldexp(b, -e[..., None]).flatten(-2)
+    v = (b * pow2(-e)[..., None]).flatten(-2)
     s = F.pad(torch.where(finite, e + 127, 255).to(torch.uint8), (0, -e.shape[-1] % 16))
     scales = s.contiguous().view(torch.float8_e8m0fnu)
     if fmt == "e4m3":
@@ -63,5 +65,5 @@ def dequantize_mx(codes: torch.Tensor, scales: torch.Tensor, k: int, dtype: torc
     if tuple(scales.shape) != want:
         raise ValueError(f"scales must be {want}, got {tuple(scales.shape)}")
     s = scales.view(torch.uint8)[..., :kp // BLOCK].int()
-    f = torch.where(s == 255, float("nan"), torch.ldexp(torch.ones((), device=codes.device), s - 127))
+    f = torch.where(s == 255, float("nan"), pow2(s - 127))
     return (v.unflatten(-1, (-1, BLOCK)) * f[..., None]).flatten(-2)[..., :k].to(dtype)

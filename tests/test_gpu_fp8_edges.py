@@ -45,3 +45,16 @@ def test_converter_on_the_gpu_is_the_one_on_the_cpu(dev):
     w = every_exponent(gen(0))
     (codes, scales), (c, s) = quantize_fp8(w), quantize_fp8(w.to(dev))
     assert torch.equal(s.cpu(), scales) and torch.equal(c.cpu().view(torch.uint8), codes.view(torch.uint8))
+
+
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
+def test_mx_converter_on_the_gpu_is_the_one_on_the_cpu(dev, fmt):
+    """Every exponent of a block's scale, and values between two codes."""
+    from krea2_svdquant_amd.quant.mx import dequantize_mx, quantize_mx
+    amp = torch.exp2(torch.arange(-140, 116).float())[:, None]
+    for x in (torch.randn(256, 32, generator=gen(1)), torch.randint(-24, 25, (256, 32), generator=gen(2)) / 4):
+        codes, scales = quantize_mx(x * amp, fmt)
+        c, s = quantize_mx((x * amp).to(dev), fmt)
+        assert torch.equal(c.cpu().view(torch.uint8), codes.view(torch.uint8))
+        assert torch.equal(s.cpu().view(torch.uint8), scales.view(torch.uint8))
+        assert torch.equal(dequantize_mx(c, s, 32).cpu(), dequantize_mx(codes, scales, 32))
