@@ -333,6 +333,9 @@ __device__ __forceinline__ int kv8_per(const Kv8Args& p, const Kv8Tile& t, int p
 // The offset of a softmax's exponent follows the maximum only where that is more than 2^KV8_LAZY above it, so the output is
 // hardly ever rescaled; probabilities up to 2^KV8_LAZY are as exact as those below 1.
 constexpr float KV8_LAZY = 8.0f;
+// score x factor - offset in one FMA is exact, the offset (a rounded product) is not: scores (log2 units) of 2^20 and more are
+// multiplied and rounded by themselves, so that the largest is at its offset however large they are.
+constexpr float KV8_LARGE = 0x1p20f;
 constexpr int KV8_SPLITS = 128;   // at most
 
 __device__ __forceinline__ float other_half_max(float v) {   // over lanes l and l ^ 32
@@ -489,12 +492,19 @@ __global__ void __launch_bounds__(256, 2) kv8_rows_kernel(Kv8Args p) {
         for (int k = 0; k < 16; ++k) hi = fmaxf(hi, S[k / 4][k % 4]);
         const float top = rows_max(hi * f);
         if (__any(top > m + KV8_LAZY)) rescale(top);
-        const float off = (m == -INFINITY ? 0.0f : m) - lv;
+        const float base = m == -INFINITY ? 0.0f : m, off = base - lv;
+        if (__any(!(fabsf(top) < KV8_LARGE))) {
+#pragma clang fp contract(off)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) S[k / 4][k % 4] = S[k / 4][k % 4] * f - base + lv;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) S[k / 4][k % 4] = __builtin_fmaf(S[k / 4][k % 4], f, -off);
+        }
         float sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < 16; k += 2) {
-          const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(S[k / 4][k % 4], f, -off));
-          const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(S[k / 4][k % 4 + 1], f, -off));
+          const float a = __builtin_amdgcn_exp2f(S[k / 4][k % 4]), b = __builtin_amdgcn_exp2f(S[k / 4][k % 4 + 1]);
           const uint32_t w = pack_bf16x2(a, b);
           pf[k / 8][k % 8 / 2] = w;
           sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3F803F80u), sum, false);
@@ -508,10 +518,13 @@ __global__ void __launch_bounds__(256, 2) kv8_rows_kernel(Kv8Args p) {
 #pragma unroll
           for (int d = 0; d < DT; ++d) vq[d] = u32x4{} | FP8_NAN4;
         }
+        {
+#pragma clang fp contract(off)
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          S[k / 4][k % 4] = key0 + k >= vis ? -INFINITY : S[k / 4][k % 4] * f;
-          hi = fmaxf(hi, S[k / 4][k % 4]);
+          for (int k = 0; k < 16; ++k) {
+            S[k / 4][k % 4] = key0 + k >= vis ? -INFINITY : S[k / 4][k % 4] * f;
+            hi = fmaxf(hi, S[k / 4][k % 4]);
+          }
         }
         const float top = rows_max(hi);
         if (__any(top > m + KV8_LAZY)) rescale(top);
@@ -678,8 +691,8 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(Kv8Args p) {
 // exp2(f s - (m - log2 vs)) = vs p, which is what the product needs; the row's sum takes the rounded values over vs, two in an
 // instruction.  The offset is a row's maximum over the first page and stays, so the output is touched by the matrix unit
 // alone; later probabilities may exceed 1, which float32 and bf16 hold as exactly.  Where a sum passes 2^64, anything is
-// not finite, or a page of which rows see different parts holds values that are no numbers, the tile is done again with an
-// offset that follows the maximum.
+// not finite, an offset is large, or a page of which rows see different parts holds values that are no numbers, the tile is done
+// again with an offset that follows the maximum.
 // Scales that are no ordinary positive numbers are dealt with as the pages come in: a factor below 0 turns the keys' signs, other
 // scales of values are multiplied into them, those that are not finite make the codes NaN.  Pages that are not there count as -infinity.
 //
@@ -856,14 +869,21 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) kv8_many_kernel(Kv8Args 
     for (int r = 1; r < 32; ++r) hi = fmaxf(hi, S[r / 16][r % 16]);
     return other_half_max(__builtin_fmaf(hi, w.f, w.at));
   };
-  auto softmax = [&](const Kv8Scale& w) __attribute__((always_inline)) {
-    const float off = (m == -INFINITY ? 0.0f : m) - w.lv;
+  auto softmax = [&](const Kv8Scale& w, auto large) __attribute__((always_inline)) {   // large: scores of any size (KV8_LARGE)
+    const float base = m == -INFINITY ? 0.0f : m, off = base - w.lv;
+    auto power = [&](float score) __attribute__((always_inline)) {
+#pragma clang fp contract(off)
+      if (large) {
+        const float rounded = score * w.f;
+        return __builtin_amdgcn_exp2f(rounded - base + w.lv);
+      }
+      return __builtin_amdgcn_exp2f(__builtin_fmaf(score, w.f, -off));
+    };
     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int r = 0; r < 32; r += 2) {
       const int hf = r / 16, q = r % 16;
-      const uint32_t x = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(S[hf][q], w.f, -off)),
-                                     __builtin_amdgcn_exp2f(__builtin_fmaf(S[hf][q + 1], w.f, -off)));
+      const uint32_t x = pack_bf16x2(power(S[hf][q]), power(S[hf][q + 1]));
       pf[hf][q / 8][q % 8 / 2] = x;
       sum[hf] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), __builtin_bit_cast(bf16x2, 0x3F803F80u), sum[hf], false);
     }
@@ -895,7 +915,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) kv8_many_kernel(Kv8Args 
       scores(buf);
       if (pg >= pe) masked(pg);
       if (pg == p0) m = top_of(now);
-      softmax(now);
+      softmax(now, std::false_type{});
       values(buf);
       store(next, buf ^ 1);
       now = scale_in(next);
@@ -907,6 +927,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) kv8_many_kernel(Kv8Args 
     }
   }
   again |= !(l <= 0x1p64f);   // infinities and NaN among them
+  again |= vis > p0 * PAGE && p0 < p1 && !(fabsf(m) < KV8_LARGE);   // -infinity too: of keys that are seen, it tells nothing of the others
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -946,7 +967,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) kv8_many_kernel(Kv8Args 
       l *= alpha;
 #pragma unroll
       for (int db = 0; db < DB; ++db) O[db] *= alpha;
-      softmax(w);
+      softmax(w, std::true_type{});
       values(0);
     }
   }

@@ -58,3 +58,58 @@ def test_mx_converter_on_the_gpu_is_the_one_on_the_cpu(dev, fmt):
         assert torch.equal(c.cpu().view(torch.uint8), codes.view(torch.uint8))
         assert torch.equal(s.cpu().view(torch.uint8), scales.view(torch.uint8))
         assert torch.equal(dequantize_mx(c, s, 32).cpu(), dequantize_mx(codes, scales, 32))
+
+
+# ---- the cache and its attention -----------------------------------------------------------------------------
+def i32(dev, x):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+def mean_of(v, seen):
+    """(o, bound) of equal probabilities of the keys `seen` [keys]: rounded to bf16 times their page's scale, which the sum
+    shares (fp8_util.attention), and the result's rounding."""
+    x = v[..., seen].double()
+    o, size = x.mean(-1), x.abs().mean(-1)
+    near = u.HALF / (1 - u.HALF) * (size + o.abs()) + size * 2.0 ** -17
+    return o, near + u.HALF * (o.abs() + near)
+
+
+@pytest.mark.parametrize("n", [3, 130])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("level", [2.0 ** 12, 2.0 ** 24, 2.0 ** 40, 2.0 ** 100])
+def test_attention_of_scores_of_any_size(dev, n, d, level):
+    """Scores of whole multiples of a level, far apart: the largest share the result evenly, whatever their page's scale; with
+    pages in every order of their largest scores."""
+    g = gen(d)
+    k = torch.randint(-6, 4, (4, 1, 64, d), generator=g).float()
+    for page, top in enumerate((2, 5, 5, 4)):
+        k[page, 0, :, 0] = torch.randint(-6, top, (64,), generator=g).float()
+        k[page, 0, 7:60:10 + page, 0] = top
+    v = torch.randint(-100, 100, (4, 1, d, 64), generator=g).float().to(torch.float8_e4m3fn)
+    s = torch.ones(4, 1, 2)
+    s[:, 0, 1] = torch.tensor([0.7, 0.013, 3.0, 1.0])
+    q = torch.zeros(n, 4, d)
+    q[..., 0] = level
+    for order in ([0, 1, 2, 3], [2, 3, 0, 1], [3, 0, 1, 2]):
+        for sign in (1.0, -1.0):
+            o = ops.kv8_attention((sign * q).to(torch.bfloat16).to(dev), i32(dev, [0, n]), i32(dev, [256]), i32(dev, [order]),
+                                  k.to(torch.float8_e4m3fn).to(dev), v.to(dev), s.to(dev), 0.3, False)
+            kv = sign * k[order, 0, :, 0].flatten()
+            vv = (v.float() * s[..., 1:, None])[order, 0].permute(1, 0, 2).flatten(1)
+            want, bound = mean_of(vv, kv == kv.max())
+            u.check(o, want.expand(n, 4, d), bound.expand(n, 4, d))
+
+
+@pytest.mark.parametrize("n", [3, 130])
+@pytest.mark.parametrize("order", [[0, 1, 2], [1, 0, 2]])
+def test_attention_of_a_page_whose_scores_pass_float32(dev, n, order):
+    """-infinity for every key of a page (the first one, too) leaves the others their part."""
+    k = torch.full((3, 1, 64, 64), -2.0 ** -9)
+    k[0] = -448.0
+    v = torch.randint(-100, 100, (3, 1, 64, 64), generator=gen(n)).float().to(torch.float8_e4m3fn)
+    q = torch.full((n, 4, 64), 3e37).to(torch.bfloat16)
+    o = ops.kv8_attention(q.to(dev), i32(dev, [0, n]), i32(dev, [192]), i32(dev, [order]), k.to(torch.float8_e4m3fn).to(dev),
+                          v.to(dev), torch.ones(3, 1, 2, device=dev), 0.125, False)
+    vv = v.float()[order, 0].permute(1, 0, 2).flatten(1)
+    want, bound = mean_of(vv, torch.tensor(order).repeat_interleave(64) != 0)
+    u.check(o, want.expand(n, 4, 64), bound.expand(n, 4, 64))
