@@ -482,7 +482,7 @@ int svdq_qk_norm_rope(const void* q, int64_t ldq, int hsq, const void* k, int64_
 
 /* Puts new keys and values (bf16 [N, Hkv, D], rows ldk, ldv apart, multiples of 8, 16-byte aligned) behind the lengths[b] tokens
  * that the sequences hold.  A page that begins with new tokens gets their scale (as svdq_fp8_quantize, over the page and
- * head); one that holds older tokens keeps its scale, or gets theirs where that is larger: the older codes are then
+ * head); one that holds older tokens keeps its scale, or gets theirs where that is larger in magnitude: the older codes are then
  * rounded again under it.  Slots behind the new tokens are left as they are, and so are the lengths. */
 int svdq_kv8_append(const void* k, int64_t ldk, const void* v, int64_t ldv, int N, const int* offsets,
                     const int* lengths, const int* table, int B, int W, void* k_codes, void* v_codes, float* scales,

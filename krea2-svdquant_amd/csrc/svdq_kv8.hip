@@ -8,8 +8,8 @@
 // Everything that comes from device memory is held to its range before it is used as an index: offsets to the rows there
 // are, lengths to the table's width, pages to the cache (others hold nothing, and nothing is written to them).
 //
-// append:  a page's scale is that of its new tokens (svdq_fp8.h), or the larger of that and the one it has where it holds
-//          tokens already; those are then rounded again under the new scale.
+// append:  a page's scale is that of its new tokens (svdq_fp8.h), or the larger (in magnitude) of that and the one it has where
+//          it holds tokens already; those are then rounded again under the new scale.
 // attend:  o = sum over visible j of softmax_j(scale q . k_j) v_j,  j < length, and with a causal mask, for the i-th of n new
 //          tokens, j <= length - n + i; 0 where nothing is visible.
 #include <type_traits>
@@ -137,16 +137,17 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(Kv8Cache c, const uint1
     s[w] = fp8_scale(max(max(tops[w][0], tops[w][1]), max(tops[w][2], tops[w][3])));
     again[w] = 1.0f;
     if (lo > 0) {
-      if (had[w] >= s[w]) s[w] = had[w];
+      if (fabsf(had[w]) >= s[w]) s[w] = had[w];
       else again[w] = had[w] / s[w];
     }
   }
   if (tid < 2) c.scales[2 * at + tid] = tid ? s[1] : s[0];
   auto encode = [](u32x4 r, float s) {
-    if (__float_as_uint(s) & 0x7FFFFFu) {   // a scale of the caller's, no power of two: the conversion takes only those
+    if (s < 0.0f || __float_as_uint(s) & 0x7FFFFFu) {   // a scale of the caller's, no power of two: the conversion takes only those
       auto over = [&](float v) {
         const float q = v / s;
-        return sticky(q, __builtin_fmaf(-q, s, v));   // s > 0: it is at least what the new tokens need
+        const float rest = __builtin_fmaf(-q, s, v);   // |s| is at least what the new tokens need
+        return sticky(q, s < 0.0f ? -rest : rest);
       };
       return u32x2{fp8_encode4(over(bf16lo(r[0])), over(bf16hi(r[0])), over(bf16lo(r[1])), over(bf16hi(r[1])), 1.0f),
                    fp8_encode4(over(bf16lo(r[2])), over(bf16hi(r[2])), over(bf16lo(r[3])), over(bf16hi(r[3])), 1.0f)};

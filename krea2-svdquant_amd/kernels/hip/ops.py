@@ -679,7 +679,7 @@ def kv8_append(k: Tensor, v: Tensor, cu_seqlens: Tensor, lengths: Tensor, block_
     each sequence, ``lengths`` [B] (int32) how many tokens it holds before the call, ``cu_seqlens`` [B + 1] (int32) which of the
     new tokens are its own: rows ``cu_seqlens[b]`` to ``cu_seqlens[b + 1]``, ascending from 0.  A page that begins with new
     tokens gets their scale (``fp8_quantize``'s, over the page and head); one that holds older tokens keeps its own or takes
-    theirs where that is larger, and the older codes are rounded again under it.  Tokens beyond the table, or whose page
+    theirs where that is larger in magnitude, and the older codes are rounded again under it.  Tokens beyond the table, or whose page
     is not in the cache, are dropped; sequences may not share a page that is written."""
     return _mx("kv8_append", k_codes, k, v, cu_seqlens, lengths, block_table, k_codes, v_codes, scales)
 

@@ -113,3 +113,25 @@ def test_attention_of_a_page_whose_scores_pass_float32(dev, n, order):
     vv = v.float()[order, 0].permute(1, 0, 2).flatten(1)
     want, bound = mean_of(vv, torch.tensor(order).repeat_interleave(64) != 0)
     u.check(o, want.expand(n, 4, 64), bound.expand(n, 4, 64))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("had", [-0.3, -2.0 ** -6, -3.7e-5, -1e30, 0.3, 2.5e-9])
+def test_append_behind_a_page_scale_of_any_sign(dev, d, had):
+    """The scale that is larger in magnitude holds the older tokens and the new ones."""
+    g = gen(d)
+    kc, vc, s = u.pages(1, 2, d, g)
+    s[:] = had
+    s[0, 1] *= 0.5
+    k, v = normal((9, 2, d), g), normal((9, 2, d), g, 0.01)
+    K, V, S = kc.to(dev), vc.to(dev), s.to(dev)
+    ops.kv8_append(k.to(dev), v.to(dev), i32(dev, [0, 9]), i32(dev, [21]), i32(dev, [[0]]), K, V, S)
+    for w, (x, codes, got) in enumerate(((k, kc, K.cpu()), (v, vc.transpose(2, 3), V.cpu().transpose(2, 3)))):
+        x, old, got = x.double().transpose(0, 1), codes.double()[0], got.double()[0]
+        need, before = u.scale_of(x.abs().amax((1, 2))), s[0, :, w].double()
+        after = torch.where(before.abs() >= need, before, need)
+        assert torch.equal(S.cpu().double()[0, :, w], after)
+        factor = (before / after).float().double()[:, None, None]   # rounded to float32
+        assert torch.equal(got[:, :21], u.e4m3(old[:, :21] * factor))
+        assert torch.equal(got[:, 21:30], u.e4m3(x / after[:, None, None]))
+        assert torch.equal(got[:, 30:], old[:, 30:])
