@@ -444,8 +444,9 @@ int svdq_residual_rms_norm_modulate_mx(const void* x, int64_t ldx, const void* v
  * 2^26 - 1.  M = 0 does nothing. */
 int svdq_fp8_quantize(const void* x, int64_t ldx, int M, int K, void* codes, float* scales, hipStream_t stream);
 
-/* y [M, ldy] bf16 = a w^T + bias, block by block in float32: each block's sum over its 128 columns is scaled (any float32
- * scales) and added.  bias [N] bf16 or null.  Within 8 consecutive k the matrix instruction drops what lies below
+/* y [M, ldy] bf16 = a w^T + bias, block by block in float32: each block's sum over its 128 columns is scaled and added.
+ * Scales are any float32; a block's two are multiplied in float32 first, so a product of 2^128 or more makes its part infinite or NaN, and
+ * one below 2^-126 leaves that part off by up to 2^-125.  bias [N] bf16 or null.  Within 8 consecutive k the matrix instruction drops what lies below
  * 2^-13 of the power of two of the largest product.  K at most 2^22, M N / 4096 (each rounded up to 64) under
  * 2^24.  M = 0 does nothing. */
 int svdq_fp8_gemm(const void* a, const float* a_scales, const void* w, const float* w_scales, const void* bias, int M,

@@ -6,7 +6,9 @@
 // v_mfma_f32_16x16x128 sums exactly one block: its result is scaled and added to the accumulator by one FMA per value
 // (the scales are any float32, so the matrix instruction's own power-of-two scales cannot take them).  The weight is the
 // first operand, so a lane holds one row m and four consecutive n: its scales are one value per row of tiles, times one per
-// block that is the same for the whole wave.
+// block that is the same for the whole wave.  Their product is a float32 too: blocks of which it is 2^128 and more are not finite, and
+// of one below 2^-126 the part is off by up to 2^-150 x 128 x 448^2.  (The scales' powers of two as the instruction's own, and what
+// they are between powers of two in the FMA, would keep the whole range: 4352 x 16384, K = 6144 391 us, so 385; 40 x 6144 10.0, 9.5.)
 #include <type_traits>
 #include <utility>
 

@@ -650,7 +650,8 @@ def fp8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
 
 def fp8_gemm(a: Tensor, a_scales: Tensor, w: Tensor, w_scales: Tensor, bias: Optional[Tensor] = None) -> Tensor:
     """``svdq::fp8_gemm``: ``a w^T + bias`` of an E4M3 activation (as ``fp8_quantize`` gives it) and an E4M3 weight ``w``
-    [N, kp] with a float32 scale for each 128 x 128 block (any values); bf16 [..., N], sums in float32."""
+    [N, kp] with a float32 scale for each 128 x 128 block; bf16 [..., N], sums in float32.  Scales may have any values; a
+    block's two are multiplied in float32 first, so below 2^-126 its part is off by up to 2^-125, from 2^128 on infinite or NaN."""
     return _mx("fp8_gemm", a, a, a_scales, w, w_scales, bias)
 
 

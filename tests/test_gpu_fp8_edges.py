@@ -135,3 +135,61 @@ def test_append_behind_a_page_scale_of_any_sign(dev, d, had):
         assert torch.equal(got[:, :21], u.e4m3(old[:, :21] * factor))
         assert torch.equal(got[:, 21:30], u.e4m3(x / after[:, None, None]))
         assert torch.equal(got[:, 30:], old[:, 30:])
+
+
+# ---- the product's kernels, each at a size that it is taken for (K = 640): (M, N) and lib.fp8_kernel's answer ----
+KERNELS = {
+    "8 rows": (5, 130, (3, 16, 16, 0)), "16 rows": (12, 131, (3, 16, 16, 0)),
+    "strip 32 x 16": (17, 50, (2, 32, 16, 0)), "strip 32 x 32": (33, 2081, (2, 32, 32, 0)),
+    "strip 64 x 32": (34, 4127, (2, 64, 32, 0)), "strip 48 x 64": (18, 8249, (2, 48, 64, 0)),
+    "strip 64 x 64": (50, 8321, (2, 64, 64, 0)), "tile 64 x 64": (5501, 262, (1, 64, 64, 0)),
+    "tile 64 x 128": (17, 16424, (1, 64, 128, 0)), "tile 128 x 128": (259, 16918, (1, 128, 128, 0)),
+    "tile 256 x 128": (133, 22092, (1, 256, 128, 0)), "tile 256 x 256": (337, 21920, (1, 256, 256, 0)),
+    "two launches": (1802, 17685, (1, 64, 128, 1792))}
+
+
+def product_on(a, sa, w, sw, bias=None):
+    """fp8_util.product on the operands' device, block by block."""
+    n, kb = w.shape[0], sa.shape[0]
+    y = mag = lost = 0.0
+    for b in range(kb):
+        p = a[:, 128 * b:128 * b + 128].double() * sa[b].double()[:, None]
+        q = w[:, 128 * b:128 * b + 128].double() * sw[:, b].double().repeat_interleave(128)[:n, None]
+        y, mag = y + p @ q.T, mag + p.abs() @ q.abs().T
+        lost = lost + 16 * 7 * 2.0 ** -13 * p.abs().amax(-1)[:, None] * q.abs().amax(-1)
+    if bias is not None:
+        y, mag = y + bias.double(), mag + bias.double().abs()
+    near = (131 + kb) * 2.0 ** -24 * mag + lost
+    return y, near + u.HALF * (y.abs() + near) + 2.0 ** -133
+
+
+def check_on(got, want, bound):
+    assert torch.isfinite(got).all() and torch.isfinite(want).all()
+    worst = ((got.double() - want).abs() / bound).max().item()
+    assert worst <= 1.0, f"off by {worst:.3g} of the bound"
+
+
+# codes' magnitude, the scales' exponents, and what a block may be off where the scales' product is subnormal: half of its last bit,
+# 2^-150, times a sum of 128 products of 448 x 448
+FAR_SCALES = {"product up to 2^127": (2.0 ** -8, 110, 15, 0.0), "product from 2^-126": (448.0, -126, 0, 0.0),
+              "subnormal activations": (448.0, -135, 20, 0.0), "subnormal weights": (8.0, 124, -138, 0.0),
+              "product of 2^-138": (448.0, -126, -12, 128 * 448.0 ** 2 * 2.0 ** -150)}
+
+
+@pytest.mark.parametrize("size", KERNELS)
+@pytest.mark.parametrize("far", FAR_SCALES)
+def test_product_of_scales_at_the_ends_of_float32(dev, size, far):
+    """Results are ordinary; rows, columns and blocks of zeros, of codes and of scales, among them."""
+    from krea2_svdquant_amd.kernels.hip import lib
+    m, n, kernel = KERNELS[size]
+    assert lib.fp8_kernel(m, n, 640) == kernel
+    amp, ea, ew, off = FAR_SCALES[far]
+    g = torch.Generator(device=dev).manual_seed(m)
+    a, w = ((torch.randn((r, 640), device=dev, generator=g) * amp / 3).clamp(-amp, amp).to(torch.float8_e4m3fn) for r in (m, n))
+    sa = ((1 + torch.rand((5, m), device=dev, generator=g).double()) * 2.0 ** ea).float()
+    sw = ((1 + torch.rand((-(-n // 128), 5), device=dev, generator=g).double()) * 2.0 ** ew).float()
+    for t in (a.view(torch.uint8)[0], a.view(torch.uint8)[1, 128:256], w.view(torch.uint8)[n - 1]):
+        t.zero_()
+    sa[3, 2], sw[0, 4] = 0.0, -sw[0, 4]
+    want, bound = product_on(a, sa, w, sw)
+    check_on(ops.fp8_gemm(a, sa, w, sw), want, bound + 5 * off)
