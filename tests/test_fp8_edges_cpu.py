@@ -47,3 +47,12 @@ def test_converter_at_every_exponent():
     s = u.scale_of(w.double().view(257, 128, 40).abs().amax((1, 2)))
     assert torch.equal(scales[:, 0].double(), s)
     assert torch.equal(codes[:, :40].double(), u.e4m3(w.double() / s.repeat_interleave(128)[:, None]))
+
+
+def test_every_product_kernel_is_tested_where_it_is_chosen():
+    from tests.test_gpu_fp8_edges import DEEP, KERNELS
+    every = ({(STRIP, *t) for t in ((32, 16), (32, 32), (64, 32), (48, 64), (64, 64))} |
+             {(TILE, *t) for t in ((64, 64), (64, 128), (128, 128), (256, 128), (256, 256))} | {(ROWS, 16, 16)})
+    for sizes in ([(m, n, 640, kernel) for m, n, kernel in KERNELS.values()], list(DEEP.values())):
+        assert all(lib.fp8_kernel(m, n, k) == kernel for m, n, k, kernel in sizes)
+        assert {kernel[:3] for *_, kernel in sizes} == every and any(kernel[3] for *_, kernel in sizes)

@@ -193,3 +193,39 @@ def test_product_of_scales_at_the_ends_of_float32(dev, size, far):
     sa[3, 2], sw[0, 4] = 0.0, -sw[0, 4]
     want, bound = product_on(a, sa, w, sw)
     check_on(ops.fp8_gemm(a, sa, w, sw), want, bound + 5 * off)
+
+
+# Each kernel at 66 blocks of K (the weights' scales are looked up 64 at a time), and layer sizes of the denoiser's.
+DEEP = {
+    "8 rows": (5, 130, 8448, (3, 16, 16, 0)), "16 rows": (12, 131, 8448, (3, 16, 16, 0)),
+    "strip 32 x 16": (17, 50, 8448, (2, 32, 16, 0)), "strip 32 x 32": (33, 2065, 8448, (2, 32, 32, 0)),
+    "strip 64 x 32": (33, 4107, 8448, (2, 64, 32, 0)), "strip 48 x 64": (18, 8198, 8448, (2, 48, 64, 0)),
+    "strip 64 x 64": (49, 8418, 8448, (2, 64, 64, 0)), "tile 64 x 64": (5634, 263, 8448, (1, 64, 64, 0)),
+    "tile 64 x 128": (65, 8207, 8448, (1, 64, 128, 0)), "tile 128 x 128": (260, 19949, 8448, (1, 128, 128, 0)),
+    "tile 256 x 128": (145, 23076, 8448, (1, 256, 128, 0)), "tile 256 x 256": (520, 18194, 8448, (1, 256, 256, 0)),
+    "two launches": (1285, 18151, 8448, (1, 64, 128, 768)),
+    "prompt": (77, 6144, 6144, (2, 48, 64, 0)), "128 tokens": (128, 6144, 6144, (2, 64, 64, 0)),
+    "320 tokens": (320, 6144, 6144, (1, 64, 128, 0)), "image, up": (4352, 16384, 6144, (1, 64, 128, 4096)),
+    "image, down": (4352, 6144, 16384, (1, 256, 256, 0))}
+
+
+@pytest.mark.parametrize("size", DEEP)
+@pytest.mark.parametrize("bias", [False, True])
+def test_product_of_small_whole_numbers_on_every_kernel(dev, size, bias):
+    """Codes and scales of which every sum is a whole number below 2^24, so only the store rounds; scales differ from block to
+    block."""
+    from krea2_svdquant_amd.kernels.hip import lib
+    m, n, k, kernel = DEEP[size]
+    assert lib.fp8_kernel(m, n, k) == kernel
+    kb, g = k // 128, torch.Generator(device=dev).manual_seed(m + bias)
+    a, w = (torch.randint(-3, 4, (r, k), device=dev, generator=g).float() for r in (m, n))
+    sa = torch.randint(1, 4, (kb, m), device=dev, generator=g).float()
+    sw = torch.randint(1, 4, (-(-n // 128), kb), device=dev, generator=g).float()
+    b = torch.randint(-100, 101, (n,), device=dev, generator=g).to(torch.bfloat16) if bias else None
+    y = ops.fp8_gemm(a.to(torch.float8_e4m3fn), sa, w.to(torch.float8_e4m3fn), sw, b)
+    ab = (a.view(m, kb, 128) * sa.T[..., None]).view(m, k).double()
+    wb = (w.view(n, kb, 128) * sw.repeat_interleave(128, 0)[:n, :, None]).view(n, k).double()
+    want = ab @ wb.T
+    if bias:
+        want += b.double()
+    assert torch.equal(y, want.to(torch.bfloat16))
