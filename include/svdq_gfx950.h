@@ -501,6 +501,11 @@ int svdq_kv8_attention(const void* q, int64_t ldq, int N, const int* offsets, co
                        int B, int W, const void* k_codes, const void* v_codes, const float* scales, int P, int H, int Hkv,
                        int D, float scale, int causal, void* o, void* workspace, hipStream_t stream);
 
+/* What svdq_kv8_attention does at these sizes: 1 the kernel for few rows, whose tiles run in *splits pieces each; 2 the one for
+ * many, in which *whole of the *tiles of an XCD run in one piece and the others in *splits; 3 the same in pieces that are about as
+ * long for sequences of different lengths; 0 where it refuses them.  (Few rows: *tiles of a key head, *whole 0.) */
+int svdq_kv8_attention_kernel(int N, int B, int W, int H, int Hkv, int D, int causal, int* splits, int* whole, int* tiles);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1032,6 +1032,18 @@ int64_t svdq_kv8_attention_workspace(int N, int B, int W, int H, int Hkv, int D,
   return svdq::kv8_attention_workspace_bytes(kv8_cache(N, nullptr, nullptr, nullptr, B, W, nullptr, nullptr, nullptr, 1, Hkv, D), H, causal);
 }
 
+int svdq_kv8_attention_kernel(int N, int B, int W, int H, int Hkv, int D, int causal, int* splits, int* whole, int* tiles) {
+  if (N <= 0 || B <= 0 || W <= 0 || W > 1 << 24 || Hkv <= 0 || H <= 0 || H % Hkv || (D != 64 && D != 128) || !kv8_fits(N, B, H, Hkv))
+    return 0;
+  int s = 0, w = 0, t = 0;
+  const int kernel = svdq::kv8_attention_kernel(kv8_cache(N, nullptr, nullptr, nullptr, B, W, nullptr, nullptr, nullptr, 1, Hkv, D), H,
+                                                causal != 0, s, w, t);
+  if (splits) *splits = s;
+  if (whole) *whole = w;
+  if (tiles) *tiles = t;
+  return kernel;
+}
+
 int svdq_kv8_attention(const void* q, int64_t ldq, int N, const int* offsets, const int* lengths, const int* table,
                        int B, int W, const void* k_codes, const void* v_codes, const float* scales, int P, int H, int Hkv,
                        int D, float scale, int causal, void* o, void* workspace, hipStream_t stream) {

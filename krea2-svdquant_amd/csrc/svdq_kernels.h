@@ -260,6 +260,9 @@ struct Kv8Attention {
   int causal;
 };
 long kv8_attention_workspace_bytes(const Kv8Cache& c, int H, int causal);
+// the kernel, pieces of a tile along the keys, an XCD's tiles that are not split, and its tiles (few rows: tiles of a head)
+constexpr int KV8_FEW = 1, KV8_MANY = 2, KV8_MANY_RAGGED = 3;
+int kv8_attention_kernel(const Kv8Cache& c, int H, int causal, int& splits, int& whole, int& tiles);
 hipError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Attention& a, void* workspace, hipStream_t st);
 
 }  // namespace svdq

@@ -1009,6 +1009,8 @@ struct Kv8Plan {
   long pieces;  // partial results
 };
 
+long kv8_all(const Kv8Plan& pl, int Hkv) { return kv8_each(pl.numbers, Hkv) * (Hkv / kv8_shared(Hkv)); }   // an XCD's tiles
+
 // Sequences are as long as the table is wide at most, and shorter ones split into shorter pieces.
 Kv8Plan kv8_plan(const Kv8Cache& c, int H, bool causal) {
   const long G = H / c.Hkv, rows = c.N * G;
@@ -1034,7 +1036,7 @@ Kv8Plan kv8_plan(const Kv8Cache& c, int H, bool causal) {
   }
   // 64 workgroups run on an XCD at a time
   const long tiles = (rows + 127) / 128 > c.B ? (rows + 127) / 128 : c.B;   // as many as there can be, all about equal
-  const long each = kv8_each(tiles, c.Hkv) * (c.Hkv / kv8_shared(c.Hkv)), all = kv8_each(pl.numbers, c.Hkv) * (c.Hkv / kv8_shared(c.Hkv));
+  const long each = kv8_each(tiles, c.Hkv) * (c.Hkv / kv8_shared(c.Hkv)), all = kv8_all(pl, c.Hkv);
   const long rounds = each / 64, rest = each % 64, most = c.W / 4;
   pl.whole = (int)all;
   pl.splits = 1;
@@ -1060,7 +1062,7 @@ Kv8Plan kv8_plan(const Kv8Cache& c, int H, bool causal) {
 template <int D>
 hipError_t launch_attention(const Kv8Args& a, const Kv8Plan& pl, hipStream_t st) {
   if (pl.many) {
-    const int all = (int)(kv8_each(pl.numbers, a.c.Hkv) * (a.c.Hkv / kv8_shared(a.c.Hkv)));
+    const int all = (int)kv8_all(pl, a.c.Hkv);
     kv8_many_kernel<D><<<(unsigned)(8 * (pl.whole + (all - pl.whole) * pl.splits)), 256, 0, st>>>(a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess || pl.pieces == 0) return e;
     kv8_join_kernel<D, 128, 1><<<(unsigned)(8 * (all - pl.whole) * 16), 256, 0, st>>>(a);
@@ -1086,6 +1088,14 @@ hipError_t launch_kv8_append(const Kv8Cache& c, const uint16_t* k, long ldk, con
 long kv8_attention_workspace_bytes(const Kv8Cache& c, int H, int causal) {
   const Kv8Plan pl = kv8_plan(c, H, causal);
   return pl.pieces * pl.rows * (c.D + 2) * 4;
+}
+
+int kv8_attention_kernel(const Kv8Cache& c, int H, int causal, int& splits, int& whole, int& tiles) {
+  const Kv8Plan pl = kv8_plan(c, H, causal);
+  splits = pl.splits;
+  whole = pl.whole;
+  tiles = pl.many ? (int)kv8_all(pl, c.Hkv) : pl.numbers;
+  return !pl.many ? KV8_FEW : pl.splits > 1 && pl.run ? KV8_MANY_RAGGED : KV8_MANY;
 }
 
 hipError_t launch_kv8_attention(const Kv8Cache& c, const Kv8Attention& a, void* workspace, hipStream_t st) {

@@ -121,6 +121,7 @@ SIGNATURES = {
                                _I, _P, _P, _P]),
     "svdq_kv8_append": (_I, [_P, _L, _P, _L, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _P]),
     "svdq_kv8_attention_workspace": (_L, [_I, _I, _I, _I, _I, _I, _I]),
+    "svdq_kv8_attention_kernel": (_I, [_I, _I, _I, _I, _I, _I, _I, ctypes.POINTER(_I), ctypes.POINTER(_I), ctypes.POINTER(_I)]),
     "svdq_kv8_attention": (_I, [_P, _L, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, ctypes.c_float, _I, _P, _P,
                                 _P]),
 }
@@ -212,6 +213,15 @@ def fp8_kernel(m: int, n: int, k: int) -> tuple[int, int, int, int]:
     rows, cols, head = _I(), _I(), _I()
     kind = load().svdq_fp8_gemm_kernel(m, n, k, ctypes.byref(rows), ctypes.byref(cols), ctypes.byref(head))
     return int(kind), rows.value, cols.value, head.value
+
+
+def kv8_kernel(n: int, batch: int, width: int, heads: int, kv: int, dim: int, causal: bool) -> tuple[int, int, int, int]:
+    """(1: few rows, 2: many, 3: many in pieces of about one length; pieces of a tile; an XCD's tiles that are not split; its
+    tiles) of attention over an 8-bit cache (``svdq_kv8_attention_kernel``)."""
+    splits, whole, tiles = _I(), _I(), _I()
+    kind = load().svdq_kv8_attention_kernel(n, batch, width, heads, kv, dim, int(causal), ctypes.byref(splits), ctypes.byref(whole),
+                                            ctypes.byref(tiles))
+    return int(kind), splits.value, whole.value, tiles.value
 
 
 def w4a4_tile_cols(m: int, n: int, k: int, group: int, operand: int) -> int:

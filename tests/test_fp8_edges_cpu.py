@@ -56,3 +56,26 @@ def test_every_product_kernel_is_tested_where_it_is_chosen():
     for sizes in ([(m, n, 640, kernel) for m, n, kernel in KERNELS.values()], list(DEEP.values())):
         assert all(lib.fp8_kernel(m, n, k) == kernel for m, n, k, kernel in sizes)
         assert {kernel[:3] for *_, kernel in sizes} == every and any(kernel[3] for *_, kernel in sizes)
+
+
+# ---- attention over the cache ----------------------------------------------------------------------------
+def test_attention_plans():
+    """An image over itself splits its last tiles alone; a long sequence's token is split, two thousand short ones' are not."""
+    kind, splits, whole, tiles = lib.kv8_kernel(4352, 1, 73, 48, 12, 128, False)
+    assert kind == 2 and splits > 1 and 0 < whole < tiles
+    assert lib.kv8_kernel(4352, 1, 73, 48, 12, 128, True)[:2] == (2, 1)
+    assert lib.kv8_kernel(1, 1, 2049, 48, 12, 128, True)[0] == 1 and lib.kv8_kernel(1, 1, 2049, 48, 12, 128, True)[1] > 8
+    assert lib.kv8_kernel(2000, 2000, 64, 48, 12, 128, True)[:2] == (1, 1)
+    assert lib.kv8_kernel(900, 5, 80, 64, 8, 64, True)[0] == 3
+    for bad in ((0, 1, 1, 4, 2, 64), (1, 0, 1, 4, 2, 64), (1, 1, 0, 4, 2, 64), (1, 1, 1, 3, 2, 64), (1, 1, 1, 4, 2, 96), (2 ** 30, 1, 1, 64, 2, 64)):
+        assert lib.kv8_kernel(*bad, True)[0] == 0
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_workspace_is_that_of_the_plan(causal):
+    load = lib.load()
+    for n, b, w, heads, kv, d in ((4352, 1, 73, 48, 12, 128), (1, 1, 2049, 48, 12, 128), (32, 32, 129, 48, 12, 128), (900, 5, 80, 64, 8, 64),
+                                  (2140, 3, 14, 32, 2, 64), (300, 2, 3, 8, 1, 64)):
+        kind, splits, whole, tiles = lib.kv8_kernel(n, b, w, heads, kv, d, causal)
+        rows, pieces = (16, tiles * kv * splits if splits > 1 else 0) if kind == 1 else (128, 8 * (tiles - whole) * splits)
+        assert load.svdq_kv8_attention_workspace(n, b, w, heads, kv, d, int(causal)) == pieces * rows * (d + 2) * 4

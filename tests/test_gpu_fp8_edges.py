@@ -165,7 +165,7 @@ def product_on(a, sa, w, sw, bias=None):
 
 def check_on(got, want, bound):
     assert torch.isfinite(got).all() and torch.isfinite(want).all()
-    worst = ((got.double() - want).abs() / bound).max().item()
+    worst = ((got.double() - want).abs() / bound.clamp_min(1e-300)).max().item()   # 0: rows that see nothing
     assert worst <= 1.0, f"off by {worst:.3g} of the bound"
 
 
@@ -229,3 +229,56 @@ def test_product_of_small_whole_numbers_on_every_kernel(dev, size, bias):
     if bias:
         want += b.double()
     assert torch.equal(y, want.to(torch.bfloat16))
+
+
+# ---- attention of which a card's last tiles alone are split ------------------------------------------------------
+def attention_on(q, offsets, lengths, table, kc, vc, scales, scale, causal):
+    """fp8_util.attention of pages that are all there and hold numbers, on the operands' device."""
+    heads, d, group = q.shape[1], q.shape[2], q.shape[1] // kc.shape[1]
+    out, bound = (torch.zeros(q.shape, dtype=torch.float64, device=q.device) for _ in range(2))
+    for b, length in enumerate(lengths):
+        row, n = offsets[b], offsets[b + 1] - offsets[b]
+        if not n or not length:
+            continue
+        pages = torch.tensor(table[b][:-(-length // u.PAGE)], device=q.device)
+        last = torch.arange(n, device=q.device)[:, None] + length - n if causal else torch.full((n, 1), length, device=q.device)
+        hidden = torch.arange(length, device=q.device) > last
+        for h in range(heads):
+            kv = h // group
+            k = (kc[pages, kv].double() * scales[pages, kv, 0].double()[:, None, None]).reshape(-1, d)[:length]
+            v = (vc[pages, kv].double() * scales[pages, kv, 1].double()[:, None, None]).transpose(1, 2).reshape(-1, d)[:length]
+            x = q[row:row + n, h].double()
+            s = (x @ k.T * scale).masked_fill_(hidden, -float("inf"))
+            mag = (x.abs() @ k.abs().T * abs(scale)).masked_fill_(hidden, 0).amax(-1, keepdim=True)
+            p = torch.exp(s - s.amax(-1, keepdim=True).clamp_min(-1e300))
+            total = p.sum(-1, keepdim=True)
+            p = p / torch.where(total == 0, 1.0, total)
+            o, size = p @ v, p @ v.abs()
+            off = 2 * ((d + 8) * 2.0 ** -24 * 1.4427 * mag + 2.0 ** -20)
+            near = u.HALF / (1 - u.HALF) * (size + o.abs()) + size * (2 * off + 2.0 ** -18)
+            out[row:row + n, h] = o
+            bound[row:row + n, h] = near + u.HALF * (o.abs() + near) + 2.0 ** -133
+    return out, bound
+
+
+# key heads, query heads of each, sequences (new tokens, tokens held): more than the 64 tiles that an XCD runs at a time, and a few
+ROUNDS = {
+    "8 heads": (8, 4, [(700, 500), (0, 300), (900, 640), (560, 64)]), "12 heads": (12, 4, [(500, 700), (300, 1), (0, 0), (900, 333)]),
+    "2 heads": (2, 16, [(2140, 700)]), "3 heads": (3, 8, [(1500, 64), (1350, 700)]), "1 head": (1, 64, [(50, 700), (1000, 129)])}
+
+
+@pytest.mark.parametrize("name", ROUNDS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_of_which_the_last_tiles_are_split(dev, name, d):
+    from krea2_svdquant_amd.kernels.hip import lib
+    from tests.test_gpu_fp8 import Cache
+    kv, group, seqs = ROUNDS[name]
+    c = Cache(dev, seqs, kv, d, len(name), width=3)
+    rows, heads = c.offsets[-1], kv * group
+    kind, splits, whole, tiles = lib.kv8_kernel(rows, len(seqs), len(c.table[0]), heads, kv, d, False)
+    assert kind == 2 and splits > 1 and 0 < whole < tiles
+    q = normal((rows + 70, heads, d), c.g).to(dev)[:rows + 5]   # the last rows are no sequence's
+    args = c.device()
+    o = ops.kv8_attention(q, *args, d ** -0.5, False)
+    check_on(o, *attention_on(q, c.offsets, c.lengths(), c.table, *args[3:], d ** -0.5, False))
+    assert not o[rows:].any()
