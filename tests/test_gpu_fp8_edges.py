@@ -282,3 +282,23 @@ def test_attention_of_which_the_last_tiles_are_split(dev, name, d):
     o = ops.kv8_attention(q, *args, d ** -0.5, False)
     check_on(o, *attention_on(q, c.offsets, c.lengths(), c.table, *args[3:], d ** -0.5, False))
     assert not o[rows:].any()
+
+
+@pytest.mark.parametrize("prompt,singles,kernel", [(1500, 40, 1), (3000, 63, 1), (2100, 7, 3), (2100, 31, 3), (3000, 64, 2)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_of_a_prompt_among_single_tokens(dev, prompt, singles, kernel, d):
+    """A batch takes one kernel, by its rows in the mean: the prompt on that for few rows (1), single tokens on that for many
+    (2, 3: in pieces of about one length)."""
+    from krea2_svdquant_amd.kernels.hip import lib
+    from tests.test_gpu_fp8 import Cache
+    seqs = [(1, 1 + 97 * b % 2000) for b in range(singles)]
+    seqs.insert(singles // 3, (prompt, prompt + 500))
+    c = Cache(dev, seqs, 2, d, singles, width=1)
+    rows = c.offsets[-1]
+    group = 4 if kernel == 1 else 8
+    assert lib.kv8_kernel(rows, len(seqs), len(c.table[0]), 2 * group, 2, d, True)[0] == kernel
+    q = normal((rows, 2 * group, d), c.g).to(dev)
+    args = c.device()
+    for causal in (True, False):
+        o = ops.kv8_attention(q, *args, d ** -0.5, causal)
+        check_on(o, *attention_on(q, c.offsets, c.lengths(), c.table, *args[3:], d ** -0.5, causal))
