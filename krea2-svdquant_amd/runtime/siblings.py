@@ -103,10 +103,10 @@ def run_grouped(x: Tensor, layers: Sequence[nn.Module]) -> list[Tensor]:
     GPU), their GEMMs run as one launch (``forward_prepared_siblings``; W4A16 where the grouped
     tiles pay), each with its layer's LoRA adapters.  ``FP8Linear`` layers run one after another on one quantised
     activation, with the same results.  Other layer sets run one after another."""
-    if _share_fp8(x, layers):
-        h = layers[0].quantize(x)
-        return [m.forward_fp8(*h) for m in layers]
     if not _groupable(x, layers):
+        if _share_fp8(x, layers):
+            h = layers[0].quantize(x)
+            return [m.forward_fp8(*h) for m in layers]
         return [m(x) for m in layers]
     from ..kernels.hip.backend import forward_prepared_siblings
     preps = [m._prepare(x.device, with_adapters=bool(m.lora_adapters)) for m in layers]

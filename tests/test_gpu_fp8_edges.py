@@ -302,3 +302,37 @@ def test_attention_of_a_prompt_among_single_tokens(dev, prompt, singles, kernel,
     for causal in (True, False):
         o = ops.kv8_attention(q, *args, d ** -0.5, causal)
         check_on(o, *attention_on(q, c.offsets, c.lengths(), c.table, *args[3:], d ** -0.5, causal))
+
+
+# ---- layers that read the same input -----------------------------------------------------------------------------
+def test_grouped_layers_are_not_asked_for_a_shared_8_bit_activation(dev, monkeypatch):
+    """SVDQuant layers take their one launch without looking for 8-bit ones first; those share their activation as before."""
+    from krea2_svdquant_amd import FP8Linear, SVDQuantLinear
+    from krea2_svdquant_amd.runtime import krea2_standin as ks, siblings
+    asked = []
+    share = siblings._share_fp8
+    monkeypatch.setattr(siblings, "_share_fp8", lambda x, layers: asked.append(1) or share(x, layers))
+    g = torch.Generator(device=dev).manual_seed(0)
+    x = torch.randn((40, 256), device=dev, generator=g).to(torch.bfloat16)
+    layers = [SVDQuantLinear(ks.random_quantized_state(n, 256, rank=32, group_size=64, device=dev, generator=g), backend="hip_gfx950")
+              for n in (256, 128)]
+    assert [y.shape for y in siblings.run_grouped(x, layers)] == [(40, 256), (40, 128)] and not asked
+    layers = [FP8Linear.from_dense(torch.randn((n, 256), device=dev, generator=g)) for n in (256, 130)]
+    quantized = []
+    monkeypatch.setattr(FP8Linear, "quantize", lambda self, z: quantized.append(1) or ops.fp8_quantize(z))
+    for y, layer in zip(siblings.run_grouped(x, layers), layers):
+        assert torch.equal(y, ops.fp8_linear(x, layer._codes(), layer.weight_scales))
+    assert len(quantized) == 1 and asked
+
+
+def test_linear_of_rows_in_any_layout(dev):
+    """Repeated, transposed, unaligned, single and no rows: as their contiguous copy."""
+    g = gen(80)
+    w, ws = torch.randint(-100, 100, (130, 256), generator=g).float().to(torch.float8_e4m3fn).to(dev), torch.rand((2, 2), generator=g).to(dev)
+    base = normal((300, 40), g).to(dev)
+    for x in (normal((1, 256), g).to(dev).expand(5, 256), base[:256].T, base.view(-1)[3:3 + 256], base[:256, 5:6].T, base[:256].T[:0],
+              base.view(-1)[1:1 + 6 * 256].view(2, 3, 256)):
+        y = ops.fp8_linear(x, w, ws)
+        assert y.shape == (*x.shape[:-1], 130) and torch.equal(y, ops.fp8_linear(x.contiguous().clone(), w, ws))
+        codes, scales = ops.fp8_quantize(x)
+        assert torch.equal(y, ops.fp8_gemm(codes, scales, w, ws))
