@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) fp8_gemm_tile_kernel(Fp8GemmP
       for (int j = 0; j < S; ++j) {
         constexpr int slots = P * S;
         const int slot = pair * S + j;
-        __builtin_amdgcn_s_setprio(1);   // a wave that has a product to issue goes first: 359 -> 353 us at 4096 x 16384 x 6144
+        __builtin_amdgcn_s_setprio(1);   // a wave that has a product to issue goes first: 340 -> 336 us at 4096 x 16384 x 6144
         v[slot & 3] = fp8_mfma16(fw[pair & 1][j % 2], fa[j / 2]);
         __builtin_amdgcn_s_setprio(0);
         if (slot < 2) scaled(slots - 2 + slot, scl);
@@ -292,7 +292,7 @@ __device__ __forceinline__ void fp8_rows_sum(const Fp8GemmParams& p, uint8_t* sm
 // 8 waves takes 16 columns of the output and all of K; the waves take blocks of 128 columns of K in turn (whole cache
 // lines of w) and add their sums through LDS in wave order.  Each wave has a ring of U blocks in LDS to itself, filled
 // by DMA, so the waves need no barrier before the sums.  MR = 8 or 16 rows of a are held; rows beyond M repeat the last.
-// HBM-bound: 1 x 6144, K = 6144 7.3 us (5.2 TB/s), 16 rows 8.6; N = 16384 18.4 (5.5 TB/s).
+// HBM-bound: 1 x 6144, K = 6144 8.1 us a call (4.7 TB/s), 16 rows 9.1; N = 16384 18.4 (5.5 TB/s).
 template <int MR, int U>
 struct Fp8Rows {
   static constexpr int NW = 8, OA = 2048, OSC = OA + 128 * MR, UNIT = OSC + 256;
@@ -363,8 +363,7 @@ __global__ void __launch_bounds__(512) fp8_gemm_rows_kernel(Fp8GemmParams p) {
 // Strips, for outputs of few tiles (16 TM rows a workgroup, 16 TN columns): as with few rows, NW waves take blocks of all of K
 // in turn, each with a ring of two in LDS to itself, and add their sums in wave order.  A lone tile spends 0.27 us on a
 // block of K, most of it waiting at one point or another for DMA, LDS, the matrix unit and the other waves; here NW such
-// chains run side by side without a barrier.  77 x 6144, K = 6144: 12.3 us, as 64 x 64 tiles 17.1, as those in pieces of K that
-// a second launch joins 16.5 (w alone takes 7.3 to read).
+// chains run side by side without a barrier.  77 x 6144, K = 6144: 11.6 us, as 64 x 64 tiles 16.5 (w alone takes 7.1 to read).
 template <int TM, int TN, int NW>
 struct Fp8Strip {
   static constexpr int OA = 2048 * TN, OSC = OA + 2048 * TM, UNIT = OSC + 512;   // w, a, scales of 16 TM rows and w's
@@ -490,9 +489,9 @@ __device__ __forceinline__ float row4_scale(const u32x4 (&v)[4]) {
 
 // The same of up to four rows of a bf16 activation, encoded by every workgroup for itself: K % 128 = 0, rows of x on 16 bytes.
 // A lane holds 32 of a block's 128 values of its row, and four lanes agree on the scale.  The conversion rounds as that of the
-// quantising kernel, so the sums are the same.  The encoding takes longer than the product's wait for w leaves, but less
-// than a launch: one row, K = 6144, N = 6144 9.8 us and (two launches) 10.2, N = 1536 5.5 and 8.1; with eight rows, N = 16384
-// it took 24.6 and 23.3, so more than four go the other way.
+// quantising kernel, so the sums are the same.  A block is encoded while its part of w is on its way; that takes longer than the wait,
+// but less than a launch: one row, K = 6144, N = 6144 9.3 us and (two launches) 10.2, N = 1536 5.4 and 8.0, N = 16384 19.8 and 20.6, four
+// rows, N = 6144 9.5 and 10.4.  Built for eight rows, N = 16384 took 24.6 and in two launches 23.3, so more than four go the other way.
 struct Fp8RowsOf {
   static constexpr int MR = 4, NW = 8, U = 3, OA = 2048, OSC = OA + 256 * MR, UNIT = OSC + 256;
   static constexpr int D = 2 + 1 + 1;   // DMA instructions of a block: w, x, the weight's scale
@@ -580,15 +579,15 @@ hipError_t launch_strip(const Fp8GemmParams& p, hipStream_t st) {
 // What a kernel's workgroups take: rows of a, of w, their threads, how many share a CU, and microseconds for a block of K with
 // n of them on a CU (us[n - 1]); a launch takes 3.5 us besides, a further round 1, and w is read from memory at 5.2 TB/s at most.
 // Measured (us, K = 6144; strips of 32 x 16, 32 x 32, 64 x 32, 48 x 64 and 64 x 64, then the tiles):
-//     32 x  1536     5.4   6.6   8.6  10.5  12.4 |  16.1  21.6  30.1  37.8  59.2
-//     77 x  1536     9.5   6.9   9.0  10.8  13.0 |  16.1  21.7  30.5  38.0  59.7
-//     32 x  6144    12.2   8.9   9.7  11.4  13.5 |  16.5  21.6  40.2  39.1  59.6
-//     64 x  6144    17.4  15.5  10.9  12.3  14.3 |  16.8  21.7  40.5  39.6  59.9
-//     77 x  6144       -  21.2  17.6  12.3  14.5 |  17.1  21.9  40.2  39.3  59.9
-//    128 x  6144       -     -  19.5  21.5  14.8 |  17.0  21.7  40.3  39.5  60.1
-//    320 x  6144       -     -  39.5  36.0  28.6 |  24.1  25.0  40.6  41.0  61.2
-//   1024 x  6144       -     -     -     -  81.1 |  64.9  57.3  51.7  45.6  63.1
-//   2381 x  6144       -     -     -     - 201   | 156   132   109   101    86.1
+//     32 x  1536     6.2   7.5   8.6  10.4  12.4 |  16.0  21.2  40.0  38.2  59.6
+//     77 x  1536     9.4   7.5   9.2  11.0  13.2 |  16.1  21.3  40.3  38.5  60.0
+//     32 x  6144    12.1   9.3   9.3  11.0  13.1 |  16.5  21.4  40.6  38.6  59.9
+//     64 x  6144    17.3  15.9  10.6  11.4  13.9 |  16.7  21.4  40.8  38.8  60.3
+//     77 x  6144    25.4  21.3  17.0  11.6  13.6 |  16.5  21.5  40.9  38.8  60.3
+//    128 x  6144    32.2  23.8  19.3  20.7  14.1 |  16.7  21.6  41.0  38.8  60.5
+//    320 x  6144    76.6  59.1  37.6  32.7  26.6 |  23.4  22.4  40.3  39.2  61.5
+//   1024 x  6144   240   167   107    94.2  76.8 |  62.4  52.9  47.9  42.2  61.7
+//   2381 x  6144   567   388   253   200   188   | 149   125   103    95.9  80.6
 struct Fp8Cost {
   int rows, cols, threads, slots;
   float us[3];
@@ -621,7 +620,7 @@ Fp8Choice choose(long M, long N, int K) {
 }
 
 // Rows ahead of the last round of the largest tiles, where the others take less in a launch of their own than in a round that is
-// nearly empty, else 0.  4352 x 16384, K = 6144: 393 us, in one launch 400 to 415 (4096 rows alone 346 to 354).
+// nearly empty, else 0.  4352 x 16384, K = 6144: 382 us, in one launch 396 (4096 rows alone 342 to 347).
 long head_rows(long M, long N, int K) {
   const Fp8Cost& t = kCosts[FP8_KERNELS - 1];
   const Fp8Choice all = choose(M, N, K);

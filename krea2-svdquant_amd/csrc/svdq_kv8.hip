@@ -277,7 +277,7 @@ __device__ __forceinline__ bool kv8_piece(const Kv8Args& p, int& number, int& hk
   uint32_t k;
   if (p.run) {
     // every tile's first piece, then their second, ...: those that a tile does not have come last.  Between others the dispatcher
-    // deals these out to few of the CUs (250 us, so 168).
+    // deals these out to few of the CUs (6 sequences of 900 to 9000 keys 192 us, so 168).
     const uint32_t tail = kv8_each(p.numbers, p.c.Hkv) * (p.c.Hkv / kv8_shared(p.c.Hkv)) - p.whole;
     split = (j - p.whole) / tail;
     k = (j - p.whole) - split * tail;
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(256, 2) kv8_rows_kernel(Kv8Args p) {
   const int tid = threadIdx.x, lane = tid & 63, lr = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   // heads one after another: a page's heads lie side by side, and the card reads them together from all of its memory (a
-  // head to an XCD reads parts of it: 131072 tokens 99 us, so 75)
+  // head to an XCD reads parts of it: 131072 tokens 94 us, so 69)
   const uint32_t hk = blockIdx.x % p.c.Hkv, rest = blockIdx.x / p.c.Hkv, split = rest % p.splits, number = rest / p.splits;
   Kv8Tile t;
   if (!kv8_tile<R>(p, number, t)) return;
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(256, 2) kv8_rows_kernel(Kv8Args p) {
     };
     look_up(0);
     int first = 0;   // the page that lane 0 holds
-    // past the caches where no other tile reads the page (131072 tokens 75 us, so 66)
+    // past the caches where no other tile reads the page (131072 tokens 77 us, so 69)
     const bool once = t.rows <= R;
     auto fetch = [&](int i) {   // page i of this wave, past the last one that again
       const int pid = max(__builtin_amdgcn_readlane(id, max(min(i, count - 1) - first, 0)), 0);
@@ -697,8 +697,8 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(Kv8Args p) {
 // Scales that are no ordinary positive numbers are dealt with as the pages come in: a factor below 0 turns the keys' signs, other
 // scales of values are multiplied into them, those that are not finite make the codes NaN.  Pages that are not there count as -infinity.
 //
-// Bound by the softmax and the conversions beside the products: 4352 tokens of 48 heads of 128 over 4608, 480 us, 1020 TFLOP/s
-// (causal, over themselves 267); heads of 64 700 TFLOP/s.
+// Bound by the softmax and the conversions beside the products: 4352 tokens of 48 heads of 128 over 4608, 483 us, 1020 TFLOP/s
+// (causal, over themselves 268); heads of 64, 4 x 2048 causal 98 us (700 TFLOP/s), 8192 all visible 919 TFLOP/s.
 //
 // Rows in LDS are not padded: chunks of 16 bytes lie at slots exchanged by the row, c ^ (row mod 16) in rows of 256 bytes, c ^
 // (row / 2 mod 8) in rows of 128, which spreads sixteen lanes' reads of a chunk, and sixteen lanes' writes of two chunks each, over the 64
@@ -1011,22 +1011,25 @@ struct Kv8Plan {
 
 long kv8_all(const Kv8Plan& pl, int Hkv) { return kv8_each(pl.numbers, Hkv) * (Hkv / kv8_shared(Hkv)); }   // an XCD's tiles
 
-// Sequences are as long as the table is wide at most, and shorter ones split into shorter pieces.
+// Sequences are as long as the table is wide at most, and shorter ones split into shorter pieces, a page or none each where the table
+// is much wider (32 tokens over 2000 keys each: a table of 33 pages 36 us, of 129 or 2049 49).
 Kv8Plan kv8_plan(const Kv8Cache& c, int H, bool causal) {
   const long G = H / c.Hkv, rows = c.N * G;
   Kv8Plan pl{};
   // A page that is read for 16 rows takes the few-rows kernel's 16 x 16 products through all of it again for the next 16; the
   // other kernel reads it once for 128 rows, but a workgroup of it that is not full takes as long as a full one.  Rows
-  // (of heads) a sequence, few / many rows kernel: 8 x 128 of 4096 keys 30 / 48 us, 8 x 256 48 / 54, 32 x 64 74 / 107,
-  // 1 x 308 of 65536 (two and a half tiles) 330 / 223.
+  // (of heads) a sequence at most, ragged up to 4096 keys, 12 heads of 128, few / many rows kernel: 8 x 128 30 / 46 us, 8 x 256
+  // 47 / 53, 32 x 64 75 / 102; 1 x 308 of 65536 (two and a half tiles) 340 / 210.
+  // One kernel serves all of a batch, by its rows in the mean: a prompt among single tokens takes longer than the two apart (2000
+  // tokens over 6096 and 31 over 4096 500 us, 286 and 65 apart; 4352 and 31 356, 260 and 65).
   pl.many = rows > 256L * c.B;
   pl.rows = pl.many ? 128 : 16;
   pl.numbers = (int)(rows / pl.rows + c.B + 1);
   if (!pl.many) {
     const long busy = ((rows + 15) / 16 > c.B ? (rows + 15) / 16 : c.B) * c.Hkv;
-    // One workgroup a CU reads fastest where there are no more (131072 tokens, 12 heads, in 252 pieces 64 us, 320 80, 512 68).
-    // Up to 512 tiles in two pieces each fill the last round better (32 sequences of 1000 to 8000 tokens, 12 heads: 88 us, in
-    // one piece 98; pieces of each by its length 92), longer tables alone (64 of 2048 in one piece 21, two 24).
+    // One workgroup a CU reads fastest where there are no more (131072 tokens, 12 heads, in 252 pieces 69 us, 312 84, 504 72).
+    // Up to 512 tiles in two pieces each fill the last round better (32 sequences of up to 8192 tokens, 12 heads: 88 us, in
+    // one piece 99), longer tables alone (64 of up to 2048, 4 heads of 64, in one piece 16, two 19.5).
     const long want = busy <= 256 ? 256 / busy : busy <= 512 ? 2 : 1, most = c.W / (busy <= 256 ? 16 : 64);
     pl.splits = (int)(want > KV8_SPLITS ? KV8_SPLITS : want);
     if (pl.splits > most) pl.splits = (int)most;
@@ -1044,8 +1047,8 @@ Kv8Plan kv8_plan(const Kv8Cache& c, int H, bool causal) {
     long want = 64 / rest;
     // Tiles that take more than half of the places are not split evenly, and the longest would run alone at the end: there a
     // batch's longer sequences are cut into up to three pieces, about as long as a place's share of all (6 sequences of 900 to
-    // 9000 keys, 12 heads of 128: 251 us, so 168; 4 of 940 to 6000, 4 heads of 64, 117 and 85).  With fewer tiles it brings
-    // nothing, as two workgroups of a CU get done 1.2 times as much as one (three chunks over 5000 keys and less 44 us, so 50).
+    // 9000 keys, 12 heads of 128: 251 us, so 168; 4 of 940 to 6000, 4 heads of 64, 117 and 86).  With fewer tiles it brings
+    // nothing, as two workgroups of a CU get done 1.2 times as much as one (three chunks over 5000 keys and less 42 us, so 53).
     if (rounds == 0 && want == 1 && c.B > 1 && c.B < 63) {   // a lane for each sequence
       want = 3;
       pl.run = (int)(512 / c.Hkv > 1 ? 512 / c.Hkv : 1);

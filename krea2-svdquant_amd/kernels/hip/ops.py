@@ -690,7 +690,8 @@ def kv8_attention(q: Tensor, cu_seqlens: Tensor, lengths: Tensor, block_table: T
     """``svdq::kv8_attention``: softmax attention of bf16 ``q`` [tokens, H, D] over an 8-bit cache (``kv8_append``), H a
     multiple of Hkv: ``sum_j softmax_j(scale q . k_j) v_j`` over the ``lengths[b]`` tokens that a sequence holds, its new ones
     among them; with ``causal`` the i-th of n new tokens sees ``lengths[b] - n + i + 1`` of them.  bf16 [tokens, H, D]; rows
-    that see nothing, and rows behind the last sequence, are 0.  A scale that is not finite makes its page's keys (or values)
+    that see nothing, and rows behind the last sequence, are 0.  One kernel serves the batch, by its rows in the mean, and the table's
+    width decides how sequences are split: prompts and single tokens are faster in calls of their own.  A scale that is not finite makes its page's keys (or values)
     NaN; pages that are not in the cache hold nothing."""
     return _mx("kv8_attention", q, q, cu_seqlens, lengths, block_table, k_codes, v_codes, scales, scale, causal)
 
