@@ -336,3 +336,58 @@ def test_linear_of_rows_in_any_layout(dev):
         assert y.shape == (*x.shape[:-1], 130) and torch.equal(y, ops.fp8_linear(x.contiguous().clone(), w, ws))
         codes, scales = ops.fp8_quantize(x)
         assert torch.equal(y, ops.fp8_gemm(codes, scales, w, ws))
+
+
+# ---- the largest sizes ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("m,n", [(3, 50), (12, 50), (20, 50), (1100, 130)])
+def test_product_of_the_longest_rows(dev, m, n):
+    """K = 2^22: codes of 1 and -1 and scales of 1, so that sums are whole numbers below 2^24."""
+    k, g = 2 ** 22, torch.Generator(device=dev).manual_seed(m)
+    a, w = (torch.randint(0, 2, (r, k), device=dev, generator=g, dtype=torch.uint8) * 128 + 0x38 for r in (m, n))
+    sa, sw = torch.ones((k // 128, m), device=dev), torch.ones((-(-n // 128), k // 128), device=dev)
+    y = ops.fp8_gemm(a.view(torch.float8_e4m3fn), sa, w.view(torch.float8_e4m3fn), sw)
+    want = torch.zeros((m, n), device=dev, dtype=torch.float64)
+    for c in range(0, k, 2 ** 17):
+        want += (1 - (a[:, c:c + 2 ** 17] >> 7).double() * 2) @ (1 - (w[:, c:c + 2 ** 17] >> 7).double() * 2).T
+    assert torch.equal(y, want.to(torch.bfloat16))
+
+
+def test_quantize_a_row_of_2_30_columns(dev):
+    g = torch.Generator(device=dev).manual_seed(0)
+    x = torch.zeros((1, 2 ** 30), dtype=torch.bfloat16, device=dev)
+    parts = (0, 2 ** 29 - 4096, 2 ** 30 - 8192)
+    for p in parts:
+        x[0, p:p + 8192] = torch.randn(8192, device=dev, generator=g).to(torch.bfloat16)
+    codes, scales = ops.fp8_quantize(x)
+    for p in parts:
+        c, s = ops.fp8_quantize(x[:, p:p + 8192].contiguous())
+        assert torch.equal(codes[:, p:p + 8192].view(torch.uint8), c.view(torch.uint8))
+        assert torch.equal(scales[p // 128:p // 128 + 64], s)
+    assert not codes[:, 10000:20000].view(torch.uint8).any()
+
+
+def test_head_norms_whose_output_passes_32_bits(dev):
+    t, h, kv, d = 600000, 48, 12, 64
+    g = torch.Generator(device=dev).manual_seed(1)
+    x = torch.empty((t, h + kv, d), dtype=torch.bfloat16, device=dev)
+    x[:] = torch.randn((1000, h + kv, d), device=dev, generator=g).to(torch.bfloat16).repeat(600, 1, 1)
+    tab = torch.randn((700, d // 2), device=dev, generator=g)
+    at = torch.randint(0, 700, (t,), device=dev, generator=g)
+    qo, ko = ops.qk_norm_rope(x[:, :h], x[:, h:], None, None, tab, tab, 1e-6, at)
+    for p in (0, t // 2, t - 100):
+        q, k = ops.qk_norm_rope(x[p:p + 100, :h], x[p:p + 100, h:], None, None, tab, tab, 1e-6, at[p:p + 100])
+        assert torch.equal(qo[p:p + 100], q) and torch.equal(ko[p:p + 100], k)
+
+
+def test_attention_whose_output_passes_32_bits(dev):
+    """1000 sequences of 300 tokens of 64 heads, which share their pages; the last ones against the definition."""
+    from tests.test_gpu_fp8 import Cache
+    n, heads, d, count = 300, 64, 128, 1000
+    c = Cache(dev, [(n, 310)], 8, d, 90)
+    _, _, _, k, v, s = c.device()
+    q = normal((n, heads, d), c.g).to(dev).repeat(count, 1, 1)
+    o = ops.kv8_attention(q, i32(dev, [n * b for b in range(count + 1)]), i32(dev, [310] * count), i32(dev, c.table * count), k, v, s,
+                          d ** -0.5)
+    want, bound = attention_on(q[:n], [0, n], [310], c.table, k, v, s, d ** -0.5, True)
+    for b in (0, count // 2, count - 1):
+        check_on(o[n * b:n * b + n], want, bound)
